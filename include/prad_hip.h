@@ -62,6 +62,7 @@ enum {
 };
 
 typedef struct prad_buf* prad_buf_t;
+typedef struct prad_index* prad_index_t; /* a vector of int32 on the device: token ids, sequence offsets, step counters */
 
 /* ---- lifecycle: replaces CudaBlas.Instance.{DeviceId,Initialize,Dispose,IsInitialized},
  *      src/RMAD/CudaBlas.cs:71-155 ------------------------------------------------------- */
@@ -375,6 +376,41 @@ int32_t prad_softmax_cce(prad_buf_t x, prad_buf_t target, prad_buf_t p, prad_buf
 int32_t prad_dense_softmax_cce(prad_buf_t A, prad_buf_t W, prad_buf_t bias, prad_buf_t target, prad_buf_t z, prad_buf_t p,
                                prad_buf_t loss, prad_buf_t dp, prad_buf_t dz, prad_buf_t dA, prad_buf_t dW, prad_buf_t dbias,
                                int32_t accumulate_dW, int32_t act, prad_buf_t act_src, double alpha);
+
+/* ---- token models: what stands between token ids and the layers above.  The reference has no fused counterpart of these:
+ *      it composes them from matrix products, softmax and elementwise nodes (src/RMAD/MatrixMultiplyOperation.cs:50-126,
+ *      src/RMAD/SoftmaxOperation.cs:45-110, src/RMAD/HadamardProductOperation.cs:50-118). ------------------------------ */
+/* Index vectors.  They live on the device so that a recorded launch sequence reads their values anew at every launch:
+ * upload the next batch's ids or offsets between launches, or change them inside the sequence with prad_index_add.
+ * prad_index_alloc zero-fills; prad_index_wrap borrows caller-owned device memory (4-byte aligned); upload and download
+ * move the whole vector (n must be its length) and wait; prad_index_add adds delta to every element (modulo 2^32). */
+int32_t prad_index_alloc(int64_t n, prad_index_t* out);
+int32_t prad_index_wrap(int64_t n, void* device_ptr, prad_index_t* out);
+int32_t prad_index_free(prad_index_t v);
+int32_t prad_index_length(prad_index_t v, int64_t* n);
+void* prad_index_device_ptr(prad_index_t v); /* getter: NULL for a bad handle */
+int32_t prad_index_upload(prad_index_t v, const void* src, int64_t n);
+int32_t prad_index_download(prad_index_t v, void* dst, int64_t n);
+int32_t prad_index_add(prad_index_t v, int32_t delta);
+
+/* Embedding: out[i] = scale * table[ids[i]]; table is vocabulary x width, out tokens x width, ids holds `tokens` elements.
+ * An id outside [0, vocabulary) - padding, usually -1 - gives a row of zeros and takes no part in the gradient. */
+int32_t prad_embedding_fwd(prad_buf_t table, prad_index_t ids, double scale, prad_buf_t out);
+/* dtable[r] = scale * (sum of dout[i] over all i with ids[i] == r), every row of dtable written; accumulate != 0 adds to what
+ * dtable holds and leaves the other rows alone.  Sums are taken in double and in one fixed order: equal calls give equal
+ * bits. */
+int32_t prad_embedding_bwd(prad_buf_t dout, prad_index_t ids, double scale, prad_buf_t dtable, int32_t accumulate);
+
+/* Dropout: y = x / (1 - p) where an element is kept, 0 where it is dropped, plus the residual (NULL: none); 0 <= p < 1, and
+ * an element is dropped with probability floor(p * 2^32) / 2^32.  What is kept is a function of (seed, site, step, position)
+ * alone - word e % 4 of the counter-based generator Philox4x32-10 on counter (e / 4 in two words, step, site) and key seed,
+ * against floor(p * 2^32), e the row-major position - so no mask is stored and backward forms it again:
+ * dx = dy / (1 - p) where kept, else 0 (the residual's gradient is dy itself).  `site` tells the places of a model apart.
+ * `step` is an index vector whose first element is read when the call runs on the device (NULL: 0): a recorded training
+ * step advances it with prad_index_add, so that every launch draws other masks.  y may be x or the residual, dx may be dy;
+ * any other overlap is refused. */
+int32_t prad_dropout_fwd(prad_buf_t x, prad_buf_t residual, prad_buf_t y, double p, int64_t seed, int32_t site, prad_index_t step);
+int32_t prad_dropout_bwd(prad_buf_t dy, prad_buf_t dx, double p, int64_t seed, int32_t site, prad_index_t step);
 
 /* ---- GradientClipper.ClipGradients, src/RMAD/GradientClipper.cs:118-157 and :212-253 (in place) */
 int32_t prad_clip(prad_buf_t g, double clip_value, double min_value);

@@ -121,6 +121,18 @@ SIGNATURES = {
     "prad_graph_launch": (_i32, [_vp]),
     "prad_graph_set_adam_iteration": (_i32, [_vp, _f64]),
     "prad_graph_destroy": (_i32, [_vp]),
+    "prad_index_alloc": (_i32, [_i64, _vpp]),
+    "prad_index_wrap": (_i32, [_i64, _vp, _vpp]),
+    "prad_index_free": (_i32, [_vp]),
+    "prad_index_length": (_i32, [_vp, _i64p]),
+    "prad_index_device_ptr": (_vp, [_vp]),
+    "prad_index_upload": (_i32, [_vp, _vp, _i64]),
+    "prad_index_download": (_i32, [_vp, _vp, _i64]),
+    "prad_index_add": (_i32, [_vp, _i32]),
+    "prad_embedding_fwd": (_i32, [_vp, _vp, _f64, _vp]),
+    "prad_embedding_bwd": (_i32, [_vp, _vp, _f64, _vp, _i32]),
+    "prad_dropout_fwd": (_i32, [_vp, _vp, _vp, _f64, _i64, _i32, _vp]),
+    "prad_dropout_bwd": (_i32, [_vp, _vp, _f64, _i64, _i32, _vp]),
     "prad_clip": (_i32, [_vp, _f64, _f64]),
     "prad_adam": (_i32, [_vp, _vp, _vp, _vp, _f64, _f64, _f64, _f64, _f64]),
     "prad_clip_multi": (_i32, [_vpp, _i32, _f64, _f64]),

@@ -432,6 +432,17 @@ hipError_t launch_window_attention_fwd(const float* QKV, float* P, float* O, int
 hipError_t launch_window_attention_bwd(const float* QKV, const float* P, const float* dO, float* dQKV, int64_t windows, int64_t heads,
                                        int64_t tokens, float scale, hipStream_t stream);
 
+// Embedding lookup and gradient, dropout, index vectors (csrc/token.hip).
+template <typename T> hipError_t launch_embedding_fwd(const T* table, const int32_t* ids, T* out, int64_t tokens, int64_t vocab, int64_t width, T scale,
+                                                      hipStream_t s);
+size_t embedding_bwd_workspace_bytes(int64_t tokens, int64_t width);
+template <typename T> hipError_t launch_embedding_bwd(const T* dout, const int32_t* ids, T* dtable, int64_t tokens, int64_t vocab, int64_t width,
+                                                      double scale, int accumulate, void* workspace, hipStream_t s);
+// residual may be nullptr; step nullptr: step 0
+template <typename T> hipError_t launch_dropout(const T* x, const T* residual, T* y, int64_t n, double p, int64_t seed, int32_t site,
+                                                const int32_t* step, hipStream_t s);
+hipError_t launch_index_add(int32_t* v, int64_t n, int32_t delta, hipStream_t s);
+
 // MatrixMultiplyAndSum
 // S = samples of a batch (each with its own A, out, dOut, dA and P slices of dB; the P slices of B are shared).
 template <typename T> hipError_t launch_matmul_sum_fwd(const T* A, const T* B, T* out, double* workspace, int64_t M, int64_t K,

@@ -16,6 +16,7 @@
 #include <cstring>
 #include <mutex>
 #include <map>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -31,6 +32,14 @@ struct prad_buf {
     size_t block_bytes;  // size class of the device block behind an owned buffer (0 for borrowed memory)
 };
 
+struct prad_index {
+    uint32_t magic;
+    int64_t n;
+    int32_t* ptr;
+    bool owned;
+    size_t block_bytes;
+};
+
 // Scratch of the allocation-free entry point (prad_clip_adam_multi_noalloc): device memory that exists from the
 // moment the code object is loaded, one copy per GPU, held until the process ends.  In host code the name is only
 // a stand-in for the symbol: its device address is asked for once per device (init_static_scratch) and every
@@ -41,6 +50,7 @@ static __device__ __align__(256) unsigned char scratch[STATIC_SCRATCH_BYTES];
 namespace {
 
 constexpr uint32_t BUF_MAGIC = 0x50524144u;  // "PRAD"
+constexpr uint32_t INDEX_MAGIC = 0x50524149u;  // "PRAI"
 constexpr size_t STAGING_CHUNK = (size_t)256 << 20;
 
 constexpr size_t COUNTER_BYTES = 4096;  // arrival counters: one per tile of a split or paired product, and a few
@@ -137,6 +147,21 @@ inline int64_t count(prad_buf_t b) { return b->depth * b->rows * b->cols; }
     do {                                                                                              \
         if (!valid(b)) return fail(PRAD_ERR_BAD_HANDLE, "%s is not a live buffer handle", #b);        \
     } while (0)
+
+inline bool valid(prad_index_t v) { return v != nullptr && v->magic == INDEX_MAGIC; }
+#define REQUIRE_INDEX(v)                                                                              \
+    do {                                                                                              \
+        if (!valid(v)) return fail(PRAD_ERR_BAD_HANDLE, "%s is not a live index vector", #v);         \
+    } while (0)
+
+inline size_t buf_bytes(prad_buf_t b) { return (size_t)count(b) * elem_size(b->dtype); }
+inline bool ranges_meet(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+// Whether two buffers share memory.
+inline bool overlap(prad_buf_t a, prad_buf_t b) { return ranges_meet(a->ptr, buf_bytes(a), b->ptr, buf_bytes(b)); }
+inline bool overlap(prad_buf_t a, prad_index_t v) { return ranges_meet(a->ptr, buf_bytes(a), v->ptr, (size_t)v->n * 4); }
 
 // Lock must be held.  Waits for everything enqueued on the library stream.
 int32_t sync_all() {
@@ -1778,6 +1803,177 @@ int32_t prad_buf_view_rows(prad_buf_t parent, int64_t row0, int64_t rows, prad_b
     char* base = static_cast<char*>(parent->ptr) + (size_t)row0 * parent->cols * elem_size(parent->dtype);
     *out = new prad_buf{BUF_MAGIC, parent->dtype, 1, rows, parent->cols, base, false, 0};
     return PRAD_OK;
+}
+
+// ---- index vectors, embedding, dropout ----------------------------------------------------------
+int32_t prad_index_alloc(int64_t n, prad_index_t* out) {
+    REQUIRE_INIT();
+    if (out == nullptr) return fail(PRAD_ERR_ARG, "out is NULL");
+    *out = nullptr;
+    if (n <= 0) return fail(PRAD_ERR_ARG, "an index vector needs at least one element");
+    prad_index* v = new (std::nothrow) prad_index{INDEX_MAGIC, n, nullptr, true, 0};
+    if (v == nullptr) return fail(PRAD_ERR_ALLOC, "out of host memory");
+    std::lock_guard<std::mutex> lock(g_ctx.mu);
+    int32_t st = PRAD_OK;
+    void* p = nullptr;
+    if (g_ctx.recording) st = fail(PRAD_ERR_RECORDING, "an allocation cannot be part of a recorded launch sequence");
+    if (st == PRAD_OK) st = pool_take((size_t)n * 4, &p, &v->block_bytes);
+    if (st == PRAD_OK) {
+        v->ptr = static_cast<int32_t*>(p);
+        const hipError_t e = launch_fill_zero<float>(static_cast<float*>(p), n, CUR_STREAM);  // (a float zero has the bits of an int32 zero)
+        if (e != hipSuccess) {
+            (void)pool_give(p, v->block_bytes);
+            st = fail(PRAD_ERR_LAUNCH, "zero fill failed: %s", hipGetErrorString(e));
+        }
+    }
+    if (st != PRAD_OK) {
+        delete v;
+        return st;
+    }
+    *out = v;
+    return PRAD_OK;
+}
+
+int32_t prad_index_wrap(int64_t n, void* device_ptr, prad_index_t* out) {
+    REQUIRE_INIT();
+    if (out == nullptr || device_ptr == nullptr) return fail(PRAD_ERR_ARG, "NULL argument");
+    *out = nullptr;
+    if (n <= 0) return fail(PRAD_ERR_ARG, "an index vector needs at least one element");
+    if (reinterpret_cast<uintptr_t>(device_ptr) % 4 != 0) return fail(PRAD_ERR_ARG, "an index vector starts on a multiple of 4 bytes");
+    prad_index* v = new (std::nothrow) prad_index{INDEX_MAGIC, n, static_cast<int32_t*>(device_ptr), false, 0};
+    if (v == nullptr) return fail(PRAD_ERR_ALLOC, "out of host memory");
+    *out = v;
+    return PRAD_OK;
+}
+
+int32_t prad_index_free(prad_index_t v) {
+    if (v == nullptr) return PRAD_OK;
+    REQUIRE_INDEX(v);
+    if (v->owned) {
+        REQUIRE_INIT();
+        ENQUEUE_LOCK();
+        NOT_WHILE_RECORDING("freeing an index vector");
+        if (int32_t st = pool_give(v->ptr, v->block_bytes)) return st;
+    }
+    v->magic = 0;
+    delete v;
+    return PRAD_OK;
+}
+
+int32_t prad_index_length(prad_index_t v, int64_t* n) {
+    REQUIRE_INDEX(v);
+    if (n == nullptr) return fail(PRAD_ERR_ARG, "n is NULL");
+    *n = v->n;
+    return PRAD_OK;
+}
+
+void* prad_index_device_ptr(prad_index_t v) { return valid(v) ? v->ptr : nullptr; }
+
+int32_t prad_index_upload(prad_index_t v, const void* src, int64_t n) {
+    REQUIRE_INIT();
+    REQUIRE_INDEX(v);
+    if (src == nullptr || n != v->n) return fail(PRAD_ERR_ARG, "upload moves the whole index vector of %lld elements", (long long)v->n);
+    ENQUEUE_LOCK();
+    NOT_WHILE_RECORDING("a copy to or from the host");
+    HIP_TRY(hipMemcpyAsync(v->ptr, src, (size_t)n * 4, hipMemcpyHostToDevice, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return sync_all();
+}
+
+int32_t prad_index_download(prad_index_t v, void* dst, int64_t n) {
+    REQUIRE_INIT();
+    REQUIRE_INDEX(v);
+    if (dst == nullptr || n != v->n) return fail(PRAD_ERR_ARG, "download moves the whole index vector of %lld elements", (long long)v->n);
+    ENQUEUE_LOCK();
+    NOT_WHILE_RECORDING("a copy to or from the host");
+    HIP_TRY(hipMemcpyAsync(dst, v->ptr, (size_t)n * 4, hipMemcpyDeviceToHost, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return sync_all();
+}
+
+int32_t prad_index_add(prad_index_t v, int32_t delta) {
+    REQUIRE_INIT();
+    REQUIRE_INDEX(v);
+    ENQUEUE_LOCK();
+    HIP_TRY(launch_index_add(v->ptr, v->n, delta, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+// rows x width against a table of the same width, `rows` ids
+static int32_t embedding_check(prad_buf_t table, prad_buf_t rows, prad_index_t ids, double scale) {
+    REQUIRE_BUF(table); REQUIRE_BUF(rows); REQUIRE_INDEX(ids);
+    if (int32_t st = same_dtype({table, rows})) return st;
+    if (table->depth != 1 || rows->depth != 1) return fail(PRAD_ERR_SHAPE, "deep buffer passed to an embedding");
+    if (table->cols != rows->cols) return fail(PRAD_ERR_SHAPE, "the table has %lld columns, the rows %lld", (long long)table->cols, (long long)rows->cols);
+    if (ids->n != rows->rows) return fail(PRAD_ERR_SHAPE, "%lld ids for %lld rows", (long long)ids->n, (long long)rows->rows);
+    if (table->rows > INT32_MAX || rows->rows > INT32_MAX || table->cols > INT32_MAX) return fail(PRAD_ERR_ARG, "an embedding holds at most 2^31 - 1 rows and columns");
+    if (!std::isfinite(scale)) return fail(PRAD_ERR_ARG, "scale must be finite");
+    return PRAD_OK;
+}
+
+int32_t prad_embedding_fwd(prad_buf_t table, prad_index_t ids, double scale, prad_buf_t out) {
+    REQUIRE_INIT();
+    if (int32_t st = embedding_check(table, out, ids, scale)) return st;
+    if (overlap(out, table) || overlap(out, ids)) return fail(PRAD_ERR_ARG, "out must not overlap an input");
+    ENQUEUE_LOCK();
+    if (table->dtype == PRAD_F64)
+        HIP_TRY(launch_embedding_fwd<double>(static_cast<const double*>(table->ptr), ids->ptr, static_cast<double*>(out->ptr), out->rows, table->rows,
+                                             table->cols, scale, CUR_STREAM), PRAD_ERR_LAUNCH);
+    else
+        HIP_TRY(launch_embedding_fwd<float>(F(table), ids->ptr, F(out), out->rows, table->rows, table->cols, (float)scale, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+int32_t prad_embedding_bwd(prad_buf_t dout, prad_index_t ids, double scale, prad_buf_t dtable, int32_t accumulate) {
+    REQUIRE_INIT();
+    if (int32_t st = embedding_check(dtable, dout, ids, scale)) return st;
+    if (overlap(dtable, dout) || overlap(dtable, ids)) return fail(PRAD_ERR_ARG, "dtable must not overlap an input");
+    ENQUEUE_LOCK();
+    if (int32_t st = ensure_workspace(embedding_bwd_workspace_bytes(dout->rows, dout->cols))) return st;
+    const int acc = accumulate != 0 ? 1 : 0;
+    if (dtable->dtype == PRAD_F64)
+        HIP_TRY(launch_embedding_bwd<double>(static_cast<const double*>(dout->ptr), ids->ptr, static_cast<double*>(dtable->ptr), dout->rows, dtable->rows,
+                                             dout->cols, scale, acc, CUR_WORKSPACE, CUR_STREAM), PRAD_ERR_LAUNCH);
+    else
+        HIP_TRY(launch_embedding_bwd<float>(F(dout), ids->ptr, F(dtable), dout->rows, dtable->rows, dout->cols, scale, acc, CUR_WORKSPACE, CUR_STREAM),
+                PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+// y may be exactly x or exactly the residual
+static int32_t dropout_check(prad_buf_t x, prad_buf_t residual, prad_buf_t y, double p, prad_index_t step) {
+    REQUIRE_BUF(x); REQUIRE_BUF(y);
+    if (residual != nullptr) REQUIRE_BUF(residual);
+    if (step != nullptr) REQUIRE_INDEX(step);
+    if (int32_t st = same_dtype({x, residual, y})) return st;
+    if (int32_t st = same_shape(x, y, "dropout")) return st;
+    if (residual != nullptr)
+        if (int32_t st = same_shape(x, residual, "dropout")) return st;
+    if (!(p >= 0.0 && p < 1.0)) return fail(PRAD_ERR_ARG, "the share of dropped elements lies in [0, 1)");
+    if ((x->ptr != y->ptr && overlap(x, y)) || (residual != nullptr && residual->ptr != y->ptr && overlap(residual, y)) ||
+        (step != nullptr && overlap(y, step)))
+        return fail(PRAD_ERR_ARG, "the output must be an input as a whole or not overlap it");
+    return PRAD_OK;
+}
+
+static int32_t dropout_enqueue(prad_buf_t x, prad_buf_t residual, prad_buf_t y, double p, int64_t seed, int32_t site, prad_index_t step) {
+    if (int32_t st = dropout_check(x, residual, y, p, step)) return st;
+    ENQUEUE_LOCK();
+    const int32_t* at = step != nullptr ? step->ptr : nullptr;
+    if (x->dtype == PRAD_F64)
+        HIP_TRY(launch_dropout<double>(static_cast<const double*>(x->ptr), residual != nullptr ? static_cast<const double*>(residual->ptr) : nullptr,
+                                       static_cast<double*>(y->ptr), count(x), p, seed, site, at, CUR_STREAM), PRAD_ERR_LAUNCH);
+    else
+        HIP_TRY(launch_dropout<float>(F(x), residual != nullptr ? F(residual) : nullptr, F(y), count(x), p, seed, site, at, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+int32_t prad_dropout_fwd(prad_buf_t x, prad_buf_t residual, prad_buf_t y, double p, int64_t seed, int32_t site, prad_index_t step) {
+    REQUIRE_INIT();
+    return dropout_enqueue(x, residual, y, p, seed, site, step);
+}
+
+int32_t prad_dropout_bwd(prad_buf_t dy, prad_buf_t dx, double p, int64_t seed, int32_t site, prad_index_t step) {
+    REQUIRE_INIT();
+    return dropout_enqueue(dy, nullptr, dx, p, seed, site, step);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -68,6 +68,13 @@ class DeviceBuffer:
         check(lib.prad_buf_alloc_output(_dtype_code(dtype), depth, rows, cols, ctypes.byref(h)))
         return cls(h, dtype, depth, rows, cols)
 
+    @classmethod
+    def wrap(cls, dtype, rows, cols, ptr, parent=None):
+        """A borrowed rows x cols matrix at a device address; parent keeps the owner of that memory alive."""
+        h = ctypes.c_void_p()
+        check(_lib.load().prad_buf_wrap(_dtype_code(dtype), rows, cols, ctypes.c_void_p(ptr), ctypes.byref(h)))
+        return cls(h, dtype, 1, rows, cols, parent=parent)
+
     def slice(self, d):
         """A borrowed 2-D view of slice d of a deep buffer."""
         lib = _lib.load()
@@ -115,6 +122,67 @@ class DeviceBuffer:
             lib = _lib.load()
             if self.handle is not None and lib.prad_is_initialized():
                 lib.prad_buf_free(self.handle)
+        except Exception:
+            pass
+        self.handle = None
+
+
+class IndexVector:
+    """Owning (or borrowing) wrapper of a prad_index_t handle: int32 values on the device (token ids, sequence offsets, step
+    counters) that a recorded launch sequence reads anew at every launch."""
+
+    def __init__(self, handle, length, parent=None):
+        self.handle = handle
+        self.length = length
+        self._parent = parent  # keeps the owner of borrowed memory alive
+
+    @classmethod
+    def alloc(cls, length):
+        """A zero-filled vector."""
+        h = ctypes.c_void_p()
+        check(_lib.load().prad_index_alloc(length, ctypes.byref(h)))
+        return cls(h, length)
+
+    @classmethod
+    def wrap(cls, ptr, length, parent=None):
+        h = ctypes.c_void_p()
+        check(_lib.load().prad_index_wrap(length, ctypes.c_void_p(ptr), ctypes.byref(h)))
+        return cls(h, length, parent=parent)
+
+    @classmethod
+    def from_values(cls, values):
+        """A vector of its own holding `values`."""
+        values = cls._as_int32(values)
+        v = cls.alloc(values.size)
+        v.upload(values)
+        return v
+
+    @staticmethod
+    def _as_int32(values):
+        given = np.asarray(values).reshape(-1)
+        if given.size == 0:
+            raise ArgumentException("an index vector needs at least one element")
+        if given.dtype.kind not in "iu" or given.min() < -2 ** 31 or given.max() >= 2 ** 31:
+            raise ArgumentException("index values must be whole numbers of 32 bits")
+        return np.ascontiguousarray(given, dtype=np.int32)
+
+    def upload(self, values):
+        values = self._as_int32(values)
+        check(_lib.load().prad_index_upload(self.handle, values.ctypes.data, values.size))
+
+    def download(self):
+        out = np.empty(self.length, dtype=np.int32)
+        check(_lib.load().prad_index_download(self.handle, out.ctypes.data, out.size))
+        return out
+
+    def add(self, delta):
+        check(_lib.load().prad_index_add(self.handle, delta))
+
+    def __del__(self):
+        try:
+            lib = _lib.load()
+            if self.handle is not None and lib.prad_is_initialized():
+                lib.prad_index_free(self.handle)
         except Exception:
             pass
         self.handle = None

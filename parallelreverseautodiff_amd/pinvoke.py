@@ -16,6 +16,8 @@ _TYPES = [
     (r"const prad_buf_t\s*\*", "IntPtr[]"),
     (r"prad_buf_t\s*\*", "out IntPtr"),
     (r"prad_buf_t", "IntPtr"),
+    (r"prad_index_t\s*\*", "out IntPtr"),
+    (r"prad_index_t", "IntPtr"),
     (r"const void\s*\*\s*const\s*\*", "IntPtr[]"),
     (r"void\s*\*\s*const\s*\*", "IntPtr[]"),
     (r"void\s*\*\*", "out IntPtr"),
