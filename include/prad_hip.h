@@ -412,6 +412,40 @@ int32_t prad_embedding_bwd(prad_buf_t dout, prad_index_t ids, double scale, prad
 int32_t prad_dropout_fwd(prad_buf_t x, prad_buf_t residual, prad_buf_t y, double p, int64_t seed, int32_t site, prad_index_t step);
 int32_t prad_dropout_bwd(prad_buf_t dy, prad_buf_t dx, double p, int64_t seed, int32_t site, prad_index_t step);
 
+/* Causal self-attention over sequences packed one after the other, with grouped heads:
+ * S = scale * Q . K^T, query i of a sequence sees its keys 0 .. i, P = softmax rows(S), O = P . V - the nodes of
+ * prad_window_attention_fwd under a causal mask, in one pass that never stores S or P.
+ *   Q, K, V:   a row per token; head h of Q lies in columns [q_col + h*head_dim, +head_dim) and works with head
+ *              h / (heads / kv_heads) of K and V, at k_col and v_col.  The three may be columns of one matrix, as one layer
+ *              writes them ([Q | K | V]: q_col = 0, k_col = heads*head_dim, v_col = (heads + kv_heads)*head_dim).
+ *   offsets:   sequence s is rows [offsets[s], offsets[s+1]); not falling, within the rows (an index vector of sequences + 1
+ *              elements, read on the device; a length of zero is fine).  Rows in front of the first and behind the last
+ *              sequence are neither read for a result nor written.  (Values that break this are cut off to rows of the
+ *              buffers; results are then undefined, memory is not harmed.)
+ *   O:         tokens x heads*head_dim.
+ *   lse:       heads x tokens, receives log sum exp of every row's visible scores, which backward needs; NULL: not kept.
+ * heads is a multiple of kv_heads, head_dim 1 .. 128; float and double.  Sums are held in the element type.
+ * A query that sees a value that is not finite, in Q, K or V, gets rows of NaN; one that does not see it is not affected. */
+int32_t prad_causal_attention_fwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                                  prad_buf_t lse, prad_index_t offsets, int64_t heads, int64_t kv_heads, int64_t head_dim, double scale);
+/* Backward from dO, with the forward call's O and lse: P = exp(S - lse), D = rowsum(dO (.) O), dV = P^T . dO,
+ * dS = P (.) (dO . V^T - D), dQ = scale * dS . K, dK = scale * dS^T . Q, summed over the heads that share a key/value head.
+ * dQ, dK, dV take the columns of their heads at dq_col, dk_col, dv_col (they may be columns of one matrix; other columns are
+ * left alone) in the rows of the sequences.  No gradient goes through an atomic: equal calls give equal bits. */
+int32_t prad_causal_attention_bwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                                  prad_buf_t lse, prad_buf_t dO, prad_buf_t dQ, int64_t dq_col, prad_buf_t dK, int64_t dk_col,
+                                  prad_buf_t dV, int64_t dv_col, prad_index_t offsets, int64_t heads, int64_t kv_heads,
+                                  int64_t head_dim, double scale);
+/* The newest tokens of each sequence against its cache (a step of a generation loop, or a chunk of a prompt): sequence s has
+ * queries [q_offsets[s], q_offsets[s+1]) and keys and values in rows [k_begin[s], k_end[s]) of K and V, its newest token's
+ * included; with n queries and m keys, query i sees keys 0 .. m - n + i (none: a row of zeros).  Key ranges may lie anywhere in
+ * the cache, overlap (a shared beginning) or be empty.  The rest as for prad_causal_attention_fwd; K and V have equally many
+ * rows, whatever Q has.  The keys are split over workgroups when there are few queries, with the workspace holding the
+ * parts. */
+int32_t prad_cached_attention(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                              prad_index_t q_offsets, prad_index_t k_begin, prad_index_t k_end, int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, double scale);
+
 /* ---- GradientClipper.ClipGradients, src/RMAD/GradientClipper.cs:118-157 and :212-253 (in place) */
 int32_t prad_clip(prad_buf_t g, double clip_value, double min_value);
 /* ---- AdamOptimizer.UpdateWeightWithAdam, src/RMAD/AdamOptimizer.cs:195-239 (in place on w, m, v) */

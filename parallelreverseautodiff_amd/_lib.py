@@ -133,6 +133,9 @@ SIGNATURES = {
     "prad_embedding_bwd": (_i32, [_vp, _vp, _f64, _vp, _i32]),
     "prad_dropout_fwd": (_i32, [_vp, _vp, _vp, _f64, _i64, _i32, _vp]),
     "prad_dropout_bwd": (_i32, [_vp, _vp, _f64, _i64, _i32, _vp]),
+    "prad_causal_attention_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _f64]),
+    "prad_causal_attention_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _f64]),
+    "prad_cached_attention": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f64]),
     "prad_clip": (_i32, [_vp, _f64, _f64]),
     "prad_adam": (_i32, [_vp, _vp, _vp, _vp, _f64, _f64, _f64, _f64, _f64]),
     "prad_clip_multi": (_i32, [_vpp, _i32, _f64, _f64]),

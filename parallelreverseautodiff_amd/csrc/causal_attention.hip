@@ -1,0 +1,821 @@
+// Causal attention over packed sequences with grouped heads, in either element type, and its form for the newest tokens of a
+// sequence against its cache.
+//
+//   S = scale Q K^T,  key j seen by query i of n (keys: m) iff j <= m - n + i,  P = softmax rows(S),  O = P V,  lse = log sum exp S
+//   D = rowsum(dO (.) O),  P = exp(S - lse),  dV = P^T dO,  dS = P (.) (dO V^T - D),  dQ = scale dS K,  dK = scale dS^T Q
+//
+// One pass over the keys with the running maximum and sum of a row: scores never reach memory.  The rows of a tile are
+// (token, head of the group) pairs - token r / group, head r % group - so the query heads that share a key/value head share its
+// tiles, and their gradients of K and V add up in one workgroup's registers in one order.
+// Statistics and sums are held in the element type (32 or 64 bits); products run on the 16 x 16 x 4 matrix instructions, whose
+// element order along the reduction is free as long as both operands agree: lane group g takes elements CH c + VEC g + t of
+// chunk c, which makes its reads whole 16-byte vectors.
+//
+// Non-finite values.  A key row that holds one (in K or V) is staged as zeros and its scores become NaN where they are seen: a
+// query that sees it has a row of NaN, a query that does not is not touched by it - a product with a masked weight of zero
+// would carry 0 * NaN into every row of the tile.
+#include "common.h"
+
+#include <algorithm>
+
+namespace prad {
+
+namespace {
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef double d4v __attribute__((ext_vector_type(4)));
+
+template <typename T> struct Num;
+template <> struct Num<float> {
+    typedef f4v Acc;
+    static __device__ __forceinline__ Acc mfma(float a, float b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ int row(int r, int g) { return 4 * g + r; }  // row of accumulator element r in lane group g
+    // scores are kept in units of log2 e: the exponential is the hardware's power of two
+    static __device__ __forceinline__ float unit() { return 1.4426950408889634f; }
+    static __device__ __forceinline__ float exp_unit(float x) { return __builtin_amdgcn_exp2f(x); }
+    static __device__ __forceinline__ float log_sum(float m, float l) { return (m + __log2f(l)) * 0.6931471805599453f; }
+};
+template <> struct Num<double> {
+    typedef d4v Acc;
+    static __device__ __forceinline__ Acc mfma(double a, double b, Acc c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ int row(int r, int g) { return 4 * r + g; }
+    static __device__ __forceinline__ double unit() { return 1.0; }
+    static __device__ __forceinline__ double exp_unit(double x) { return exp(x); }
+    static __device__ __forceinline__ double log_sum(double m, double l) { return m + log(l); }
+};
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+template <typename T> __device__ __forceinline__ bool is_finite(T x) { return fabs(x) < (T)INFINITY; }
+template <typename T> __device__ __forceinline__ T nan_of() { return (T)NAN; }
+
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Reductions over the 16 lanes that share a lane group (a row of an accumulator).
+template <typename T> __device__ __forceinline__ T max16(T v) {
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) v = fmax(v, __shfl_xor(v, m, 64));
+    return v;
+}
+template <typename T> __device__ __forceinline__ T sum16(T v) {
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) v += __shfl_xor(v, m, 64);
+    return v;
+}
+
+// The rows and keys of one sequence.  Values that do not describe rows of the buffers are cut off to some that do.
+struct Span {
+    int64_t q0, nq, k0, nk;
+};
+__device__ __forceinline__ int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const CausalArgs<T>& p, int s) {
+    Span r;
+    r.q0 = clamped(p.q_off[s], p.q_rows);
+    const int64_t q1 = clamped(p.q_off[s + 1], p.q_rows);
+    r.nq = q1 > r.q0 ? q1 - r.q0 : 0;
+    if (p.k_begin == nullptr) {
+        r.k0 = r.q0;
+        r.nk = r.nq;
+    } else {
+        r.k0 = clamped(p.k_begin[s], p.k_rows);
+        const int64_t k1 = clamped(p.k_end[s], p.k_rows);
+        r.nk = k1 > r.k0 ? k1 - r.k0 : 0;
+    }
+    return r;
+}
+
+// Tiles of R packed rows are numbered through all sequences without a table: sequence s begins at number
+// floor(offset G / R) + s, which leaves room for its ceil(n G / R) tiles.  Finds the sequence of a tile and the tile's number
+// inside it; false: no such tile.
+template <int R, typename T>
+__device__ __forceinline__ bool find_tile(const CausalArgs<T>& p, int group, int64_t tile, int* sequence, int64_t* inside) {
+    int lo = 0, hi = p.sequences;  // the last s whose first tile is not behind `tile` lies in [lo - 1, hi)
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (clamped(p.q_off[mid], p.q_rows) * group / R + mid <= tile) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo == 0) return false;
+    *sequence = lo - 1;
+    *inside = tile - (clamped(p.q_off[lo - 1], p.q_rows) * group / R + (lo - 1));
+    return true;
+}
+
+// Elements [d0, d0 + VEC) of a row of head_dim elements, zeros past it.
+template <typename T>
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_pack(const T* __restrict__ row, int d0, int head_dim, bool vec) {
+    constexpr int VEC = 16 / sizeof(T);
+    Pack<T, VEC> v;
+#pragma unroll
+    for (int t = 0; t < VEC; ++t) v.v[t] = (T)0;
+    if (vec) {
+        if (d0 < head_dim) v = *reinterpret_cast<const Pack<T, VEC>*>(row + d0);
+    } else {
+#pragma unroll
+        for (int t = 0; t < VEC; ++t)
+            if (d0 + t < head_dim) v.v[t] = row[d0 + t];
+    }
+    return v;
+}
+
+// A row as the A operand of the matrix instructions: frag[c][t] = element CH c + VEC g + t.
+template <typename T, int HDP>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int g, int head_dim, bool vec, Pack<T, 16 / sizeof(T)> (&frag)[HDP / (64 / sizeof(T))]) {
+    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
+#pragma unroll
+    for (int c = 0; c < HDP / CH; ++c) {
+        if (row != nullptr) {
+            frag[c] = load_pack(row, CH * c + VEC * g, head_dim, vec);
+        } else {
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) frag[c].v[t] = (T)0;
+        }
+    }
+}
+// Makes a row that holds a non-finite value NaN throughout.
+template <typename T, int CHUNKS>
+__device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNKS]) {
+    constexpr int VEC = 16 / sizeof(T);
+    int bad = 0;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int t = 0; t < VEC; ++t) bad |= is_finite(frag[c].v[t]) ? 0 : 1;
+    bad |= __shfl_xor(bad, 16, 64);
+    bad |= __shfl_xor(bad, 32, 64);
+    if (bad) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) frag[c].v[t] = nan_of<T>();
+    }
+}
+
+// Stages two tiles of ROWS rows (of K and V, or of Q and dO) by 256 threads.  row_of(j, which) is the address of row j, nullptr
+// for a row that is not there: zeros.  A row with a non-finite value in either tile is staged as zeros in that tile and marked
+// with `tag`.
+template <typename T, int HDP, int ROWS, int PITCH, typename RowOf>
+__device__ __forceinline__ void stage_two(T* __restrict__ first, T* __restrict__ second, int* __restrict__ bad, int tag, int head_dim, bool vec, RowOf row_of) {
+    constexpr int VEC = 16 / sizeof(T), PER_ROW = HDP / VEC, COUNT = ROWS * PER_ROW / 256;
+    static_assert(ROWS * PER_ROW % 256 == 0, "whole rounds");
+    Pack<T, VEC> v[2][COUNT];
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int u = 0; u < COUNT; ++u) {
+            const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * VEC;
+            const T* __restrict__ row = row_of(j, which);
+            if (row != nullptr) {
+                v[which][u] = load_pack(row, d, head_dim, vec);
+            } else {
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) v[which][u].v[t] = (T)0;
+            }
+        }
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+#pragma unroll
+        for (int u = 0; u < COUNT; ++u) {
+            const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * VEC;
+            bool fine = true;
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) fine = fine && is_finite(v[which][u].v[t]);
+            if (!fine) {
+                bad[j] = tag;
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) v[which][u].v[t] = is_finite(v[which][u].v[t]) ? v[which][u].v[t] : (T)0;
+            }
+            *reinterpret_cast<Pack<T, VEC>*>((which == 0 ? first : second) + j * PITCH + d) = v[which][u];
+        }
+}
+
+// C[16 x 16 y] = A . B^T over the head dimension: A fragments in registers, rows 16 y + li of a staged tile.
+template <typename T, int HDP, int PITCH, int NY>
+__device__ __forceinline__ void rows_product(const Pack<T, 16 / sizeof(T)> (&a)[HDP / (64 / sizeof(T))], const T* __restrict__ tile, int li, int g,
+                                             typename Num<T>::Acc (&acc)[NY]) {
+    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
+#pragma unroll
+    for (int y = 0; y < NY; ++y) acc[y] = typename Num<T>::Acc{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < HDP / CH; ++c) {
+        Pack<T, VEC> b[NY];
+#pragma unroll
+        for (int y = 0; y < NY; ++y) b[y] = *reinterpret_cast<const Pack<T, VEC>*>(tile + (16 * y + li) * PITCH + CH * c + VEC * g);
+#pragma unroll
+        for (int t = 0; t < VEC; ++t)
+#pragma unroll
+            for (int y = 0; y < NY; ++y) acc[y] = Num<T>::mfma(a[c].v[t], b[y].v[t], acc[y]);
+    }
+}
+
+// out[16 x HDP] += W . X: weights of 16 rows over COLS columns in the wavefront's tile w, staged rows of X.
+template <typename T, int HDP, int COLS, int WPITCH, int PITCH>
+__device__ __forceinline__ void weights_product(const T* __restrict__ w, const T* __restrict__ x, int li, int g, typename Num<T>::Acc (&out)[HDP / 16]) {
+    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
+#pragma unroll
+    for (int c = 0; c < COLS / CH; ++c) {
+        const Pack<T, VEC> a = *reinterpret_cast<const Pack<T, VEC>*>(w + li * WPITCH + CH * c + VEC * g);
+#pragma unroll
+        for (int t = 0; t < VEC; ++t)
+#pragma unroll
+            for (int y = 0; y < HDP / 16; ++y) out[y] = Num<T>::mfma(a.v[t], x[(CH * c + VEC * g + t) * PITCH + 16 * y + li], out[y]);
+    }
+}
+
+// Columns of a tile and the pitches of the staged tiles: a 16-byte pad spreads the rows over the LDS banks.
+template <typename T, int HDP> struct Tile {
+    static constexpr int VEC = 16 / sizeof(T);
+    static constexpr int COLS = sizeof(T) * HDP > 512 ? 16 : 32;
+    static constexpr int PITCH = HDP + VEC, WPITCH = COLS + VEC, NY = COLS / 16;
+};
+
+// Running softmax statistics of the four rows a lane holds, over one tile of scores.  On return s holds the weights and the
+// factors of the old sums.
+template <typename T, int NY>
+__device__ __forceinline__ void softmax_tile(typename Num<T>::Acc (&s)[NY], T (&m)[4], T (&l)[4], T (&factor)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        T top = s[0][r];
+#pragma unroll
+        for (int y = 1; y < NY; ++y) top = fmax(top, s[y][r]);
+        top = fmax(m[r], max16(top));
+        const T ref = top == -(T)INFINITY ? (T)0 : top;  // nothing seen yet: every weight below is exp(-inf) = 0
+        factor[r] = Num<T>::exp_unit(m[r] - ref);
+        T sum = 0;
+#pragma unroll
+        for (int y = 0; y < NY; ++y) {
+            s[y][r] = Num<T>::exp_unit(s[y][r] - ref);
+            sum += s[y][r];
+        }
+        l[r] = l[r] * factor[r] + sum16(sum);
+        m[r] = top;
+    }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------
+// A workgroup takes 64 packed rows of a key/value head, a wavefront 16 of them; K and V pass through LDS in tiles of COLS keys.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(256) causal_fwd_kernel(const CausalArgs<T> p) {
+    typedef Tile<T, HDP> TL;
+    typedef typename Num<T>::Acc Acc;
+    constexpr int CHUNKS = HDP / (4 * TL::VEC);
+    __shared__ __attribute__((aligned(16))) T ks[TL::COLS * TL::PITCH], vs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
+    __shared__ int bad[TL::COLS];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kv = blockIdx.y;
+    int s;
+    int64_t inside;
+    if (!find_tile<64>(p, p.group, (int64_t)gridDim.x - 1 - blockIdx.x, &s, &inside)) return;  // (late tiles see the most keys: first)
+    const Span sp = span_of(p, s);
+    const int64_t rows = sp.nq * p.group, row0 = inside * 64;
+    if (row0 >= rows) return;
+    if (threadIdx.x < TL::COLS) bad[threadIdx.x] = -1;
+    const int64_t lead = sp.nk - sp.nq;  // query i sees keys up to lead + i
+    Pack<T, TL::VEC> q[CHUNKS];
+    {
+        const int64_t r = row0 + 16 * wave + li;
+        const T* row = r < rows ? p.Q + (sp.q0 + r / p.group) * p.ldq + (kv * p.group + r % p.group) * (int64_t)p.head_dim : nullptr;
+        load_row<T, HDP>(row, g, p.head_dim, p.vec_q, q);
+        poison_row<T, CHUNKS>(q);
+    }
+    int64_t last[4];  // the last key that each of the lane's rows sees
+#pragma unroll
+    for (int r = 0; r < 4; ++r) last[r] = lead + (row0 + 16 * wave + Num<T>::row(r, g)) / p.group;
+    T m[4], l[4];
+    Acc o[HDP / 16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { m[r] = -(T)INFINITY; l[r] = 0; }
+#pragma unroll
+    for (int y = 0; y < HDP / 16; ++y) o[y] = Acc{0, 0, 0, 0};
+    const int64_t last_row = row0 + 63 < rows ? row0 + 63 : rows - 1;
+    const int64_t seen = clamped(lead + last_row / p.group + 1, sp.nk);
+    const T factor = p.scale * Num<T>::unit();
+    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
+    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
+    for (int64_t k0 = 0; k0 < seen; k0 += TL::COLS) {
+        const int tag = (int)(k0 / TL::COLS);
+        __syncthreads();
+        stage_two<T, HDP, TL::COLS, TL::PITCH>(ks, vs, bad, tag, p.head_dim, p.vec_kv, [&](int j, int which) -> const T* {
+            if (k0 + j >= sp.nk) return nullptr;
+            return which == 0 ? K + (k0 + j) * p.ldk : V + (k0 + j) * p.ldv;
+        });
+        __syncthreads();
+        Acc acc[TL::NY];
+        rows_product<T, HDP, TL::PITCH, TL::NY>(q, ks, li, g, acc);
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y) {
+            const int64_t j = k0 + 16 * y + li;
+            const bool poisoned = bad[16 * y + li] == tag;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[y][r] = j > last[r] ? -(T)INFINITY : poisoned ? nan_of<T>() : acc[y][r] * factor;
+        }
+        T fac[4];
+        softmax_tile<T, TL::NY>(acc, m, l, fac);
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[y][r] *= fac[r];
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ws[wave][Num<T>::row(r, g) * TL::WPITCH + 16 * y + li] = acc[y][r];
+        wave_sync();
+        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], vs, li, g, o);
+        wave_sync();
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
+        if (row >= rows) continue;
+        const int64_t token = sp.q0 + row / p.group;
+        const int head = kv * p.group + (int)(row % p.group);
+        const bool any = last[r] >= 0;
+        const T inv = any ? (T)1 / l[r] : (T)0;
+        T* dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y)
+            if (16 * y + li < p.head_dim) dst[16 * y + li] = any ? o[y][r] * inv : (T)0;
+        if (p.lse != nullptr && li == 0) p.lse[head * p.q_rows + token] = any ? Num<T>::log_sum(m[r], l[r]) : -(T)INFINITY;
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------------
+// D = rowsum(dO (.) O) per token and head, 16 lanes to a row; NaN for a row of dO with a non-finite value.
+template <typename T>
+__global__ void __launch_bounds__(256) causal_dot_kernel(const CausalArgs<T> p) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int lane = threadIdx.x & 15;
+    if (at >= p.q_rows * p.heads) return;
+    const int64_t token = at / p.heads;
+    const int head = (int)(at % p.heads);
+    const T* __restrict__ o = p.O + token * p.ldo + head * (int64_t)p.head_dim;
+    const T* __restrict__ g = p.dO + token * p.ldo + head * (int64_t)p.head_dim;
+    T sum = 0, check = 0;
+    for (int d = lane; d < p.head_dim; d += 16) {
+        sum += o[d] * g[d];
+        check += is_finite(g[d]) ? (T)0 : nan_of<T>();
+    }
+    sum = sum16(sum + check);
+    if (lane == 0) p.D[head * p.q_rows + token] = is_finite(sum) ? sum : nan_of<T>();
+}
+
+// Gradients of K and V: a workgroup owns 64 keys of a key/value head (a wavefront 16, its rows of K and V in registers) and
+// walks the packed query rows that see them, all heads of the group among them, in tiles of COLS.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(256) causal_bwd_kv_kernel(const CausalArgs<T> p) {
+    typedef Tile<T, HDP> TL;
+    typedef typename Num<T>::Acc Acc;
+    constexpr int CHUNKS = HDP / (4 * TL::VEC);
+    __shared__ __attribute__((aligned(16))) T qs[TL::COLS * TL::PITCH], gs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
+    __shared__ T row_lse[TL::COLS], row_dot[TL::COLS];
+    __shared__ int bad[TL::COLS];  // written by the staging; rows with a non-finite value already have a NaN in lse or D
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kv = blockIdx.y;
+    int s;
+    int64_t inside;
+    if (!find_tile<64>(p, 1, blockIdx.x, &s, &inside)) return;  // (tiles of keys are numbered like packed rows of one head)
+    const Span sp = span_of(p, s);
+    const int64_t key0 = inside * 64, rows = sp.nq * p.group;
+    if (key0 >= sp.nk) return;
+    const int64_t key = key0 + 16 * wave + li;
+    Pack<T, TL::VEC> k[CHUNKS], v[CHUNKS];
+    load_row<T, HDP>(key < sp.nk ? p.K + (sp.k0 + key) * p.ldk + kv * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_kv, k);
+    load_row<T, HDP>(key < sp.nk ? p.V + (sp.k0 + key) * p.ldv + kv * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_kv, v);
+    Acc dk[HDP / 16], dv[HDP / 16];
+#pragma unroll
+    for (int y = 0; y < HDP / 16; ++y) dk[y] = dv[y] = Acc{0, 0, 0, 0};
+    const T factor = p.scale * Num<T>::unit();
+    // (queries and keys are the same rows here: token i sees key j iff j <= i)
+    for (int64_t r0 = key0 * p.group / TL::COLS * TL::COLS; r0 < rows; r0 += TL::COLS) {
+        __syncthreads();
+        if (threadIdx.x < TL::COLS) {
+            const int64_t r = r0 + threadIdx.x;
+            T lse = 0, dot = 0;
+            if (r < rows) {
+                const int64_t at = (kv * p.group + r % p.group) * p.q_rows + sp.q0 + r / p.group;
+                dot = p.D[at];
+                lse = p.lse[at] * Num<T>::unit() + (dot - dot);  // NaN where D is
+            }
+            row_lse[threadIdx.x] = lse;
+            row_dot[threadIdx.x] = dot;
+        }
+        stage_two<T, HDP, TL::COLS, TL::PITCH>(qs, gs, bad, 0, p.head_dim, p.vec_q && p.vec_o, [&](int j, int which) -> const T* {
+            const int64_t r = r0 + j;
+            if (r >= rows) return nullptr;
+            const int64_t token = sp.q0 + r / p.group, col = (kv * p.group + r % p.group) * (int64_t)p.head_dim;
+            return which == 0 ? p.Q + token * p.ldq + col : p.dO + token * p.ldo + col;
+        });
+        __syncthreads();
+        Acc st[TL::NY], dp[TL::NY];
+        rows_product<T, HDP, TL::PITCH, TL::NY>(k, qs, li, g, st);   // S^T: rows are keys, columns query rows
+        rows_product<T, HDP, TL::PITCH, TL::NY>(v, gs, li, g, dp);   // (dO V^T)^T
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y) {
+            const int64_t r = r0 + 16 * y + li, token = r / p.group;
+            const T lse = row_lse[16 * y + li], dot = row_dot[16 * y + li];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool seen = r < rows && key0 + 16 * wave + Num<T>::row(e, g) <= token;
+                const T w = seen ? Num<T>::exp_unit(st[y][e] * factor - lse) : (T)0;
+                st[y][e] = w;
+                dp[y][e] = seen ? w * (dp[y][e] - dot) : (T)0;
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ws[wave][Num<T>::row(e, g) * TL::WPITCH + 16 * y + li] = st[y][e];
+        wave_sync();
+        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], gs, li, g, dv);
+        wave_sync();
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ws[wave][Num<T>::row(e, g) * TL::WPITCH + 16 * y + li] = dp[y][e];
+        wave_sync();
+        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], qs, li, g, dk);
+        wave_sync();
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t j = key0 + 16 * wave + Num<T>::row(e, g);
+        if (j >= sp.nk) continue;
+        T* dst_k = p.dK + (sp.k0 + j) * p.lddk + kv * (int64_t)p.head_dim;
+        T* dst_v = p.dV + (sp.k0 + j) * p.lddv + kv * (int64_t)p.head_dim;
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y)
+            if (16 * y + li < p.head_dim) {
+                dst_k[16 * y + li] = dk[y][e] * p.scale;
+                dst_v[16 * y + li] = dv[y][e];
+            }
+    }
+}
+
+// Gradient of Q: tiles as in the forward kernel, the rows of Q and dO in registers.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(256) causal_bwd_q_kernel(const CausalArgs<T> p) {
+    typedef Tile<T, HDP> TL;
+    typedef typename Num<T>::Acc Acc;
+    constexpr int CHUNKS = HDP / (4 * TL::VEC);
+    __shared__ __attribute__((aligned(16))) T ks[TL::COLS * TL::PITCH], vs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
+    __shared__ int bad[TL::COLS];  // written by the staging; rows that see such a key already have a NaN in lse
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kv = blockIdx.y;
+    int s;
+    int64_t inside;
+    if (!find_tile<64>(p, p.group, (int64_t)gridDim.x - 1 - blockIdx.x, &s, &inside)) return;
+    const Span sp = span_of(p, s);
+    const int64_t rows = sp.nq * p.group, row0 = inside * 64;
+    if (row0 >= rows) return;
+    Pack<T, TL::VEC> q[CHUNKS], go[CHUNKS];
+    {
+        const int64_t r = row0 + 16 * wave + li;
+        const int64_t token = sp.q0 + r / p.group, col = (kv * p.group + r % p.group) * (int64_t)p.head_dim;
+        load_row<T, HDP>(r < rows ? p.Q + token * p.ldq + col : nullptr, g, p.head_dim, p.vec_q, q);
+        load_row<T, HDP>(r < rows ? p.dO + token * p.ldo + col : nullptr, g, p.head_dim, p.vec_o, go);
+    }
+    int64_t last[4];
+    T lse[4], dot[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
+        last[r] = row < rows ? row / p.group : -1;
+        lse[r] = dot[r] = 0;
+        if (row < rows) {
+            const int64_t at = (kv * p.group + row % p.group) * p.q_rows + sp.q0 + row / p.group;
+            dot[r] = p.D[at];
+            lse[r] = p.lse[at] * Num<T>::unit() + (dot[r] - dot[r]);
+        }
+    }
+    Acc dq[HDP / 16];
+#pragma unroll
+    for (int y = 0; y < HDP / 16; ++y) dq[y] = Acc{0, 0, 0, 0};
+    const int64_t last_row = row0 + 63 < rows ? row0 + 63 : rows - 1;
+    const int64_t seen = last_row / p.group + 1;
+    const T factor = p.scale * Num<T>::unit();
+    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
+    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
+    for (int64_t k0 = 0; k0 < seen; k0 += TL::COLS) {
+        __syncthreads();
+        stage_two<T, HDP, TL::COLS, TL::PITCH>(ks, vs, bad, 0, p.head_dim, p.vec_kv, [&](int j, int which) -> const T* {
+            if (k0 + j >= sp.nk) return nullptr;
+            return which == 0 ? K + (k0 + j) * p.ldk : V + (k0 + j) * p.ldv;
+        });
+        __syncthreads();
+        Acc st[TL::NY], dp[TL::NY];
+        rows_product<T, HDP, TL::PITCH, TL::NY>(q, ks, li, g, st);
+        rows_product<T, HDP, TL::PITCH, TL::NY>(go, vs, li, g, dp);
+#pragma unroll
+        for (int y = 0; y < TL::NY; ++y) {
+            const int64_t j = k0 + 16 * y + li;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const T w = Num<T>::exp_unit(st[y][r] * factor - lse[r]);
+                ws[wave][Num<T>::row(r, g) * TL::WPITCH + 16 * y + li] = j <= last[r] ? w * (dp[y][r] - dot[r]) : (T)0;
+            }
+        }
+        wave_sync();
+        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], ks, li, g, dq);
+        wave_sync();
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
+        if (row >= rows) continue;
+        T* dst = p.dQ + (sp.q0 + row / p.group) * p.lddq + (kv * p.group + row % p.group) * (int64_t)p.head_dim;
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y)
+            if (16 * y + li < p.head_dim) dst[16 * y + li] = dq[y][r] * p.scale;
+    }
+}
+
+// ---- the newest tokens against the cache ----------------------------------------------------------------------------------
+// A step of a generation loop reads every key and value once and does little with it: it is bound by memory.  A workgroup takes
+// 16 packed rows (a single token of up to 16 heads that share a key/value head) and one of `splits` parts of the keys; its four
+// wavefronts take every fourth tile of 16 keys, straight from memory into the operand registers.  Their sums meet in LDS;
+// with more than one part, (maximum, sum, weighted values) go to the workspace and a second launch joins them.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(256) cached_attention_kernel(const CausalArgs<T> p, int splits, T* __restrict__ part) {
+    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC, CHUNKS = HDP / CH, WPITCH = 16 + VEC;
+    typedef typename Num<T>::Acc Acc;
+    __shared__ __attribute__((aligned(16))) T ws[4][16 * WPITCH];
+    __shared__ T stat[4][2][16];
+    __shared__ T sums[16 * (HDP + 1)];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kv = blockIdx.y, split = blockIdx.z;
+    int s;
+    int64_t inside;
+    if (!find_tile<16>(p, p.group, blockIdx.x, &s, &inside)) return;
+    const Span sp = span_of(p, s);
+    const int64_t rows = sp.nq * p.group, row0 = inside * 16;
+    if (row0 >= rows) return;
+    const int64_t lead = sp.nk - sp.nq;
+    Pack<T, VEC> q[CHUNKS];
+    {
+        const int64_t r = row0 + li;
+        const T* row = r < rows ? p.Q + (sp.q0 + r / p.group) * p.ldq + (kv * p.group + r % p.group) * (int64_t)p.head_dim : nullptr;
+        load_row<T, HDP>(row, g, p.head_dim, p.vec_q, q);
+        poison_row<T, CHUNKS>(q);
+    }
+    int64_t last[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) last[r] = lead + (row0 + Num<T>::row(r, g)) / p.group;
+    T m[4], l[4];
+    Acc o[HDP / 16];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) { m[r] = -(T)INFINITY; l[r] = 0; }
+#pragma unroll
+    for (int y = 0; y < HDP / 16; ++y) o[y] = Acc{0, 0, 0, 0};
+    const int64_t last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
+    const int64_t tiles = (clamped(lead + last_row / p.group + 1, sp.nk) + 15) / 16;
+    const int64_t per = (tiles + splits - 1) / splits;
+    const int64_t from = split * per, to = from + per < tiles ? from + per : tiles;
+    const T factor = p.scale * Num<T>::unit();
+    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
+    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
+    for (int64_t tile = from + wave; tile < to; tile += 4) {
+        const int64_t k0 = tile * 16;
+        // keys past the last are the last one again: their scores are masked
+        const int64_t key = k0 + li < sp.nk ? k0 + li : sp.nk - 1;
+        Pack<T, VEC> k[CHUNKS];
+        load_row<T, HDP>(K + key * p.ldk, g, p.head_dim, p.vec_kv, k);
+        T v[16 / 4][HDP / 16];  // value rows CH c + VEC g + t, columns 16 y + li
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int64_t j = k0 + CH * (x / VEC) + VEC * g + x % VEC;
+            const T* __restrict__ row = V + (j < sp.nk ? j : sp.nk - 1) * p.ldv;
+#pragma unroll
+            for (int y = 0; y < HDP / 16; ++y) v[x][y] = 16 * y + li < p.head_dim ? row[16 * y + li] : (T)0;
+        }
+        Acc acc[1] = {Acc{0, 0, 0, 0}};
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) acc[0] = Num<T>::mfma(q[c].v[t], k[c].v[t], acc[0]);
+        // a key row with a non-finite value: NaN for the rows that see it, zeros elsewhere
+        uint32_t poisoned = 0;  // bit j: key k0 + j
+        {
+            bool fine = true;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) fine = fine && is_finite(k[c].v[t]);
+            uint64_t b = __ballot(!fine);
+            poisoned = (uint32_t)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xFFFFu);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                fine = true;
+#pragma unroll
+                for (int y = 0; y < HDP / 16; ++y) {
+                    fine = fine && is_finite(v[x][y]);
+                }
+                b = __ballot(!fine);
+                if (b != 0) {
+#pragma unroll
+                    for (int y = 0; y < HDP / 16; ++y) v[x][y] = is_finite(v[x][y]) ? v[x][y] : (T)0;
+#pragma unroll
+                    for (int gg = 0; gg < 4; ++gg)
+                        if ((b >> (16 * gg)) & 0xFFFFu) poisoned |= 1u << (CH * (x / VEC) + VEC * gg + x % VEC);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            acc[0][r] = k0 + li > last[r] ? -(T)INFINITY : (poisoned >> li) & 1 ? nan_of<T>() : acc[0][r] * factor;
+        T fac[4];
+        softmax_tile<T, 1>(acc, m, l, fac);
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[y][r] *= fac[r];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[wave][Num<T>::row(r, g) * WPITCH + li] = acc[0][r];
+        wave_sync();
+#pragma unroll
+        for (int c = 0; c < 16 / CH; ++c) {
+            const Pack<T, VEC> a = *reinterpret_cast<const Pack<T, VEC>*>(&ws[wave][li * WPITCH + CH * c + VEC * g]);
+#pragma unroll
+            for (int t = 0; t < VEC; ++t)
+#pragma unroll
+                for (int y = 0; y < HDP / 16; ++y) o[y] = Num<T>::mfma(a.v[t], v[c * VEC + t][y], o[y]);
+        }
+        wave_sync();
+    }
+    // the four wavefronts' sums, added in their order
+    if (li == 0) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            stat[wave][0][Num<T>::row(r, g)] = m[r];
+            stat[wave][1][Num<T>::row(r, g)] = l[r];
+        }
+    }
+    __syncthreads();
+    T top[4], total[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = Num<T>::row(r, g);
+        top[r] = fmax(fmax(stat[0][0][row], stat[1][0][row]), fmax(stat[2][0][row], stat[3][0][row]));
+        const T ref = top[r] == -(T)INFINITY ? (T)0 : top[r];
+        total[r] = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) total[r] += stat[w][1][row] * Num<T>::exp_unit(stat[w][0][row] - ref);
+        const T mine = Num<T>::exp_unit(m[r] - ref);
+#pragma unroll
+        for (int y = 0; y < HDP / 16; ++y) o[y][r] *= mine;
+    }
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int y = 0; y < HDP / 16; ++y) {
+                    T* at = &sums[Num<T>::row(r, g) * (HDP + 1) + 16 * y + li];
+                    *at = w == 0 ? o[y][r] : *at + o[y][r];
+                }
+        }
+        __syncthreads();
+    }
+    // wavefront w finishes rows w, w + 4, ...
+    for (int row = wave; row < 16; row += 4) {
+        const int64_t r = row0 + row;
+        if (r >= rows) break;
+        T mm = fmax(fmax(stat[0][0][row], stat[1][0][row]), fmax(stat[2][0][row], stat[3][0][row]));
+        const T ref = mm == -(T)INFINITY ? (T)0 : mm;
+        T ll = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ll += stat[w][1][row] * Num<T>::exp_unit(stat[w][0][row] - ref);
+        const int64_t token = sp.q0 + r / p.group;
+        const int head = kv * p.group + (int)(r % p.group);
+        if (splits == 1) {
+            const bool any = lead + r / p.group >= 0 && sp.nk > 0;
+            T* dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
+            for (int d = lane; d < p.head_dim; d += 64) dst[d] = any ? sums[row * (HDP + 1) + d] / ll : (T)0;
+        } else {
+            T* dst = part + ((token * p.heads + head) * splits + split) * (int64_t)(p.head_dim + 2);
+            for (int d = lane; d < p.head_dim; d += 64) dst[2 + d] = sums[row * (HDP + 1) + d];
+            if (lane == 0) { dst[0] = mm; dst[1] = ll; }
+        }
+    }
+}
+
+// Joins the parts of a row: a wavefront per (token, head).
+template <typename T>
+__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, int splits, const T* __restrict__ part) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (at >= p.q_rows * p.heads) return;
+    const int64_t token = at / p.heads;
+    const int head = (int)(at % p.heads);
+    // the sequence of the token: rows in front of the first and behind the last are left as they are
+    int lo = 0, hi = p.sequences + 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (clamped(p.q_off[mid], p.q_rows) <= token) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo == 0 || lo > p.sequences) return;
+    const Span sp = span_of(p, lo - 1);
+    if (token < sp.q0 || token >= sp.q0 + sp.nq) return;
+    const bool any = sp.nk - sp.nq + (token - sp.q0) >= 0 && sp.nk > 0;
+    const int stride = p.head_dim + 2;
+    const T* __restrict__ mine = part + at * splits * (int64_t)stride;
+    T top = -(T)INFINITY;
+    for (int i = 0; i < splits; ++i) top = fmax(top, mine[i * stride]);
+    const T ref = top == -(T)INFINITY ? (T)0 : top;
+    for (int d = lane; d < p.head_dim; d += 64) {
+        T sum = 0, total = 0;
+        for (int i = 0; i < splits; ++i) {
+            const T f = Num<T>::exp_unit(mine[i * stride] - ref);
+            total += mine[i * stride + 1] * f;
+            sum += mine[i * stride + 2 + d] * f;
+        }
+        p.O[token * p.ldo + head * (int64_t)p.head_dim + d] = any ? sum / total : (T)0;
+    }
+}
+
+inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
+inline int64_t tile_slots(int64_t rows, int64_t group, int64_t per_tile, int64_t sequences) { return rows * group / per_tile + sequences; }
+
+}  // namespace
+
+// A launch of KERNEL<T, HDP> for the smallest padded head dimension that holds head_dim.
+#define BY_HEAD_DIM(KERNEL, GRID, ...)                                                                                  \
+    do {                                                                                                                \
+        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32>), GRID, dim3(256), 0, s, __VA_ARGS__);                  \
+        else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(256), 0, s, __VA_ARGS__);             \
+        else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(256), 0, s, __VA_ARGS__);                                  \
+        if (hipError_t e = hipGetLastError()) return e;                                                                 \
+    } while (0)
+
+template <typename T>
+hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s) {
+    const int64_t slots = tile_slots(a.q_rows, a.group, 64, a.sequences);
+    if (!grid_fits(slots, 256)) return hipErrorInvalidValue;
+    BY_HEAD_DIM(causal_fwd_kernel, dim3((unsigned)slots, a.kv_heads), a);
+    return hipSuccess;
+}
+
+template <typename T>
+size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a) {
+    return (size_t)a.heads * a.q_rows * sizeof(T);
+}
+
+template <typename T>
+hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
+    a.D = static_cast<T*>(workspace);
+    const int64_t dots = (a.q_rows * a.heads + 15) / 16, key_slots = tile_slots(a.q_rows, 1, 64, a.sequences), slots = tile_slots(a.q_rows, a.group, 64, a.sequences);
+    if (!grid_fits(dots, 256) || !grid_fits(slots, 256)) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(causal_dot_kernel<T>, dim3((unsigned)dots), dim3(256), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    BY_HEAD_DIM(causal_bwd_kv_kernel, dim3((unsigned)key_slots, a.kv_heads), a);
+    BY_HEAD_DIM(causal_bwd_q_kernel, dim3((unsigned)slots, a.kv_heads), a);
+    return hipSuccess;
+}
+
+// Parts of the keys for a cached call: enough workgroups to fill the chip, none with less than a tile per wavefront of a cache
+// that fills the whole of K.
+static int cached_splits(int64_t q_rows, int64_t k_rows, int sequences, int kv_heads, int group) {
+    const int64_t groups = tile_slots(q_rows, group, 16, sequences) * kv_heads;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + groups - 1) / groups, (k_rows + 63) / 64, 32}));
+}
+
+template <typename T>
+size_t cached_workspace_bytes(const CausalArgs<T>& a) {
+    const int splits = cached_splits(a.q_rows, a.k_rows, a.sequences, a.kv_heads, a.group);
+    return splits == 1 ? 0 : (size_t)a.q_rows * a.heads * splits * (a.head_dim + 2) * sizeof(T);
+}
+
+template <typename T>
+hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s) {
+    const int splits = cached_splits(a.q_rows, a.k_rows, a.sequences, a.kv_heads, a.group);
+    const int64_t slots = tile_slots(a.q_rows, a.group, 16, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
+    if (!grid_fits(slots, 256) || !grid_fits(rows, 256)) return hipErrorInvalidValue;
+    T* part = static_cast<T*>(workspace);
+    BY_HEAD_DIM(cached_attention_kernel, dim3((unsigned)slots, a.kv_heads, splits), a, splits, part);
+    if (splits > 1) {
+        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, splits, part);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
+
+#define INSTANTIATE(T)                                                              \
+    template hipError_t launch_causal_fwd<T>(const CausalArgs<T>&, hipStream_t);    \
+    template size_t causal_bwd_workspace_bytes<T>(const CausalArgs<T>&);            \
+    template hipError_t launch_causal_bwd<T>(CausalArgs<T>, void*, hipStream_t);    \
+    template size_t cached_workspace_bytes<T>(const CausalArgs<T>&);                \
+    template hipError_t launch_cached_attention<T>(const CausalArgs<T>&, void*, hipStream_t);
+INSTANTIATE(float)
+INSTANTIATE(double)
+#undef INSTANTIATE
+
+}  // namespace prad

@@ -443,6 +443,31 @@ template <typename T> hipError_t launch_dropout(const T* x, const T* residual, T
                                                 const int32_t* step, hipStream_t s);
 hipError_t launch_index_add(int32_t* v, int64_t n, int32_t delta, hipStream_t s);
 
+// Causal attention over packed sequences (csrc/causal_attention.hip).  Column offsets of Q, K, V and their gradients are part of
+// the pointers; rows are ld* elements apart and a head's columns head_dim apart.  group = heads / kv_heads.
+template <typename T>
+struct CausalArgs {
+    const T* Q; const T* K; const T* V;
+    int64_t ldq, ldk, ldv;
+    T* O; int64_t ldo;
+    T* lse;                        // heads x q_rows, may be nullptr forward
+    const int32_t* q_off;          // sequences + 1 row numbers
+    const int32_t* k_begin; const int32_t* k_end;  // rows of K and V per sequence; nullptr: those of Q
+    int sequences, heads, kv_heads, group, head_dim;
+    int64_t q_rows, k_rows;
+    T scale;
+    bool vec_q, vec_kv, vec_o;     // rows and heads start on multiples of 16 bytes
+    const T* dO;                   // rows ldo apart
+    T* D;                          // heads x q_rows of workspace
+    T* dQ; T* dK; T* dV;
+    int64_t lddq, lddk, lddv;
+};
+template <typename T> hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s);
+template <typename T> size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a);
+template <typename T> hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s);
+template <typename T> size_t cached_workspace_bytes(const CausalArgs<T>& a);
+template <typename T> hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s);
+
 // MatrixMultiplyAndSum
 // S = samples of a batch (each with its own A, out, dOut, dA and P slices of dB; the P slices of B are shared).
 template <typename T> hipError_t launch_matmul_sum_fwd(const T* A, const T* B, T* out, double* workspace, int64_t M, int64_t K,

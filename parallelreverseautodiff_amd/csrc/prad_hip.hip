@@ -1976,6 +1976,170 @@ int32_t prad_dropout_bwd(prad_buf_t dy, prad_buf_t dx, double p, int64_t seed, i
     return dropout_enqueue(dy, nullptr, dx, p, seed, site, step);
 }
 
+// ---- causal attention -----------------------------------------------------------------------------
+// The head columns [col, col + heads * head_dim) of a matrix.
+struct HeadColumns {
+    prad_buf_t buf;
+    int64_t col, width;
+    const char* name;
+};
+static bool columns_meet(const HeadColumns& a, const HeadColumns& b) {
+    if (a.buf->ptr == b.buf->ptr && a.buf->cols == b.buf->cols && a.buf->dtype == b.buf->dtype) return a.col < b.col + b.width && b.col < a.col + a.width;
+    return overlap(a.buf, b.buf);
+}
+static int32_t columns_check(const HeadColumns& c, int64_t rows) {
+    if (c.buf->depth != 1 || c.buf->rows != rows) return fail(PRAD_ERR_SHAPE, "%s must have %lld rows", c.name, (long long)rows);
+    if (c.col < 0 || c.width > c.buf->cols || c.col > c.buf->cols - c.width)
+        return fail(PRAD_ERR_SHAPE, "%s: columns [%lld, %lld) lie outside its %lld", c.name, (long long)c.col, (long long)(c.col + c.width), (long long)c.buf->cols);
+    return PRAD_OK;
+}
+static int32_t heads_check(int64_t heads, int64_t kv_heads, int64_t head_dim, double scale) {
+    if (heads < 1 || kv_heads < 1 || heads > 65535 || kv_heads > heads || heads % kv_heads != 0)
+        return fail(PRAD_ERR_ARG, "the heads must be a multiple of the key/value heads, 1 to 65535 of them");
+    if (head_dim < 1 || head_dim > 128) return fail(PRAD_ERR_ARG, "the head dimension must be 1 to 128");
+    if (!std::isfinite(scale)) return fail(PRAD_ERR_ARG, "scale must be finite");
+    return PRAD_OK;
+}
+extern "C++" {
+template <typename T>
+static bool packs_of_16(std::initializer_list<HeadColumns> list, int64_t head_dim) {
+    for (const HeadColumns& c : list)
+        if (reinterpret_cast<uintptr_t>(c.buf->ptr) % 16 != 0 || c.buf->cols * sizeof(T) % 16 != 0 || c.col * sizeof(T) % 16 != 0) return false;
+    return head_dim * sizeof(T) % 16 == 0;
+}
+template <typename T>
+static const T* at_column(const HeadColumns& c) { return static_cast<const T*>(c.buf->ptr) + c.col; }
+template <typename T>
+static T* out_column(const HeadColumns& c) { return static_cast<T*>(c.buf->ptr) + c.col; }
+
+template <typename T>
+static CausalArgs<T> causal_args(const HeadColumns& Q, const HeadColumns& K, const HeadColumns& V, prad_buf_t O, int64_t heads, int64_t kv_heads,
+                                 int64_t head_dim, double scale) {
+    CausalArgs<T> a{};
+    a.Q = at_column<T>(Q); a.K = at_column<T>(K); a.V = at_column<T>(V);
+    a.ldq = Q.buf->cols; a.ldk = K.buf->cols; a.ldv = V.buf->cols;
+    a.O = static_cast<T*>(O->ptr); a.ldo = O->cols;
+    a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.group = (int)(heads / kv_heads); a.head_dim = (int)head_dim;
+    a.q_rows = Q.buf->rows; a.k_rows = K.buf->rows;
+    a.scale = (T)scale;
+    a.vec_q = packs_of_16<T>({Q}, head_dim);
+    a.vec_kv = packs_of_16<T>({K, V}, head_dim);
+    a.vec_o = packs_of_16<T>({{O, 0, O->cols, "O"}}, head_dim);
+    return a;
+}
+
+template <typename T>
+static int32_t causal_fwd_t(CausalArgs<T> a, prad_buf_t lse, prad_index_t offsets) {
+    a.lse = lse != nullptr ? static_cast<T*>(lse->ptr) : nullptr;
+    a.q_off = offsets->ptr; a.sequences = (int)(offsets->n - 1);
+    HIP_TRY(launch_causal_fwd<T>(a, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+template <typename T>
+static int32_t causal_bwd_t(CausalArgs<T> a, prad_buf_t lse, prad_buf_t dO, const HeadColumns& dQ, const HeadColumns& dK, const HeadColumns& dV,
+                            prad_index_t offsets) {
+    a.lse = static_cast<T*>(lse->ptr);
+    a.q_off = offsets->ptr; a.sequences = (int)(offsets->n - 1);
+    a.dO = static_cast<const T*>(dO->ptr);
+    a.vec_o = a.vec_o && reinterpret_cast<uintptr_t>(dO->ptr) % 16 == 0;
+    a.dQ = out_column<T>(dQ); a.dK = out_column<T>(dK); a.dV = out_column<T>(dV);
+    a.lddq = dQ.buf->cols; a.lddk = dK.buf->cols; a.lddv = dV.buf->cols;
+    if (int32_t st = ensure_workspace(causal_bwd_workspace_bytes<T>(a))) return st;
+    HIP_TRY(launch_causal_bwd<T>(a, CUR_WORKSPACE, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+
+template <typename T>
+static int32_t cached_t(CausalArgs<T> a, prad_index_t q_offsets, prad_index_t k_begin, prad_index_t k_end) {
+    a.q_off = q_offsets->ptr; a.sequences = (int)(q_offsets->n - 1);
+    a.k_begin = k_begin->ptr; a.k_end = k_end->ptr;
+    if (int32_t st = ensure_workspace(cached_workspace_bytes<T>(a))) return st;
+    HIP_TRY(launch_cached_attention<T>(a, CUR_WORKSPACE, CUR_STREAM), PRAD_ERR_LAUNCH);
+    return PRAD_OK;
+}
+}  // extern "C++"
+
+// Operands common to the three calls; rows of K and V may differ from Q's with a cache.
+static int32_t causal_check(const HeadColumns& Q, const HeadColumns& K, const HeadColumns& V, prad_buf_t O, prad_index_t offsets, int64_t heads,
+                            int64_t head_dim, bool cache) {
+    REQUIRE_BUF(Q.buf); REQUIRE_BUF(K.buf); REQUIRE_BUF(V.buf); REQUIRE_BUF(O); REQUIRE_INDEX(offsets);
+    if (int32_t st = same_dtype({Q.buf, K.buf, V.buf, O})) return st;
+    if (int32_t st = columns_check(Q, Q.buf->rows)) return st;
+    if (int32_t st = columns_check(K, cache ? K.buf->rows : Q.buf->rows)) return st;
+    if (int32_t st = columns_check(V, K.buf->rows)) return st;
+    if (O->depth != 1 || O->rows != Q.buf->rows || O->cols != heads * head_dim)
+        return fail(PRAD_ERR_SHAPE, "O must be %lld x %lld", (long long)Q.buf->rows, (long long)(heads * head_dim));
+    if (Q.buf->rows > INT32_MAX || K.buf->rows > INT32_MAX) return fail(PRAD_ERR_ARG, "at most 2^31 - 1 rows");
+    if (offsets->n < 2 || offsets->n > INT32_MAX) return fail(PRAD_ERR_SHAPE, "the offsets of n sequences are n + 1 elements");
+    return PRAD_OK;
+}
+
+int32_t prad_causal_attention_fwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                                  prad_buf_t lse, prad_index_t offsets, int64_t heads, int64_t kv_heads, int64_t head_dim, double scale) {
+    REQUIRE_INIT();
+    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
+    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, false)) return st;
+    if (lse != nullptr) {
+        REQUIRE_BUF(lse);
+        if (int32_t st = same_dtype({Q, lse})) return st;
+        if (int32_t st = expect_rows(lse, heads, Q->rows, "lse")) return st;
+    }
+    for (prad_buf_t out : {O, lse}) {
+        if (out == nullptr) continue;
+        if (overlap(out, Q) || overlap(out, K) || overlap(out, V) || overlap(out, offsets)) return fail(PRAD_ERR_ARG, "an output must not overlap an input");
+    }
+    if (lse != nullptr && overlap(O, lse)) return fail(PRAD_ERR_ARG, "O and lse must not overlap");
+    ENQUEUE_LOCK();
+    if (Q->dtype == PRAD_F64) return causal_fwd_t<double>(causal_args<double>(q, k, v, O, heads, kv_heads, head_dim, scale), lse, offsets);
+    return causal_fwd_t<float>(causal_args<float>(q, k, v, O, heads, kv_heads, head_dim, scale), lse, offsets);
+}
+
+int32_t prad_causal_attention_bwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                                  prad_buf_t lse, prad_buf_t dO, prad_buf_t dQ, int64_t dq_col, prad_buf_t dK, int64_t dk_col,
+                                  prad_buf_t dV, int64_t dv_col, prad_index_t offsets, int64_t heads, int64_t kv_heads,
+                                  int64_t head_dim, double scale) {
+    REQUIRE_INIT();
+    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
+    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, false)) return st;
+    REQUIRE_BUF(lse); REQUIRE_BUF(dO); REQUIRE_BUF(dQ); REQUIRE_BUF(dK); REQUIRE_BUF(dV);
+    if (int32_t st = same_dtype({Q, lse, dO, dQ, dK, dV})) return st;
+    if (int32_t st = expect_rows(lse, heads, Q->rows, "lse")) return st;
+    if (int32_t st = expect_rows(dO, Q->rows, heads * head_dim, "dO")) return st;
+    const HeadColumns grads[3] = {{dQ, dq_col, heads * head_dim, "dQ"}, {dK, dk_col, kv_heads * head_dim, "dK"}, {dV, dv_col, kv_heads * head_dim, "dV"}};
+    for (const HeadColumns& g : grads) {
+        if (int32_t st = columns_check(g, Q->rows)) return st;
+        for (prad_buf_t in : {Q, K, V, O, lse, dO})
+            if (overlap(g.buf, in)) return fail(PRAD_ERR_ARG, "%s must not overlap an input", g.name);
+        if (overlap(g.buf, offsets)) return fail(PRAD_ERR_ARG, "%s must not overlap an input", g.name);
+    }
+    if (columns_meet(grads[0], grads[1]) || columns_meet(grads[0], grads[2]) || columns_meet(grads[1], grads[2]))
+        return fail(PRAD_ERR_ARG, "the columns of dQ, dK and dV must not overlap");
+    ENQUEUE_LOCK();
+    if (Q->dtype == PRAD_F64)
+        return causal_bwd_t<double>(causal_args<double>(q, k, v, O, heads, kv_heads, head_dim, scale), lse, dO, grads[0], grads[1], grads[2], offsets);
+    return causal_bwd_t<float>(causal_args<float>(q, k, v, O, heads, kv_heads, head_dim, scale), lse, dO, grads[0], grads[1], grads[2], offsets);
+}
+
+int32_t prad_cached_attention(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
+                              prad_index_t q_offsets, prad_index_t k_begin, prad_index_t k_end, int64_t heads, int64_t kv_heads,
+                              int64_t head_dim, double scale) {
+    REQUIRE_INIT();
+    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
+    if (int32_t st = causal_check(q, k, v, O, q_offsets, heads, head_dim, true)) return st;
+    REQUIRE_INDEX(k_begin); REQUIRE_INDEX(k_end);
+    if (k_begin->n != q_offsets->n - 1 || k_end->n != q_offsets->n - 1)
+        return fail(PRAD_ERR_SHAPE, "%lld sequences need as many key ranges", (long long)(q_offsets->n - 1));
+    if (overlap(O, Q) || overlap(O, K) || overlap(O, V) || overlap(O, q_offsets) || overlap(O, k_begin) || overlap(O, k_end))
+        return fail(PRAD_ERR_ARG, "O must not overlap an input");
+    ENQUEUE_LOCK();
+    if (Q->dtype == PRAD_F64) return cached_t<double>(causal_args<double>(q, k, v, O, heads, kv_heads, head_dim, scale), q_offsets, k_begin, k_end);
+    return cached_t<float>(causal_args<float>(q, k, v, O, heads, kv_heads, head_dim, scale), q_offsets, k_begin, k_end);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Recording.  The stream is captured in thread-local mode and the context remembers which thread records:
 // every enqueueing entry point called from another thread while a recording is open returns

@@ -63,3 +63,38 @@ def attention(q, k, v, scale, g=None):
             dk[:seen] += np.outer(ds, q[i])
             dv[:seen] += np.outer(p, gi)
     return (o, lse) if g is None else (o, lse, dq, dk, dv)
+
+
+def attention_bounds(q, k, v, scale, u, g):
+    """How far o, lse, dq, dk, dv of one head may be off in arithmetic of unit roundoff u, whatever the order of the sums,
+    counted term by term to first order in u (the factor 1.1 of the comparison covers the rest):
+      a score: d products and their sum, the scaling (d + 4 roundings of |scale| sum |q||k|);
+      a weight exp(s - top) / sum: the errors of two scores, an exponential good to 4 u, a sum of m terms, a division;
+      backward's weight exp(s - lse): a score's error, lse's own and its rounding, 4 u;  and so on along the formulas."""
+    q, k, v, g = (np.asarray(x, np.float64) for x in (q, k, v, g))
+    n, m, d = len(q), len(k), q.shape[1]
+    seen = np.arange(m)[None, :] <= np.arange(n)[:, None] + (m - n)
+    s = np.where(seen, q @ k.T * scale, -np.inf)
+    some = seen.any(axis=1)
+    top = np.where(some, s.max(axis=1, initial=-np.inf), 0)
+    e = np.exp(s - top[:, None])
+    total = np.where(some, e.sum(axis=1), 1)
+    p = e / total[:, None]
+    lse = top + np.log(total)
+    ds_score = np.where(seen, (d + 4) * u * (np.abs(q) @ np.abs(k).T) * abs(scale), 0)
+    row = ds_score.max(axis=1, initial=0)[:, None] + u * (np.abs(s, where=seen, out=np.zeros_like(s)) + np.abs(top)[:, None])
+    weight = 2 * row + (m + 8) * u
+    o_size = p @ np.abs(v)
+    e_o = (p * weight) @ np.abs(v) + (m + 4) * u * o_size
+    e_lse = row.max(axis=1, initial=0) + (m + 8) * u + 4 * u * np.abs(lse)
+    o = p @ v
+    again = row + e_lse[:, None] + (4 * np.abs(lse)[:, None] + 8) * u     # backward's weights, relative
+    dp, dp_size = g @ v.T, np.abs(g) @ np.abs(v).T
+    dot = (g * o).sum(axis=1)[:, None]
+    e_dot = ((d + 2) * u * (np.abs(g) * np.abs(o)).sum(axis=1) + (np.abs(g) * e_o).sum(axis=1))[:, None]
+    e_ds = p * (np.abs(dp - dot) * (again + 4 * u) + (d + 2) * u * dp_size + e_dot + 2 * u * (np.abs(dp) + np.abs(dot)))
+    ds = p * np.abs(dp - dot)
+    e_dq = abs(scale) * ((e_ds + (m + 4) * u * ds) @ np.abs(k))
+    e_dk = abs(scale) * ((e_ds + (n + 4) * u * ds).T @ np.abs(q))
+    e_dv = (p * (again + (n + 4) * u)).T @ np.abs(g)
+    return e_o, np.where(some, e_lse, 0), e_dq, e_dk, e_dv
