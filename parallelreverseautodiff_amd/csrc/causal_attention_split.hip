@@ -1,0 +1,628 @@
+// Causal attention in float for long batches: the products run on the half-precision matrix instructions.
+//
+// A float x scaled by a power of two is held as two halves, x = hi + lo with hi the nearest half and lo the nearest half to the
+// rest: 22 bits.  A product of two such numbers is three products of halves, hi hi + hi lo + lo hi, summed in float by the matrix
+// instruction; what is left out, lo lo and the rest behind lo, is below 2^-21 of the product, the size of a float's own
+// rounding.  The half instructions run at sixteen times the rate of the float ones, so three of them take a fifth of the time
+// (library products on this card: 1060 TFLOP/s in half, 153 in float) - and they overlap with vector instructions, which the
+// float ones do not.
+//
+// Scaling.  Halves reach from 2^-24 to 2^16, so the rows of a tile (64 rows of one head) are scaled by one power of two that
+// takes the largest magnitude in it to [2^11, 2^12).  An element 2^-26 times that still has its 11 + 11 bits, one further down
+// an absolute error of 2^-37 of the largest.  Weights P <= 1 are scaled by a constant.  Where tiles are summed in one
+// accumulator, the ratio of a tile's power to the largest one of all tiles that go into the sum is folded into the weights.
+//
+// Layout.  A first launch splits the operands and writes them in the order in which the 32 x 32 x 16 matrix instruction takes
+// its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the reduction; a fragment is
+// 1 KB, copied to LDS as it is and read back without bank conflicts.  Rows and columns past the end are zeros, so the
+// main kernels check no bounds.  Which element of the reduction sits where is free as long as both operands agree: the weights
+// come out of the first product with a column per lane and 4-row groups alternating between the lane halves, and the transposed
+// operands are written in that order, so weights go from one product into the next without leaving their lane.
+//
+// A non-finite value is replaced by zero in the split operands and its row marked: where it is seen, scores (forward) or
+// lse / D (backward) are NaN.
+#include "common.h"
+
+#include <algorithm>
+
+namespace prad {
+
+namespace {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int NO_EXPONENT = -1000;   // of a tile that holds nothing but zeros
+constexpr int WEIGHT_BITS = 14;      // P is scaled by 2^14
+
+// What the first launch notes about a tile of 64 rows.
+struct Header {
+    int e;                  // values were scaled by 2^-e
+    uint32_t bad[2];        // rows that hold a non-finite value
+    int e_dot;              // of dO: |D| < 2^e_dot
+};
+
+__device__ __forceinline__ int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
+__device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+// 2^e, within the normal numbers
+__device__ __forceinline__ float pow2(int e) { return __builtin_ldexpf(1.0f, e < -126 ? -126 : e > 127 ? 127 : e); }
+
+// Tiles of 64 packed rows (token, head of the group) are numbered as in causal_attention.hip: sequence s begins at
+// floor(offset G / R) + s.
+__device__ __forceinline__ int64_t first_tile(const CausalArgs<float>& p, int s, int group, int R) { return clamped(p.q_off[s], p.q_rows) * group / R + s; }
+__device__ __forceinline__ bool find_tile(const CausalArgs<float>& p, int group, int R, int64_t tile, int* sequence, int64_t* inside) {
+    int lo = 0, hi = p.sequences;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (first_tile(p, mid, group, R) <= tile) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo == 0) return false;
+    *sequence = lo - 1;
+    *inside = tile - first_tile(p, lo - 1, group, R);
+    return true;
+}
+__device__ __forceinline__ void sequence_rows(const CausalArgs<float>& p, int s, int64_t* q0, int64_t* n) {
+    *q0 = clamped(p.q_off[s], p.q_rows);
+    const int64_t q1 = clamped(p.q_off[s + 1], p.q_rows);
+    *n = q1 > *q0 ? q1 - *q0 : 0;
+}
+
+// hi = nearest halves, lo = nearest halves to the rest.  `minus_one` is a register the compiler does not see through, which
+// makes x - hi one mixed-precision instruction instead of a conversion and a subtraction.
+__device__ __forceinline__ void split2(float a, float b, float minus_one, h2* hi, h2* lo) {
+    const f2 v = {a, b};
+    const h2 h = __builtin_convertvector(v, h2);
+    const f2 r = {__builtin_fmaf((float)h.x, minus_one, a), __builtin_fmaf((float)h.y, minus_one, b)};
+    *hi = h;
+    *lo = __builtin_convertvector(r, h2);
+}
+__device__ __forceinline__ float opaque_minus_one() {
+    float m = -1.0f;
+    asm("" : "+s"(m));
+    return m;
+}
+template <int N>
+__device__ __forceinline__ void split_regs(const float (&x)[N], float minus_one, h8 (&hi)[N / 8], h8 (&lo)[N / 8]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        h2 h, l;
+        split2(x[i], x[i + 1], minus_one, &h, &l);
+        hi[i / 8][i % 8] = h.x; hi[i / 8][i % 8 + 1] = h.y;
+        lo[i / 8][i % 8] = l.x; lo[i / 8][i % 8 + 1] = l.y;
+    }
+}
+
+// acc += (a_hi + a_lo) (b_hi + b_lo) without lo lo, the small parts first
+__device__ __forceinline__ void mfma3(h8 a_hi, h8 a_lo, h8 b_hi, h8 b_lo, f16v& acc) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a_lo, b_hi, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a_hi, b_lo, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a_hi, b_hi, acc, 0, 0, 0);
+}
+// Row of accumulator element r in lane half h.
+__device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// ---- first launch: split operands ------------------------------------------------------------------------------------------
+// A block of 32 rows of a tile is 128 HDP bytes:
+//   rows form:        [plane][HDP / 16][lane][8]            row l % 32, columns 16 k + 8 (l / 32) + e
+//   transposed form:  [plane][HDP / 32][2][lane][8]         column 32 c + l % 32, rows acc_row(8 t + e, l / 32)
+// A tile is two blocks; tile and head (slot, kv) lie at (slot kv_heads + kv) 256 HDP bytes.
+struct SplitSource {
+    const float* src;
+    int64_t ld;
+    int group;         // heads per packed row group (1: keys)
+    int vec;
+    _Float16* rows;    // nullptr: form not needed
+    _Float16* columns;
+    Header* header;
+    int dots;          // dO: D and lse of the rows as well
+};
+struct SplitArgs {
+    CausalArgs<float> p;
+    SplitSource t[4];
+    float* row_lse;    // [slot][kv][64]: WEIGHT_BITS - lse log2 e, -inf for a row that is not there
+    float* row_dot;    // D
+};
+
+template <int HDP>
+__global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
+    constexpr int PITCH = HDP + 4, PER_ROW = HDP / 4, COUNT = 64 * PER_ROW / 256;
+    __shared__ __attribute__((aligned(16))) float tile[64 * PITCH];
+    __shared__ float wave_max[4], wave_dot[4];
+    __shared__ int bad[64];
+    const SplitSource t = a.t[blockIdx.z];
+    const CausalArgs<float>& p = a.p;
+    const int kv = blockIdx.y;
+    int s;
+    int64_t inside, q0, n;
+    if (!find_tile(p, t.group, 64, blockIdx.x, &s, &inside)) return;
+    sequence_rows(p, s, &q0, &n);
+    const int64_t rows = n * t.group, row0 = inside * 64;
+    if (row0 >= rows) return;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (threadIdx.x < 64) bad[threadIdx.x] = 0;
+    __syncthreads();
+    f4 v[COUNT];
+    float top = 0.f;
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+        const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
+        const int64_t r = row0 + j;
+        v[u] = f4{0.f, 0.f, 0.f, 0.f};
+        if (r < rows && d < p.head_dim) {
+            const float* __restrict__ src = t.src + (q0 + r / t.group) * t.ld + (kv * t.group + r % t.group) * (int64_t)p.head_dim + d;
+            if (t.vec) {
+                v[u] = *reinterpret_cast<const f4*>(src);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < p.head_dim) v[u][e] = src[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+        const int j = (threadIdx.x + 256 * u) / PER_ROW;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (!is_finite(v[u][e])) {
+                v[u][e] = 0.f;
+                bad[j] = 1;
+            }
+            top = fmaxf(top, fabsf(v[u][e]));
+        }
+    }
+    top = wave_max_t(top);
+    if (lane == 0) wave_max[wave] = top;
+    // D = rowsum(dO (.) O): four lanes to a row
+    if (t.dots) {
+        const int j = threadIdx.x >> 2;
+        const int64_t r = row0 + j;
+        float dot = 0.f, size = 0.f;
+        if (r < rows) {
+            const int64_t token = q0 + r / t.group, head = kv * t.group + r % t.group;
+            const float* __restrict__ g = t.src + token * t.ld + head * p.head_dim;
+            const float* __restrict__ o = p.O + token * p.ldo + head * p.head_dim;
+            float check = 0.f;
+            for (int d = threadIdx.x & 3; d < p.head_dim; d += 4) {
+                dot = __builtin_fmaf(g[d], o[d], dot);
+                check += is_finite(g[d]) ? 0.f : NAN;
+            }
+            dot += check;
+            dot += __shfl_xor(dot, 1, 64);
+            dot += __shfl_xor(dot, 2, 64);
+            if (!is_finite(dot)) dot = NAN;
+            size = is_finite(dot) ? fabsf(dot) : 0.f;
+            if ((threadIdx.x & 3) == 0) {
+                const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + j;
+                a.row_lse[at] = (WEIGHT_BITS - p.lse[head * p.q_rows + token] * LOG2E) + (dot - dot);  // NaN where D is
+                a.row_dot[at] = dot;
+            }
+        } else if ((threadIdx.x & 3) == 0) {
+            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + j;
+            a.row_lse[at] = -INFINITY;
+            a.row_dot[at] = 0.f;
+        }
+        size = wave_max_t(size);
+        if (lane == 0) wave_dot[wave] = size;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
+    int e = NO_EXPONENT;
+    if (top > 0.f) {
+        (void)frexpf(top, &e);  // top = m 2^e, m in [1/2, 1)
+        e -= 12;
+    }
+    if (threadIdx.x < 64) {
+        const uint64_t marks = __ballot(bad[threadIdx.x] != 0);
+        if (threadIdx.x == 0) {
+            Header h;
+            h.e = e;
+            h.bad[0] = (uint32_t)marks;
+            h.bad[1] = (uint32_t)(marks >> 32);
+            h.e_dot = NO_EXPONENT;
+            if (t.dots) {
+                const float size = fmaxf(fmaxf(wave_dot[0], wave_dot[1]), fmaxf(wave_dot[2], wave_dot[3]));
+                if (size > 0.f) (void)frexpf(size, &h.e_dot);
+            }
+            t.header[(int64_t)blockIdx.x * p.kv_heads + kv] = h;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < COUNT; ++u) {
+        const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
+        f4 w;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = top > 0.f ? __builtin_ldexpf(v[u][c], -e) : 0.f;
+        *reinterpret_cast<f4*>(tile + j * PITCH + d) = w;
+    }
+    __syncthreads();
+    const float minus_one = opaque_minus_one();
+    const int64_t base = ((int64_t)blockIdx.x * p.kv_heads + kv) * (128 * HDP);  // halves
+    constexpr int FRAGS = HDP / 16;  // per block and plane, in either form
+#pragma unroll
+    for (int u = 0; u < 2 * FRAGS * 64 / 256; ++u) {
+        const int at = threadIdx.x + 256 * u, l = at & 63, f = (at >> 6) % FRAGS, block = (at >> 6) / FRAGS;
+        const int64_t hi_at = base + (int64_t)(block * 2 * FRAGS + f) * 512 + l * 8, lo_at = hi_at + FRAGS * 512;
+        float x[8];
+        h8 hi[1], lo[1];
+        if (t.rows != nullptr) {
+            const float* __restrict__ row = tile + (32 * block + (l & 31)) * PITCH + 16 * f + 8 * (l >> 5);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] = row[c];
+            split_regs<8>(x, minus_one, hi, lo);
+            *reinterpret_cast<h8*>(t.rows + hi_at) = hi[0];
+            *reinterpret_cast<h8*>(t.rows + lo_at) = lo[0];
+        }
+        if (t.columns != nullptr) {
+            const float* __restrict__ col = tile + 32 * block * PITCH + 32 * (f >> 1) + (l & 31);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[c] = col[acc_row(8 * (f & 1) + c, l >> 5) * PITCH];
+            split_regs<8>(x, minus_one, hi, lo);
+            *reinterpret_cast<h8*>(t.columns + hi_at) = hi[0];
+            *reinterpret_cast<h8*>(t.columns + lo_at) = lo[0];
+        }
+    }
+}
+
+// ---- staging ----------------------------------------------------------------------------------------------------------------
+// Copies BYTES of split operands to LDS without passing through registers: 1 KB per instruction and wavefront.
+template <int BYTES, int WAVES>
+__device__ __forceinline__ void stage(const _Float16* __restrict__ src, _Float16* dst, int wave, int lane) {
+    static_assert(BYTES % (1024 * WAVES) == 0, "whole rounds");
+#pragma unroll
+    for (int i = 0; i < BYTES / 1024 / WAVES; ++i) {
+        const int at = (i * WAVES + wave) * 512;
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + at + lane * 8),
+                                         (__attribute__((address_space(3))) void*)(dst + at), 16, 0, 0);
+    }
+}
+// The copies of every wavefront have arrived, and every wavefront is done with what they replace next.
+__device__ __forceinline__ void staged() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+__device__ __forceinline__ h8 frag(const _Float16* base, int f, int lane) { return *reinterpret_cast<const h8*>(base + f * 512 + lane * 8); }
+
+// acc[32 rows x 32 columns] = A . B over the head dimension: a block's rows form against a column per lane.
+template <int HDP>
+__device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b_hi)[HDP / 16], const h8 (&b_lo)[HDP / 16], int lane, f16v& acc) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < HDP / 16; ++k) mfma3(frag(block, k, lane), frag(block, HDP / 16 + k, lane), b_hi[k], b_lo[k], acc);
+}
+// out[HDP x 32 columns] += A^T . W: a block's transposed form against the weights of its 32 rows.
+template <int HDP>
+__device__ __forceinline__ void columns_product(const _Float16* block, const h8 (&w_hi)[2], const h8 (&w_lo)[2], int lane, f16v (&out)[HDP / 32]) {
+#pragma unroll
+    for (int c = 0; c < HDP / 32; ++c)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) mfma3(frag(block, 2 * c + t, lane), frag(block, HDP / 16 + 2 * c + t, lane), w_hi[t], w_lo[t], out[c]);
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// ---- forward ----------------------------------------------------------------------------------------------------------------
+struct ForwardArgs {
+    CausalArgs<float> p;
+    const _Float16* k_rows;
+    const _Float16* v_columns;
+    const Header* hk;
+    const Header* hv;
+};
+
+// A workgroup takes 128 packed rows of a key/value head, a wavefront 32 of them, a row per lane (of either half): S^T = K Q^T has
+// a query's scores in its lane, its statistics are sums over registers.  K and V pass through LDS in tiles of 64 keys, the next
+// one copied while this one is used.
+template <int HDP, int KEYS>
+struct ForwardTile {
+    static constexpr int BLOCKS = KEYS / 32;
+    _Float16 k[BLOCKS][64 * HDP];   // (a block of 32 rows: 2 planes of 32 HDP halves)
+    _Float16 v[BLOCKS][64 * HDP];
+};
+
+// What the headers of a tile of keys say; asked for before the copies of the tile are, so that no wait for it is a wait for them.
+struct KeyNotes {
+    int e_k, e_v;
+    uint32_t bad[2];
+    __device__ __forceinline__ void ask(const Header* __restrict__ hk, const Header* __restrict__ hv, int64_t at) {
+        e_k = hk[at].e;
+        e_v = hv[at].e;
+        bad[0] = hk[at].bad[0] | hv[at].bad[0];
+        bad[1] = hk[at].bad[1] | hv[at].bad[1];
+    }
+    // the same value in every lane: to scalar registers
+    __device__ __forceinline__ KeyNotes uniform() const {
+        KeyNotes n;
+        n.e_k = __builtin_amdgcn_readfirstlane(e_k);
+        n.e_v = __builtin_amdgcn_readfirstlane(e_v);
+        n.bad[0] = __builtin_amdgcn_readfirstlane(bad[0]);
+        n.bad[1] = __builtin_amdgcn_readfirstlane(bad[1]);
+        return n;
+    }
+};
+
+template <int HDP, int KEYS>
+__device__ __forceinline__ void forward_stage(const ForwardArgs& a, ForwardTile<HDP, KEYS>& t, KeyNotes& notes, int64_t tile0, int kv, int64_t k0, int wave,
+                                              int lane) {
+    const int64_t tile_at = (tile0 + k0 / 64) * a.p.kv_heads + kv;
+    const int64_t at = tile_at * (128 * HDP) + (k0 / KEYS % (64 / KEYS)) * (2 * KEYS * HDP);
+    notes.ask(a.hk, a.hv, tile_at);
+    stage<4 * KEYS * HDP, 4>(a.k_rows + at, &t.k[0][0], wave, lane);
+    stage<4 * KEYS * HDP, 4>(a.v_columns + at, &t.v[0][0], wave, lane);
+}
+
+template <int HDP>
+struct ForwardState {
+    h8 q_hi[HDP / 16], q_lo[HDP / 16];
+    f16v o[HDP / 32];
+    float m, l;        // the maximum the weights refer to (in units of log2 e) and their sum, this lane half's share
+    int e_row, e_v;    // exponent of the row of Q; exponent that o is kept at
+    int64_t last;      // the last key that the lane's row sees
+};
+
+template <int HDP, int KEYS>
+__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int64_t k0, int64_t wave_first, float minus_one, int lane, ForwardState<HDP>& st) {
+    constexpr int NB = KEYS / 32;
+    const int h = lane >> 5;
+    f16v s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) rows_product<HDP>(&t.k[b][0], st.q_hi, st.q_lo, lane, s[b]);
+    const float c = pow2(st.e_row + notes.e_k);
+    // masks and marks: only where some row does not see all the keys, or some key holds a non-finite value
+    if (k0 + KEYS - 1 > wave_first || (notes.bad[0] | notes.bad[1]) != 0) {
+        const int part = (int)(k0 / KEYS % (64 / KEYS));
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = 32 * b + acc_row(r, h), bit = part * KEYS + j;
+                const bool marked = (notes.bad[bit >> 5] >> (bit & 31)) & 1;
+                s[b][r] = k0 + j > st.last ? -INFINITY : marked ? NAN : s[b][r];
+            }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    top = fmaxf(top, other_half(top)) * c;
+    // The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach 2^6 2^8, and the
+    // accumulators are rarely rescaled.  (No key seen yet: m = -inf, and a top of -inf keeps the weights at 0.)
+    const bool raise = top > st.m + 6.f;
+    const int e_v = notes.e_v > st.e_v ? notes.e_v : st.e_v;
+    if (__ballot(raise) != 0 || e_v != st.e_v) {
+        const float m = raise ? top : st.m;
+        const float f = raise ? __builtin_amdgcn_exp2f(st.m - m) : 1.f;  // (m = -inf before: 0)
+        const float fo = __builtin_ldexpf(f, st.e_v - e_v < -200 ? -200 : st.e_v - e_v);
+        st.l *= f;
+#pragma unroll
+        for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st.o[d][r] *= fo;
+        st.m = m;
+        st.e_v = e_v;
+    }
+    const float ref = st.m == -INFINITY ? 0.f : st.m - 8.f;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float w[NB][16];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            w[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c, -ref));
+            sum[r & 3] += w[b][r];
+        }
+    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    if (notes.e_v != st.e_v) {  // a tile of smaller values: its weights carry the ratio
+        const float f = pow2(notes.e_v - st.e_v);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w[b][r] *= f;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        h8 hi[2], lo[2];
+        split_regs<16>(w[b], minus_one, hi, lo);
+        columns_product<HDP>(&t.v[b][0], hi, lo, lane, st.o);
+    }
+}
+
+template <int HDP, int KEYS>
+__global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardArgs a) {
+    __shared__ __attribute__((aligned(16))) ForwardTile<HDP, KEYS> even, odd;
+    const CausalArgs<float>& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    // all heads of a tile next to each other: consecutive workgroups go to different chiplets, so a chiplet's cache serves few
+    // heads; late tiles see the most keys and go first, so that the last ones to finish are short
+    const int kv = blockIdx.x % (unsigned)p.kv_heads;
+    int s;
+    int64_t inside, q0, n;
+    if (!find_tile(p, p.group, 128, (int64_t)(gridDim.x / (unsigned)p.kv_heads) - 1 - blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;
+    sequence_rows(p, s, &q0, &n);
+    const int64_t rows = n * p.group, row0 = inside * 128 + 32 * wave, row = row0 + (lane & 31);
+    if (inside * 128 >= rows) return;
+    const float minus_one = opaque_minus_one();
+    ForwardState<HDP> st;
+    const int64_t token = q0 + row / p.group;
+    const int head = kv * p.group + (int)(row % p.group);
+    bool row_bad = false;
+    {
+        // the row of Q, scaled by a power of two of its own; scale log2 e goes in as a factor in [1/2, 1) and another power
+        const float* __restrict__ src = p.Q + token * p.ldq + head * (int64_t)p.head_dim;
+        int e_factor = 0;
+        const float factor = frexpf(p.scale * LOG2E, &e_factor);
+        float x[HDP / 16][8], top = 0.f;
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k)
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const int d = 16 * k + 8 * h + 4 * v;
+                f4 y = {0.f, 0.f, 0.f, 0.f};
+                if (row < rows && d < p.head_dim) {
+                    if (p.vec_q) {
+                        y = *reinterpret_cast<const f4*>(src + d);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (d + e < p.head_dim) y[e] = src[d + e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    row_bad = row_bad || !is_finite(y[e]);
+                    x[k][4 * v + e] = is_finite(y[e]) ? y[e] : 0.f;
+                    top = fmaxf(top, fabsf(x[k][4 * v + e]));
+                }
+            }
+        top = fmaxf(top, other_half(top));
+        row_bad = __shfl_xor((int)row_bad, 32, 64) != 0 || row_bad;
+        int e = 0;
+        if (top > 0.f) {
+            (void)frexpf(top, &e);
+            e -= 12;
+        }
+        st.e_row = e + e_factor;
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k) {
+            h8 hi[1], lo[1];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) x[k][c] = __builtin_ldexpf(x[k][c], -e) * factor;
+            split_regs<8>(x[k], minus_one, hi, lo);
+            st.q_hi[k] = hi[0];
+            st.q_lo[k] = lo[0];
+        }
+    }
+    st.last = row < rows ? row / p.group : rows / p.group - 1;
+    st.m = -INFINITY;
+    st.l = 0.f;
+    st.e_v = NO_EXPONENT;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.o[d][r] = 0.f;
+    // keys seen by the workgroup and by the wavefront; the first key that a row of the wavefront does not see is wave_first + 1
+    const int64_t last_row = inside * 128 + 127 < rows ? inside * 128 + 127 : rows - 1;
+    const int64_t seen = last_row / p.group + 1;
+    const int64_t wave_first = row0 < rows ? row0 / p.group : -1;
+    const int64_t wave_row = row0 + 31 < rows ? row0 + 31 : rows - 1;
+    const int64_t wave_seen = row0 < rows ? wave_row / p.group + 1 : 0;
+    const int64_t tile0 = first_tile(p, s, 1, 64);
+    KeyNotes notes_even, notes_odd;
+    forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, 0, wave, lane);
+    for (int64_t k0 = 0; k0 < seen; k0 += 2 * KEYS) {
+        staged();
+        KeyNotes notes = notes_even.uniform();
+        if (k0 + KEYS < seen) forward_stage<HDP, KEYS>(a, odd, notes_odd, tile0, kv, k0 + KEYS, wave, lane);
+        if (k0 < wave_seen) forward_tile<HDP, KEYS>(even, notes, k0, wave_first, minus_one, lane, st);
+        if (k0 + KEYS >= seen) break;
+        staged();
+        notes = notes_odd.uniform();
+        if (k0 + 2 * KEYS < seen) forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, k0 + 2 * KEYS, wave, lane);
+        if (k0 + KEYS < wave_seen) forward_tile<HDP, KEYS>(odd, notes, k0 + KEYS, wave_first, minus_one, lane, st);
+    }
+    if (row >= rows) return;
+    const float l = st.l + other_half(st.l);
+    const float inv = row_bad ? NAN : 1.f / l;
+    float* __restrict__ dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * h;
+            f4 y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(st.o[d][4 * q + e] * inv, st.e_v);
+            if (at >= p.head_dim) continue;
+            if (p.vec_o) {
+                *reinterpret_cast<f4*>(dst + at) = y;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < p.head_dim) dst[at + e] = y[e];
+            }
+        }
+    if (p.lse != nullptr && h == 0) {
+        const float ref = st.m == -INFINITY ? 0.f : st.m - 8.f;
+        p.lse[head * p.q_rows + token] = row_bad ? NAN : (ref + __log2f(l)) * LN2;
+    }
+}
+
+// ---- workspace --------------------------------------------------------------------------------------------------------------
+inline size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
+inline int64_t tile_slots(int64_t rows, int64_t group, int64_t per_tile, int64_t sequences) { return rows * group / per_tile + sequences; }
+inline int padded(int head_dim) { return head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128; }
+
+// Hands out parts of the workspace; with a null base it only counts.
+struct Carver {
+    char* base;
+    size_t used = 0;
+    template <typename U>
+    U* take(size_t bytes) {
+        U* at = base == nullptr ? nullptr : reinterpret_cast<U*>(base + used);
+        used += round256(bytes);
+        return at;
+    }
+};
+
+struct ForwardPlan {
+    SplitArgs split;
+    ForwardArgs main;
+    size_t bytes;
+};
+ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
+    const int hdp = padded(p.head_dim);
+    const int64_t key_tiles = tile_slots(p.q_rows, 1, 64, p.sequences) * p.kv_heads;
+    Carver c{static_cast<char*>(workspace)};
+    ForwardPlan f{};
+    _Float16* k = c.take<_Float16>((size_t)key_tiles * 256 * hdp);
+    _Float16* v = c.take<_Float16>((size_t)key_tiles * 256 * hdp);
+    Header* hk = c.take<Header>((size_t)key_tiles * sizeof(Header));
+    Header* hv = c.take<Header>((size_t)key_tiles * sizeof(Header));
+    f.split.p = p;
+    f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, nullptr, hk, 0};
+    f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, nullptr, v, hv, 0};
+    f.main = {p, k, v, hk, hv};
+    f.bytes = c.used;
+    return f;
+}
+
+inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
+
+}  // namespace
+
+bool causal_split_eligible(const CausalArgs<float>& p, bool backward) {
+    return !backward && p.q_rows >= 512;
+}
+
+size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
+
+hipError_t launch_causal_split_fwd(const CausalArgs<float>& p, void* workspace, hipStream_t s) {
+    const ForwardPlan f = forward_plan(p, workspace);
+    const int64_t key_slots = tile_slots(p.q_rows, 1, 64, p.sequences), slots = tile_slots(p.q_rows, p.group, 128, p.sequences);
+    if (!grid_fits(key_slots, 256) || !grid_fits(slots * p.kv_heads, 256)) return hipErrorInvalidValue;
+    const dim3 split((unsigned)key_slots, p.kv_heads, 2), grid((unsigned)(slots * p.kv_heads)), block(256);
+    switch (padded(p.head_dim)) {
+        case 32:
+            hipLaunchKernelGGL(causal_split_kernel<32>, split, block, 0, s, f.split);
+            hipLaunchKernelGGL((causal_split_fwd_kernel<32, 64>), grid, block, 0, s, f.main);
+            break;
+        case 64:
+            hipLaunchKernelGGL(causal_split_kernel<64>, split, block, 0, s, f.split);
+            hipLaunchKernelGGL((causal_split_fwd_kernel<64, 64>), grid, block, 0, s, f.main);
+            break;
+        default:
+            hipLaunchKernelGGL(causal_split_kernel<128>, split, block, 0, s, f.split);
+            hipLaunchKernelGGL((causal_split_fwd_kernel<128, 32>), grid, block, 0, s, f.main);
+            break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace prad

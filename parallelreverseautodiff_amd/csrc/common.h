@@ -465,6 +465,10 @@ struct CausalArgs {
 template <typename T> hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s);
 template <typename T> size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a);
 template <typename T> hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s);
+// The same in float on the half-precision matrix instructions (csrc/causal_attention_split.hip), for batches long enough.
+bool causal_split_eligible(const CausalArgs<float>& a, bool backward);
+size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& a);
+hipError_t launch_causal_split_fwd(const CausalArgs<float>& a, void* workspace, hipStream_t s);
 template <typename T> size_t cached_workspace_bytes(const CausalArgs<T>& a);
 template <typename T> hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s);
 

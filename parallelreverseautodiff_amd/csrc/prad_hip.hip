@@ -2032,6 +2032,13 @@ template <typename T>
 static int32_t causal_fwd_t(CausalArgs<T> a, prad_buf_t lse, prad_index_t offsets) {
     a.lse = lse != nullptr ? static_cast<T*>(lse->ptr) : nullptr;
     a.q_off = offsets->ptr; a.sequences = (int)(offsets->n - 1);
+    if constexpr (sizeof(T) == 4) {
+        if (causal_split_eligible(a, false)) {
+            if (int32_t st = ensure_workspace(causal_split_fwd_workspace_bytes(a))) return st;
+            HIP_TRY(launch_causal_split_fwd(a, CUR_WORKSPACE, CUR_STREAM), PRAD_ERR_LAUNCH);
+            return PRAD_OK;
+        }
+    }
     HIP_TRY(launch_causal_fwd<T>(a, CUR_STREAM), PRAD_ERR_LAUNCH);
     return PRAD_OK;
 }

@@ -165,7 +165,10 @@ def compare(batch, parity=True):
 CASES = [([1], 1, 1, 1, "fused"), ([5], 2, 1, 3, "apart"), ([0, 0], 2, 2, 8, "fused"), ([0, 3, 0, 1, 2, 0], 2, 2, 16, "fused"), ([49, 1, 17, 33], 3, 3, 32, "fused"),
          ([16, 15, 17], 4, 2, 33, "apart"), ([64, 63, 65, 1], 2, 1, 40, "fused"), ([31, 32, 33], 6, 2, 64, "fused"), ([130, 2], 5, 1, 64, "apart"),
          ([20, 100], 3, 1, 65, "apart"), ([70, 0, 129], 4, 4, 80, "fused"), ([129], 8, 1, 128, "fused"), ([90, 45], 2, 2, 127, "apart"), ([200], 6, 3, 96, "apart"),
-         ([260, 90], 4, 2, 128, "apart")]
+         ([260, 90], 4, 2, 128, "apart"),
+         # long batches
+         ([300, 0, 129, 64, 1, 77, 40], 4, 2, 64, "fused"), ([520], 3, 1, 40, "apart"), ([63, 65, 130, 255, 100], 2, 2, 32, "fused"), ([257, 256, 31], 4, 1, 128, "fused"),
+         ([600, 32], 5, 1, 80, "apart"), ([1] * 530, 2, 1, 64, "fused"), ([1300], 1, 1, 16, "fused"), ([130, 400], 6, 2, 127, "apart")]
 
 
 @DTYPES
@@ -174,10 +177,14 @@ def test_attention_against_its_definition(gpu, dtype, case):
     compare(Batch(dtype, *case))
 
 
+LONG = pytest.mark.parametrize("long", [False, True], ids=["short", "long"])
+
+
 @DTYPES
-def test_scores_far_apart_and_far_from_zero(gpu, dtype):
+@LONG
+def test_scores_far_apart_and_far_from_zero(gpu, dtype, long):
     """Scores of several hundreds: the running maximum moves, most weights vanish."""
-    batch = Batch(dtype, [150, 40], 2, 1, 64, "fused")
+    batch = Batch(dtype, [550, 40] if long else [150, 40], 2, 1, 64, "fused")
     batch.q *= 12
     batch.k *= 12
     batch.upload()
@@ -185,8 +192,35 @@ def test_scores_far_apart_and_far_from_zero(gpu, dtype):
 
 
 @DTYPES
-def test_equal_calls_give_equal_bits(gpu, dtype):
-    batch = Batch(dtype, [300, 77, 1, 130], 6, 2, 64, "fused")
+@LONG
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_a_scale_that_is_not_positive(gpu, dtype, long, scale):
+    batch = Batch(dtype, [540] if long else [70], 2, 1, 32, "fused")
+    batch.scale = scale
+    batch.tail = batch.tail[:3] + (scale,)
+    compare(batch)
+
+
+@DTYPES
+@LONG
+def test_rows_of_very_different_size(gpu, dtype, long):
+    """Tokens whose values differ by thousands, tiles of zeros among them, everything far below one: every element stays within
+    its bound (which grows with the largest values a row mixes)."""
+    batch = Batch(dtype, [560, 30] if long else [190, 30], 2, 1, 64, "fused")
+    size = 2.0 ** (np.arange(batch.rows) // 37 % 5 * 3.0 - 12)
+    for x in (batch.v, batch.g):
+        x *= (size * 2.0 ** -20)[:, None].astype(dtype)
+    batch.v[70:140] = 0
+    batch.k *= size[::-1, None].astype(dtype)
+    batch.q[100:170] = 0
+    batch.upload()
+    compare(batch, parity=False)
+
+
+@DTYPES
+@LONG
+def test_equal_calls_give_equal_bits(gpu, dtype, long):
+    batch = Batch(dtype, [900, 77, 1, 130] if long else [300, 77, 1, 130], 6, 2, 64, "fused")
     first = batch.forward()
     grads = batch.backward(*first)
     for _ in range(2):
@@ -196,13 +230,14 @@ def test_equal_calls_give_equal_bits(gpu, dtype):
 
 
 @DTYPES
+@LONG
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", ["q", "k", "v", "g"])
-def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, value):
+def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, value, long):
     """Token 20 of the second sequence holds one: earlier tokens and other sequences keep every bit of O and of the gradients
     that do not depend on it; whoever sees it gets NaN."""
-    clean = Batch(dtype, [33, 50, 40], 2, 1, 40, "fused")
-    dirty = Batch(dtype, [33, 50, 40], 2, 1, 40, "fused")
+    lengths = [33, 450, 140] if long else [33, 50, 40]
+    clean, dirty = Batch(dtype, lengths, 2, 1, 40, "fused"), Batch(dtype, lengths, 2, 1, 40, "fused")
     at = int(clean.starts[1]) + 20
     getattr(dirty, where)[at, 7] = value        # (head 0)
     dirty.upload()
@@ -239,9 +274,9 @@ def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, 
         assert np.isnan(dk[int(clean.starts[1]):second_end]).all()
 
 
-def test_rows_of_nobody_are_not_read_for_a_result(gpu):
-    clean = Batch(np.float32, [70, 20], 4, 2, 64, "fused", front=70, behind=70)
-    dirty = Batch(np.float32, [70, 20], 4, 2, 64, "fused", front=70, behind=70)
+@LONG
+def test_rows_of_nobody_are_not_read_for_a_result(gpu, long):
+    clean, dirty = (Batch(np.float32, [470, 20] if long else [70, 20], 4, 2, 64, "fused", front=70, behind=70) for _ in range(2))
     first, last = int(clean.starts[0]), int(clean.starts[-1])
     for x in (dirty.q, dirty.k, dirty.v, dirty.g):
         x[:first] = np.nan
@@ -253,9 +288,10 @@ def test_rows_of_nobody_are_not_read_for_a_result(gpu):
 
 
 @DTYPES
-def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype):
-    lib = _lib.load()
-    batch = Batch(dtype, [60, 60, 30], 4, 2, 64, "fused", front=0, behind=0)
+@LONG
+def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype, long):
+    lib, times = _lib.load(), 5 if long else 1
+    batch = Batch(dtype, [60 * times, 60 * times, 30 * times], 4, 2, 64, "fused", front=0, behind=0)
     o, l = unfilled(dtype, batch.rows, 256), unfilled(dtype, 4, batch.rows)
     g, d = dev(batch.g), unfilled(dtype, batch.rows, batch.full[0])
     grads = [x for c in batch.cols for x in (d.handle, c)]
@@ -272,7 +308,7 @@ def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype):
         gr = ctypes.c_void_p()
         check(lib.prad_graph_end(ctypes.byref(gr)))
     for lengths in ([150, 0, 0], [1, 148, 1], [50, 50, 50], [0, 75, 75]):
-        batch.offsets.upload(np.concatenate([[0], np.cumsum(lengths)]))
+        batch.offsets.upload(times * np.concatenate([[0], np.cumsum(lengths)]))
         check(lib.prad_graph_launch(gr))
         got = o.download(), l.download(), d.download()
         o.zero(), l.zero(), d.zero()
@@ -281,10 +317,11 @@ def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype):
     check(lib.prad_graph_destroy(gr))
 
 
-def test_offsets_that_describe_no_rows_do_no_harm(gpu):
+@LONG
+def test_offsets_that_describe_no_rows_do_no_harm(gpu, long):
     """Offsets past the rows, negative or falling: cut off to rows of the buffers, nothing outside is touched."""
     lib = _lib.load()
-    batch = Batch(np.float32, [40, 40], 2, 1, 32, "fused", front=0, behind=0)
+    batch = Batch(np.float32, [40, 540] if long else [40, 40], 2, 1, 32, "fused", front=0, behind=0)
     room = DeviceBuffer.alloc(np.float32, batch.rows + 64, 64)
     room.upload(np.full((batch.rows + 64, 64), 7, np.float32))
     o = room.view_rows(32, batch.rows)
