@@ -9,8 +9,10 @@
 //
 // Scaling.  Halves reach from 2^-24 to 2^16, so the rows of a tile (64 rows of one head) are scaled by one power of two that
 // takes the largest magnitude in it to [2^11, 2^12).  An element 2^-26 times that still has its 11 + 11 bits, one further down
-// an absolute error of 2^-37 of the largest.  Weights P <= 1 are scaled by a constant.  Where tiles are summed in one
-// accumulator, the ratio of a tile's power to the largest one of all tiles that go into the sum is folded into the weights.
+// an absolute error of 2^-37 of the largest.  Where tiles are summed in one accumulator, the ratio of a tile's power to the
+// largest one of all tiles that go into the sum is folded into the weights.  The weights of a column (a query forward, a key or a
+// query backward) are scaled by a power of two that belongs to the column and falls when a weight no longer fits, the
+// accumulators of the column with it: forward that is the running maximum of the softmax, backward `fit`.
 //
 // Layout.  A first launch splits the operands and writes them in the order in which the 32 x 32 x 16 matrix instruction takes
 // its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the reduction; a fragment is
@@ -37,7 +39,6 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int NO_EXPONENT = -1000;   // of a tile that holds nothing but zeros
-constexpr int WEIGHT_BITS = 14;      // P is scaled by 2^14
 
 // What the first launch notes about a tile of 64 rows.
 struct Header {
@@ -124,7 +125,7 @@ struct SplitSource {
 struct SplitArgs {
     CausalArgs<float> p;
     SplitSource t[4];
-    float* row_lse;    // [slot][kv][64]: WEIGHT_BITS - lse log2 e, -inf for a row that is not there
+    float* row_lse;    // [slot][kv][64]: -lse log2 e, -inf for a row that is not there
     float* row_dot;    // D
 };
 
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
             size = is_finite(dot) ? fabsf(dot) : 0.f;
             if ((threadIdx.x & 3) == 0) {
                 const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + j;
-                a.row_lse[at] = (WEIGHT_BITS - p.lse[head * p.q_rows + token] * LOG2E) + (dot - dot);  // NaN where D is
+                a.row_lse[at] = (dot - dot) - p.lse[head * p.q_rows + token] * LOG2E;  // NaN where D is
                 a.row_dot[at] = dot;
             }
         } else if ((threadIdx.x & 3) == 0) {
@@ -305,7 +306,15 @@ __device__ __forceinline__ void columns_product(const _Float16* block, const h8 
         for (int t = 0; t < 2; ++t) mfma3(frag(block, 2 * c + t, lane), frag(block, HDP / 16 + 2 * c + t, lane), w_hi[t], w_lo[t], out[c]);
 }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// Over the two lanes that share a column (lane halves).
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 struct ForwardArgs {
@@ -391,7 +400,7 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = fmaxf(top, other_half(top)) * c;
+    top = max_halves(top) * c;
     // The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach 2^6 2^8, and the
     // accumulators are rarely rescaled.  (No key seen yet: m = -inf, and a top of -inf keeps the weights at 0.)
     const bool raise = top > st.m + 6.f;
@@ -481,7 +490,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
                     top = fmaxf(top, fabsf(x[k][4 * v + e]));
                 }
             }
-        top = fmaxf(top, other_half(top));
+        top = max_halves(top);
         row_bad = __shfl_xor((int)row_bad, 32, 64) != 0 || row_bad;
         int e = 0;
         if (top > 0.f) {
@@ -528,7 +537,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
         if (k0 + KEYS < wave_seen) forward_tile<HDP, KEYS>(odd, notes, k0 + KEYS, wave_first, minus_one, lane, st);
     }
     if (row >= rows) return;
-    const float l = st.l + other_half(st.l);
+    const float l = sum_halves(st.l);
     const float inv = row_bad ? NAN : 1.f / l;
     float* __restrict__ dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
 #pragma unroll
@@ -552,6 +561,352 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
         const float ref = st.m == -INFINITY ? 0.f : st.m - 8.f;
         p.lse[head * p.q_rows + token] = row_bad ? NAN : (ref + __log2f(l)) * LN2;
     }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------------
+struct BackwardArgs {
+    CausalArgs<float> p;
+    const _Float16* q_rows; const _Float16* q_columns;
+    const _Float16* g_rows; const _Float16* g_columns;   // dO
+    const _Float16* k_rows; const _Float16* k_columns;
+    const _Float16* v_rows;
+    const Header* hq; const Header* hg; const Header* hk; const Header* hv;
+    const float* row_lse; const float* row_dot;
+};
+
+__device__ __forceinline__ int wave_max_int(int v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+// dP - D is below 2^(e - 1) in magnitude, e from the exponents of dO, V and D: a sum of up to 2^7 products of values below 2^12
+__device__ __forceinline__ int e_difference(int e_g, int e_v, int e_dot) { return max(31 + e_g + e_v, e_dot + 1) + 1; }
+
+// Makes weights fit into halves: where a column's largest has passed 2^15, the column and its accumulators come down to 2^11, so
+// that it takes another factor of 16 before the next time.  x: the power of two that the column is scaled by.
+constexpr int FIT_FROM = 110;  // (the smallest normal weight, 2^-126, still shows)
+template <int N>
+__device__ __forceinline__ void fit(float (&w)[16], int& x, f16v (&acc)[N]) {
+    float top = fabsf(w[0]);
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, fabsf(w[r]));
+    top = max_halves(top);
+    const bool over = top >= 32768.f;
+    if (__ballot(over) != 0) {
+        int e = 0;
+        (void)frexpf(top, &e);
+        const int down = over ? e - 11 : 0;
+        const float f = pow2(-down);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] *= f;
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] *= f;
+        x -= down;
+    }
+}
+
+template <int HDP>
+__device__ __forceinline__ void load_fragments(const _Float16* __restrict__ block, int lane, h8 (&hi)[HDP / 16], h8 (&lo)[HDP / 16]) {
+#pragma unroll
+    for (int k = 0; k < HDP / 16; ++k) {
+        hi[k] = frag(block, k, lane);
+        lo[k] = frag(block, HDP / 16 + k, lane);
+    }
+}
+// A column per lane of an accumulator to a row of `head_dim` floats.
+template <int HDP>
+__device__ __forceinline__ void store_column(float* __restrict__ dst, const f16v (&acc)[HDP / 32], float factor, int e, int h, int head_dim, bool vec) {
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * h;
+            f4 y;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) y[c] = __builtin_ldexpf(acc[d][4 * q + c], e) * factor;
+            if (at >= head_dim) continue;
+            if (vec) {
+                *reinterpret_cast<f4*>(dst + at) = y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (at + c < head_dim) dst[at + c] = y[c];
+            }
+        }
+}
+
+// Gradients of K and V.  A workgroup owns 128 keys of a key/value head, a wavefront 32 of them, a key per lane, with their K and V
+// in registers; blocks of 32 packed rows (all heads of the group) of Q and dO pass through LDS in both forms.  S = Q K^T and
+// dP = dO V^T come out with a key per lane, so P and dS go straight into dV^T += dO^T P and dK^T += Q^T dS.
+template <int HDP>
+struct RowBlock {
+    _Float16 q[64 * HDP], g[64 * HDP], q_columns[64 * HDP], g_columns[64 * HDP];
+    float lse[32], dot[32];
+};
+struct RowNotes {
+    int e_q, e_g;
+};
+
+template <int HDP>
+__device__ __forceinline__ void row_stage(const BackwardArgs& a, RowBlock<HDP>& t, RowNotes& notes, int64_t tile0, int kv, int64_t block, int wave, int lane) {
+    const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
+    notes.e_q = a.hq[tile_at].e;
+    notes.e_g = a.hg[tile_at].e;
+    stage<128 * HDP, 4>(a.q_rows + at, t.q, wave, lane);
+    stage<128 * HDP, 4>(a.g_rows + at, t.g, wave, lane);
+    stage<128 * HDP, 4>(a.q_columns + at, t.q_columns, wave, lane);
+    stage<128 * HDP, 4>(a.g_columns + at, t.g_columns, wave, lane);
+    if (wave == 0) {
+        const float* src = (lane < 32 ? a.row_lse : a.row_dot) + tile_at * 64 + (block & 1) * 32 + (lane & 31);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)t.lse, 4, 0, 0);
+    }
+}
+
+template <int HDP>
+struct KeyState {
+    h8 k_hi[HDP / 16], k_lo[HDP / 16], v_hi[HDP / 16], v_lo[HDP / 16];
+    f16v dk[HDP / 32], dv[HDP / 32];
+    int e_k, e_v;            // of the lane's keys
+    int top_q, top_g, top_t; // the largest exponents of Q, dO and dP - D over all rows that go into the sums
+    int x_v, x_k;            // the powers of two that the lane's key is scaled by in the weights of dV and dK
+    int64_t first_row;       // the first packed row that sees the lane's key
+};
+
+template <int HDP>
+__device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes& notes, int64_t row0, int64_t wave_last, float factor, float minus_one, int lane,
+                                          KeyState<HDP>& st) {
+    const int h = lane >> 5;
+    f16v s, dp;
+    rows_product<HDP>(t.q, st.k_hi, st.k_lo, lane, s);
+    rows_product<HDP>(t.g, st.v_hi, st.v_lo, lane, dp);
+    const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
+    const int e_ratio = notes.e_q - st.top_q;
+    const float x_v = (float)st.x_v;
+    float w[16], ds[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f4 lse = *reinterpret_cast<const f4*>(t.lse + 8 * q + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e]) + x_v);
+    }
+    if (row0 < wave_last) {  // some key is not seen by some row
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = row0 + acc_row(r, h) >= st.first_row ? w[r] : 0.f;
+    }
+    fit(w, st.x_v, st.dv);
+    // |P (dP - D)| 2^(1 - top_t) is at most 1; the ratio of Q's powers goes in, the weights' own power comes out
+    const int e_one = 1 - st.top_t + e_ratio + st.x_k - st.x_v;
+    const float a1 = __builtin_ldexpf(1.f, notes.e_g + st.e_v + e_one);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const f4 dot = *reinterpret_cast<const f4*>(t.dot + 8 * q + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ds[4 * q + e] = w[4 * q + e] * __builtin_fmaf(dp[4 * q + e], a1, -__builtin_ldexpf(dot[e], e_one));
+    }
+    if (row0 < wave_last) {  // (a weight of zero times a D that is not finite)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = row0 + acc_row(r, h) >= st.first_row ? ds[r] : 0.f;
+    }
+    if (notes.e_g != st.top_g) {
+        const float f = pow2(notes.e_g - st.top_g);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] *= f;
+    }
+    h8 hi[2], lo[2];
+    split_regs<16>(w, minus_one, hi, lo);
+    columns_product<HDP>(t.g_columns, hi, lo, lane, st.dv);
+    fit(ds, st.x_k, st.dk);
+    split_regs<16>(ds, minus_one, hi, lo);
+    columns_product<HDP>(t.q_columns, hi, lo, lane, st.dk);
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_kernel(const BackwardArgs a) {
+    __shared__ __attribute__((aligned(16))) RowBlock<HDP> even, odd;
+    const CausalArgs<float>& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int kv = blockIdx.x % (unsigned)p.kv_heads;
+    int s;
+    int64_t inside, q0, n;
+    if (!find_tile(p, 1, 128, blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;  // (early keys are seen by the most rows: first)
+    sequence_rows(p, s, &q0, &n);
+    const int64_t group_key0 = inside * 128;
+    if (group_key0 >= n) return;
+    const int64_t key0 = group_key0 + 32 * wave, rows = n * p.group;
+    const bool active = key0 < n;
+    const float minus_one = opaque_minus_one();
+    const int64_t row_tile0 = first_tile(p, s, p.group, 64);
+    KeyState<HDP> st;
+    {
+        const int64_t tile_at = (first_tile(p, s, 1, 64) + (active ? key0 : group_key0) / 64) * p.kv_heads + kv;
+        const int64_t at = tile_at * (128 * HDP) + (active ? key0 / 32 % 2 : 0) * (64 * HDP);
+        load_fragments<HDP>(a.k_rows + at, lane, st.k_hi, st.k_lo);
+        load_fragments<HDP>(a.v_rows + at, lane, st.v_hi, st.v_lo);
+        st.e_k = a.hk[tile_at].e;
+        st.e_v = a.hv[tile_at].e;
+    }
+    const int64_t first_block = group_key0 * p.group / 32, blocks = (rows + 31) / 32;
+    {
+        int tq = NO_EXPONENT, tg = NO_EXPONENT, tt = 2 * NO_EXPONENT;
+        for (int64_t tile = first_block / 2 + lane; tile < (blocks + 1) / 2; tile += 64) {
+            const int64_t at = (row_tile0 + tile) * p.kv_heads + kv;
+            const int e_g = a.hg[at].e;
+            tq = max(tq, a.hq[at].e);
+            tg = max(tg, e_g);
+            tt = max(tt, e_difference(e_g, st.e_v, a.hg[at].e_dot));
+        }
+        st.top_q = wave_max_int(tq);
+        st.top_g = wave_max_int(tg);
+        st.top_t = wave_max_int(tt);
+        st.e_k = __builtin_amdgcn_readfirstlane(st.e_k);
+        st.e_v = __builtin_amdgcn_readfirstlane(st.e_v);
+    }
+    st.x_v = st.x_k = FIT_FROM;
+    st.first_row = (key0 + (lane & 31)) * p.group;
+    const int64_t wave_first = key0 * p.group, wave_last = (key0 + 31) * p.group;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.dk[d][r] = st.dv[d][r] = 0.f;
+    const float factor = p.scale * LOG2E;
+    RowNotes notes_even, notes_odd;
+    auto uniform = [](const RowNotes& x) { return RowNotes{__builtin_amdgcn_readfirstlane(x.e_q), __builtin_amdgcn_readfirstlane(x.e_g)}; };
+    row_stage<HDP>(a, even, notes_even, row_tile0, kv, first_block, wave, lane);
+    for (int64_t b = first_block; b < blocks; b += 2) {
+        staged();
+        RowNotes notes = uniform(notes_even);
+        if (b + 1 < blocks) row_stage<HDP>(a, odd, notes_odd, row_tile0, kv, b + 1, wave, lane);
+        if (active && 32 * b + 31 >= wave_first) row_block<HDP>(even, notes, 32 * b, wave_last, factor, minus_one, lane, st);
+        if (b + 1 >= blocks) break;
+        staged();
+        notes = uniform(notes_odd);
+        if (b + 2 < blocks) row_stage<HDP>(a, even, notes_even, row_tile0, kv, b + 2, wave, lane);
+        if (active && 32 * (b + 1) + 31 >= wave_first) row_block<HDP>(odd, notes, 32 * (b + 1), wave_last, factor, minus_one, lane, st);
+    }
+    const int64_t key = key0 + (lane & 31);
+    if (key >= n) return;
+    store_column<HDP>(p.dK + (q0 + key) * p.lddk + kv * (int64_t)p.head_dim, st.dk, p.scale, st.top_t - 1 + st.top_q - st.x_k, h, p.head_dim, p.vec_dkv);
+    store_column<HDP>(p.dV + (q0 + key) * p.lddv + kv * (int64_t)p.head_dim, st.dv, 1.f, st.top_g - st.x_v, h, p.head_dim, p.vec_dkv);
+}
+
+// Gradient of Q: 128 packed rows to a workgroup, a row per lane, Q and dO in registers; blocks of 32 keys of K (both forms) and V
+// pass through LDS.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
+template <int HDP>
+struct KeyBlock {
+    _Float16 k[64 * HDP], v[64 * HDP], k_columns[64 * HDP];
+};
+struct BlockNotes {
+    int e_k, e_v;
+};
+
+template <int HDP>
+__device__ __forceinline__ void key_stage(const BackwardArgs& a, KeyBlock<HDP>& t, BlockNotes& notes, int64_t tile0, int kv, int64_t block, int wave, int lane) {
+    const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
+    notes.e_k = a.hk[tile_at].e;
+    notes.e_v = a.hv[tile_at].e;
+    stage<128 * HDP, 4>(a.k_rows + at, t.k, wave, lane);
+    stage<128 * HDP, 4>(a.v_rows + at, t.v, wave, lane);
+    stage<128 * HDP, 4>(a.k_columns + at, t.k_columns, wave, lane);
+}
+
+template <int HDP>
+struct RowState {
+    h8 q_hi[HDP / 16], q_lo[HDP / 16], g_hi[HDP / 16], g_lo[HDP / 16];
+    f16v dq[HDP / 32];
+    float lse, dot;
+    int e_q, e_g, top_k, top_t;
+    int x_q;        // the power of two that the lane's row is scaled by in the weights
+    int64_t last;   // the last key that the lane's row sees
+};
+
+template <int HDP>
+__device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNotes& notes, int64_t k0, int64_t wave_first, float factor, float minus_one, int lane,
+                                          RowState<HDP>& st) {
+    const int h = lane >> 5;
+    f16v s, dp;
+    rows_product<HDP>(t.k, st.q_hi, st.q_lo, lane, s);
+    rows_product<HDP>(t.v, st.g_hi, st.g_lo, lane, dp);
+    const float c = __builtin_ldexpf(factor, st.e_q + notes.e_k);
+    const int e_ratio = notes.e_k - st.top_k;
+    const int e_one = 1 - st.top_t + e_ratio + st.x_q;
+    const float a1 = __builtin_ldexpf(1.f, st.e_g + notes.e_v + e_one), b = -__builtin_ldexpf(st.dot, e_one);
+    float ds[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, st.lse)) * __builtin_fmaf(dp[r], a1, b);
+    if (k0 + 31 > wave_first) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = k0 + acc_row(r, h) <= st.last ? ds[r] : 0.f;
+    }
+    fit(ds, st.x_q, st.dq);
+    h8 hi[2], lo[2];
+    split_regs<16>(ds, minus_one, hi, lo);
+    columns_product<HDP>(t.k_columns, hi, lo, lane, st.dq);
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const BackwardArgs a) {
+    __shared__ __attribute__((aligned(16))) KeyBlock<HDP> even, odd;
+    const CausalArgs<float>& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int kv = blockIdx.x % (unsigned)p.kv_heads;
+    int s;
+    int64_t inside, q0, n;
+    if (!find_tile(p, p.group, 128, (int64_t)(gridDim.x / (unsigned)p.kv_heads) - 1 - blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;
+    sequence_rows(p, s, &q0, &n);
+    const int64_t rows = n * p.group, group_row0 = inside * 128;
+    if (group_row0 >= rows) return;
+    const int64_t row0 = group_row0 + 32 * wave, row = row0 + (lane & 31);
+    const bool active = row0 < rows;
+    const float minus_one = opaque_minus_one();
+    const int64_t key_tile0 = first_tile(p, s, 1, 64);
+    const int64_t last_row = group_row0 + 127 < rows ? group_row0 + 127 : rows - 1;
+    const int64_t seen = last_row / p.group + 1, blocks = (seen + 31) / 32;
+    RowState<HDP> st;
+    {
+        const int64_t from = active ? row0 : group_row0;
+        const int64_t tile_at = (first_tile(p, s, p.group, 64) + from / 64) * p.kv_heads + kv, at = tile_at * (128 * HDP) + (from / 32 % 2) * (64 * HDP);
+        load_fragments<HDP>(a.q_rows + at, lane, st.q_hi, st.q_lo);
+        load_fragments<HDP>(a.g_rows + at, lane, st.g_hi, st.g_lo);
+        st.lse = a.row_lse[tile_at * 64 + from % 64 + (lane & 31)];
+        st.dot = a.row_dot[tile_at * 64 + from % 64 + (lane & 31)];
+        st.e_q = __builtin_amdgcn_readfirstlane(a.hq[tile_at].e);
+        st.e_g = __builtin_amdgcn_readfirstlane(a.hg[tile_at].e);
+        int tk = NO_EXPONENT, tv = NO_EXPONENT;
+        for (int64_t tile = lane; tile < (blocks + 1) / 2; tile += 64) {
+            tk = max(tk, a.hk[(key_tile0 + tile) * p.kv_heads + kv].e);
+            tv = max(tv, a.hv[(key_tile0 + tile) * p.kv_heads + kv].e);
+        }
+        st.top_k = wave_max_int(tk);
+        st.top_t = e_difference(st.e_g, wave_max_int(tv), __builtin_amdgcn_readfirstlane(a.hg[tile_at].e_dot));
+    }
+    st.x_q = FIT_FROM;
+    st.last = row < rows ? row / p.group : n - 1;
+    const int64_t wave_row = row0 + 31 < rows ? row0 + 31 : rows - 1;
+    const int64_t wave_first = row0 / p.group, wave_seen = active ? wave_row / p.group + 1 : 0;
+#pragma unroll
+    for (int d = 0; d < HDP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st.dq[d][r] = 0.f;
+    const float factor = p.scale * LOG2E;
+    BlockNotes notes_even, notes_odd;
+    auto uniform = [](const BlockNotes& x) { return BlockNotes{__builtin_amdgcn_readfirstlane(x.e_k), __builtin_amdgcn_readfirstlane(x.e_v)}; };
+    key_stage<HDP>(a, even, notes_even, key_tile0, kv, 0, wave, lane);
+    for (int64_t b = 0; b < blocks; b += 2) {
+        staged();
+        BlockNotes notes = uniform(notes_even);
+        if (b + 1 < blocks) key_stage<HDP>(a, odd, notes_odd, key_tile0, kv, b + 1, wave, lane);
+        if (32 * b < wave_seen) key_block<HDP>(even, notes, 32 * b, wave_first, factor, minus_one, lane, st);
+        if (b + 1 >= blocks) break;
+        staged();
+        notes = uniform(notes_odd);
+        if (b + 2 < blocks) key_stage<HDP>(a, even, notes_even, key_tile0, kv, b + 2, wave, lane);
+        if (32 * (b + 1) < wave_seen) key_block<HDP>(odd, notes, 32 * (b + 1), wave_first, factor, minus_one, lane, st);
+    }
+    if (row >= rows) return;
+    store_column<HDP>(p.dQ + (q0 + row / p.group) * p.lddq + (kv * p.group + row % p.group) * (int64_t)p.head_dim, st.dq, p.scale,
+                      st.top_t - 1 + st.top_k - st.x_q, h, p.head_dim, p.vec_dq);
 }
 
 // ---- workspace --------------------------------------------------------------------------------------------------------------
@@ -593,13 +948,44 @@ ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
     return f;
 }
 
+struct BackwardPlan {
+    SplitArgs split;
+    BackwardArgs main;
+    size_t bytes;
+};
+BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
+    const int hdp = padded(p.head_dim);
+    const int64_t key_tiles = tile_slots(p.q_rows, 1, 64, p.sequences) * p.kv_heads, row_tiles = tile_slots(p.q_rows, p.group, 64, p.sequences) * p.kv_heads;
+    Carver c{static_cast<char*>(workspace)};
+    BackwardPlan b{};
+    _Float16* rows[4];
+    _Float16* columns[4];
+    Header* headers[4];
+    for (int i = 0; i < 4; ++i) {  // Q, dO, K, V
+        const int64_t tiles = i < 2 ? row_tiles : key_tiles;
+        rows[i] = c.take<_Float16>((size_t)tiles * 256 * hdp);
+        columns[i] = i < 3 ? c.take<_Float16>((size_t)tiles * 256 * hdp) : nullptr;
+        headers[i] = c.take<Header>((size_t)tiles * sizeof(Header));
+    }
+    float* lse = c.take<float>((size_t)row_tiles * 64 * 4);
+    float* dot = c.take<float>((size_t)row_tiles * 64 * 4);
+    b.split.p = p;
+    b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, rows[0], columns[0], headers[0], 0};
+    b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, rows[1], columns[1], headers[1], 1};
+    b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, rows[2], columns[2], headers[2], 0};
+    b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, rows[3], columns[3], headers[3], 0};
+    b.split.row_lse = lse;
+    b.split.row_dot = dot;
+    b.main = {p, rows[0], columns[0], rows[1], columns[1], rows[2], columns[2], rows[3], headers[0], headers[1], headers[2], headers[3], lse, dot};
+    b.bytes = c.used;
+    return b;
+}
+
 inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
 
 }  // namespace
 
-bool causal_split_eligible(const CausalArgs<float>& p, bool backward) {
-    return !backward && p.q_rows >= 512;
-}
+bool causal_split_eligible(const CausalArgs<float>& p) { return p.q_rows >= 512; }
 
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
 
@@ -621,6 +1007,29 @@ hipError_t launch_causal_split_fwd(const CausalArgs<float>& p, void* workspace, 
             hipLaunchKernelGGL(causal_split_kernel<128>, split, block, 0, s, f.split);
             hipLaunchKernelGGL((causal_split_fwd_kernel<128, 32>), grid, block, 0, s, f.main);
             break;
+    }
+    return hipGetLastError();
+}
+
+size_t causal_split_bwd_workspace_bytes(const CausalArgs<float>& p) { return backward_plan(p, nullptr).bytes; }
+
+template <int HDP>
+static void enqueue_backward(const BackwardPlan& b, dim3 split, dim3 key_grid, dim3 row_grid, hipStream_t s) {
+    hipLaunchKernelGGL(causal_split_kernel<HDP>, split, dim3(256), 0, s, b.split);
+    hipLaunchKernelGGL(causal_split_bwd_kv_kernel<HDP>, key_grid, dim3(256), 0, s, b.main);
+    hipLaunchKernelGGL(causal_split_bwd_q_kernel<HDP>, row_grid, dim3(256), 0, s, b.main);
+}
+
+hipError_t launch_causal_split_bwd(const CausalArgs<float>& p, void* workspace, hipStream_t s) {
+    const BackwardPlan b = backward_plan(p, workspace);
+    const int64_t row_tiles = tile_slots(p.q_rows, p.group, 64, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences),
+                  row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
+    if (!grid_fits(row_tiles, 256) || !grid_fits(row_groups * p.kv_heads, 256)) return hipErrorInvalidValue;
+    const dim3 split((unsigned)row_tiles, p.kv_heads, 4), key_grid((unsigned)(key_groups * p.kv_heads)), row_grid((unsigned)(row_groups * p.kv_heads));
+    switch (padded(p.head_dim)) {
+        case 32: enqueue_backward<32>(b, split, key_grid, row_grid, s); break;
+        case 64: enqueue_backward<64>(b, split, key_grid, row_grid, s); break;
+        default: enqueue_backward<128>(b, split, key_grid, row_grid, s); break;
     }
     return hipGetLastError();
 }

@@ -461,12 +461,15 @@ struct CausalArgs {
     T* D;                          // heads x q_rows of workspace
     T* dQ; T* dK; T* dV;
     int64_t lddq, lddk, lddv;
+    bool vec_dq, vec_dkv;
 };
 template <typename T> hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s);
 template <typename T> size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a);
 template <typename T> hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s);
 // The same in float on the half-precision matrix instructions (csrc/causal_attention_split.hip), for batches long enough.
-bool causal_split_eligible(const CausalArgs<float>& a, bool backward);
+bool causal_split_eligible(const CausalArgs<float>& a);
+size_t causal_split_bwd_workspace_bytes(const CausalArgs<float>& a);
+hipError_t launch_causal_split_bwd(const CausalArgs<float>& a, void* workspace, hipStream_t s);
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& a);
 hipError_t launch_causal_split_fwd(const CausalArgs<float>& a, void* workspace, hipStream_t s);
 template <typename T> size_t cached_workspace_bytes(const CausalArgs<T>& a);
