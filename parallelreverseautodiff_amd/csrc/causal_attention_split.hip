@@ -125,18 +125,75 @@ struct SplitSource {
 struct SplitArgs {
     CausalArgs<float> p;
     SplitSource t[4];
+    int tensors;
+    int4* order;       // schedules for the main kernels, see below
+    int order_slots[2];
+    int shift;
     float* row_lse;    // [slot][kv][64]: -lse log2 e, -inf for a row that is not there
     float* row_dot;    // D
 };
 
+// The groups of 128 packed rows (which = 0) or 128 keys (1) of all sequences as (sequence, number inside it), those with the most
+// work first: the last workgroups to finish are then short ones.  Which of two with about equal work comes first is left to
+// chance and shows in no result.  One workgroup, beside the ones that split.
+constexpr int ORDER_BINS = 1024;
+__device__ __forceinline__ void write_order(const CausalArgs<float>& p, int which, int slots, int shift, int4* __restrict__ order, int* bins) {
+    __shared__ int wave_total[4];
+    const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    const int group = which == 0 ? p.group : 1;
+    for (int i = threadIdx.x; i < ORDER_BINS; i += 256) bins[i] = 0;
+    __syncthreads();
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int slot = threadIdx.x; slot < slots; slot += 256) {
+            int s = -1;
+            int64_t inside = 0, q0 = 0, n = 0, work = -1;  // in tiles of 64 keys or tokens
+            if (find_tile(p, group, 128, slot, &s, &inside)) {
+                sequence_rows(p, s, &q0, &n);
+                if (inside * 128 < n * group) work = which == 0 ? (inside * 128 + 127) / group / 64 : (n - 1 - inside * 128) / 64;
+            }
+            const int64_t bin = work < 0 ? ORDER_BINS - 1 : (work >> shift) > ORDER_BINS - 2 ? 0 : ORDER_BINS - 2 - (work >> shift);
+            const int at = atomicAdd(&bins[bin], 1);
+            if (pass == 1) order[at] = int4{work < 0 ? -1 : s, (int)inside, 0, 0};
+        }
+        __syncthreads();
+        if (pass == 1) break;
+        // counts to first places
+        int mine[ORDER_BINS / 256], total = 0;
+#pragma unroll
+        for (int i = 0; i < ORDER_BINS / 256; ++i) {
+            mine[i] = total;
+            total += bins[threadIdx.x * (ORDER_BINS / 256) + i];
+        }
+        int before = total;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int v = __shfl_up(before, off, 64);
+            if (lane >= off) before += v;
+        }
+        if (lane == 63) wave_total[wave] = before;
+        __syncthreads();
+        int base = before - total;
+        for (int w = 0; w < wave; ++w) base += wave_total[w];
+#pragma unroll
+        for (int i = 0; i < ORDER_BINS / 256; ++i) bins[threadIdx.x * (ORDER_BINS / 256) + i] = base + mine[i];
+        __syncthreads();
+    }
+}
+
 template <int HDP>
 __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     constexpr int PITCH = HDP + 4, PER_ROW = HDP / 4, COUNT = 64 * PER_ROW / 256;
+    static_assert(64 * PITCH >= ORDER_BINS, "the tile's room also holds the bins of a schedule");
     __shared__ __attribute__((aligned(16))) float tile[64 * PITCH];
-    __shared__ float wave_max[4], wave_dot[4];
+    __shared__ float wave_max[4], row_dots[64], largest_dot;
     __shared__ int bad[64];
-    const SplitSource t = a.t[blockIdx.z];
     const CausalArgs<float>& p = a.p;
+    if ((int)blockIdx.z == a.tensors) {
+        if (blockIdx.y == 0 && blockIdx.x < 2 && a.order_slots[blockIdx.x] > 0)
+            write_order(p, blockIdx.x, a.order_slots[blockIdx.x], a.shift, a.order + (blockIdx.x == 0 ? 0 : a.order_slots[0]), reinterpret_cast<int*>(tile));
+        return;
+    }
+    const SplitSource t = a.t[blockIdx.z];
     const int kv = blockIdx.y;
     int s;
     int64_t inside, q0, n;
@@ -179,37 +236,46 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     }
     top = wave_max_t(top);
     if (lane == 0) wave_max[wave] = top;
-    // D = rowsum(dO (.) O): four lanes to a row
+    // D = rowsum(dO (.) O): the PER_ROW lanes that hold a row of dO
     if (t.dots) {
-        const int j = threadIdx.x >> 2;
-        const int64_t r = row0 + j;
-        float dot = 0.f, size = 0.f;
-        if (r < rows) {
-            const int64_t token = q0 + r / t.group, head = kv * t.group + r % t.group;
-            const float* __restrict__ g = t.src + token * t.ld + head * p.head_dim;
-            const float* __restrict__ o = p.O + token * p.ldo + head * p.head_dim;
-            float check = 0.f;
-            for (int d = threadIdx.x & 3; d < p.head_dim; d += 4) {
-                dot = __builtin_fmaf(g[d], o[d], dot);
-                check += is_finite(g[d]) ? 0.f : NAN;
+        float size = 0.f;
+#pragma unroll
+        for (int u = 0; u < COUNT; ++u) {
+            const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
+            const int64_t r = row0 + j, token = q0 + r / t.group, head = kv * t.group + r % t.group;
+            float dot = 0.f;
+            if (r < rows && d < p.head_dim) {
+                const float* __restrict__ o = p.O + token * p.ldo + head * p.head_dim + d;
+                f4 y = {0.f, 0.f, 0.f, 0.f};
+                if (t.vec) {
+                    y = *reinterpret_cast<const f4*>(o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < p.head_dim) y[e] = o[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(v[u][e], y[e], dot);
             }
-            dot += check;
-            dot += __shfl_xor(dot, 1, 64);
-            dot += __shfl_xor(dot, 2, 64);
-            if (!is_finite(dot)) dot = NAN;
-            size = is_finite(dot) ? fabsf(dot) : 0.f;
-            if ((threadIdx.x & 3) == 0) {
-                const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + j;
-                a.row_lse[at] = (dot - dot) - p.lse[head * p.q_rows + token] * LOG2E;  // NaN where D is
-                a.row_dot[at] = dot;
-            }
-        } else if ((threadIdx.x & 3) == 0) {
-            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + j;
-            a.row_lse[at] = -INFINITY;
-            a.row_dot[at] = 0.f;
+#pragma unroll
+            for (int m = 1; m < PER_ROW; m <<= 1) dot += __shfl_xor(dot, m, 64);
+            row_dots[j] = dot;  // (every lane of the row the same)
         }
-        size = wave_max_t(size);
-        if (lane == 0) wave_dot[wave] = size;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            const int64_t r = row0 + threadIdx.x, token = q0 + r / t.group, head = kv * t.group + r % t.group;
+            float dot = row_dots[threadIdx.x], lse = -INFINITY;
+            if (r < rows) {
+                if (!is_finite(dot) || bad[threadIdx.x] != 0) dot = NAN;
+                else size = fabsf(dot);
+                lse = (dot - dot) - p.lse[head * p.q_rows + token] * LOG2E;  // NaN where D is
+            }
+            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + threadIdx.x;
+            a.row_lse[at] = lse;
+            a.row_dot[at] = dot;
+            size = wave_max_t(size);
+            if (lane == 0) largest_dot = size;
+        }
     }
     __syncthreads();
     top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
@@ -227,8 +293,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
             h.bad[1] = (uint32_t)(marks >> 32);
             h.e_dot = NO_EXPONENT;
             if (t.dots) {
-                const float size = fmaxf(fmaxf(wave_dot[0], wave_dot[1]), fmaxf(wave_dot[2], wave_dot[3]));
-                if (size > 0.f) (void)frexpf(size, &h.e_dot);
+                if (largest_dot > 0.f) (void)frexpf(largest_dot, &h.e_dot);
             }
             t.header[(int64_t)blockIdx.x * p.kv_heads + kv] = h;
         }
@@ -323,6 +388,7 @@ struct ForwardArgs {
     const _Float16* v_columns;
     const Header* hk;
     const Header* hv;
+    const int4* order;
 };
 
 // A workgroup takes 128 packed rows of a key/value head, a wavefront 32 of them, a row per lane (of either half): S^T = K Q^T has
@@ -448,15 +514,17 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     __shared__ __attribute__((aligned(16))) ForwardTile<HDP, KEYS> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-    // all heads of a tile next to each other: consecutive workgroups go to different chiplets, so a chiplet's cache serves few
-    // heads; late tiles see the most keys and go first, so that the last ones to finish are short
+    // all heads of a group of rows next to each other: consecutive workgroups go to different chiplets, so a chiplet's cache
+    // serves few heads
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
-    int s;
-    int64_t inside, q0, n;
-    if (!find_tile(p, p.group, 128, (int64_t)(gridDim.x / (unsigned)p.kv_heads) - 1 - blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;
+    const int4 job = a.order[blockIdx.x / (unsigned)p.kv_heads];
+    const int s = job.x;
+    const int64_t inside = job.y;
+    if (s < 0) return;
+    int64_t q0, n;
     sequence_rows(p, s, &q0, &n);
     const int64_t rows = n * p.group, row0 = inside * 128 + 32 * wave, row = row0 + (lane & 31);
-    if (inside * 128 >= rows) return;
+    if (inside * 128 >= rows) return;  // (cannot be, with offsets that have not changed since the first launch)
     const float minus_one = opaque_minus_one();
     ForwardState<HDP> st;
     const int64_t token = q0 + row / p.group;
@@ -572,6 +640,10 @@ struct BackwardArgs {
     const _Float16* v_rows;
     const Header* hq; const Header* hg; const Header* hk; const Header* hv;
     const float* row_lse; const float* row_dot;
+    const int4* row_order; const int4* key_order;
+    int chunk_blocks, chunks;   // blocks of rows that a workgroup of the key kernel takes at most, and parts that makes of the longest
+    float* part;                // [chunk][token][kv][dK | dV][hd4] where a group of keys has more than one part
+    int hd4;                    // head_dim rounded up to whole vectors
 };
 
 __device__ __forceinline__ int wave_max_int(int v) {
@@ -727,17 +799,21 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     __shared__ __attribute__((aligned(16))) RowBlock<HDP> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-    const int kv = blockIdx.x % (unsigned)p.kv_heads;
-    int s;
-    int64_t inside, q0, n;
-    if (!find_tile(p, 1, 128, blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;  // (early keys are seen by the most rows: first)
+    const int kv = blockIdx.x % (unsigned)p.kv_heads, chunk = blockIdx.x / (unsigned)p.kv_heads % (unsigned)a.chunks;
+    const int4 job = a.key_order[blockIdx.x / (unsigned)p.kv_heads / (unsigned)a.chunks];
+    const int s = job.x;
+    const int64_t group_key0 = (int64_t)job.y * 128;
+    if (s < 0) return;
+    int64_t q0, n;
     sequence_rows(p, s, &q0, &n);
-    const int64_t group_key0 = inside * 128;
-    if (group_key0 >= n) return;
     const int64_t key0 = group_key0 + 32 * wave, rows = n * p.group;
     const bool active = key0 < n;
     const float minus_one = opaque_minus_one();
     const int64_t row_tile0 = first_tile(p, s, p.group, 64);
+    const int64_t all_first = group_key0 * p.group / 32, all_blocks = (rows + 31) / 32;
+    const int64_t first_block = all_first + (int64_t)chunk * a.chunk_blocks;
+    const int64_t blocks = first_block + a.chunk_blocks < all_blocks ? first_block + a.chunk_blocks : all_blocks;
+    if (first_block >= all_blocks) return;
     KeyState<HDP> st;
     {
         const int64_t tile_at = (first_tile(p, s, 1, 64) + (active ? key0 : group_key0) / 64) * p.kv_heads + kv;
@@ -747,7 +823,6 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
         st.e_k = a.hk[tile_at].e;
         st.e_v = a.hv[tile_at].e;
     }
-    const int64_t first_block = group_key0 * p.group / 32, blocks = (rows + 31) / 32;
     {
         int tq = NO_EXPONENT, tg = NO_EXPONENT, tt = 2 * NO_EXPONENT;
         for (int64_t tile = first_block / 2 + lane; tile < (blocks + 1) / 2; tile += 64) {
@@ -787,8 +862,49 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     }
     const int64_t key = key0 + (lane & 31);
     if (key >= n) return;
-    store_column<HDP>(p.dK + (q0 + key) * p.lddk + kv * (int64_t)p.head_dim, st.dk, p.scale, st.top_t - 1 + st.top_q - st.x_k, h, p.head_dim, p.vec_dkv);
-    store_column<HDP>(p.dV + (q0 + key) * p.lddv + kv * (int64_t)p.head_dim, st.dv, 1.f, st.top_g - st.x_v, h, p.head_dim, p.vec_dkv);
+    float* dst_k = p.dK + (q0 + key) * p.lddk + kv * (int64_t)p.head_dim;
+    float* dst_v = p.dV + (q0 + key) * p.lddv + kv * (int64_t)p.head_dim;
+    int width = p.head_dim;
+    bool vec = p.vec_dkv;
+    if (all_blocks - all_first > a.chunk_blocks) {
+        dst_k = a.part + ((chunk * p.q_rows + q0 + key) * p.kv_heads + kv) * (2 * a.hd4);
+        dst_v = dst_k + a.hd4;
+        width = a.hd4;  // (columns past the head dimension are zeros)
+        vec = true;
+    }
+    store_column<HDP>(dst_k, st.dk, p.scale, st.top_t - 1 + st.top_q - st.x_k, h, width, vec);
+    store_column<HDP>(dst_v, st.dv, 1.f, st.top_g - st.x_v, h, width, vec);
+}
+
+// Adds the parts of the groups of keys that have several, in their order.
+__global__ void __launch_bounds__(256) causal_split_join_kernel(const BackwardArgs a) {
+    const CausalArgs<float>& p = a.p;
+    const int kv = blockIdx.x % (unsigned)p.kv_heads;
+    const int4 job = a.key_order[blockIdx.x / (unsigned)p.kv_heads];
+    if (job.x < 0) return;
+    int64_t q0, n;
+    sequence_rows(p, job.x, &q0, &n);
+    const int64_t key0 = (int64_t)job.y * 128, total = (n * p.group + 31) / 32 - key0 * p.group / 32;
+    const int parts = (int)((total + a.chunk_blocks - 1) / a.chunk_blocks);
+    if (parts <= 1) return;
+    const int per_row = a.hd4 / 2;  // vectors of both gradients
+    for (int i = (int)(blockIdx.y * 256 + threadIdx.x); i < 128 * per_row; i += 256 * gridDim.y) {
+        const int64_t key = key0 + i / per_row;
+        const int c = i % per_row * 4;
+        if (key >= n) break;
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < parts; ++x) sum += *reinterpret_cast<const f4*>(a.part + ((x * p.q_rows + q0 + key) * p.kv_heads + kv) * (2 * a.hd4) + c);
+        const bool is_v = c >= a.hd4;
+        const int d = is_v ? c - a.hd4 : c;
+        float* dst = (is_v ? p.dV + (q0 + key) * p.lddv : p.dK + (q0 + key) * p.lddk) + kv * (int64_t)p.head_dim + d;
+        if (p.vec_dkv) {
+            *reinterpret_cast<f4*>(dst) = sum;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < p.head_dim) dst[e] = sum[e];
+        }
+    }
 }
 
 // Gradient of Q: 128 packed rows to a workgroup, a row per lane, Q and dO in registers; blocks of 32 keys of K (both forms) and V
@@ -851,11 +967,12 @@ __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const Backwa
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
-    int s;
-    int64_t inside, q0, n;
-    if (!find_tile(p, p.group, 128, (int64_t)(gridDim.x / (unsigned)p.kv_heads) - 1 - blockIdx.x / (unsigned)p.kv_heads, &s, &inside)) return;
+    const int4 job = a.row_order[blockIdx.x / (unsigned)p.kv_heads];
+    const int s = job.x;
+    if (s < 0) return;
+    int64_t q0, n;
     sequence_rows(p, s, &q0, &n);
-    const int64_t rows = n * p.group, group_row0 = inside * 128;
+    const int64_t rows = n * p.group, group_row0 = (int64_t)job.y * 128;
     if (group_row0 >= rows) return;
     const int64_t row0 = group_row0 + 32 * wave, row = row0 + (lane & 31);
     const bool active = row0 < rows;
@@ -926,6 +1043,13 @@ struct Carver {
     }
 };
 
+// Work is at most q_rows / 64 tiles: this many bits less of it tell ORDER_BINS - 1 kinds apart.
+inline int order_shift(int64_t q_rows) {
+    int shift = 0;
+    while ((q_rows / 64) >> shift >= ORDER_BINS - 1) ++shift;
+    return shift;
+}
+
 struct ForwardPlan {
     SplitArgs split;
     ForwardArgs main;
@@ -940,10 +1064,15 @@ ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
     _Float16* v = c.take<_Float16>((size_t)key_tiles * 256 * hdp);
     Header* hk = c.take<Header>((size_t)key_tiles * sizeof(Header));
     Header* hv = c.take<Header>((size_t)key_tiles * sizeof(Header));
+    const int64_t row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
+    f.split.order = c.take<int4>((size_t)row_groups * sizeof(int4));
+    f.split.order_slots[0] = (int)row_groups;
+    f.split.tensors = 2;
+    f.split.shift = order_shift(p.q_rows);
     f.split.p = p;
     f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, nullptr, hk, 0};
     f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, nullptr, v, hv, 0};
-    f.main = {p, k, v, hk, hv};
+    f.main = {p, k, v, hk, hv, f.split.order};
     f.bytes = c.used;
     return f;
 }
@@ -974,9 +1103,26 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, rows[1], columns[1], headers[1], 1};
     b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, rows[2], columns[2], headers[2], 0};
     b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, rows[3], columns[3], headers[3], 0};
+    const int64_t row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences);
+    b.split.order = c.take<int4>((size_t)(row_groups + key_groups) * sizeof(int4));
+    b.split.order_slots[0] = (int)row_groups;
+    b.split.order_slots[1] = (int)key_groups;
+    b.split.tensors = 4;
+    b.split.shift = order_shift(p.q_rows);
+    // Parts of the rows that see a group of keys.  If the sequences were equally long, 512 workgroups (two to a compute unit) would
+    // have this many blocks of rows each; half of it keeps the longest group from being what the others wait for.  At most 16 parts
+    // and 256 MB of them.
+    const int hd4 = (p.head_dim + 3) & ~3;
+    const int64_t part_bytes = p.q_rows * p.kv_heads * 2 * hd4 * 4, most_blocks = (p.q_rows * p.group + 31) / 32;
+    const int64_t most_parts = std::max<int64_t>(1, std::min<int64_t>(16, ((int64_t)256 << 20) / part_bytes));
+    const int64_t share = (int64_t)((double)p.q_rows * p.q_rows / p.sequences * p.group * p.kv_heads / (2.0 * 128 * 32 * 512));
+    const int64_t chunk = std::max<int64_t>({32, share / 2, (most_blocks + most_parts - 1) / most_parts});
+    const int chunks = (int)((most_blocks + chunk - 1) / chunk);
+    float* part = chunks > 1 ? c.take<float>((size_t)(part_bytes * chunks)) : nullptr;
     b.split.row_lse = lse;
     b.split.row_dot = dot;
-    b.main = {p, rows[0], columns[0], rows[1], columns[1], rows[2], columns[2], rows[3], headers[0], headers[1], headers[2], headers[3], lse, dot};
+    b.main = {p, rows[0], columns[0], rows[1], columns[1], rows[2], columns[2], rows[3], headers[0], headers[1], headers[2], headers[3], lse, dot,
+              b.split.order, b.split.order + row_groups, (int)chunk, chunks, part, hd4};
     b.bytes = c.used;
     return b;
 }
@@ -993,7 +1139,7 @@ hipError_t launch_causal_split_fwd(const CausalArgs<float>& p, void* workspace, 
     const ForwardPlan f = forward_plan(p, workspace);
     const int64_t key_slots = tile_slots(p.q_rows, 1, 64, p.sequences), slots = tile_slots(p.q_rows, p.group, 128, p.sequences);
     if (!grid_fits(key_slots, 256) || !grid_fits(slots * p.kv_heads, 256)) return hipErrorInvalidValue;
-    const dim3 split((unsigned)key_slots, p.kv_heads, 2), grid((unsigned)(slots * p.kv_heads)), block(256);
+    const dim3 split((unsigned)key_slots, p.kv_heads, 3), grid((unsigned)(slots * p.kv_heads)), block(256);
     switch (padded(p.head_dim)) {
         case 32:
             hipLaunchKernelGGL(causal_split_kernel<32>, split, block, 0, s, f.split);
@@ -1014,9 +1160,10 @@ hipError_t launch_causal_split_fwd(const CausalArgs<float>& p, void* workspace, 
 size_t causal_split_bwd_workspace_bytes(const CausalArgs<float>& p) { return backward_plan(p, nullptr).bytes; }
 
 template <int HDP>
-static void enqueue_backward(const BackwardPlan& b, dim3 split, dim3 key_grid, dim3 row_grid, hipStream_t s) {
+static void enqueue_backward(const BackwardPlan& b, dim3 split, unsigned key_groups, dim3 row_grid, hipStream_t s) {
     hipLaunchKernelGGL(causal_split_kernel<HDP>, split, dim3(256), 0, s, b.split);
-    hipLaunchKernelGGL(causal_split_bwd_kv_kernel<HDP>, key_grid, dim3(256), 0, s, b.main);
+    hipLaunchKernelGGL(causal_split_bwd_kv_kernel<HDP>, dim3(key_groups * b.main.chunks), dim3(256), 0, s, b.main);
+    if (b.main.chunks > 1) hipLaunchKernelGGL(causal_split_join_kernel, dim3(key_groups, HDP / 32), dim3(256), 0, s, b.main);
     hipLaunchKernelGGL(causal_split_bwd_q_kernel<HDP>, row_grid, dim3(256), 0, s, b.main);
 }
 
@@ -1024,12 +1171,13 @@ hipError_t launch_causal_split_bwd(const CausalArgs<float>& p, void* workspace, 
     const BackwardPlan b = backward_plan(p, workspace);
     const int64_t row_tiles = tile_slots(p.q_rows, p.group, 64, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences),
                   row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
-    if (!grid_fits(row_tiles, 256) || !grid_fits(row_groups * p.kv_heads, 256)) return hipErrorInvalidValue;
-    const dim3 split((unsigned)row_tiles, p.kv_heads, 4), key_grid((unsigned)(key_groups * p.kv_heads)), row_grid((unsigned)(row_groups * p.kv_heads));
+    if (!grid_fits(row_tiles, 256) || !grid_fits(row_groups * p.kv_heads, 256) || !grid_fits(key_groups * p.kv_heads * b.main.chunks, 256))
+        return hipErrorInvalidValue;
+    const dim3 split((unsigned)row_tiles, p.kv_heads, 5), row_grid((unsigned)(row_groups * p.kv_heads));
     switch (padded(p.head_dim)) {
-        case 32: enqueue_backward<32>(b, split, key_grid, row_grid, s); break;
-        case 64: enqueue_backward<64>(b, split, key_grid, row_grid, s); break;
-        default: enqueue_backward<128>(b, split, key_grid, row_grid, s); break;
+        case 32: enqueue_backward<32>(b, split, (unsigned)(key_groups * p.kv_heads), row_grid, s); break;
+        case 64: enqueue_backward<64>(b, split, (unsigned)(key_groups * p.kv_heads), row_grid, s); break;
+        default: enqueue_backward<128>(b, split, (unsigned)(key_groups * p.kv_heads), row_grid, s); break;
     }
     return hipGetLastError();
 }
