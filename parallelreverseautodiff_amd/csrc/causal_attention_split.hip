@@ -799,8 +799,11 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     __shared__ __attribute__((aligned(16))) RowBlock<HDP> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-    const int kv = blockIdx.x % (unsigned)p.kv_heads, chunk = blockIdx.x / (unsigned)p.kv_heads % (unsigned)a.chunks;
-    const int4 job = a.key_order[blockIdx.x / (unsigned)p.kv_heads / (unsigned)a.chunks];
+    // later parts exist for long groups only and are as large as a part gets: first.  (The parts of a group must not be neighbours:
+    // with consecutive workgroups on different chiplets, every second chiplet would only get parts that do not exist.)
+    const unsigned per_chunk = gridDim.x / (unsigned)a.chunks;
+    const int kv = blockIdx.x % (unsigned)p.kv_heads, chunk = a.chunks - 1 - (int)(blockIdx.x / per_chunk);
+    const int4 job = a.key_order[blockIdx.x % per_chunk / (unsigned)p.kv_heads];
     const int s = job.x;
     const int64_t group_key0 = (int64_t)job.y * 128;
     if (s < 0) return;
