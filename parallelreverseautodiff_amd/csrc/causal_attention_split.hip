@@ -15,11 +15,12 @@
 // accumulators of the column with it: forward that is the running maximum of the softmax, backward `fit`.
 //
 // Layout.  A first launch splits the operands and writes them in the order in which the 32 x 32 x 16 matrix instruction takes
-// its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the reduction; a fragment is
+// its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the head dimension; a fragment is
 // 1 KB, copied to LDS as it is and read back without bank conflicts.  Rows and columns past the end are zeros, so the
 // main kernels check no bounds.  Which element of the reduction sits where is free as long as both operands agree: the weights
-// come out of the first product with a column per lane and 4-row groups alternating between the lane halves, and the transposed
-// operands are written in that order, so weights go from one product into the next without leaving their lane.
+// come out of the first product with a column per lane and 4-row groups alternating between the lane halves, and the same
+// fragments, read across by the transposing LDS loads, take the rows in that order, so weights go from one product into the next
+// without leaving their lane and an operand is held once, whichever side it is needed from.
 //
 // A non-finite value is replaced by zero in the split operands and its row marked: where it is seen, scores (forward) or
 // lse / D (backward) are NaN.
@@ -108,17 +109,14 @@ __device__ __forceinline__ void mfma3(h8 a_hi, h8 a_lo, h8 b_hi, h8 b_lo, f16v& 
 __device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
 
 // ---- first launch: split operands ------------------------------------------------------------------------------------------
-// A block of 32 rows of a tile is 128 HDP bytes:
-//   rows form:        [plane][HDP / 16][lane][8]            row l % 32, columns 16 k + 8 (l / 32) + e
-//   transposed form:  [plane][HDP / 32][2][lane][8]         column 32 c + l % 32, rows acc_row(8 t + e, l / 32)
-// A tile is two blocks; tile and head (slot, kv) lie at (slot kv_heads + kv) 256 HDP bytes.
+// A block of 32 rows of a tile is 128 HDP bytes, [plane][HDP / 16][lane][8] with row l % 32 and columns 16 k + 8 (l / 32) + e in
+// lane l of fragment k.  A tile is two blocks; tile and head (slot, kv) lie at (slot kv_heads + kv) 256 HDP bytes.
 struct SplitSource {
     const float* src;
     int64_t ld;
     int group;         // heads per packed row group (1: keys)
     int vec;
-    _Float16* rows;    // nullptr: form not needed
-    _Float16* columns;
+    _Float16* split;
     Header* header;
     int dots;          // dO: D and lse of the rows as well
 };
@@ -309,29 +307,19 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     __syncthreads();
     const float minus_one = opaque_minus_one();
     const int64_t base = ((int64_t)blockIdx.x * p.kv_heads + kv) * (128 * HDP);  // halves
-    constexpr int FRAGS = HDP / 16;  // per block and plane, in either form
+    constexpr int FRAGS = HDP / 16;  // per block and plane
 #pragma unroll
     for (int u = 0; u < 2 * FRAGS * 64 / 256; ++u) {
         const int at = threadIdx.x + 256 * u, l = at & 63, f = (at >> 6) % FRAGS, block = (at >> 6) / FRAGS;
         const int64_t hi_at = base + (int64_t)(block * 2 * FRAGS + f) * 512 + l * 8, lo_at = hi_at + FRAGS * 512;
         float x[8];
         h8 hi[1], lo[1];
-        if (t.rows != nullptr) {
-            const float* __restrict__ row = tile + (32 * block + (l & 31)) * PITCH + 16 * f + 8 * (l >> 5);
+        const float* __restrict__ row = tile + (32 * block + (l & 31)) * PITCH + 16 * f + 8 * (l >> 5);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] = row[c];
-            split_regs<8>(x, minus_one, hi, lo);
-            *reinterpret_cast<h8*>(t.rows + hi_at) = hi[0];
-            *reinterpret_cast<h8*>(t.rows + lo_at) = lo[0];
-        }
-        if (t.columns != nullptr) {
-            const float* __restrict__ col = tile + 32 * block * PITCH + 32 * (f >> 1) + (l & 31);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) x[c] = col[acc_row(8 * (f & 1) + c, l >> 5) * PITCH];
-            split_regs<8>(x, minus_one, hi, lo);
-            *reinterpret_cast<h8*>(t.columns + hi_at) = hi[0];
-            *reinterpret_cast<h8*>(t.columns + lo_at) = lo[0];
-        }
+        for (int c = 0; c < 8; ++c) x[c] = row[c];
+        split_regs<8>(x, minus_one, hi, lo);
+        *reinterpret_cast<h8*>(t.split + hi_at) = hi[0];
+        *reinterpret_cast<h8*>(t.split + lo_at) = lo[0];
     }
 }
 
@@ -354,7 +342,7 @@ __device__ __forceinline__ void staged() {
 }
 __device__ __forceinline__ h8 frag(const _Float16* base, int f, int lane) { return *reinterpret_cast<const h8*>(base + f * 512 + lane * 8); }
 
-// acc[32 rows x 32 columns] = A . B over the head dimension: a block's rows form against a column per lane.
+// acc[32 rows x 32 columns] = A . B over the head dimension: a block against a column per lane.
 template <int HDP>
 __device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b_hi)[HDP / 16], const h8 (&b_lo)[HDP / 16], int lane, f16v& acc) {
 #pragma unroll
@@ -362,13 +350,30 @@ __device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b
 #pragma unroll
     for (int k = 0; k < HDP / 16; ++k) mfma3(frag(block, k, lane), frag(block, HDP / 16 + k, lane), b_hi[k], b_lo[k], acc);
 }
-// out[HDP x 32 columns] += A^T . W: a block's transposed form against the weights of its 32 rows.
+// Fragment of a block read across, from LDS: lane l gets column 32 c + l % 32, rows acc_row(8 t + e, l / 32).  One transposing load
+// gives each 16 lanes 4 rows of 16 columns: its lane i asks for columns 4 (i % 4) .. + 3 of row i / 4 and receives column i.
+typedef short s4 __attribute__((ext_vector_type(4)));
+struct Across {
+    int at;  // of the lane, in halves
+    __device__ __forceinline__ explicit Across(int lane) {
+        const int i = lane & 15;
+        at = ((lane >> 4) & 1) * 512 + (4 * (lane >> 5) + (i >> 2) + 32 * ((i >> 1) & 1)) * 8 + (i & 1) * 4;
+    }
+    __device__ __forceinline__ h8 frag(const _Float16* plane, int c, int t) const {
+        typedef __attribute__((address_space(3))) s4* lds;
+        const _Float16* first = plane + at + c * 1024 + t * 128;
+        const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)first), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(first + 64));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    }
+};
+// out[HDP x 32 columns] += A^T . W: a block read across against the weights of its 32 rows.
 template <int HDP>
-__device__ __forceinline__ void columns_product(const _Float16* block, const h8 (&w_hi)[2], const h8 (&w_lo)[2], int lane, f16v (&out)[HDP / 32]) {
+__device__ __forceinline__ void columns_product(const _Float16* block, const h8 (&w_hi)[2], const h8 (&w_lo)[2], const Across& across, f16v (&out)[HDP / 32]) {
 #pragma unroll
     for (int c = 0; c < HDP / 32; ++c)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) mfma3(frag(block, 2 * c + t, lane), frag(block, HDP / 16 + 2 * c + t, lane), w_hi[t], w_lo[t], out[c]);
+        for (int t = 0; t < 2; ++t) mfma3(across.frag(block, c, t), across.frag(block + 32 * HDP, c, t), w_hi[t], w_lo[t], out[c]);
 }
 
 // Over the two lanes that share a column (lane halves).
@@ -384,8 +389,8 @@ __device__ __forceinline__ float sum_halves(float x) {
 // ---- forward ----------------------------------------------------------------------------------------------------------------
 struct ForwardArgs {
     CausalArgs<float> p;
-    const _Float16* k_rows;
-    const _Float16* v_columns;
+    const _Float16* k;
+    const _Float16* v;
     const Header* hk;
     const Header* hv;
     const int4* order;
@@ -428,8 +433,8 @@ __device__ __forceinline__ void forward_stage(const ForwardArgs& a, ForwardTile<
     const int64_t tile_at = (tile0 + k0 / 64) * a.p.kv_heads + kv;
     const int64_t at = tile_at * (128 * HDP) + (k0 / KEYS % (64 / KEYS)) * (2 * KEYS * HDP);
     notes.ask(a.hk, a.hv, tile_at);
-    stage<4 * KEYS * HDP, 4>(a.k_rows + at, &t.k[0][0], wave, lane);
-    stage<4 * KEYS * HDP, 4>(a.v_columns + at, &t.v[0][0], wave, lane);
+    stage<4 * KEYS * HDP, 4>(a.k + at, &t.k[0][0], wave, lane);
+    stage<4 * KEYS * HDP, 4>(a.v + at, &t.v[0][0], wave, lane);
 }
 
 template <int HDP>
@@ -445,6 +450,7 @@ template <int HDP, int KEYS>
 __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int64_t k0, int64_t wave_first, float minus_one, int lane, ForwardState<HDP>& st) {
     constexpr int NB = KEYS / 32;
     const int h = lane >> 5;
+    const Across across(lane);
     f16v s[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) rows_product<HDP>(&t.k[b][0], st.q_hi, st.q_lo, lane, s[b]);
@@ -505,7 +511,7 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
     for (int b = 0; b < NB; ++b) {
         h8 hi[2], lo[2];
         split_regs<16>(w[b], minus_one, hi, lo);
-        columns_product<HDP>(&t.v[b][0], hi, lo, lane, st.o);
+        columns_product<HDP>(&t.v[b][0], hi, lo, across, st.o);
     }
 }
 
@@ -634,10 +640,8 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
 // ---- backward ---------------------------------------------------------------------------------------------------------------
 struct BackwardArgs {
     CausalArgs<float> p;
-    const _Float16* q_rows; const _Float16* q_columns;
-    const _Float16* g_rows; const _Float16* g_columns;   // dO
-    const _Float16* k_rows; const _Float16* k_columns;
-    const _Float16* v_rows;
+    const _Float16* q; const _Float16* g;   // g: dO
+    const _Float16* k; const _Float16* v;
     const Header* hq; const Header* hg; const Header* hk; const Header* hv;
     const float* row_lse; const float* row_dot;
     const int4* row_order; const int4* key_order;
@@ -710,11 +714,11 @@ __device__ __forceinline__ void store_column(float* __restrict__ dst, const f16v
 }
 
 // Gradients of K and V.  A workgroup owns 128 keys of a key/value head, a wavefront 32 of them, a key per lane, with their K and V
-// in registers; blocks of 32 packed rows (all heads of the group) of Q and dO pass through LDS in both forms.  S = Q K^T and
+// in registers; blocks of 32 packed rows (all heads of the group) of Q and dO pass through LDS.  S = Q K^T and
 // dP = dO V^T come out with a key per lane, so P and dS go straight into dV^T += dO^T P and dK^T += Q^T dS.
 template <int HDP>
 struct RowBlock {
-    _Float16 q[64 * HDP], g[64 * HDP], q_columns[64 * HDP], g_columns[64 * HDP];
+    _Float16 q[64 * HDP], g[64 * HDP];
     float lse[32], dot[32];
 };
 struct RowNotes {
@@ -726,10 +730,8 @@ __device__ __forceinline__ void row_stage(const BackwardArgs& a, RowBlock<HDP>& 
     const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
     notes.e_q = a.hq[tile_at].e;
     notes.e_g = a.hg[tile_at].e;
-    stage<128 * HDP, 4>(a.q_rows + at, t.q, wave, lane);
-    stage<128 * HDP, 4>(a.g_rows + at, t.g, wave, lane);
-    stage<128 * HDP, 4>(a.q_columns + at, t.q_columns, wave, lane);
-    stage<128 * HDP, 4>(a.g_columns + at, t.g_columns, wave, lane);
+    stage<128 * HDP, 4>(a.q + at, t.q, wave, lane);
+    stage<128 * HDP, 4>(a.g + at, t.g, wave, lane);
     if (wave == 0) {
         const float* src = (lane < 32 ? a.row_lse : a.row_dot) + tile_at * 64 + (block & 1) * 32 + (lane & 31);
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)t.lse, 4, 0, 0);
@@ -750,6 +752,7 @@ template <int HDP>
 __device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes& notes, int64_t row0, int64_t wave_last, float factor, float minus_one, int lane,
                                           KeyState<HDP>& st) {
     const int h = lane >> 5;
+    const Across across(lane);
     f16v s, dp;
     rows_product<HDP>(t.q, st.k_hi, st.k_lo, lane, s);
     rows_product<HDP>(t.g, st.v_hi, st.v_lo, lane, dp);
@@ -788,10 +791,10 @@ __device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes
     }
     h8 hi[2], lo[2];
     split_regs<16>(w, minus_one, hi, lo);
-    columns_product<HDP>(t.g_columns, hi, lo, lane, st.dv);
+    columns_product<HDP>(t.g, hi, lo, across, st.dv);
     fit(ds, st.x_k, st.dk);
     split_regs<16>(ds, minus_one, hi, lo);
-    columns_product<HDP>(t.q_columns, hi, lo, lane, st.dk);
+    columns_product<HDP>(t.q, hi, lo, across, st.dk);
 }
 
 template <int HDP>
@@ -821,8 +824,8 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     {
         const int64_t tile_at = (first_tile(p, s, 1, 64) + (active ? key0 : group_key0) / 64) * p.kv_heads + kv;
         const int64_t at = tile_at * (128 * HDP) + (active ? key0 / 32 % 2 : 0) * (64 * HDP);
-        load_fragments<HDP>(a.k_rows + at, lane, st.k_hi, st.k_lo);
-        load_fragments<HDP>(a.v_rows + at, lane, st.v_hi, st.v_lo);
+        load_fragments<HDP>(a.k + at, lane, st.k_hi, st.k_lo);
+        load_fragments<HDP>(a.v + at, lane, st.v_hi, st.v_lo);
         st.e_k = a.hk[tile_at].e;
         st.e_v = a.hv[tile_at].e;
     }
@@ -910,11 +913,11 @@ __global__ void __launch_bounds__(256) causal_split_join_kernel(const BackwardAr
     }
 }
 
-// Gradient of Q: 128 packed rows to a workgroup, a row per lane, Q and dO in registers; blocks of 32 keys of K (both forms) and V
-// pass through LDS.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
+// Gradient of Q: 128 packed rows to a workgroup, a row per lane, Q and dO in registers; blocks of 32 keys of K and V pass
+// through LDS.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
 template <int HDP>
 struct KeyBlock {
-    _Float16 k[64 * HDP], v[64 * HDP], k_columns[64 * HDP];
+    _Float16 k[64 * HDP], v[64 * HDP];
 };
 struct BlockNotes {
     int e_k, e_v;
@@ -925,9 +928,8 @@ __device__ __forceinline__ void key_stage(const BackwardArgs& a, KeyBlock<HDP>& 
     const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
     notes.e_k = a.hk[tile_at].e;
     notes.e_v = a.hv[tile_at].e;
-    stage<128 * HDP, 4>(a.k_rows + at, t.k, wave, lane);
-    stage<128 * HDP, 4>(a.v_rows + at, t.v, wave, lane);
-    stage<128 * HDP, 4>(a.k_columns + at, t.k_columns, wave, lane);
+    stage<128 * HDP, 4>(a.k + at, t.k, wave, lane);
+    stage<128 * HDP, 4>(a.v + at, t.v, wave, lane);
 }
 
 template <int HDP>
@@ -944,6 +946,7 @@ template <int HDP>
 __device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNotes& notes, int64_t k0, int64_t wave_first, float factor, float minus_one, int lane,
                                           RowState<HDP>& st) {
     const int h = lane >> 5;
+    const Across across(lane);
     f16v s, dp;
     rows_product<HDP>(t.k, st.q_hi, st.q_lo, lane, s);
     rows_product<HDP>(t.v, st.g_hi, st.g_lo, lane, dp);
@@ -961,7 +964,7 @@ __device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNot
     fit(ds, st.x_q, st.dq);
     h8 hi[2], lo[2];
     split_regs<16>(ds, minus_one, hi, lo);
-    columns_product<HDP>(t.k_columns, hi, lo, lane, st.dq);
+    columns_product<HDP>(t.k, hi, lo, across, st.dq);
 }
 
 template <int HDP>
@@ -987,8 +990,8 @@ __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const Backwa
     {
         const int64_t from = active ? row0 : group_row0;
         const int64_t tile_at = (first_tile(p, s, p.group, 64) + from / 64) * p.kv_heads + kv, at = tile_at * (128 * HDP) + (from / 32 % 2) * (64 * HDP);
-        load_fragments<HDP>(a.q_rows + at, lane, st.q_hi, st.q_lo);
-        load_fragments<HDP>(a.g_rows + at, lane, st.g_hi, st.g_lo);
+        load_fragments<HDP>(a.q + at, lane, st.q_hi, st.q_lo);
+        load_fragments<HDP>(a.g + at, lane, st.g_hi, st.g_lo);
         st.lse = a.row_lse[tile_at * 64 + from % 64 + (lane & 31)];
         st.dot = a.row_dot[tile_at * 64 + from % 64 + (lane & 31)];
         st.e_q = __builtin_amdgcn_readfirstlane(a.hq[tile_at].e);
@@ -1073,8 +1076,8 @@ ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
     f.split.tensors = 2;
     f.split.shift = order_shift(p.q_rows);
     f.split.p = p;
-    f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, nullptr, hk, 0};
-    f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, nullptr, v, hv, 0};
+    f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, hk, 0};
+    f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, v, hv, 0};
     f.main = {p, k, v, hk, hv, f.split.order};
     f.bytes = c.used;
     return f;
@@ -1090,22 +1093,20 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     const int64_t key_tiles = tile_slots(p.q_rows, 1, 64, p.sequences) * p.kv_heads, row_tiles = tile_slots(p.q_rows, p.group, 64, p.sequences) * p.kv_heads;
     Carver c{static_cast<char*>(workspace)};
     BackwardPlan b{};
-    _Float16* rows[4];
-    _Float16* columns[4];
+    _Float16* split[4];
     Header* headers[4];
     for (int i = 0; i < 4; ++i) {  // Q, dO, K, V
         const int64_t tiles = i < 2 ? row_tiles : key_tiles;
-        rows[i] = c.take<_Float16>((size_t)tiles * 256 * hdp);
-        columns[i] = i < 3 ? c.take<_Float16>((size_t)tiles * 256 * hdp) : nullptr;
+        split[i] = c.take<_Float16>((size_t)tiles * 256 * hdp);
         headers[i] = c.take<Header>((size_t)tiles * sizeof(Header));
     }
     float* lse = c.take<float>((size_t)row_tiles * 64 * 4);
     float* dot = c.take<float>((size_t)row_tiles * 64 * 4);
     b.split.p = p;
-    b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, rows[0], columns[0], headers[0], 0};
-    b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, rows[1], columns[1], headers[1], 1};
-    b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, rows[2], columns[2], headers[2], 0};
-    b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, rows[3], columns[3], headers[3], 0};
+    b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, split[0], headers[0], 0};
+    b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, split[1], headers[1], 1};
+    b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, split[2], headers[2], 0};
+    b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, split[3], headers[3], 0};
     const int64_t row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences);
     b.split.order = c.take<int4>((size_t)(row_groups + key_groups) * sizeof(int4));
     b.split.order_slots[0] = (int)row_groups;
@@ -1124,7 +1125,7 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     float* part = chunks > 1 ? c.take<float>((size_t)(part_bytes * chunks)) : nullptr;
     b.split.row_lse = lse;
     b.split.row_dot = dot;
-    b.main = {p, rows[0], columns[0], rows[1], columns[1], rows[2], columns[2], rows[3], headers[0], headers[1], headers[2], headers[3], lse, dot,
+    b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], lse, dot,
               b.split.order, b.split.order + row_groups, (int)chunk, chunks, part, hd4};
     b.bytes = c.used;
     return b;
