@@ -27,6 +27,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace prad {
 
@@ -342,13 +343,61 @@ __device__ __forceinline__ void staged() {
 }
 __device__ __forceinline__ h8 frag(const _Float16* base, int f, int lane) { return *reinterpret_cast<const h8*>(base + f * 512 + lane * 8); }
 
-// acc[32 rows x 32 columns] = A . B over the head dimension: a block against a column per lane.
-template <int HDP>
-__device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b_hi)[HDP / 16], const h8 (&b_lo)[HDP / 16], int lane, f16v& acc) {
+// Asks the scheduler for this order of instructions in a basic block: `n` LDS reads, `n` matrix instructions.  Without it the
+// fragments are read right before they are used and every step waits for LDS.
+__device__ __forceinline__ void then_reads(std::integral_constant<int, 2>) { __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+__device__ __forceinline__ void then_reads(std::integral_constant<int, 4>) { __builtin_amdgcn_sched_group_barrier(0x100, 4, 0); }
+__device__ __forceinline__ void then_products() { __builtin_amdgcn_sched_group_barrier(0x008, 3, 0); }
+
+// A chain of STEPS products of fragments, the fragments of a step read while the step before it multiplies.  read(i, hi, lo),
+// multiply(i, hi, lo).
+template <int STEPS, int READS, typename Read, typename Multiply>
+__device__ __forceinline__ void product_chain(Read read, Multiply multiply) {
+    h8 hi[2], lo[2];
+    read(0, hi[0], lo[0]);
+    then_reads(std::integral_constant<int, READS>());
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        if (i + 1 < STEPS) {
+            read(i + 1, hi[(i + 1) & 1], lo[(i + 1) & 1]);
+            then_reads(std::integral_constant<int, READS>());
+        }
+        multiply(i, hi[i & 1], lo[i & 1]);
+        then_products();
+    }
+}
+__device__ __forceinline__ void clear(f16v& acc) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-#pragma unroll
-    for (int k = 0; k < HDP / 16; ++k) mfma3(frag(block, k, lane), frag(block, HDP / 16 + k, lane), b_hi[k], b_lo[k], acc);
+}
+// first, second [32 rows x 32 columns] = A . B over the head dimension: two blocks, each against a column per lane.
+template <int HDP>
+__device__ __forceinline__ void rows_products(const _Float16* first_block, const h8 (&f_hi)[HDP / 16], const h8 (&f_lo)[HDP / 16], f16v& first,
+                                              const _Float16* second_block, const h8 (&s_hi)[HDP / 16], const h8 (&s_lo)[HDP / 16], f16v& second, int lane) {
+    constexpr int K = HDP / 16;
+    clear(first);
+    clear(second);
+    product_chain<2 * K, 2>(
+        [&](int i, h8& hi, h8& lo) {
+            const _Float16* block = i < K ? first_block : second_block;
+            hi = frag(block, i % K, lane);
+            lo = frag(block, K + i % K, lane);
+        },
+        [&](int i, h8 hi, h8 lo) {
+            if (i < K) mfma3(hi, lo, f_hi[i % K], f_lo[i % K], first);
+            else mfma3(hi, lo, s_hi[i % K], s_lo[i % K], second);
+        });
+}
+template <int HDP>
+__device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b_hi)[HDP / 16], const h8 (&b_lo)[HDP / 16], f16v& acc, int lane) {
+    constexpr int K = HDP / 16;
+    clear(acc);
+    product_chain<K, 2>(
+        [&](int i, h8& hi, h8& lo) {
+            hi = frag(block, i, lane);
+            lo = frag(block, K + i, lane);
+        },
+        [&](int i, h8 hi, h8 lo) { mfma3(hi, lo, b_hi[i], b_lo[i], acc); });
 }
 // Fragment of a block read across, from LDS: lane l gets column 32 c + l % 32, rows acc_row(8 t + e, l / 32).  One transposing load
 // gives each 16 lanes 4 rows of 16 columns: its lane i asks for columns 4 (i % 4) .. + 3 of row i / 4 and receives column i.
@@ -370,10 +419,12 @@ struct Across {
 // out[HDP x 32 columns] += A^T . W: a block read across against the weights of its 32 rows.
 template <int HDP>
 __device__ __forceinline__ void columns_product(const _Float16* block, const h8 (&w_hi)[2], const h8 (&w_lo)[2], const Across& across, f16v (&out)[HDP / 32]) {
-#pragma unroll
-    for (int c = 0; c < HDP / 32; ++c)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) mfma3(across.frag(block, c, t), across.frag(block + 32 * HDP, c, t), w_hi[t], w_lo[t], out[c]);
+    product_chain<HDP / 16, 4>(
+        [&](int i, h8& hi, h8& lo) {
+            hi = across.frag(block, i / 2, i % 2);
+            lo = across.frag(block + 32 * HDP, i / 2, i % 2);
+        },
+        [&](int i, h8 hi, h8 lo) { mfma3(hi, lo, w_hi[i % 2], w_lo[i % 2], out[i / 2]); });
 }
 
 // Over the two lanes that share a column (lane halves).
@@ -406,23 +457,17 @@ struct ForwardTile {
     _Float16 v[BLOCKS][64 * HDP];
 };
 
-// What the headers of a tile of keys say; asked for before the copies of the tile are, so that no wait for it is a wait for them.
+// What the headers of a tile of keys say.  They are asked for with the copies of the tile and looked at (`uniform`) once those have
+// arrived: touching them earlier would wait for the copies.
 struct KeyNotes {
-    int e_k, e_v;
-    uint32_t bad[2];
-    __device__ __forceinline__ void ask(const Header* __restrict__ hk, const Header* __restrict__ hv, int64_t at) {
-        e_k = hk[at].e;
-        e_v = hv[at].e;
-        bad[0] = hk[at].bad[0] | hv[at].bad[0];
-        bad[1] = hk[at].bad[1] | hv[at].bad[1];
-    }
+    Header k, v;
     // the same value in every lane: to scalar registers
     __device__ __forceinline__ KeyNotes uniform() const {
         KeyNotes n;
-        n.e_k = __builtin_amdgcn_readfirstlane(e_k);
-        n.e_v = __builtin_amdgcn_readfirstlane(e_v);
-        n.bad[0] = __builtin_amdgcn_readfirstlane(bad[0]);
-        n.bad[1] = __builtin_amdgcn_readfirstlane(bad[1]);
+        n.k.e = __builtin_amdgcn_readfirstlane(k.e);
+        n.v.e = __builtin_amdgcn_readfirstlane(v.e);
+        n.k.bad[0] = __builtin_amdgcn_readfirstlane(k.bad[0] | v.bad[0]);
+        n.k.bad[1] = __builtin_amdgcn_readfirstlane(k.bad[1] | v.bad[1]);
         return n;
     }
 };
@@ -432,7 +477,8 @@ __device__ __forceinline__ void forward_stage(const ForwardArgs& a, ForwardTile<
                                               int lane) {
     const int64_t tile_at = (tile0 + k0 / 64) * a.p.kv_heads + kv;
     const int64_t at = tile_at * (128 * HDP) + (k0 / KEYS % (64 / KEYS)) * (2 * KEYS * HDP);
-    notes.ask(a.hk, a.hv, tile_at);
+    notes.k = a.hk[tile_at];
+    notes.v = a.hv[tile_at];
     stage<4 * KEYS * HDP, 4>(a.k + at, &t.k[0][0], wave, lane);
     stage<4 * KEYS * HDP, 4>(a.v + at, &t.v[0][0], wave, lane);
 }
@@ -452,18 +498,18 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
     const int h = lane >> 5;
     const Across across(lane);
     f16v s[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) rows_product<HDP>(&t.k[b][0], st.q_hi, st.q_lo, lane, s[b]);
-    const float c = pow2(st.e_row + notes.e_k);
+    if constexpr (NB == 2) rows_products<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], &t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
+    else rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
+    const float c = pow2(st.e_row + notes.k.e);
     // masks and marks: only where some row does not see all the keys, or some key holds a non-finite value
-    if (k0 + KEYS - 1 > wave_first || (notes.bad[0] | notes.bad[1]) != 0) {
+    if (k0 + KEYS - 1 > wave_first || (notes.k.bad[0] | notes.k.bad[1]) != 0) {
         const int part = (int)(k0 / KEYS % (64 / KEYS));
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int j = 32 * b + acc_row(r, h), bit = part * KEYS + j;
-                const bool marked = (notes.bad[bit >> 5] >> (bit & 31)) & 1;
+                const bool marked = (notes.k.bad[bit >> 5] >> (bit & 31)) & 1;
                 s[b][r] = k0 + j > st.last ? -INFINITY : marked ? NAN : s[b][r];
             }
     }
@@ -476,7 +522,7 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
     // The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach 2^6 2^8, and the
     // accumulators are rarely rescaled.  (No key seen yet: m = -inf, and a top of -inf keeps the weights at 0.)
     const bool raise = top > st.m + 6.f;
-    const int e_v = notes.e_v > st.e_v ? notes.e_v : st.e_v;
+    const int e_v = notes.v.e > st.e_v ? notes.v.e : st.e_v;
     if (__ballot(raise) != 0 || e_v != st.e_v) {
         const float m = raise ? top : st.m;
         const float f = raise ? __builtin_amdgcn_exp2f(st.m - m) : 1.f;  // (m = -inf before: 0)
@@ -500,8 +546,8 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
             sum[r & 3] += w[b][r];
         }
     st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (notes.e_v != st.e_v) {  // a tile of smaller values: its weights carry the ratio
-        const float f = pow2(notes.e_v - st.e_v);
+    if (notes.v.e != st.e_v) {  // a tile of smaller values: its weights carry the ratio
+        const float f = pow2(notes.v.e - st.e_v);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -754,8 +800,7 @@ __device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
-    rows_product<HDP>(t.q, st.k_hi, st.k_lo, lane, s);
-    rows_product<HDP>(t.g, st.v_hi, st.v_lo, lane, dp);
+    rows_products<HDP>(t.q, st.k_hi, st.k_lo, s, t.g, st.v_hi, st.v_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
     const int e_ratio = notes.e_q - st.top_q;
     const float x_v = (float)st.x_v;
@@ -948,8 +993,7 @@ __device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNot
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
-    rows_product<HDP>(t.k, st.q_hi, st.q_lo, lane, s);
-    rows_product<HDP>(t.v, st.g_hi, st.g_lo, lane, dp);
+    rows_products<HDP>(t.k, st.q_hi, st.q_lo, s, t.v, st.g_hi, st.g_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, st.e_q + notes.e_k);
     const int e_ratio = notes.e_k - st.top_k;
     const int e_one = 1 - st.top_t + e_ratio + st.x_q;
