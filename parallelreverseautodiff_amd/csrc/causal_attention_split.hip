@@ -128,8 +128,7 @@ struct SplitArgs {
     int4* order;       // schedules for the main kernels, see below
     int order_slots[2];
     int shift;
-    float* row_lse;    // [slot][kv][64]: -lse log2 e, -inf for a row that is not there
-    float* row_dot;    // D
+    float* row_notes;  // [slot][kv][2][64]: -lse log2 e (-inf for a row that is not there), then D
 };
 
 // The groups of 128 packed rows (which = 0) or 128 keys (1) of all sequences as (sequence, number inside it), those with the most
@@ -269,9 +268,9 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
                 else size = fabsf(dot);
                 lse = (dot - dot) - p.lse[head * p.q_rows + token] * LOG2E;  // NaN where D is
             }
-            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 64 + threadIdx.x;
-            a.row_lse[at] = lse;
-            a.row_dot[at] = dot;
+            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 128 + threadIdx.x;
+            a.row_notes[at] = lse;
+            a.row_notes[at + 64] = dot;
             size = wave_max_t(size);
             if (lane == 0) largest_dot = size;
         }
@@ -325,16 +324,19 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
 }
 
 // ---- staging ----------------------------------------------------------------------------------------------------------------
-// Copies BYTES of split operands to LDS without passing through registers: 1 KB per instruction and wavefront.
+// Copies BYTES of split operands to LDS without passing through registers: 1 KB per instruction and wavefront.  As buffer loads:
+// their flat form would count as an LDS access to the compiler, which then waits for all LDS reads wherever it waits for one.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+}
 template <int BYTES, int WAVES>
 __device__ __forceinline__ void stage(const _Float16* __restrict__ src, _Float16* dst, int wave, int lane) {
     static_assert(BYTES % (1024 * WAVES) == 0, "whole rounds");
+    const __amdgpu_buffer_rsrc_t from = buffer_of(src, BYTES);
 #pragma unroll
-    for (int i = 0; i < BYTES / 1024 / WAVES; ++i) {
-        const int at = (i * WAVES + wave) * 512;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + at + lane * 8),
-                                         (__attribute__((address_space(3))) void*)(dst + at), 16, 0, 0);
-    }
+    for (int i = 0; i < BYTES / 1024 / WAVES; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(dst + (i * WAVES + wave) * 512), 16, lane * 16,
+                                                 (i * WAVES + wave) * 1024, 0, 0);
 }
 // The copies of every wavefront have arrived, and every wavefront is done with what they replace next.
 __device__ __forceinline__ void staged() {
@@ -689,7 +691,7 @@ struct BackwardArgs {
     const _Float16* q; const _Float16* g;   // g: dO
     const _Float16* k; const _Float16* v;
     const Header* hq; const Header* hg; const Header* hk; const Header* hv;
-    const float* row_lse; const float* row_dot;
+    const float* row_notes;
     const int4* row_order; const int4* key_order;
     int chunk_blocks, chunks;   // blocks of rows that a workgroup of the key kernel takes at most, and parts that makes of the longest
     float* part;                // [chunk][token][kv][dK | dV][hd4] where a group of keys has more than one part
@@ -779,8 +781,9 @@ __device__ __forceinline__ void row_stage(const BackwardArgs& a, RowBlock<HDP>& 
     stage<128 * HDP, 4>(a.q + at, t.q, wave, lane);
     stage<128 * HDP, 4>(a.g + at, t.g, wave, lane);
     if (wave == 0) {
-        const float* src = (lane < 32 ? a.row_lse : a.row_dot) + tile_at * 64 + (block & 1) * 32 + (lane & 31);
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)t.lse, 4, 0, 0);
+        const __amdgpu_buffer_rsrc_t from = buffer_of(a.row_notes + tile_at * 128, 512);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)t.lse, 4, (lane < 32 ? 0 : 256) + (lane & 31) * 4,
+                                                 (int)(block & 1) * 128, 0, 0);
     }
 }
 
@@ -1036,8 +1039,8 @@ __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const Backwa
         const int64_t tile_at = (first_tile(p, s, p.group, 64) + from / 64) * p.kv_heads + kv, at = tile_at * (128 * HDP) + (from / 32 % 2) * (64 * HDP);
         load_fragments<HDP>(a.q + at, lane, st.q_hi, st.q_lo);
         load_fragments<HDP>(a.g + at, lane, st.g_hi, st.g_lo);
-        st.lse = a.row_lse[tile_at * 64 + from % 64 + (lane & 31)];
-        st.dot = a.row_dot[tile_at * 64 + from % 64 + (lane & 31)];
+        st.lse = a.row_notes[tile_at * 128 + from % 64 + (lane & 31)];
+        st.dot = a.row_notes[tile_at * 128 + 64 + from % 64 + (lane & 31)];
         st.e_q = __builtin_amdgcn_readfirstlane(a.hq[tile_at].e);
         st.e_g = __builtin_amdgcn_readfirstlane(a.hg[tile_at].e);
         int tk = NO_EXPONENT, tv = NO_EXPONENT;
@@ -1144,8 +1147,7 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
         split[i] = c.take<_Float16>((size_t)tiles * 256 * hdp);
         headers[i] = c.take<Header>((size_t)tiles * sizeof(Header));
     }
-    float* lse = c.take<float>((size_t)row_tiles * 64 * 4);
-    float* dot = c.take<float>((size_t)row_tiles * 64 * 4);
+    float* notes = c.take<float>((size_t)row_tiles * 128 * 4);
     b.split.p = p;
     b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, split[0], headers[0], 0};
     b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, split[1], headers[1], 1};
@@ -1167,9 +1169,8 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     const int64_t chunk = std::max<int64_t>({32, share / 2, (most_blocks + most_parts - 1) / most_parts});
     const int chunks = (int)((most_blocks + chunk - 1) / chunk);
     float* part = chunks > 1 ? c.take<float>((size_t)(part_bytes * chunks)) : nullptr;
-    b.split.row_lse = lse;
-    b.split.row_dot = dot;
-    b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], lse, dot,
+    b.split.row_notes = notes;
+    b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], notes,
               b.split.order, b.split.order + row_groups, (int)chunk, chunks, part, hd4};
     b.bytes = c.used;
     return b;
