@@ -89,6 +89,9 @@ __device__ __forceinline__ float opaque_minus_one() {
     asm("" : "+s"(m));
     return m;
 }
+// Values are formed before this point: the compiler would otherwise move them past the next branch, towards their use and away
+// from the matrix instructions they are meant to run beside.
+__device__ __forceinline__ void keep_here(h8 (&hi)[2], h8 (&lo)[2]) { asm volatile("" : "+v"(hi[0]), "+v"(hi[1]), "+v"(lo[0]), "+v"(lo[1])); }
 template <int N>
 __device__ __forceinline__ void split_regs(const float (&x)[N], float minus_one, h8 (&hi)[N / 8], h8 (&lo)[N / 8]) {
 #pragma unroll
@@ -352,8 +355,9 @@ __device__ __forceinline__ void then_reads(std::integral_constant<int, 4>) { __b
 __device__ __forceinline__ void then_products() { __builtin_amdgcn_sched_group_barrier(0x008, 3, 0); }
 
 // A chain of STEPS products of fragments, the fragments of a step read while the step before it multiplies.  read(i, hi, lo),
-// multiply(i, hi, lo).
-template <int STEPS, int READS, typename Read, typename Multiply>
+// multiply(i, hi, lo).  BESIDE: vector instructions of the same basic block that do not depend on the chain go between its
+// matrix instructions.
+template <int STEPS, int READS, bool BESIDE = false, typename Read, typename Multiply>
 __device__ __forceinline__ void product_chain(Read read, Multiply multiply) {
     h8 hi[2], lo[2];
     read(0, hi[0], lo[0]);
@@ -365,7 +369,16 @@ __device__ __forceinline__ void product_chain(Read read, Multiply multiply) {
             then_reads(std::integral_constant<int, READS>());
         }
         multiply(i, hi[i & 1], lo[i & 1]);
-        then_products();
+        if constexpr (BESIDE) {
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+            }
+        } else {
+            then_products();
+        }
     }
 }
 __device__ __forceinline__ void clear(f16v& acc) {
@@ -390,11 +403,11 @@ __device__ __forceinline__ void rows_products(const _Float16* first_block, const
             else mfma3(hi, lo, s_hi[i % K], s_lo[i % K], second);
         });
 }
-template <int HDP>
+template <int HDP, bool BESIDE = false>
 __device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b_hi)[HDP / 16], const h8 (&b_lo)[HDP / 16], f16v& acc, int lane) {
     constexpr int K = HDP / 16;
     clear(acc);
-    product_chain<K, 2>(
+    product_chain<K, 2, BESIDE>(
         [&](int i, h8& hi, h8& lo) {
             hi = frag(block, i, lane);
             lo = frag(block, K + i, lane);
@@ -419,9 +432,9 @@ struct Across {
     }
 };
 // out[HDP x 32 columns] += A^T . W: a block read across against the weights of its 32 rows.
-template <int HDP>
+template <int HDP, bool BESIDE = false>
 __device__ __forceinline__ void columns_product(const _Float16* block, const h8 (&w_hi)[2], const h8 (&w_lo)[2], const Across& across, f16v (&out)[HDP / 32]) {
-    product_chain<HDP / 16, 4>(
+    product_chain<HDP / 16, 4, BESIDE>(
         [&](int i, h8& hi, h8& lo) {
             hi = across.frag(block, i / 2, i % 2);
             lo = across.frag(block + 32 * HDP, i / 2, i % 2);
@@ -494,72 +507,91 @@ struct ForwardState {
     int64_t last;      // the last key that the lane's row sees
 };
 
-template <int HDP, int KEYS>
-__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int64_t k0, int64_t wave_first, float minus_one, int lane, ForwardState<HDP>& st) {
-    constexpr int NB = KEYS / 32;
-    const int h = lane >> 5;
-    const Across across(lane);
-    f16v s[NB];
-    if constexpr (NB == 2) rows_products<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], &t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
-    else rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
-    const float c = pow2(st.e_row + notes.k.e);
-    // masks and marks: only where some row does not see all the keys, or some key holds a non-finite value
-    if (k0 + KEYS - 1 > wave_first || (notes.k.bad[0] | notes.k.bad[1]) != 0) {
-        const int part = (int)(k0 / KEYS % (64 / KEYS));
+// Masks and marks of a block of 32 scores per row, the first of them of key k0: only where some row does not see all the keys, or
+// some key holds a non-finite value.
+template <int HDP>
+__device__ __forceinline__ void forward_mask(f16v& s, uint32_t marks, int64_t k0, int64_t wave_first, int h, const ForwardState<HDP>& st) {
+    if (k0 + 31 > wave_first || marks != 0) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = 32 * b + acc_row(r, h), bit = part * KEYS + j;
-                const bool marked = (notes.k.bad[bit >> 5] >> (bit & 31)) & 1;
-                s[b][r] = k0 + j > st.last ? -INFINITY : marked ? NAN : s[b][r];
-            }
+        for (int r = 0; r < 16; ++r) {
+            const int j = acc_row(r, h);
+            s[r] = k0 + j > st.last ? -INFINITY : ((marks >> j) & 1) != 0 ? NAN : s[r];
+        }
     }
-    float top = s[0][0];
+}
+// Scores to weights, split.  The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach
+// 2^6 2^8, and the accumulators are rarely rescaled (by the factor returned).  No key seen yet: m = -inf, and a top of -inf
+// keeps the weights at 0.
+template <int HDP>
+__device__ __forceinline__ float forward_weights(f16v& s, float c, float minus_one, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2]) {
+    float top = s[0];
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top = max_halves(top) * c;
-    // The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach 2^6 2^8, and the
-    // accumulators are rarely rescaled.  (No key seen yet: m = -inf, and a top of -inf keeps the weights at 0.)
     const bool raise = top > st.m + 6.f;
-    const int e_v = notes.v.e > st.e_v ? notes.v.e : st.e_v;
-    if (__ballot(raise) != 0 || e_v != st.e_v) {
-        const float m = raise ? top : st.m;
-        const float f = raise ? __builtin_amdgcn_exp2f(st.m - m) : 1.f;  // (m = -inf before: 0)
-        const float fo = __builtin_ldexpf(f, st.e_v - e_v < -200 ? -200 : st.e_v - e_v);
-        st.l *= f;
+    const float m = raise ? top : st.m;
+    const float f = __builtin_amdgcn_exp2f(raise ? st.m - m : 0.f);  // (m = -inf before: 0)
+    st.m = m;
+    const float ref = m == -INFINITY ? 0.f : m - 8.f;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    float w[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
+        sum[r & 3] += w[r];
+    }
+    st.l = __builtin_fmaf(st.l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    split_regs<16>(w, minus_one, hi, lo);
+    keep_here(hi, lo);
+    return f;
+}
+// Before the weights of a block meet V: the accumulators follow the weights' reference, and the larger of their exponent and the
+// tile's; a tile of smaller values has the ratio in its weights (a power of two: exact, down to where halves end).
+template <int HDP>
+__device__ __forceinline__ void forward_rescale(float f, int e_tile, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2]) {
+    const int e_v = max(e_tile, st.e_v);
+    if (__ballot(f != 1.f) != 0 || e_v != st.e_v) {
+        const float fo = __builtin_ldexpf(f, max(st.e_v - e_v, -200));
 #pragma unroll
         for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) st.o[d][r] *= fo;
-        st.m = m;
         st.e_v = e_v;
     }
-    const float ref = st.m == -INFINITY ? 0.f : st.m - 8.f;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    float w[NB][16];
+    if (e_tile != st.e_v) {
+        const _Float16 ratio = (_Float16)pow2(max(e_tile - st.e_v, -40));
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            w[b][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c, -ref));
-            sum[r & 3] += w[b][r];
+        for (int i = 0; i < 2; ++i) {
+            hi[i] *= ratio;
+            lo[i] *= ratio;
         }
-    st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    if (notes.v.e != st.e_v) {  // a tile of smaller values: its weights carry the ratio
-        const float f = pow2(notes.v.e - st.e_v);
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w[b][r] *= f;
     }
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        h8 hi[2], lo[2];
-        split_regs<16>(w[b], minus_one, hi, lo);
-        columns_product<HDP>(&t.v[b][0], hi, lo, across, st.o);
+}
+
+// A tile of KEYS keys against the wavefront's rows, block by block: the second block's scores are formed beside the first one's
+// softmax, the first one's product with V beside the second one's softmax.
+template <int HDP, int KEYS>
+__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int64_t k0, int64_t wave_first, float minus_one,
+                                             int lane, ForwardState<HDP>& st) {
+    const int h = lane >> 5, first_mark = (int)(k0 / 32 % 2);
+    const Across across(lane);
+    const float c = pow2(st.e_row + notes.k.e);
+    f16v s[KEYS / 32];
+    h8 hi[2], lo[2];
+    rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
+    forward_mask<HDP>(s[0], notes.k.bad[KEYS == 64 ? 0 : first_mark], k0, wave_first, h, st);
+    if constexpr (KEYS == 64) rows_product<HDP, true>(&t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
+    float f = forward_weights<HDP>(s[0], c, minus_one, st, hi, lo);
+    forward_rescale<HDP>(f, notes.v.e, st, hi, lo);
+    if constexpr (KEYS == 64) {
+        forward_mask<HDP>(s[1], notes.k.bad[1], k0 + 32, wave_first, h, st);
+        columns_product<HDP, true>(&t.v[0][0], hi, lo, across, st.o);
+        h8 hi2[2], lo2[2];
+        f = forward_weights<HDP>(s[1], c, minus_one, st, hi2, lo2);
+        forward_rescale<HDP>(f, notes.v.e, st, hi2, lo2);
+        columns_product<HDP>(&t.v[1][0], hi2, lo2, across, st.o);
+    } else {
+        columns_product<HDP>(&t.v[0][0], hi, lo, across, st.o);
     }
 }
 
