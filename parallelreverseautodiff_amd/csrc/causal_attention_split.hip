@@ -134,9 +134,10 @@ struct SplitArgs {
     float* row_notes;  // [slot][kv][2][64]: -lse log2 e (-inf for a row that is not there), then D
 };
 
-// The groups of 128 packed rows (which = 0) or 128 keys (1) of all sequences as (sequence, number inside it), those with the most
+// The groups of 128 packed rows (which = 0) or 128 keys (1) of all sequences as (sequence, number inside it, first row of the
+// sequence, its length), those with the most
 // work first: the last workgroups to finish are then short ones.  Which of two with about equal work comes first is left to
-// chance and shows in no result.  One workgroup, beside the ones that split.
+// chance and shows in no result.  With an entry a workgroup knows all its addresses: its first copies wait for one load.  One workgroup, beside the ones that split.
 constexpr int ORDER_BINS = 1024;
 __device__ __forceinline__ void write_order(const CausalArgs<float>& p, int which, int slots, int shift, int4* __restrict__ order, int* bins) {
     __shared__ int wave_total[4];
@@ -154,7 +155,7 @@ __device__ __forceinline__ void write_order(const CausalArgs<float>& p, int whic
             }
             const int64_t bin = work < 0 ? ORDER_BINS - 1 : (work >> shift) > ORDER_BINS - 2 ? 0 : ORDER_BINS - 2 - (work >> shift);
             const int at = atomicAdd(&bins[bin], 1);
-            if (pass == 1) order[at] = int4{work < 0 ? -1 : s, (int)inside, 0, 0};
+            if (pass == 1) order[at] = int4{work < 0 ? -1 : s, (int)inside, (int)q0, (int)n};
         }
         __syncthreads();
         if (pass == 1) break;
@@ -488,7 +489,7 @@ struct KeyNotes {
 };
 
 template <int HDP, int KEYS>
-__device__ __forceinline__ void forward_stage(const ForwardArgs& a, ForwardTile<HDP, KEYS>& t, KeyNotes& notes, int64_t tile0, int kv, int64_t k0, int wave,
+__device__ __forceinline__ void forward_stage(const ForwardArgs& a, ForwardTile<HDP, KEYS>& t, KeyNotes& notes, int64_t tile0, int kv, int k0, int wave,
                                               int lane) {
     const int64_t tile_at = (tile0 + k0 / 64) * a.p.kv_heads + kv;
     const int64_t at = tile_at * (128 * HDP) + (k0 / KEYS % (64 / KEYS)) * (2 * KEYS * HDP);
@@ -504,13 +505,13 @@ struct ForwardState {
     f16v o[HDP / 32];
     float m, l;        // the maximum the weights refer to (in units of log2 e) and their sum, this lane half's share
     int e_row, e_v;    // exponent of the row of Q; exponent that o is kept at
-    int64_t last;      // the last key that the lane's row sees
+    int last;          // the last key that the lane's row sees
 };
 
 // Masks and marks of a block of 32 scores per row, the first of them of key k0: only where some row does not see all the keys, or
 // some key holds a non-finite value.
 template <int HDP>
-__device__ __forceinline__ void forward_mask(f16v& s, uint32_t marks, int64_t k0, int64_t wave_first, int h, const ForwardState<HDP>& st) {
+__device__ __forceinline__ void forward_mask(f16v& s, uint32_t marks, int k0, int wave_first, int h, const ForwardState<HDP>& st) {
     if (k0 + 31 > wave_first || marks != 0) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -571,9 +572,9 @@ __device__ __forceinline__ void forward_rescale(float f, int e_tile, ForwardStat
 // A tile of KEYS keys against the wavefront's rows, block by block: the second block's scores are formed beside the first one's
 // softmax, the first one's product with V beside the second one's softmax.
 template <int HDP, int KEYS>
-__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int64_t k0, int64_t wave_first, float minus_one,
+__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int k0, int wave_first, float minus_one,
                                              int lane, ForwardState<HDP>& st) {
-    const int h = lane >> 5, first_mark = (int)(k0 / 32 % 2);
+    const int h = lane >> 5, first_mark = k0 / 32 % 2;
     const Across across(lane);
     const float c = pow2(st.e_row + notes.k.e);
     f16v s[KEYS / 32];
@@ -604,17 +605,18 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     // serves few heads
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
     const int4 job = a.order[blockIdx.x / (unsigned)p.kv_heads];
-    const int s = job.x;
-    const int64_t inside = job.y;
-    if (s < 0) return;
-    int64_t q0, n;
-    sequence_rows(p, s, &q0, &n);
-    const int64_t rows = n * p.group, row0 = inside * 128 + 32 * wave, row = row0 + (lane & 31);
-    if (inside * 128 >= rows) return;  // (cannot be, with offsets that have not changed since the first launch)
+    if (job.x < 0) return;
+    const int q0 = job.z, rows = job.w * p.group, group_row0 = job.y * 128, row0 = group_row0 + 32 * wave, row = row0 + (lane & 31);
+    // keys seen by the workgroup and by the wavefront; the first key that a row of the wavefront does not see is wave_first + 1
+    const int seen = (min(group_row0 + 128, rows) - 1) / p.group + 1;
+    const int wave_first = row0 < rows ? row0 / p.group : -1, wave_seen = row0 < rows ? (min(row0 + 32, rows) - 1) / p.group + 1 : 0;
+    const int64_t tile0 = q0 / 64 + job.x;
+    KeyNotes notes_even, notes_odd;
+    forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, 0, wave, lane);
     const float minus_one = opaque_minus_one();
     ForwardState<HDP> st;
-    const int64_t token = q0 + row / p.group;
-    const int head = kv * p.group + (int)(row % p.group);
+    const int seen_by_row = row / p.group, head = kv * p.group + row - seen_by_row * p.group;
+    const int64_t token = q0 + seen_by_row;
     bool row_bad = false;
     {
         // the row of Q, scaled by a power of two of its own; scale log2 e goes in as a factor in [1/2, 1) and another power
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
             st.q_lo[k] = lo[0];
         }
     }
-    st.last = row < rows ? row / p.group : rows / p.group - 1;
+    st.last = row < rows ? seen_by_row : job.w - 1;
     st.m = -INFINITY;
     st.l = 0.f;
     st.e_v = NO_EXPONENT;
@@ -670,16 +672,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.o[d][r] = 0.f;
-    // keys seen by the workgroup and by the wavefront; the first key that a row of the wavefront does not see is wave_first + 1
-    const int64_t last_row = inside * 128 + 127 < rows ? inside * 128 + 127 : rows - 1;
-    const int64_t seen = last_row / p.group + 1;
-    const int64_t wave_first = row0 < rows ? row0 / p.group : -1;
-    const int64_t wave_row = row0 + 31 < rows ? row0 + 31 : rows - 1;
-    const int64_t wave_seen = row0 < rows ? wave_row / p.group + 1 : 0;
-    const int64_t tile0 = first_tile(p, s, 1, 64);
-    KeyNotes notes_even, notes_odd;
-    forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, 0, wave, lane);
-    for (int64_t k0 = 0; k0 < seen; k0 += 2 * KEYS) {
+    for (int k0 = 0; k0 < seen; k0 += 2 * KEYS) {
         staged();
         KeyNotes notes = notes_even.uniform();
         if (k0 + KEYS < seen) forward_stage<HDP, KEYS>(a, odd, notes_odd, tile0, kv, k0 + KEYS, wave, lane);
@@ -725,7 +718,7 @@ struct BackwardArgs {
     const Header* hq; const Header* hg; const Header* hk; const Header* hv;
     const float* row_notes;
     const int4* row_order; const int4* key_order;
-    int chunk_blocks, chunks;   // blocks of rows that a workgroup of the key kernel takes at most, and parts that makes of the longest
+    int chunk_tiles, chunks;    // tiles of rows that a workgroup of the key kernel takes at most, and parts that makes of the longest
     float* part;                // [chunk][token][kv][dK | dV][hd4] where a group of keys has more than one part
     int hd4;                    // head_dim rounded up to whole vectors
 };
@@ -797,25 +790,23 @@ __device__ __forceinline__ void store_column(float* __restrict__ dst, const f16v
 // in registers; blocks of 32 packed rows (all heads of the group) of Q and dO pass through LDS.  S = Q K^T and
 // dP = dO V^T come out with a key per lane, so P and dS go straight into dV^T += dO^T P and dK^T += Q^T dS.
 template <int HDP>
-struct RowBlock {
-    _Float16 q[64 * HDP], g[64 * HDP];
-    float lse[32], dot[32];
+struct RowTile {
+    _Float16 q[2][64 * HDP], g[2][64 * HDP];   // two blocks of 32 rows
+    float lse[64], dot[64];
 };
 struct RowNotes {
     int e_q, e_g;
 };
 
 template <int HDP>
-__device__ __forceinline__ void row_stage(const BackwardArgs& a, RowBlock<HDP>& t, RowNotes& notes, int64_t tile0, int kv, int64_t block, int wave, int lane) {
-    const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
+__device__ __forceinline__ void row_stage(const BackwardArgs& a, RowTile<HDP>& t, RowNotes& notes, int64_t tile_at, int wave, int lane) {
     notes.e_q = a.hq[tile_at].e;
     notes.e_g = a.hg[tile_at].e;
-    stage<128 * HDP, 4>(a.q + at, t.q, wave, lane);
-    stage<128 * HDP, 4>(a.g + at, t.g, wave, lane);
-    if (wave == 0) {
+    stage<256 * HDP, 4>(a.q + tile_at * (128 * HDP), &t.q[0][0], wave, lane);
+    stage<256 * HDP, 4>(a.g + tile_at * (128 * HDP), &t.g[0][0], wave, lane);
+    if (wave < 2) {
         const __amdgpu_buffer_rsrc_t from = buffer_of(a.row_notes + tile_at * 128, 512);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)t.lse, 4, (lane < 32 ? 0 : 256) + (lane & 31) * 4,
-                                                 (int)(block & 1) * 128, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(t.lse + 64 * wave), 4, lane * 4, wave * 256, 0, 0);
     }
 }
 
@@ -826,23 +817,23 @@ struct KeyState {
     int e_k, e_v;            // of the lane's keys
     int top_q, top_g, top_t; // the largest exponents of Q, dO and dP - D over all rows that go into the sums
     int x_v, x_k;            // the powers of two that the lane's key is scaled by in the weights of dV and dK
-    int64_t first_row;       // the first packed row that sees the lane's key
+    int first_row;           // the first packed row that sees the lane's key
 };
 
 template <int HDP>
-__device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes& notes, int64_t row0, int64_t wave_last, float factor, float minus_one, int lane,
+__device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, const RowNotes& notes, int row0, int wave_last, float factor, float minus_one, int lane,
                                           KeyState<HDP>& st) {
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
-    rows_products<HDP>(t.q, st.k_hi, st.k_lo, s, t.g, st.v_hi, st.v_lo, dp, lane);
+    rows_products<HDP>(t.q[block], st.k_hi, st.k_lo, s, t.g[block], st.v_hi, st.v_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
     const int e_ratio = notes.e_q - st.top_q;
     const float x_v = (float)st.x_v;
     float w[16], ds[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const f4 lse = *reinterpret_cast<const f4*>(t.lse + 8 * q + 4 * h);
+        const f4 lse = *reinterpret_cast<const f4*>(t.lse + 32 * block + 8 * q + 4 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e]) + x_v);
     }
@@ -856,7 +847,7 @@ __device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes
     const float a1 = __builtin_ldexpf(1.f, notes.e_g + st.e_v + e_one);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const f4 dot = *reinterpret_cast<const f4*>(t.dot + 8 * q + 4 * h);
+        const f4 dot = *reinterpret_cast<const f4*>(t.dot + 32 * block + 8 * q + 4 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ds[4 * q + e] = w[4 * q + e] * __builtin_fmaf(dp[4 * q + e], a1, -__builtin_ldexpf(dot[e], e_one));
     }
@@ -871,15 +862,15 @@ __device__ __forceinline__ void row_block(const RowBlock<HDP>& t, const RowNotes
     }
     h8 hi[2], lo[2];
     split_regs<16>(w, minus_one, hi, lo);
-    columns_product<HDP>(t.g, hi, lo, across, st.dv);
+    columns_product<HDP>(t.g[block], hi, lo, across, st.dv);
     fit(ds, st.x_k, st.dk);
     split_regs<16>(ds, minus_one, hi, lo);
-    columns_product<HDP>(t.q, hi, lo, across, st.dk);
+    columns_product<HDP>(t.q[block], hi, lo, across, st.dk);
 }
 
 template <int HDP>
 __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_kernel(const BackwardArgs a) {
-    __shared__ __attribute__((aligned(16))) RowBlock<HDP> even, odd;
+    __shared__ __attribute__((aligned(16))) RowTile<HDP> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     // later parts exist for long groups only and are as large as a part gets: first.  (The parts of a group must not be neighbours:
@@ -887,64 +878,63 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     const unsigned per_chunk = gridDim.x / (unsigned)a.chunks;
     const int kv = blockIdx.x % (unsigned)p.kv_heads, chunk = a.chunks - 1 - (int)(blockIdx.x / per_chunk);
     const int4 job = a.key_order[blockIdx.x % per_chunk / (unsigned)p.kv_heads];
-    const int s = job.x;
-    const int64_t group_key0 = (int64_t)job.y * 128;
-    if (s < 0) return;
-    int64_t q0, n;
-    sequence_rows(p, s, &q0, &n);
-    const int64_t key0 = group_key0 + 32 * wave, rows = n * p.group;
+    if (job.x < 0) return;
+    const int q0 = job.z, n = job.w, rows = n * p.group, group_key0 = job.y * 128, key0 = group_key0 + 32 * wave;
     const bool active = key0 < n;
+    const int64_t row_tile0 = (int64_t)q0 * p.group / 64 + job.x;
+    // tiles of rows: the last part is a whole one, the first what remains
+    const int all_first = group_key0 * p.group / 64, all_tiles = (rows + 63) / 64, parts = (all_tiles - all_first + a.chunk_tiles - 1) / a.chunk_tiles;
+    if (chunk >= parts) return;
+    const int first = max(all_first, all_tiles - (parts - chunk) * a.chunk_tiles), tiles = all_tiles - (parts - 1 - chunk) * a.chunk_tiles;
+    RowNotes notes_even, notes_odd;
+    auto tile_at = [&](int i) { return (row_tile0 + i) * p.kv_heads + kv; };
+    row_stage<HDP>(a, even, notes_even, tile_at(first), wave, lane);
     const float minus_one = opaque_minus_one();
-    const int64_t row_tile0 = first_tile(p, s, p.group, 64);
-    const int64_t all_first = group_key0 * p.group / 32, all_blocks = (rows + 31) / 32;
-    const int64_t first_block = all_first + (int64_t)chunk * a.chunk_blocks;
-    const int64_t blocks = first_block + a.chunk_blocks < all_blocks ? first_block + a.chunk_blocks : all_blocks;
-    if (first_block >= all_blocks) return;
     KeyState<HDP> st;
     {
-        const int64_t tile_at = (first_tile(p, s, 1, 64) + (active ? key0 : group_key0) / 64) * p.kv_heads + kv;
-        const int64_t at = tile_at * (128 * HDP) + (active ? key0 / 32 % 2 : 0) * (64 * HDP);
+        const int from = active ? key0 : group_key0;
+        const int64_t key_tile = ((int64_t)q0 / 64 + job.x + from / 64) * p.kv_heads + kv;
+        const int64_t at = key_tile * (128 * HDP) + from / 32 % 2 * (64 * HDP);
         load_fragments<HDP>(a.k + at, lane, st.k_hi, st.k_lo);
         load_fragments<HDP>(a.v + at, lane, st.v_hi, st.v_lo);
-        st.e_k = a.hk[tile_at].e;
-        st.e_v = a.hv[tile_at].e;
-    }
-    {
-        int tq = NO_EXPONENT, tg = NO_EXPONENT, tt = 2 * NO_EXPONENT;
-        for (int64_t tile = first_block / 2 + lane; tile < (blocks + 1) / 2; tile += 64) {
-            const int64_t at = (row_tile0 + tile) * p.kv_heads + kv;
-            const int e_g = a.hg[at].e;
-            tq = max(tq, a.hq[at].e);
-            tg = max(tg, e_g);
-            tt = max(tt, e_difference(e_g, st.e_v, a.hg[at].e_dot));
+        st.e_k = a.hk[key_tile].e;
+        st.e_v = a.hv[key_tile].e;
+        int tq = NO_EXPONENT, tg = NO_EXPONENT, td = NO_EXPONENT;
+        for (int tile = first + lane; tile < tiles; tile += 64) {
+            tq = max(tq, a.hq[tile_at(tile)].e);
+            tg = max(tg, a.hg[tile_at(tile)].e);
+            td = max(td, a.hg[tile_at(tile)].e_dot);
         }
         st.top_q = wave_max_int(tq);
         st.top_g = wave_max_int(tg);
-        st.top_t = wave_max_int(tt);
         st.e_k = __builtin_amdgcn_readfirstlane(st.e_k);
         st.e_v = __builtin_amdgcn_readfirstlane(st.e_v);
+        st.top_t = e_difference(st.top_g, st.e_v, wave_max_int(td));
     }
     st.x_v = st.x_k = FIT_FROM;
     st.first_row = (key0 + (lane & 31)) * p.group;
-    const int64_t wave_first = key0 * p.group, wave_last = (key0 + 31) * p.group;
+    const int wave_first = key0 * p.group, wave_last = (key0 + 31) * p.group;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.dk[d][r] = st.dv[d][r] = 0.f;
     const float factor = p.scale * LOG2E;
-    RowNotes notes_even, notes_odd;
     auto uniform = [](const RowNotes& x) { return RowNotes{__builtin_amdgcn_readfirstlane(x.e_q), __builtin_amdgcn_readfirstlane(x.e_g)}; };
-    row_stage<HDP>(a, even, notes_even, row_tile0, kv, first_block, wave, lane);
-    for (int64_t b = first_block; b < blocks; b += 2) {
+    auto use = [&](const RowTile<HDP>& t, const RowNotes& notes, int i) {
+#pragma unroll
+        for (int block = 0; block < 2; ++block)
+            if (active && 64 * i + 32 * block + 31 >= wave_first) row_block<HDP>(t, block, notes, 64 * i + 32 * block, wave_last, factor, minus_one, lane, st);
+    };
+    for (int i = first; i < tiles; i += 2) {
         staged();
         RowNotes notes = uniform(notes_even);
-        if (b + 1 < blocks) row_stage<HDP>(a, odd, notes_odd, row_tile0, kv, b + 1, wave, lane);
-        if (active && 32 * b + 31 >= wave_first) row_block<HDP>(even, notes, 32 * b, wave_last, factor, minus_one, lane, st);
-        if (b + 1 >= blocks) break;
+        if (i + 1 < tiles) row_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
+        use(even, notes, i);
+        if (i + 1 >= tiles) break;
         staged();
         notes = uniform(notes_odd);
-        if (b + 2 < blocks) row_stage<HDP>(a, even, notes_even, row_tile0, kv, b + 2, wave, lane);
-        if (active && 32 * (b + 1) + 31 >= wave_first) row_block<HDP>(odd, notes, 32 * (b + 1), wave_last, factor, minus_one, lane, st);
+        if (i + 2 < tiles) row_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
+        use(odd, notes, i + 1);
     }
     const int64_t key = key0 + (lane & 31);
     if (key >= n) return;
@@ -952,7 +942,7 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     float* dst_v = p.dV + (q0 + key) * p.lddv + kv * (int64_t)p.head_dim;
     int width = p.head_dim;
     bool vec = p.vec_dkv;
-    if (all_blocks - all_first > a.chunk_blocks) {
+    if (parts > 1) {
         dst_k = a.part + ((chunk * p.q_rows + q0 + key) * p.kv_heads + kv) * (2 * a.hd4);
         dst_v = dst_k + a.hd4;
         width = a.hd4;  // (columns past the head dimension are zeros)
@@ -968,10 +958,9 @@ __global__ void __launch_bounds__(256) causal_split_join_kernel(const BackwardAr
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
     const int4 job = a.key_order[blockIdx.x / (unsigned)p.kv_heads];
     if (job.x < 0) return;
-    int64_t q0, n;
-    sequence_rows(p, job.x, &q0, &n);
-    const int64_t key0 = (int64_t)job.y * 128, total = (n * p.group + 31) / 32 - key0 * p.group / 32;
-    const int parts = (int)((total + a.chunk_blocks - 1) / a.chunk_blocks);
+    const int64_t q0 = job.z;
+    const int n = job.w, key0 = job.y * 128, total = (n * p.group + 63) / 64 - key0 * p.group / 64;
+    const int parts = (total + a.chunk_tiles - 1) / a.chunk_tiles;
     if (parts <= 1) return;
     const int per_row = a.hd4 / 2;  // vectors of both gradients
     for (int i = (int)(blockIdx.y * 256 + threadIdx.x); i < 128 * per_row; i += 256 * gridDim.y) {
@@ -996,20 +985,19 @@ __global__ void __launch_bounds__(256) causal_split_join_kernel(const BackwardAr
 // Gradient of Q: 128 packed rows to a workgroup, a row per lane, Q and dO in registers; blocks of 32 keys of K and V pass
 // through LDS.  S^T = K Q^T and dP^T = V dO^T, then dQ^T += K^T dS^T.
 template <int HDP>
-struct KeyBlock {
-    _Float16 k[64 * HDP], v[64 * HDP];
+struct KeyTile {
+    _Float16 k[2][64 * HDP], v[2][64 * HDP];   // two blocks of 32 keys
 };
 struct BlockNotes {
     int e_k, e_v;
 };
 
 template <int HDP>
-__device__ __forceinline__ void key_stage(const BackwardArgs& a, KeyBlock<HDP>& t, BlockNotes& notes, int64_t tile0, int kv, int64_t block, int wave, int lane) {
-    const int64_t tile_at = (tile0 + block / 2) * a.p.kv_heads + kv, at = tile_at * (128 * HDP) + (block & 1) * (64 * HDP);
+__device__ __forceinline__ void key_stage(const BackwardArgs& a, KeyTile<HDP>& t, BlockNotes& notes, int64_t tile_at, int wave, int lane) {
     notes.e_k = a.hk[tile_at].e;
     notes.e_v = a.hv[tile_at].e;
-    stage<128 * HDP, 4>(a.k + at, t.k, wave, lane);
-    stage<128 * HDP, 4>(a.v + at, t.v, wave, lane);
+    stage<256 * HDP, 4>(a.k + tile_at * (128 * HDP), &t.k[0][0], wave, lane);
+    stage<256 * HDP, 4>(a.v + tile_at * (128 * HDP), &t.v[0][0], wave, lane);
 }
 
 template <int HDP>
@@ -1019,16 +1007,16 @@ struct RowState {
     float lse, dot;
     int e_q, e_g, top_k, top_t;
     int x_q;        // the power of two that the lane's row is scaled by in the weights
-    int64_t last;   // the last key that the lane's row sees
+    int last;       // the last key that the lane's row sees
 };
 
 template <int HDP>
-__device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNotes& notes, int64_t k0, int64_t wave_first, float factor, float minus_one, int lane,
+__device__ __forceinline__ void key_block(const KeyTile<HDP>& t, int block, const BlockNotes& notes, int k0, int wave_first, float factor, float minus_one, int lane,
                                           RowState<HDP>& st) {
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
-    rows_products<HDP>(t.k, st.q_hi, st.q_lo, s, t.v, st.g_hi, st.g_lo, dp, lane);
+    rows_products<HDP>(t.k[block], st.q_hi, st.q_lo, s, t.v[block], st.g_hi, st.g_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, st.e_q + notes.e_k);
     const int e_ratio = notes.e_k - st.top_k;
     const int e_one = 1 - st.top_t + e_ratio + st.x_q;
@@ -1043,71 +1031,72 @@ __device__ __forceinline__ void key_block(const KeyBlock<HDP>& t, const BlockNot
     fit(ds, st.x_q, st.dq);
     h8 hi[2], lo[2];
     split_regs<16>(ds, minus_one, hi, lo);
-    columns_product<HDP>(t.k, hi, lo, across, st.dq);
+    columns_product<HDP>(t.k[block], hi, lo, across, st.dq);
 }
 
 template <int HDP>
 __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const BackwardArgs a) {
-    __shared__ __attribute__((aligned(16))) KeyBlock<HDP> even, odd;
+    __shared__ __attribute__((aligned(16))) KeyTile<HDP> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
     const int4 job = a.row_order[blockIdx.x / (unsigned)p.kv_heads];
-    const int s = job.x;
-    if (s < 0) return;
-    int64_t q0, n;
-    sequence_rows(p, s, &q0, &n);
-    const int64_t rows = n * p.group, group_row0 = (int64_t)job.y * 128;
-    if (group_row0 >= rows) return;
-    const int64_t row0 = group_row0 + 32 * wave, row = row0 + (lane & 31);
+    if (job.x < 0) return;
+    const int q0 = job.z, rows = job.w * p.group, group_row0 = job.y * 128, row0 = group_row0 + 32 * wave, row = row0 + (lane & 31);
     const bool active = row0 < rows;
+    const int seen = (min(group_row0 + 128, rows) - 1) / p.group + 1, tiles = (seen + 63) / 64;
+    const int wave_first = row0 / p.group, wave_seen = active ? (min(row0 + 32, rows) - 1) / p.group + 1 : 0;
+    const int64_t key_tile0 = q0 / 64 + job.x;
+    BlockNotes notes_even, notes_odd;
+    auto tile_at = [&](int i) { return (key_tile0 + i) * p.kv_heads + kv; };
+    key_stage<HDP>(a, even, notes_even, tile_at(0), wave, lane);
     const float minus_one = opaque_minus_one();
-    const int64_t key_tile0 = first_tile(p, s, 1, 64);
-    const int64_t last_row = group_row0 + 127 < rows ? group_row0 + 127 : rows - 1;
-    const int64_t seen = last_row / p.group + 1, blocks = (seen + 31) / 32;
     RowState<HDP> st;
     {
-        const int64_t from = active ? row0 : group_row0;
-        const int64_t tile_at = (first_tile(p, s, p.group, 64) + from / 64) * p.kv_heads + kv, at = tile_at * (128 * HDP) + (from / 32 % 2) * (64 * HDP);
+        const int from = active ? row0 : group_row0;
+        const int64_t row_tile = ((int64_t)q0 * p.group / 64 + job.x + from / 64) * p.kv_heads + kv, at = row_tile * (128 * HDP) + from / 32 % 2 * (64 * HDP);
         load_fragments<HDP>(a.q + at, lane, st.q_hi, st.q_lo);
         load_fragments<HDP>(a.g + at, lane, st.g_hi, st.g_lo);
-        st.lse = a.row_notes[tile_at * 128 + from % 64 + (lane & 31)];
-        st.dot = a.row_notes[tile_at * 128 + 64 + from % 64 + (lane & 31)];
-        st.e_q = __builtin_amdgcn_readfirstlane(a.hq[tile_at].e);
-        st.e_g = __builtin_amdgcn_readfirstlane(a.hg[tile_at].e);
+        st.lse = a.row_notes[row_tile * 128 + from % 64 + (lane & 31)];
+        st.dot = a.row_notes[row_tile * 128 + 64 + from % 64 + (lane & 31)];
+        const Header hq = a.hq[row_tile], hg = a.hg[row_tile];
         int tk = NO_EXPONENT, tv = NO_EXPONENT;
-        for (int64_t tile = lane; tile < (blocks + 1) / 2; tile += 64) {
-            tk = max(tk, a.hk[(key_tile0 + tile) * p.kv_heads + kv].e);
-            tv = max(tv, a.hv[(key_tile0 + tile) * p.kv_heads + kv].e);
+        for (int tile = lane; tile < tiles; tile += 64) {
+            tk = max(tk, a.hk[tile_at(tile)].e);
+            tv = max(tv, a.hv[tile_at(tile)].e);
         }
+        st.e_q = __builtin_amdgcn_readfirstlane(hq.e);
+        st.e_g = __builtin_amdgcn_readfirstlane(hg.e);
         st.top_k = wave_max_int(tk);
-        st.top_t = e_difference(st.e_g, wave_max_int(tv), __builtin_amdgcn_readfirstlane(a.hg[tile_at].e_dot));
+        st.top_t = e_difference(st.e_g, wave_max_int(tv), __builtin_amdgcn_readfirstlane(hg.e_dot));
     }
     st.x_q = FIT_FROM;
-    st.last = row < rows ? row / p.group : n - 1;
-    const int64_t wave_row = row0 + 31 < rows ? row0 + 31 : rows - 1;
-    const int64_t wave_first = row0 / p.group, wave_seen = active ? wave_row / p.group + 1 : 0;
+    const int seen_by_row = row / p.group;
+    st.last = row < rows ? seen_by_row : job.w - 1;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.dq[d][r] = 0.f;
     const float factor = p.scale * LOG2E;
-    BlockNotes notes_even, notes_odd;
     auto uniform = [](const BlockNotes& x) { return BlockNotes{__builtin_amdgcn_readfirstlane(x.e_k), __builtin_amdgcn_readfirstlane(x.e_v)}; };
-    key_stage<HDP>(a, even, notes_even, key_tile0, kv, 0, wave, lane);
-    for (int64_t b = 0; b < blocks; b += 2) {
+    auto use = [&](const KeyTile<HDP>& t, const BlockNotes& notes, int i) {
+#pragma unroll
+        for (int block = 0; block < 2; ++block)
+            if (64 * i + 32 * block < wave_seen) key_block<HDP>(t, block, notes, 64 * i + 32 * block, wave_first, factor, minus_one, lane, st);
+    };
+    for (int i = 0; i < tiles; i += 2) {
         staged();
         BlockNotes notes = uniform(notes_even);
-        if (b + 1 < blocks) key_stage<HDP>(a, odd, notes_odd, key_tile0, kv, b + 1, wave, lane);
-        if (32 * b < wave_seen) key_block<HDP>(even, notes, 32 * b, wave_first, factor, minus_one, lane, st);
-        if (b + 1 >= blocks) break;
+        if (i + 1 < tiles) key_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
+        use(even, notes, i);
+        if (i + 1 >= tiles) break;
         staged();
         notes = uniform(notes_odd);
-        if (b + 2 < blocks) key_stage<HDP>(a, even, notes_even, key_tile0, kv, b + 2, wave, lane);
-        if (32 * (b + 1) < wave_seen) key_block<HDP>(odd, notes, 32 * (b + 1), wave_first, factor, minus_one, lane, st);
+        if (i + 2 < tiles) key_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
+        use(odd, notes, i + 1);
     }
     if (row >= rows) return;
-    store_column<HDP>(p.dQ + (q0 + row / p.group) * p.lddq + (kv * p.group + row % p.group) * (int64_t)p.head_dim, st.dq, p.scale,
+    store_column<HDP>(p.dQ + ((int64_t)q0 + seen_by_row) * p.lddq + (kv * p.group + row - seen_by_row * p.group) * (int64_t)p.head_dim, st.dq, p.scale,
                       st.top_t - 1 + st.top_k - st.x_q, h, p.head_dim, p.vec_dq);
 }
 
@@ -1162,6 +1151,7 @@ ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
     return f;
 }
 
+constexpr int MOST_PARTS = 32, CHUNK_FROM = 16;
 struct BackwardPlan {
     SplitArgs split;
     BackwardArgs main;
@@ -1192,14 +1182,14 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     b.split.tensors = 4;
     b.split.shift = order_shift(p.q_rows);
     // Parts of the rows that see a group of keys.  If the sequences were equally long, 512 workgroups (two to a compute unit) would
-    // have this many blocks of rows each; half of it keeps the longest group from being what the others wait for.  At most 16 parts
-    // and 256 MB of them.
+    // have `share` tiles of rows each; half of it keeps the longest group from being what the others wait for.  At most
+    // MOST_PARTS parts and 256 MB of them.
     const int hd4 = (p.head_dim + 3) & ~3;
-    const int64_t part_bytes = p.q_rows * p.kv_heads * 2 * hd4 * 4, most_blocks = (p.q_rows * p.group + 31) / 32;
-    const int64_t most_parts = std::max<int64_t>(1, std::min<int64_t>(16, ((int64_t)256 << 20) / part_bytes));
-    const int64_t share = (int64_t)((double)p.q_rows * p.q_rows / p.sequences * p.group * p.kv_heads / (2.0 * 128 * 32 * 512));
-    const int64_t chunk = std::max<int64_t>({32, share / 2, (most_blocks + most_parts - 1) / most_parts});
-    const int chunks = (int)((most_blocks + chunk - 1) / chunk);
+    const int64_t part_bytes = p.q_rows * p.kv_heads * 2 * hd4 * 4, most_tiles = (p.q_rows * p.group + 63) / 64;
+    const int64_t most_parts = std::max<int64_t>(1, std::min<int64_t>(MOST_PARTS, ((int64_t)256 << 20) / part_bytes));
+    const int64_t share = (int64_t)((double)p.q_rows * p.q_rows / p.sequences * p.group * p.kv_heads / (2.0 * 128 * 64 * 512));
+    const int64_t chunk = std::max<int64_t>({CHUNK_FROM, share / 2, (most_tiles + most_parts - 1) / most_parts});
+    const int chunks = (int)((most_tiles + chunk - 1) / chunk);
     float* part = chunks > 1 ? c.take<float>((size_t)(part_bytes * chunks)) : nullptr;
     b.split.row_notes = notes;
     b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], notes,
@@ -1212,7 +1202,8 @@ inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < (
 
 }  // namespace
 
-bool causal_split_eligible(const CausalArgs<float>& p) { return p.q_rows >= 512; }
+// (Packed rows of a sequence are counted in 32 bits.)
+bool causal_split_eligible(const CausalArgs<float>& p) { return p.q_rows >= 512 && p.q_rows * p.group < ((int64_t)1 << 31) - 256; }
 
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
 
