@@ -538,208 +538,327 @@ __global__ void __launch_bounds__(256) causal_bwd_q_kernel(const CausalArgs<T> p
     }
 }
 
-// ---- the newest tokens against the cache ----------------------------------------------------------------------------------
-// A step of a generation loop reads every key and value once and does little with it: it is bound by memory.  A workgroup takes
-// 16 packed rows (a single token of up to 16 heads that share a key/value head) and one of `splits` parts of the keys; its four
-// wavefronts take every fourth tile of 16 keys, straight from memory into the operand registers.  Their sums meet in LDS;
-// with more than one part, (maximum, sum, weighted values) go to the workspace and a second launch joins them.
-template <typename T, int HDP>
-__global__ void __launch_bounds__(256) cached_attention_kernel(const CausalArgs<T> p, int splits, T* __restrict__ part) {
-    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC, CHUNKS = HDP / CH, WPITCH = 16 + VEC;
-    typedef typename Num<T>::Acc Acc;
-    __shared__ __attribute__((aligned(16))) T ws[4][16 * WPITCH];
-    __shared__ T stat[4][2][16];
-    __shared__ T sums[16 * (HDP + 1)];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.y, split = blockIdx.z;
-    int s;
-    int64_t inside;
-    if (!find_tile<16>(p, p.group, blockIdx.x, &s, &inside)) return;
-    const Span sp = span_of(p, s);
-    const int64_t rows = sp.nq * p.group, row0 = inside * 16;
-    if (row0 >= rows) return;
-    const int64_t lead = sp.nk - sp.nq;
-    Pack<T, VEC> q[CHUNKS];
-    {
-        const int64_t r = row0 + li;
-        const T* row = r < rows ? p.Q + (sp.q0 + r / p.group) * p.ldq + (kv * p.group + r % p.group) * (int64_t)p.head_dim : nullptr;
-        load_row<T, HDP>(row, g, p.head_dim, p.vec_q, q);
-        poison_row<T, CHUNKS>(q);
-    }
-    int64_t last[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) last[r] = lead + (row0 + Num<T>::row(r, g)) / p.group;
-    T m[4], l[4];
-    Acc o[HDP / 16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) { m[r] = -(T)INFINITY; l[r] = 0; }
-#pragma unroll
-    for (int y = 0; y < HDP / 16; ++y) o[y] = Acc{0, 0, 0, 0};
-    const int64_t last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
-    const int64_t tiles = (clamped(lead + last_row / p.group + 1, sp.nk) + 15) / 16;
-    const int64_t per = (tiles + splits - 1) / splits;
-    const int64_t from = split * per, to = from + per < tiles ? from + per : tiles;
-    const T factor = p.scale * Num<T>::unit();
-    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
-    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
-    for (int64_t tile = from + wave; tile < to; tile += 4) {
-        const int64_t k0 = tile * 16;
-        // keys past the last are the last one again: their scores are masked
-        const int64_t key = k0 + li < sp.nk ? k0 + li : sp.nk - 1;
-        Pack<T, VEC> k[CHUNKS];
-        load_row<T, HDP>(K + key * p.ldk, g, p.head_dim, p.vec_kv, k);
-        T v[16 / 4][HDP / 16];  // value rows CH c + VEC g + t, columns 16 y + li
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int64_t j = k0 + CH * (x / VEC) + VEC * g + x % VEC;
-            const T* __restrict__ row = V + (j < sp.nk ? j : sp.nk - 1) * p.ldv;
-#pragma unroll
-            for (int y = 0; y < HDP / 16; ++y) v[x][y] = 16 * y + li < p.head_dim ? row[16 * y + li] : (T)0;
+// ---- the newest tokens of a sequence against its cache --------------------------------------------------------------------
+// Bound by reading the cache once.  Work is cut into units of one sequence: 16 packed rows against one part of its keys, one
+// workgroup each, numbered through all sequences by a scan that every workgroup does for itself (lengths live on the device).
+// A wavefront takes every fourth tile of 16 keys.  Everything is transposed - S^T = K Q^T, O^T = V^T P^T - so that the weights
+// come out of the first product in the lanes where the second wants them, a row's statistics sit in a lane, and K and V go
+// from memory to the registers of the matrix instructions without LDS.  Each operand's registers are filled again for the next
+// tile as soon as its product has read them, so that loads are always in flight.
+template <typename T>
+struct CachedPlan {
+    int most_parts;      // of a sequence
+    T *stat, *data;      // of part i of packed row r: {maximum, sum} and the weighted sum of values, at r * most_parts + i
+};
+constexpr int CACHED_WAVES = 4, CACHED_CHUNK = 256;
+
+// Keys of each part of a sequence, whole tiles.
+__device__ __forceinline__ int64_t part_keys(int64_t keys, int most_parts) {
+    const int64_t least = (keys + most_parts - 1) / most_parts;
+    return ((least > CACHED_CHUNK ? least : CACHED_CHUNK) + 15) / 16 * 16;
+}
+__device__ __forceinline__ int part_count(int64_t keys, int most_parts) {
+    const int64_t size = part_keys(keys, most_parts);
+    return keys <= size || most_parts == 1 ? 1 : (int)((keys + size - 1) / size);
+}
+
+// The sequence and the number inside it of unit `unit`, by a whole wavefront; false: there are not so many.
+template <typename T>
+__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts, int64_t unit, int lane, int* sequence, int64_t* inside) {
+    int64_t before = 0;
+    for (int s0 = 0; s0 < p.sequences; s0 += 64) {
+        int64_t units = 0;
+        if (s0 + lane < p.sequences) {
+            const Span sp = span_of(p, s0 + lane);
+            units = (sp.nq * p.group + 15) / 16 * part_count(sp.nk, most_parts);
         }
-        Acc acc[1] = {Acc{0, 0, 0, 0}};
+        int64_t upto = units;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t other = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += other;
+        }
+        const uint64_t behind = __ballot(before + upto > unit);
+        if (behind != 0) {
+            const int at = __builtin_ctzll(behind);
+            *sequence = s0 + at;
+            *inside = unit - before - __shfl(upto - units, at, 64);
+            return true;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return false;
+}
+
+// N consecutive elements; columns past the row's end are read at its start, for which nothing uses the result.
+template <typename T, int N, bool ALIGNED>
+__device__ __forceinline__ Pack<T, N> load_some(const T* __restrict__ row, int d0, int head_dim) {
+    Pack<T, N> v;
+    if constexpr (ALIGNED) {
+        v = *reinterpret_cast<const Pack<T, N>*>(row + (d0 < head_dim ? d0 : 0));
+    } else {
 #pragma unroll
-            for (int t = 0; t < VEC; ++t) acc[0] = Num<T>::mfma(q[c].v[t], k[c].v[t], acc[0]);
-        // a key row with a non-finite value: NaN for the rows that see it, zeros elsewhere
-        uint32_t poisoned = 0;  // bit j: key k0 + j
-        {
-            bool fine = true;
+        for (int t = 0; t < N; ++t) v.v[t] = row[d0 + t < head_dim ? d0 + t : 0];
+    }
+    return v;
+}
+
+template <typename T, int HDP, bool ALIGNED>
+__global__ void __launch_bounds__(64 * CACHED_WAVES) cached_attention_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
+    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC, CHUNKS = HDP / CH, NY = HDP / 16, N = VEC < NY ? VEC : NY, W = CACHED_WAVES, PITCH = HDP + VEC;
+    typedef typename Num<T>::Acc Acc;
+    __shared__ __attribute__((aligned(16))) T sums[W / 2][16 * PITCH];
+    __shared__ T stat[W][2][16];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const int kv = blockIdx.y;
+    for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+        int s;
+        int64_t inside;
+        if (!find_unit(p, plan.most_parts, unit, lane, &s, &inside)) return;
+        s = __builtin_amdgcn_readfirstlane(s);
+        const Span sp = span_of(p, s);
+        const int parts = part_count(sp.nk, plan.most_parts), part = (int)(inside % parts);
+        const int64_t rows = sp.nq * p.group, row0 = inside / parts * 16;
+        const int64_t lead = sp.nk - sp.nq;
+        const int64_t r = row0 + li;  // the lane's row
+        const int64_t token = sp.q0 + r / p.group;
+        const int head = kv * p.group + (int)(r % p.group);
+        Pack<T, VEC> q[CHUNKS];
+        load_row<T, HDP>(r < rows ? p.Q + token * p.ldq + head * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_q, q);
+        poison_row<T, CHUNKS>(q);
+        const int64_t last = lead + r / p.group, first_last = lead + row0 / p.group;  // the last key that the row sees, of all the least
+        const int64_t last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
+        const int64_t size = part_keys(sp.nk, plan.most_parts), seen = clamped(lead + last_row / p.group + 1, sp.nk);
+        const int64_t from = parts == 1 ? 0 : part * size, to = parts == 1 || seen < from + size ? seen : from + size;
+        const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
+        const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
+        T m = -(T)INFINITY, l = 0;
+        Acc o[NY];  // element r of o[N y + t]: column 16 N y + N row(r, g) + t of row li
+#pragma unroll
+        for (int y = 0; y < NY; ++y) o[y] = Acc{0, 0, 0, 0};
+        const T factor = p.scale * Num<T>::unit();
+        Pack<T, VEC> k[CHUNKS];   // key li, elements CH c + VEC g + t
+        Pack<T, N> v[4][NY / N];  // keys row(x, g), columns 16 N y + N li + t
+        // keys past the last are the last one again: their scores are masked
+        auto load_k = [&](int64_t k0) {
+            const int most = (int)(to - 1 - k0 < 15 ? to - 1 - k0 : 15);
+            const T* __restrict__ row = K + k0 * p.ldk + (li < most ? li : most) * p.ldk;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) k[c] = load_some<T, VEC, ALIGNED>(row, CH * c + VEC * g, p.head_dim);
+        };
+        auto load_v = [&](int64_t k0) {
+            const int most = (int)(to - 1 - k0 < 15 ? to - 1 - k0 : 15);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int j = Num<T>::row(x, g);
+                const T* __restrict__ row = V + k0 * p.ldv + (j < most ? j : most) * p.ldv;
+#pragma unroll
+                for (int y = 0; y < NY / N; ++y) v[x][y] = load_some<T, N, ALIGNED>(row, 16 * N * y + N * li, p.head_dim);
+            }
+        };
+        int64_t k0 = from + 16 * wave;
+        if (k0 < to) {
+            load_k(k0);
+            load_v(k0);
+        }
+        for (; k0 < to; k0 += 16 * W) {
+            Acc sc = Acc{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                for (int t = 0; t < VEC; ++t) fine = fine && is_finite(k[c].v[t]);
-            uint64_t b = __ballot(!fine);
-            poisoned = (uint32_t)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xFFFFu);
+                for (int t = 0; t < VEC; ++t) sc = Num<T>::mfma(k[c].v[t], q[c].v[t], sc);
+            // A key with a non-finite value is NaN for the rows that see it and zeros for the others.  In K it makes the scores
+            // of its key non-finite whatever the rows hold, so that K is looked at only after such a score.
+            uint32_t poisoned = 0;  // bit j: key k0 + j
+            T odd = 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                fine = true;
+            for (int x = 0; x < 4; ++x) odd = fma(sc[x], (T)0, odd);
+            if (__any(!(odd == 0))) {
+                bool fine = true;
 #pragma unroll
-                for (int y = 0; y < HDP / 16; ++y) {
-                    fine = fine && is_finite(v[x][y]);
-                }
-                b = __ballot(!fine);
-                if (b != 0) {
+                for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-                    for (int y = 0; y < HDP / 16; ++y) v[x][y] = is_finite(v[x][y]) ? v[x][y] : (T)0;
+                    for (int t = 0; t < VEC; ++t) fine = fine && is_finite(k[c].v[t]);
+                const uint64_t b = __ballot(!fine);
+                poisoned = (uint32_t)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xFFFFu);
+            }
+            load_k(k0 + 16 * W);
+            odd = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < NY / N; ++y)
+#pragma unroll
+                    for (int t = 0; t < N; ++t) odd = fma(v[x][y].v[t], (T)0, odd);
+            if (__any(!(odd == 0))) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    bool fine = true;
+#pragma unroll
+                    for (int y = 0; y < NY / N; ++y)
+#pragma unroll
+                        for (int t = 0; t < N; ++t) {
+                            fine = fine && is_finite(v[x][y].v[t]);
+                            v[x][y].v[t] = is_finite(v[x][y].v[t]) ? v[x][y].v[t] : (T)0;
+                        }
+                    const uint64_t b = __ballot(!fine);
 #pragma unroll
                     for (int gg = 0; gg < 4; ++gg)
-                        if ((b >> (16 * gg)) & 0xFFFFu) poisoned |= 1u << (CH * (x / VEC) + VEC * gg + x % VEC);
+                        if ((b >> (16 * gg)) & 0xFFFFu) poisoned |= 1u << Num<T>::row(x, gg);
                 }
             }
+            T top = -(T)INFINITY;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[x] *= factor;
+            if (poisoned != 0 || k0 + 15 > first_last) {
+                const int most = (int)clamped(last - k0 + 1, 16);  // keys of the tile that the row sees
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int j = Num<T>::row(x, g);
+                    sc[x] = j >= most ? -(T)INFINITY : (poisoned >> j) & 1 ? nan_of<T>() : sc[x];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) top = fmax(top, sc[x]);
+            // the maximum is raised for a tile only if one of its scores is above it
+            if (__any(top > m)) {
+                top = fmax(top, __shfl_xor(top, 16, 64));
+                top = fmax(top, __shfl_xor(top, 32, 64));
+                top = fmax(top, m);
+                const T f = top == -(T)INFINITY ? (T)1 : Num<T>::exp_unit(m - top);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int y = 0; y < NY; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[y][x] *= f;
+            }
+            const T ref = m == -(T)INFINITY ? (T)0 : m;  // nothing seen yet: every weight is exp(-inf) = 0
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                sc[x] = Num<T>::exp_unit(sc[x] - ref);
+                l += sc[x];
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+#pragma unroll
+                for (int y = 0; y < NY; ++y) o[y] = Num<T>::mfma(v[x][y / N].v[y % N], sc[x], o[y]);
+            load_v(k0 + 16 * W);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            acc[0][r] = k0 + li > last[r] ? -(T)INFINITY : (poisoned >> li) & 1 ? nan_of<T>() : acc[0][r] * factor;
-        T fac[4];
-        softmax_tile<T, 1>(acc, m, l, fac);
-#pragma unroll
-        for (int y = 0; y < HDP / 16; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[y][r] *= fac[r];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ws[wave][Num<T>::row(r, g) * WPITCH + li] = acc[0][r];
-        wave_sync();
-#pragma unroll
-        for (int c = 0; c < 16 / CH; ++c) {
-            const Pack<T, VEC> a = *reinterpret_cast<const Pack<T, VEC>*>(&ws[wave][li * WPITCH + CH * c + VEC * g]);
-#pragma unroll
-            for (int t = 0; t < VEC; ++t)
-#pragma unroll
-                for (int y = 0; y < HDP / 16; ++y) o[y] = Num<T>::mfma(a.v[t], v[c * VEC + t][y], o[y]);
+        // the wavefronts' sums, added in pairs
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) {
+            stat[wave][0][li] = m;
+            stat[wave][1][li] = l;
         }
-        wave_sync();
-    }
-    // the four wavefronts' sums, added in their order
-    if (li == 0) {
+        __syncthreads();
+        T top = stat[0][0][li];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            stat[wave][0][Num<T>::row(r, g)] = m[r];
-            stat[wave][1][Num<T>::row(r, g)] = l[r];
+        for (int w = 1; w < W; ++w) top = fmax(top, stat[w][0][li]);
+        const T ref = top == -(T)INFINITY ? (T)0 : top;
+        const T mine = Num<T>::exp_unit(m - ref);
+        T total = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) total += stat[w][1][li] * Num<T>::exp_unit(stat[w][0][li] - ref);
+#pragma unroll
+        for (int y = 0; y < NY; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[y][x] *= mine;
+#pragma unroll
+        for (int half = W / 2; half > 0; half /= 2) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int y = 0; y < NY / N; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        Pack<T, N> e;
+#pragma unroll
+                        for (int t = 0; t < N; ++t) e.v[t] = o[N * y + t][x];
+                        *reinterpret_cast<Pack<T, N>*>(&sums[wave - half][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]) = e;
+                    }
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int y = 0; y < NY / N; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const Pack<T, N> e = *reinterpret_cast<const Pack<T, N>*>(&sums[wave][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]);
+#pragma unroll
+                        for (int t = 0; t < N; ++t) o[N * y + t][x] += e.v[t];
+                    }
+            }
         }
-    }
-    __syncthreads();
-    T top[4], total[4];
+        if (wave == 0 && r < rows) {
+            T by = 1;
+            T* __restrict__ dst;
+            if (parts == 1) {
+                by = last >= 0 && sp.nk > 0 ? 1 / total : (T)0;
+                dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
+            } else {
+                const int64_t at = (token * p.heads + head) * plan.most_parts + part;
+                dst = plan.data + at * p.head_dim;
+                if (g == 0) {
+                    plan.stat[2 * at] = top;
+                    plan.stat[2 * at + 1] = total;
+                }
+            }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = Num<T>::row(r, g);
-        top[r] = fmax(fmax(stat[0][0][row], stat[1][0][row]), fmax(stat[2][0][row], stat[3][0][row]));
-        const T ref = top[r] == -(T)INFINITY ? (T)0 : top[r];
-        total[r] = 0;
+            for (int y = 0; y < NY / N; ++y)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) total[r] += stat[w][1][row] * Num<T>::exp_unit(stat[w][0][row] - ref);
-        const T mine = Num<T>::exp_unit(m[r] - ref);
+                for (int x = 0; x < 4; ++x) {
+                    const int d = 16 * N * y + N * Num<T>::row(x, g);
 #pragma unroll
-        for (int y = 0; y < HDP / 16; ++y) o[y][r] *= mine;
-    }
-    for (int w = 0; w < 4; ++w) {
-        if (wave == w) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int y = 0; y < HDP / 16; ++y) {
-                    T* at = &sums[Num<T>::row(r, g) * (HDP + 1) + 16 * y + li];
-                    *at = w == 0 ? o[y][r] : *at + o[y][r];
+                    for (int t = 0; t < N; ++t)
+                        if (d + t < p.head_dim) dst[d + t] = o[N * y + t][x] * by;
                 }
         }
         __syncthreads();
-    }
-    // wavefront w finishes rows w, w + 4, ...
-    for (int row = wave; row < 16; row += 4) {
-        const int64_t r = row0 + row;
-        if (r >= rows) break;
-        T mm = fmax(fmax(stat[0][0][row], stat[1][0][row]), fmax(stat[2][0][row], stat[3][0][row]));
-        const T ref = mm == -(T)INFINITY ? (T)0 : mm;
-        T ll = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) ll += stat[w][1][row] * Num<T>::exp_unit(stat[w][0][row] - ref);
-        const int64_t token = sp.q0 + r / p.group;
-        const int head = kv * p.group + (int)(r % p.group);
-        if (splits == 1) {
-            const bool any = lead + r / p.group >= 0 && sp.nk > 0;
-            T* dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
-            for (int d = lane; d < p.head_dim; d += 64) dst[d] = any ? sums[row * (HDP + 1) + d] / ll : (T)0;
-        } else {
-            T* dst = part + ((token * p.heads + head) * splits + split) * (int64_t)(p.head_dim + 2);
-            for (int d = lane; d < p.head_dim; d += 64) dst[2 + d] = sums[row * (HDP + 1) + d];
-            if (lane == 0) { dst[0] = mm; dst[1] = ll; }
-        }
     }
 }
 
 // Joins the parts of a row: a wavefront per (token, head).
 template <typename T>
-__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, int splits, const T* __restrict__ part) {
+__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
     const int lane = threadIdx.x & 63;
     const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (at >= p.q_rows * p.heads) return;
     const int64_t token = at / p.heads;
-    const int head = (int)(at % p.heads);
     // the sequence of the token: rows in front of the first and behind the last are left as they are
-    int lo = 0, hi = p.sequences + 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (clamped(p.q_off[mid], p.q_rows) <= token) lo = mid + 1;
-        else hi = mid;
+    int begun = 0;  // offsets that are not behind the token
+    for (int s0 = 0; s0 <= p.sequences; s0 += 64) {
+        const int here = __popcll(__ballot(s0 + lane <= p.sequences && clamped(p.q_off[s0 + lane], p.q_rows) <= token));
+        begun += here;
+        if (here < 64) break;
     }
-    if (lo == 0 || lo > p.sequences) return;
-    const Span sp = span_of(p, lo - 1);
+    begun = __builtin_amdgcn_readfirstlane(begun);
+    if (begun == 0 || begun > p.sequences) return;
+    const Span sp = span_of(p, begun - 1);
     if (token < sp.q0 || token >= sp.q0 + sp.nq) return;
-    const bool any = sp.nk - sp.nq + (token - sp.q0) >= 0 && sp.nk > 0;
-    const int stride = p.head_dim + 2;
-    const T* __restrict__ mine = part + at * splits * (int64_t)stride;
-    T top = -(T)INFINITY;
-    for (int i = 0; i < splits; ++i) top = fmax(top, mine[i * stride]);
-    const T ref = top == -(T)INFINITY ? (T)0 : top;
-    for (int d = lane; d < p.head_dim; d += 64) {
-        T sum = 0, total = 0;
-        for (int i = 0; i < splits; ++i) {
-            const T f = Num<T>::exp_unit(mine[i * stride] - ref);
-            total += mine[i * stride + 1] * f;
-            sum += mine[i * stride + 2 + d] * f;
-        }
-        p.O[token * p.ldo + head * (int64_t)p.head_dim + d] = any ? sum / total : (T)0;
+    const int parts = part_count(sp.nk, plan.most_parts);
+    if (parts == 1) return;
+    const T m = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane)] : -(T)INFINITY;
+    const T l = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane) + 1] : (T)0;
+    T top = m;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d, 64));
+    T f = Num<T>::exp_unit(m - (top == -(T)INFINITY ? (T)0 : top)), total = l * f;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
+    f = sp.nk - sp.nq + (token - sp.q0) >= 0 ? f / total : (T)0;
+    const T* __restrict__ mine = plan.data + at * plan.most_parts * (int64_t)p.head_dim;
+    T sum[2] = {0, 0};
+    const int d0 = lane < p.head_dim ? lane : 0, d1 = lane + 64 < p.head_dim ? lane + 64 : 0;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+        const T w = __shfl(f, i, 64);
+        sum[0] += mine[(int64_t)i * p.head_dim + d0] * w;
+        sum[1] += mine[(int64_t)i * p.head_dim + d1] * w;
     }
+    T* __restrict__ dst = p.O + token * p.ldo + at % p.heads * (int64_t)p.head_dim;
+    if (lane < p.head_dim) dst[lane] = sum[0];
+    if (lane + 64 < p.head_dim) dst[lane + 64] = sum[1];
 }
 
 inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
@@ -754,6 +873,14 @@ inline int64_t tile_slots(int64_t rows, int64_t group, int64_t per_tile, int64_t
         else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(256), 0, s, __VA_ARGS__);             \
         else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(256), 0, s, __VA_ARGS__);                                  \
         if (hipError_t e = hipGetLastError()) return e;                                                                 \
+    } while (0)
+
+#define BY_HEAD_DIM_CACHED(ALIGNED)                                                                                                       \
+    do {                                                                                                                                  \
+        const dim3 block(64 * CACHED_WAVES);                                                                                              \
+        if (a.head_dim <= 32) hipLaunchKernelGGL((cached_attention_kernel<T, 32, ALIGNED>), grid, block, 0, s, a, plan);                  \
+        else if (a.head_dim <= 64) hipLaunchKernelGGL((cached_attention_kernel<T, 64, ALIGNED>), grid, block, 0, s, a, plan);             \
+        else hipLaunchKernelGGL((cached_attention_kernel<T, 128, ALIGNED>), grid, block, 0, s, a, plan);                                  \
     } while (0)
 
 template <typename T>
@@ -781,28 +908,30 @@ hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     return hipSuccess;
 }
 
-// Parts of the keys for a cached call: enough workgroups to fill the chip, none with less than a tile per wavefront of a cache
-// that fills the whole of K.
-static int cached_splits(int64_t q_rows, int64_t k_rows, int sequences, int kv_heads, int group) {
-    const int64_t groups = tile_slots(q_rows, group, 16, sequences) * kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({(2048 + groups - 1) / groups, (k_rows + 63) / 64, 32}));
-}
+// Parts of a sequence's keys: none where a part would hold all of a cache.
+static int most_cached_parts(int64_t k_rows) { return k_rows <= 2 * CACHED_CHUNK ? 1 : (int)std::min<int64_t>((k_rows + CACHED_CHUNK - 1) / CACHED_CHUNK, 64); }
 
 template <typename T>
 size_t cached_workspace_bytes(const CausalArgs<T>& a) {
-    const int splits = cached_splits(a.q_rows, a.k_rows, a.sequences, a.kv_heads, a.group);
-    return splits == 1 ? 0 : (size_t)a.q_rows * a.heads * splits * (a.head_dim + 2) * sizeof(T);
+    const int parts = most_cached_parts(a.k_rows);
+    return parts == 1 ? 0 : (size_t)a.q_rows * a.heads * parts * (a.head_dim + 2) * sizeof(T);
 }
 
 template <typename T>
 hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s) {
-    const int splits = cached_splits(a.q_rows, a.k_rows, a.sequences, a.kv_heads, a.group);
-    const int64_t slots = tile_slots(a.q_rows, a.group, 16, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
-    if (!grid_fits(slots, 256) || !grid_fits(rows, 256)) return hipErrorInvalidValue;
-    T* part = static_cast<T*>(workspace);
-    BY_HEAD_DIM(cached_attention_kernel, dim3((unsigned)slots, a.kv_heads, splits), a, splits, part);
-    if (splits > 1) {
-        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, splits, part);
+    CachedPlan<T> plan;
+    plan.most_parts = most_cached_parts(a.k_rows);
+    plan.data = static_cast<T*>(workspace);
+    plan.stat = plan.data + a.q_rows * a.heads * (int64_t)plan.most_parts * a.head_dim;
+    // a workgroup per unit if the sequences' keys are apart from each other; where they share keys, some take several
+    const int64_t tiles = tile_slots(a.q_rows, a.group, 16, a.sequences), each = std::max<int64_t>(1, tiles / a.sequences);
+    const int64_t units = std::min<int64_t>(tiles + (plan.most_parts == 1 ? 0 : each * (a.k_rows / CACHED_CHUNK)), 65536), rows = (a.q_rows * a.heads + 3) / 4;
+    if (!grid_fits(rows, 256)) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)units, a.kv_heads);
+    if (a.vec_kv) BY_HEAD_DIM_CACHED(true); else BY_HEAD_DIM_CACHED(false);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (plan.most_parts > 1) {
+        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, plan);
         if (hipError_t e = hipGetLastError()) return e;
     }
     return hipSuccess;
