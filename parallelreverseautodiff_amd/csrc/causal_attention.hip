@@ -547,47 +547,85 @@ __global__ void __launch_bounds__(256) causal_bwd_q_kernel(const CausalArgs<T> p
 // tile as soon as its product has read them, so that loads are always in flight.
 template <typename T>
 struct CachedPlan {
-    int most_parts;      // of a sequence
-    T *stat, *data;      // of part i of packed row r: {maximum, sum} and the weighted sum of values, at r * most_parts + i
+    int most_parts;     // of a sequence
+    T *stat, *data;     // of part i of packed row r: {maximum, sum} and the weighted sum of values, at r * most_parts + i
+    int32_t* part_keys; // how many keys make a part, for the join
 };
-constexpr int CACHED_WAVES = 4, CACHED_CHUNK = 256;
+constexpr int CACHED_WAVES = 4, CACHED_LEAST = 128, CACHED_WHOLE = 512, CACHED_GROUPS = 512;
 
-// Keys of each part of a sequence, whole tiles.
-__device__ __forceinline__ int64_t part_keys(int64_t keys, int most_parts) {
-    const int64_t least = (keys + most_parts - 1) / most_parts;
-    return ((least > CACHED_CHUNK ? least : CACHED_CHUNK) + 15) / 16 * 16;
+// Parts of a sequence's keys: of `size` keys, or of more if there would be too many parts, whole tiles.
+__device__ __forceinline__ int64_t part_keys(int64_t keys, int64_t size, int most_parts) {
+    if (keys <= size * most_parts) return size;
+    return ((keys + most_parts - 1) / most_parts + 15) / 16 * 16;
 }
-__device__ __forceinline__ int part_count(int64_t keys, int most_parts) {
-    const int64_t size = part_keys(keys, most_parts);
-    return keys <= size || most_parts == 1 ? 1 : (int)((keys + size - 1) / size);
+__device__ __forceinline__ uint32_t part_count(int64_t keys, uint32_t size, int most_parts) {
+    if (keys <= CACHED_WHOLE || keys <= size || most_parts == 1) return 1;
+    if (keys <= (int64_t)size * most_parts) return ((uint32_t)keys + size - 1) / size;
+    const int64_t larger = part_keys(keys, size, most_parts);
+    return (uint32_t)((keys + larger - 1) / larger);
 }
 
-// The sequence and the number inside it of unit `unit`, by a whole wavefront; false: there are not so many.
+// Sums over the lanes up to this one.
+__device__ __forceinline__ uint32_t scan64(uint32_t x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // one lane up inside each 16, two, four, eight
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last lane of the 16 before; of the 32 before
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
+// The sequence of unit `unit` and the unit's number inside it, by a whole wavefront; false: there are not so many.  (Rows fit
+// into 31 bits, so a sequence has less than 2^32 units.  Offsets that overlap may wrap the sum: the caller checks the number.)
 template <typename T>
-__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts, int64_t unit, int lane, int* sequence, int64_t* inside) {
-    int64_t before = 0;
+__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts, uint32_t size, uint32_t unit, int lane, Span* span, uint32_t* parts, uint32_t* inside) {
+    uint32_t before = 0;
     for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-        int64_t units = 0;
+        Span sp = {0, 0, 0, 0};
+        uint32_t units = 0, count = 1;
         if (s0 + lane < p.sequences) {
-            const Span sp = span_of(p, s0 + lane);
-            units = (sp.nq * p.group + 15) / 16 * part_count(sp.nk, most_parts);
+            sp = span_of(p, s0 + lane);
+            count = part_count(sp.nk, size, most_parts);
+            units = ((uint32_t)sp.nq * (uint32_t)p.group + 15) / 16 * count;
         }
-        int64_t upto = units;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t other = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += other;
-        }
-        const uint64_t behind = __ballot(before + upto > unit);
+        const uint32_t upto = before + scan64(units);
+        const uint64_t behind = __ballot(upto > unit);
         if (behind != 0) {
             const int at = __builtin_ctzll(behind);
-            *sequence = s0 + at;
-            *inside = unit - before - __shfl(upto - units, at, 64);
+            // (none of these passes 31 bits)
+            span->q0 = __builtin_amdgcn_readlane((int)sp.q0, at);
+            span->nq = __builtin_amdgcn_readlane((int)sp.nq, at);
+            span->k0 = __builtin_amdgcn_readlane((int)sp.k0, at);
+            span->nk = __builtin_amdgcn_readlane((int)sp.nk, at);
+            *parts = __builtin_amdgcn_readlane(count, at);
+            *inside = unit - __builtin_amdgcn_readlane(upto - units, at);
             return true;
         }
-        before += __shfl(upto, 63, 64);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
+}
+
+// Keys per part that make all units of a call few enough to run at once, each sequence having a part that is not whole.
+template <typename T>
+__device__ __forceinline__ uint32_t keys_per_part(const CausalArgs<T>& p, int most_parts, int lane) {
+    if (most_parts == 1) return 0;
+    float keys = 0, tiles = 0;
+    for (int s0 = 0; s0 < p.sequences; s0 += 64) {
+        if (s0 + lane >= p.sequences) break;
+        const Span sp = span_of(p, s0 + lane);
+        const float here = (float)(((uint32_t)sp.nq * (uint32_t)p.group + 15) / 16);
+        tiles += here;
+        keys += here * (float)sp.nk;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        keys += __shfl_xor(keys, d, 64);
+        tiles += __shfl_xor(tiles, d, 64);
+    }
+    const float room = fmaxf((float)(CACHED_GROUPS / 2), CACHED_GROUPS - tiles * p.kv_heads), share = keys * p.kv_heads / room;
+    return __builtin_amdgcn_readfirstlane(((uint32_t)fminf(fmaxf(share, (float)CACHED_LEAST), 1e9f) + 63) / 64 * 64);
 }
 
 // N consecutive elements; columns past the row's end are read at its start, for which nothing uses the result.
@@ -604,32 +642,37 @@ __device__ __forceinline__ Pack<T, N> load_some(const T* __restrict__ row, int d
 }
 
 template <typename T, int HDP, bool ALIGNED>
-__global__ void __launch_bounds__(64 * CACHED_WAVES) cached_attention_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
+__global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) cached_attention_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
     constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC, CHUNKS = HDP / CH, NY = HDP / 16, N = VEC < NY ? VEC : NY, W = CACHED_WAVES, PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
-    __shared__ __attribute__((aligned(16))) T sums[W / 2][16 * PITCH];
+    __shared__ __attribute__((aligned(16))) T sums[W][16 * PITCH];
     __shared__ T stat[W][2][16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.y;
-    for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
-        int s;
-        int64_t inside;
-        if (!find_unit(p, plan.most_parts, unit, lane, &s, &inside)) return;
-        s = __builtin_amdgcn_readfirstlane(s);
-        const Span sp = span_of(p, s);
-        const int parts = part_count(sp.nk, plan.most_parts), part = (int)(inside % parts);
-        const int64_t rows = sp.nq * p.group, row0 = inside / parts * 16;
+    // heads of a unit are neighbours, so that workgroups without a unit come last
+    const uint32_t stride = gridDim.x / p.kv_heads;
+    const int kv = (int)(blockIdx.x % p.kv_heads);
+    const uint32_t keys_each = keys_per_part(p, plan.most_parts, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && plan.most_parts > 1) *plan.part_keys = (int32_t)keys_each;
+    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+        Span sp;
+        uint32_t parts, inside;
+        if (!find_unit(p, plan.most_parts, keys_each, unit, lane, &sp, &parts, &inside)) return;
+        const uint32_t rows = (uint32_t)sp.nq * (uint32_t)p.group, tile = inside / parts, part = inside % parts, row0 = tile * 16;
+        if (tile >= (rows + 15) / 16) return;  // (a wrapped sum)
         const int64_t lead = sp.nk - sp.nq;
-        const int64_t r = row0 + li;  // the lane's row
-        const int64_t token = sp.q0 + r / p.group;
-        const int head = kv * p.group + (int)(r % p.group);
+        const uint32_t r = row0 + li < rows ? row0 + li : rows - 1;  // the lane's row; past the last it is the last one again
+        const uint32_t first_token = row0 / p.group, ahead = (row0 % p.group + (r - row0)) / p.group;  // of the tile; of the row, from there
+        const int64_t token = sp.q0 + first_token + ahead;
+        const int head = kv * p.group + (int)(r - (first_token + ahead) * p.group);
         Pack<T, VEC> q[CHUNKS];
-        load_row<T, HDP>(r < rows ? p.Q + token * p.ldq + head * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_q, q);
-        poison_row<T, CHUNKS>(q);
-        const int64_t last = lead + r / p.group, first_last = lead + row0 / p.group;  // the last key that the row sees, of all the least
-        const int64_t last_row = row0 + 15 < rows ? row0 + 15 : rows - 1;
-        const int64_t size = part_keys(sp.nk, plan.most_parts), seen = clamped(lead + last_row / p.group + 1, sp.nk);
-        const int64_t from = parts == 1 ? 0 : part * size, to = parts == 1 || seen < from + size ? seen : from + size;
+        {
+            const T* __restrict__ row = p.Q + token * p.ldq + head * (int64_t)p.head_dim;
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) q[c] = load_some<T, VEC, ALIGNED>(row, CH * c + VEC * g, p.head_dim);
+        }
+        const int64_t first_last = lead + first_token, last = first_last + ahead;  // the last key that the tile's first row sees, that this one does
+        const int64_t size = part_keys(sp.nk, keys_each, plan.most_parts), seen = clamped(first_last + (int)__builtin_amdgcn_readlane(ahead, 15) + 1, sp.nk);
+        const int64_t from = part * size, to = parts == 1 || seen < from + size ? seen : from + size;
         const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
         const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
         T m = -(T)INFINITY, l = 0;
@@ -661,6 +704,11 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES) cached_attention_kernel(con
             load_k(k0);
             load_v(k0);
         }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) q[c].v[t] = CH * c + VEC * g + t < p.head_dim ? q[c].v[t] : (T)0;
+        poison_row<T, CHUNKS>(q);
         for (; k0 < to; k0 += 16 * W) {
             Acc sc = Acc{0, 0, 0, 0};
 #pragma unroll
@@ -745,75 +793,65 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES) cached_attention_kernel(con
                 for (int y = 0; y < NY; ++y) o[y] = Num<T>::mfma(v[x][y / N].v[y % N], sc[x], o[y]);
             load_v(k0 + 16 * W);
         }
-        // the wavefronts' sums, added in pairs
+        // the wavefronts' sums, added in their order
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0) {
             stat[wave][0][li] = m;
             stat[wave][1][li] = l;
         }
-        __syncthreads();
-        T top = stat[0][0][li];
-#pragma unroll
-        for (int w = 1; w < W; ++w) top = fmax(top, stat[w][0][li]);
-        const T ref = top == -(T)INFINITY ? (T)0 : top;
-        const T mine = Num<T>::exp_unit(m - ref);
-        T total = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) total += stat[w][1][li] * Num<T>::exp_unit(stat[w][0][li] - ref);
-#pragma unroll
-        for (int y = 0; y < NY; ++y)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[y][x] *= mine;
-#pragma unroll
-        for (int half = W / 2; half > 0; half /= 2) {
-            if (wave >= half && wave < 2 * half) {
-#pragma unroll
-                for (int y = 0; y < NY / N; ++y)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        Pack<T, N> e;
-#pragma unroll
-                        for (int t = 0; t < N; ++t) e.v[t] = o[N * y + t][x];
-                        *reinterpret_cast<Pack<T, N>*>(&sums[wave - half][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]) = e;
-                    }
-            }
-            __syncthreads();
-            if (wave < half) {
-#pragma unroll
-                for (int y = 0; y < NY / N; ++y)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const Pack<T, N> e = *reinterpret_cast<const Pack<T, N>*>(&sums[wave][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]);
-#pragma unroll
-                        for (int t = 0; t < N; ++t) o[N * y + t][x] += e.v[t];
-                    }
-            }
-        }
-        if (wave == 0 && r < rows) {
-            T by = 1;
-            T* __restrict__ dst;
-            if (parts == 1) {
-                by = last >= 0 && sp.nk > 0 ? 1 / total : (T)0;
-                dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
-            } else {
-                const int64_t at = (token * p.heads + head) * plan.most_parts + part;
-                dst = plan.data + at * p.head_dim;
-                if (g == 0) {
-                    plan.stat[2 * at] = top;
-                    plan.stat[2 * at + 1] = total;
-                }
-            }
+        const int here = (int)(rows - row0 < 16 ? rows - row0 : 16);
+        if (li < here) {
 #pragma unroll
             for (int y = 0; y < NY / N; ++y)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const int d = 16 * N * y + N * Num<T>::row(x, g);
+                    Pack<T, N> e;
 #pragma unroll
-                    for (int t = 0; t < N; ++t)
-                        if (d + t < p.head_dim) dst[d + t] = o[N * y + t][x] * by;
+                    for (int t = 0; t < N; ++t) e.v[t] = o[N * y + t][x];
+                    *reinterpret_cast<Pack<T, N>*>(&sums[wave][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]) = e;
                 }
         }
+        __syncthreads();
+        for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * W) {
+            const uint32_t row = at / (HDP / VEC), ahead_of = (row0 % p.group + row) / p.group;
+            const int d = at % (HDP / VEC) * VEC;
+            if (d >= p.head_dim) continue;
+            const int64_t to_token = sp.q0 + first_token + ahead_of;
+            const int to_head = kv * p.group + (int)(row0 + row - (first_token + ahead_of) * p.group);
+            T top = stat[0][0][row], total = 0, sum[VEC];
+#pragma unroll
+            for (int w = 1; w < W; ++w) top = fmax(top, stat[w][0][row]);
+            const T ref = top == -(T)INFINITY ? (T)0 : top;
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) sum[t] = 0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const T f = Num<T>::exp_unit(stat[w][0][row] - ref);
+                total = fma(stat[w][1][row], f, total);
+                const Pack<T, VEC> e = *reinterpret_cast<const Pack<T, VEC>*>(&sums[w][row * PITCH + d]);
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) sum[t] = fma(e.v[t], f, sum[t]);
+            }
+            T* __restrict__ dst;
+            if (parts == 1) {
+                const T by = first_last + ahead_of >= 0 && sp.nk > 0 ? 1 / total : (T)0;
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) sum[t] *= by;
+                dst = p.O + to_token * p.ldo + to_head * (int64_t)p.head_dim;
+            } else {
+                const int64_t place = (to_token * p.heads + to_head) * plan.most_parts + part;
+                dst = plan.data + place * p.head_dim;
+                if (d == 0) {
+                    plan.stat[2 * place] = top;
+                    plan.stat[2 * place + 1] = total;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < VEC; ++t)
+                if (d + t < p.head_dim) dst[d + t] = sum[t];
+        }
+        if (unit > ~0u - stride) return;
         __syncthreads();
     }
 }
@@ -836,7 +874,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p,
     if (begun == 0 || begun > p.sequences) return;
     const Span sp = span_of(p, begun - 1);
     if (token < sp.q0 || token >= sp.q0 + sp.nq) return;
-    const int parts = part_count(sp.nk, plan.most_parts);
+    const int parts = (int)part_count(sp.nk, (uint32_t)*plan.part_keys, plan.most_parts);
     if (parts == 1) return;
     const T m = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane)] : -(T)INFINITY;
     const T l = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane) + 1] : (T)0;
@@ -908,27 +946,34 @@ hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     return hipSuccess;
 }
 
-// Parts of a sequence's keys: none where a part would hold all of a cache.
-static int most_cached_parts(int64_t k_rows) { return k_rows <= 2 * CACHED_CHUNK ? 1 : (int)std::min<int64_t>((k_rows + CACHED_CHUNK - 1) / CACHED_CHUNK, 64); }
+// Parts of a sequence's keys at most: one where a cache is short, no more than a lane each, and few enough that rows with many
+// units do not need a large workspace.
+template <typename T>
+static int most_cached_parts(const CausalArgs<T>& a) {
+    if (a.k_rows <= CACHED_WHOLE) return 1;
+    const int64_t units = tile_slots(a.q_rows, a.group, 16, a.sequences) * a.kv_heads;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({64, (a.k_rows + CACHED_LEAST - 1) / CACHED_LEAST, 8 * CACHED_GROUPS / units}));
+}
 
 template <typename T>
 size_t cached_workspace_bytes(const CausalArgs<T>& a) {
-    const int parts = most_cached_parts(a.k_rows);
-    return parts == 1 ? 0 : (size_t)a.q_rows * a.heads * parts * (a.head_dim + 2) * sizeof(T);
+    const int parts = most_cached_parts(a);
+    return parts == 1 ? 0 : 16 + (size_t)a.q_rows * a.heads * parts * (a.head_dim + 2) * sizeof(T);
 }
 
 template <typename T>
 hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s) {
     CachedPlan<T> plan;
-    plan.most_parts = most_cached_parts(a.k_rows);
-    plan.data = static_cast<T*>(workspace);
+    plan.most_parts = most_cached_parts(a);
+    plan.part_keys = static_cast<int32_t*>(workspace);
+    plan.data = static_cast<T*>(workspace) + 16 / sizeof(T);
     plan.stat = plan.data + a.q_rows * a.heads * (int64_t)plan.most_parts * a.head_dim;
-    // a workgroup per unit if the sequences' keys are apart from each other; where they share keys, some take several
-    const int64_t tiles = tile_slots(a.q_rows, a.group, 16, a.sequences), each = std::max<int64_t>(1, tiles / a.sequences);
-    const int64_t units = std::min<int64_t>(tiles + (plan.most_parts == 1 ? 0 : each * (a.k_rows / CACHED_CHUNK)), 65536), rows = (a.q_rows * a.heads + 3) / 4;
-    if (!grid_fits(rows, 256)) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)units, a.kv_heads);
-    if (a.vec_kv) BY_HEAD_DIM_CACHED(true); else BY_HEAD_DIM_CACHED(false);
+    // a workgroup per unit of a call whose units run at once; of larger calls some take several
+    const int64_t tiles = tile_slots(a.q_rows, a.group, 16, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
+    const int64_t groups = std::min(tiles * plan.most_parts, std::max<int64_t>(1, (tiles * a.kv_heads <= CACHED_GROUPS / 2 ? 1 : 4) * CACHED_GROUPS / a.kv_heads));
+    if (!grid_fits(rows, 256) || a.q_rows > INT32_MAX / a.group - 16 || a.k_rows > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(groups * a.kv_heads));
+    if (a.vec_q && a.vec_kv) BY_HEAD_DIM_CACHED(true); else BY_HEAD_DIM_CACHED(false);
     if (hipError_t e = hipGetLastError()) return e;
     if (plan.most_parts > 1) {
         hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, plan);
