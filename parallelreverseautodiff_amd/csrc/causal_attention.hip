@@ -52,24 +52,6 @@ struct alignas(sizeof(T) * N) Pack {
 template <typename T> __device__ __forceinline__ bool is_finite(T x) { return fabs(x) < (T)INFINITY; }
 template <typename T> __device__ __forceinline__ T nan_of() { return (T)NAN; }
 
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-// Reductions over the 16 lanes that share a lane group (a row of an accumulator).
-template <typename T> __device__ __forceinline__ T max16(T v) {
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) v = fmax(v, __shfl_xor(v, m, 64));
-    return v;
-}
-template <typename T> __device__ __forceinline__ T sum16(T v) {
-#pragma unroll
-    for (int m = 1; m < 16; m <<= 1) v += __shfl_xor(v, m, 64);
-    return v;
-}
-
 // The rows and keys of one sequence.  Values that do not describe rows of the buffers are cut off to some that do.
 struct Span {
     int64_t q0, nq, k0, nk;
@@ -93,54 +75,6 @@ __device__ __forceinline__ Span span_of(const CausalArgs<T>& p, int s) {
     return r;
 }
 
-// Tiles of R packed rows are numbered through all sequences without a table: sequence s begins at number
-// floor(offset G / R) + s, which leaves room for its ceil(n G / R) tiles.  Finds the sequence of a tile and the tile's number
-// inside it; false: no such tile.
-template <int R, typename T>
-__device__ __forceinline__ bool find_tile(const CausalArgs<T>& p, int group, int64_t tile, int* sequence, int64_t* inside) {
-    int lo = 0, hi = p.sequences;  // the last s whose first tile is not behind `tile` lies in [lo - 1, hi)
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (clamped(p.q_off[mid], p.q_rows) * group / R + mid <= tile) lo = mid + 1;
-        else hi = mid;
-    }
-    if (lo == 0) return false;
-    *sequence = lo - 1;
-    *inside = tile - (clamped(p.q_off[lo - 1], p.q_rows) * group / R + (lo - 1));
-    return true;
-}
-
-// Elements [d0, d0 + VEC) of a row of head_dim elements, zeros past it.
-template <typename T>
-__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_pack(const T* __restrict__ row, int d0, int head_dim, bool vec) {
-    constexpr int VEC = 16 / sizeof(T);
-    Pack<T, VEC> v;
-#pragma unroll
-    for (int t = 0; t < VEC; ++t) v.v[t] = (T)0;
-    if (vec) {
-        if (d0 < head_dim) v = *reinterpret_cast<const Pack<T, VEC>*>(row + d0);
-    } else {
-#pragma unroll
-        for (int t = 0; t < VEC; ++t)
-            if (d0 + t < head_dim) v.v[t] = row[d0 + t];
-    }
-    return v;
-}
-
-// A row as the A operand of the matrix instructions: frag[c][t] = element CH c + VEC g + t.
-template <typename T, int HDP>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int g, int head_dim, bool vec, Pack<T, 16 / sizeof(T)> (&frag)[HDP / (64 / sizeof(T))]) {
-    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
-#pragma unroll
-    for (int c = 0; c < HDP / CH; ++c) {
-        if (row != nullptr) {
-            frag[c] = load_pack(row, CH * c + VEC * g, head_dim, vec);
-        } else {
-#pragma unroll
-            for (int t = 0; t < VEC; ++t) frag[c].v[t] = (T)0;
-        }
-    }
-}
 // Makes a row that holds a non-finite value NaN throughout.
 template <typename T, int CHUNKS>
 __device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNKS]) {
@@ -160,398 +94,25 @@ __device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNK
     }
 }
 
-// Stages two tiles of ROWS rows (of K and V, or of Q and dO) by 256 threads.  row_of(j, which) is the address of row j, nullptr
-// for a row that is not there: zeros.  A row with a non-finite value in either tile is staged as zeros in that tile and marked
-// with `tag`.
-template <typename T, int HDP, int ROWS, int PITCH, typename RowOf>
-__device__ __forceinline__ void stage_two(T* __restrict__ first, T* __restrict__ second, int* __restrict__ bad, int tag, int head_dim, bool vec, RowOf row_of) {
-    constexpr int VEC = 16 / sizeof(T), PER_ROW = HDP / VEC, COUNT = ROWS * PER_ROW / 256;
-    static_assert(ROWS * PER_ROW % 256 == 0, "whole rounds");
-    Pack<T, VEC> v[2][COUNT];
-#pragma unroll
-    for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int u = 0; u < COUNT; ++u) {
-            const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * VEC;
-            const T* __restrict__ row = row_of(j, which);
-            if (row != nullptr) {
-                v[which][u] = load_pack(row, d, head_dim, vec);
-            } else {
-#pragma unroll
-                for (int t = 0; t < VEC; ++t) v[which][u].v[t] = (T)0;
-            }
-        }
-#pragma unroll
-    for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int u = 0; u < COUNT; ++u) {
-            const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * VEC;
-            bool fine = true;
-#pragma unroll
-            for (int t = 0; t < VEC; ++t) fine = fine && is_finite(v[which][u].v[t]);
-            if (!fine) {
-                bad[j] = tag;
-#pragma unroll
-                for (int t = 0; t < VEC; ++t) v[which][u].v[t] = is_finite(v[which][u].v[t]) ? v[which][u].v[t] : (T)0;
-            }
-            *reinterpret_cast<Pack<T, VEC>*>((which == 0 ? first : second) + j * PITCH + d) = v[which][u];
-        }
-}
+// ---- units of work ----------------------------------------------------------------------------------------------------------
+// A unit is 16 packed rows of one sequence and key/value head against its keys or a part of them, one workgroup each; in the
+// gradients of K and V it is 16 keys against the rows.  Units are numbered through all sequences by a scan that every workgroup
+// does for itself: lengths live on the device.  The wavefronts take every fourth tile of 16 keys (or rows) and add their sums
+// up in LDS at the end, which gives short sequences four times the wavefronts.
+// Everything is transposed - S^T = K Q^T, O^T = V^T P^T - so that the weights come out of the first product in the lanes where
+// the second wants them and a row's statistics sit in a lane; rows go from memory to the registers of the matrix instructions
+// without LDS, along for a product over the head dimension and across for one over the rows.  The registers of an operand are
+// filled again for the next tile as soon as its product has read them, so that loads are always in flight.
+constexpr int WAVES = 4;
+// parts of the keys: the least keys in one, sequences that are not cut, units that run at once (two workgroups per compute unit)
+constexpr int LEAST_KEYS = 128, WHOLE_KEYS = 512, RUNNING = 512;
 
-// C[16 x 16 y] = A . B^T over the head dimension: A fragments in registers, rows 16 y + li of a staged tile.
-template <typename T, int HDP, int PITCH, int NY>
-__device__ __forceinline__ void rows_product(const Pack<T, 16 / sizeof(T)> (&a)[HDP / (64 / sizeof(T))], const T* __restrict__ tile, int li, int g,
-                                             typename Num<T>::Acc (&acc)[NY]) {
-    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
-#pragma unroll
-    for (int y = 0; y < NY; ++y) acc[y] = typename Num<T>::Acc{0, 0, 0, 0};
-#pragma unroll
-    for (int c = 0; c < HDP / CH; ++c) {
-        Pack<T, VEC> b[NY];
-#pragma unroll
-        for (int y = 0; y < NY; ++y) b[y] = *reinterpret_cast<const Pack<T, VEC>*>(tile + (16 * y + li) * PITCH + CH * c + VEC * g);
-#pragma unroll
-        for (int t = 0; t < VEC; ++t)
-#pragma unroll
-            for (int y = 0; y < NY; ++y) acc[y] = Num<T>::mfma(a[c].v[t], b[y].v[t], acc[y]);
-    }
-}
-
-// out[16 x HDP] += W . X: weights of 16 rows over COLS columns in the wavefront's tile w, staged rows of X.
-template <typename T, int HDP, int COLS, int WPITCH, int PITCH>
-__device__ __forceinline__ void weights_product(const T* __restrict__ w, const T* __restrict__ x, int li, int g, typename Num<T>::Acc (&out)[HDP / 16]) {
-    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC;
-#pragma unroll
-    for (int c = 0; c < COLS / CH; ++c) {
-        const Pack<T, VEC> a = *reinterpret_cast<const Pack<T, VEC>*>(w + li * WPITCH + CH * c + VEC * g);
-#pragma unroll
-        for (int t = 0; t < VEC; ++t)
-#pragma unroll
-            for (int y = 0; y < HDP / 16; ++y) out[y] = Num<T>::mfma(a.v[t], x[(CH * c + VEC * g + t) * PITCH + 16 * y + li], out[y]);
-    }
-}
-
-// Columns of a tile and the pitches of the staged tiles: a 16-byte pad spreads the rows over the LDS banks.
-template <typename T, int HDP> struct Tile {
-    static constexpr int VEC = 16 / sizeof(T);
-    static constexpr int COLS = sizeof(T) * HDP > 512 ? 16 : 32;
-    static constexpr int PITCH = HDP + VEC, WPITCH = COLS + VEC, NY = COLS / 16;
-};
-
-// Running softmax statistics of the four rows a lane holds, over one tile of scores.  On return s holds the weights and the
-// factors of the old sums.
-template <typename T, int NY>
-__device__ __forceinline__ void softmax_tile(typename Num<T>::Acc (&s)[NY], T (&m)[4], T (&l)[4], T (&factor)[4]) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        T top = s[0][r];
-#pragma unroll
-        for (int y = 1; y < NY; ++y) top = fmax(top, s[y][r]);
-        top = fmax(m[r], max16(top));
-        const T ref = top == -(T)INFINITY ? (T)0 : top;  // nothing seen yet: every weight below is exp(-inf) = 0
-        factor[r] = Num<T>::exp_unit(m[r] - ref);
-        T sum = 0;
-#pragma unroll
-        for (int y = 0; y < NY; ++y) {
-            s[y][r] = Num<T>::exp_unit(s[y][r] - ref);
-            sum += s[y][r];
-        }
-        l[r] = l[r] * factor[r] + sum16(sum);
-        m[r] = top;
-    }
-}
-
-// ---- forward ------------------------------------------------------------------------------------------------------------
-// A workgroup takes 64 packed rows of a key/value head, a wavefront 16 of them; K and V pass through LDS in tiles of COLS keys.
-template <typename T, int HDP>
-__global__ void __launch_bounds__(256) causal_fwd_kernel(const CausalArgs<T> p) {
-    typedef Tile<T, HDP> TL;
-    typedef typename Num<T>::Acc Acc;
-    constexpr int CHUNKS = HDP / (4 * TL::VEC);
-    __shared__ __attribute__((aligned(16))) T ks[TL::COLS * TL::PITCH], vs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
-    __shared__ int bad[TL::COLS];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.y;
-    int s;
-    int64_t inside;
-    if (!find_tile<64>(p, p.group, (int64_t)gridDim.x - 1 - blockIdx.x, &s, &inside)) return;  // (late tiles see the most keys: first)
-    const Span sp = span_of(p, s);
-    const int64_t rows = sp.nq * p.group, row0 = inside * 64;
-    if (row0 >= rows) return;
-    if (threadIdx.x < TL::COLS) bad[threadIdx.x] = -1;
-    const int64_t lead = sp.nk - sp.nq;  // query i sees keys up to lead + i
-    Pack<T, TL::VEC> q[CHUNKS];
-    {
-        const int64_t r = row0 + 16 * wave + li;
-        const T* row = r < rows ? p.Q + (sp.q0 + r / p.group) * p.ldq + (kv * p.group + r % p.group) * (int64_t)p.head_dim : nullptr;
-        load_row<T, HDP>(row, g, p.head_dim, p.vec_q, q);
-        poison_row<T, CHUNKS>(q);
-    }
-    int64_t last[4];  // the last key that each of the lane's rows sees
-#pragma unroll
-    for (int r = 0; r < 4; ++r) last[r] = lead + (row0 + 16 * wave + Num<T>::row(r, g)) / p.group;
-    T m[4], l[4];
-    Acc o[HDP / 16];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) { m[r] = -(T)INFINITY; l[r] = 0; }
-#pragma unroll
-    for (int y = 0; y < HDP / 16; ++y) o[y] = Acc{0, 0, 0, 0};
-    const int64_t last_row = row0 + 63 < rows ? row0 + 63 : rows - 1;
-    const int64_t seen = clamped(lead + last_row / p.group + 1, sp.nk);
-    const T factor = p.scale * Num<T>::unit();
-    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
-    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
-    for (int64_t k0 = 0; k0 < seen; k0 += TL::COLS) {
-        const int tag = (int)(k0 / TL::COLS);
-        __syncthreads();
-        stage_two<T, HDP, TL::COLS, TL::PITCH>(ks, vs, bad, tag, p.head_dim, p.vec_kv, [&](int j, int which) -> const T* {
-            if (k0 + j >= sp.nk) return nullptr;
-            return which == 0 ? K + (k0 + j) * p.ldk : V + (k0 + j) * p.ldv;
-        });
-        __syncthreads();
-        Acc acc[TL::NY];
-        rows_product<T, HDP, TL::PITCH, TL::NY>(q, ks, li, g, acc);
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y) {
-            const int64_t j = k0 + 16 * y + li;
-            const bool poisoned = bad[16 * y + li] == tag;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[y][r] = j > last[r] ? -(T)INFINITY : poisoned ? nan_of<T>() : acc[y][r] * factor;
-        }
-        T fac[4];
-        softmax_tile<T, TL::NY>(acc, m, l, fac);
-#pragma unroll
-        for (int y = 0; y < HDP / 16; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[y][r] *= fac[r];
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ws[wave][Num<T>::row(r, g) * TL::WPITCH + 16 * y + li] = acc[y][r];
-        wave_sync();
-        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], vs, li, g, o);
-        wave_sync();
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
-        if (row >= rows) continue;
-        const int64_t token = sp.q0 + row / p.group;
-        const int head = kv * p.group + (int)(row % p.group);
-        const bool any = last[r] >= 0;
-        const T inv = any ? (T)1 / l[r] : (T)0;
-        T* dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
-#pragma unroll
-        for (int y = 0; y < HDP / 16; ++y)
-            if (16 * y + li < p.head_dim) dst[16 * y + li] = any ? o[y][r] * inv : (T)0;
-        if (p.lse != nullptr && li == 0) p.lse[head * p.q_rows + token] = any ? Num<T>::log_sum(m[r], l[r]) : -(T)INFINITY;
-    }
-}
-
-// ---- backward -----------------------------------------------------------------------------------------------------------
-// D = rowsum(dO (.) O) per token and head, 16 lanes to a row; NaN for a row of dO with a non-finite value.
 template <typename T>
-__global__ void __launch_bounds__(256) causal_dot_kernel(const CausalArgs<T> p) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-    const int lane = threadIdx.x & 15;
-    if (at >= p.q_rows * p.heads) return;
-    const int64_t token = at / p.heads;
-    const int head = (int)(at % p.heads);
-    const T* __restrict__ o = p.O + token * p.ldo + head * (int64_t)p.head_dim;
-    const T* __restrict__ g = p.dO + token * p.ldo + head * (int64_t)p.head_dim;
-    T sum = 0, check = 0;
-    for (int d = lane; d < p.head_dim; d += 16) {
-        sum += o[d] * g[d];
-        check += is_finite(g[d]) ? (T)0 : nan_of<T>();
-    }
-    sum = sum16(sum + check);
-    if (lane == 0) p.D[head * p.q_rows + token] = is_finite(sum) ? sum : nan_of<T>();
-}
-
-// Gradients of K and V: a workgroup owns 64 keys of a key/value head (a wavefront 16, its rows of K and V in registers) and
-// walks the packed query rows that see them, all heads of the group among them, in tiles of COLS.
-template <typename T, int HDP>
-__global__ void __launch_bounds__(256) causal_bwd_kv_kernel(const CausalArgs<T> p) {
-    typedef Tile<T, HDP> TL;
-    typedef typename Num<T>::Acc Acc;
-    constexpr int CHUNKS = HDP / (4 * TL::VEC);
-    __shared__ __attribute__((aligned(16))) T qs[TL::COLS * TL::PITCH], gs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
-    __shared__ T row_lse[TL::COLS], row_dot[TL::COLS];
-    __shared__ int bad[TL::COLS];  // written by the staging; rows with a non-finite value already have a NaN in lse or D
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.y;
-    int s;
-    int64_t inside;
-    if (!find_tile<64>(p, 1, blockIdx.x, &s, &inside)) return;  // (tiles of keys are numbered like packed rows of one head)
-    const Span sp = span_of(p, s);
-    const int64_t key0 = inside * 64, rows = sp.nq * p.group;
-    if (key0 >= sp.nk) return;
-    const int64_t key = key0 + 16 * wave + li;
-    Pack<T, TL::VEC> k[CHUNKS], v[CHUNKS];
-    load_row<T, HDP>(key < sp.nk ? p.K + (sp.k0 + key) * p.ldk + kv * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_kv, k);
-    load_row<T, HDP>(key < sp.nk ? p.V + (sp.k0 + key) * p.ldv + kv * (int64_t)p.head_dim : nullptr, g, p.head_dim, p.vec_kv, v);
-    Acc dk[HDP / 16], dv[HDP / 16];
-#pragma unroll
-    for (int y = 0; y < HDP / 16; ++y) dk[y] = dv[y] = Acc{0, 0, 0, 0};
-    const T factor = p.scale * Num<T>::unit();
-    // (queries and keys are the same rows here: token i sees key j iff j <= i)
-    for (int64_t r0 = key0 * p.group / TL::COLS * TL::COLS; r0 < rows; r0 += TL::COLS) {
-        __syncthreads();
-        if (threadIdx.x < TL::COLS) {
-            const int64_t r = r0 + threadIdx.x;
-            T lse = 0, dot = 0;
-            if (r < rows) {
-                const int64_t at = (kv * p.group + r % p.group) * p.q_rows + sp.q0 + r / p.group;
-                dot = p.D[at];
-                lse = p.lse[at] * Num<T>::unit() + (dot - dot);  // NaN where D is
-            }
-            row_lse[threadIdx.x] = lse;
-            row_dot[threadIdx.x] = dot;
-        }
-        stage_two<T, HDP, TL::COLS, TL::PITCH>(qs, gs, bad, 0, p.head_dim, p.vec_q && p.vec_o, [&](int j, int which) -> const T* {
-            const int64_t r = r0 + j;
-            if (r >= rows) return nullptr;
-            const int64_t token = sp.q0 + r / p.group, col = (kv * p.group + r % p.group) * (int64_t)p.head_dim;
-            return which == 0 ? p.Q + token * p.ldq + col : p.dO + token * p.ldo + col;
-        });
-        __syncthreads();
-        Acc st[TL::NY], dp[TL::NY];
-        rows_product<T, HDP, TL::PITCH, TL::NY>(k, qs, li, g, st);   // S^T: rows are keys, columns query rows
-        rows_product<T, HDP, TL::PITCH, TL::NY>(v, gs, li, g, dp);   // (dO V^T)^T
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y) {
-            const int64_t r = r0 + 16 * y + li, token = r / p.group;
-            const T lse = row_lse[16 * y + li], dot = row_dot[16 * y + li];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool seen = r < rows && key0 + 16 * wave + Num<T>::row(e, g) <= token;
-                const T w = seen ? Num<T>::exp_unit(st[y][e] * factor - lse) : (T)0;
-                st[y][e] = w;
-                dp[y][e] = seen ? w * (dp[y][e] - dot) : (T)0;
-            }
-        }
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ws[wave][Num<T>::row(e, g) * TL::WPITCH + 16 * y + li] = st[y][e];
-        wave_sync();
-        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], gs, li, g, dv);
-        wave_sync();
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) ws[wave][Num<T>::row(e, g) * TL::WPITCH + 16 * y + li] = dp[y][e];
-        wave_sync();
-        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], qs, li, g, dk);
-        wave_sync();
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int64_t j = key0 + 16 * wave + Num<T>::row(e, g);
-        if (j >= sp.nk) continue;
-        T* dst_k = p.dK + (sp.k0 + j) * p.lddk + kv * (int64_t)p.head_dim;
-        T* dst_v = p.dV + (sp.k0 + j) * p.lddv + kv * (int64_t)p.head_dim;
-#pragma unroll
-        for (int y = 0; y < HDP / 16; ++y)
-            if (16 * y + li < p.head_dim) {
-                dst_k[16 * y + li] = dk[y][e] * p.scale;
-                dst_v[16 * y + li] = dv[y][e];
-            }
-    }
-}
-
-// Gradient of Q: tiles as in the forward kernel, the rows of Q and dO in registers.
-template <typename T, int HDP>
-__global__ void __launch_bounds__(256) causal_bwd_q_kernel(const CausalArgs<T> p) {
-    typedef Tile<T, HDP> TL;
-    typedef typename Num<T>::Acc Acc;
-    constexpr int CHUNKS = HDP / (4 * TL::VEC);
-    __shared__ __attribute__((aligned(16))) T ks[TL::COLS * TL::PITCH], vs[TL::COLS * TL::PITCH], ws[4][16 * TL::WPITCH];
-    __shared__ int bad[TL::COLS];  // written by the staging; rows that see such a key already have a NaN in lse
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
-    const int kv = blockIdx.y;
-    int s;
-    int64_t inside;
-    if (!find_tile<64>(p, p.group, (int64_t)gridDim.x - 1 - blockIdx.x, &s, &inside)) return;
-    const Span sp = span_of(p, s);
-    const int64_t rows = sp.nq * p.group, row0 = inside * 64;
-    if (row0 >= rows) return;
-    Pack<T, TL::VEC> q[CHUNKS], go[CHUNKS];
-    {
-        const int64_t r = row0 + 16 * wave + li;
-        const int64_t token = sp.q0 + r / p.group, col = (kv * p.group + r % p.group) * (int64_t)p.head_dim;
-        load_row<T, HDP>(r < rows ? p.Q + token * p.ldq + col : nullptr, g, p.head_dim, p.vec_q, q);
-        load_row<T, HDP>(r < rows ? p.dO + token * p.ldo + col : nullptr, g, p.head_dim, p.vec_o, go);
-    }
-    int64_t last[4];
-    T lse[4], dot[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
-        last[r] = row < rows ? row / p.group : -1;
-        lse[r] = dot[r] = 0;
-        if (row < rows) {
-            const int64_t at = (kv * p.group + row % p.group) * p.q_rows + sp.q0 + row / p.group;
-            dot[r] = p.D[at];
-            lse[r] = p.lse[at] * Num<T>::unit() + (dot[r] - dot[r]);
-        }
-    }
-    Acc dq[HDP / 16];
-#pragma unroll
-    for (int y = 0; y < HDP / 16; ++y) dq[y] = Acc{0, 0, 0, 0};
-    const int64_t last_row = row0 + 63 < rows ? row0 + 63 : rows - 1;
-    const int64_t seen = last_row / p.group + 1;
-    const T factor = p.scale * Num<T>::unit();
-    const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
-    const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
-    for (int64_t k0 = 0; k0 < seen; k0 += TL::COLS) {
-        __syncthreads();
-        stage_two<T, HDP, TL::COLS, TL::PITCH>(ks, vs, bad, 0, p.head_dim, p.vec_kv, [&](int j, int which) -> const T* {
-            if (k0 + j >= sp.nk) return nullptr;
-            return which == 0 ? K + (k0 + j) * p.ldk : V + (k0 + j) * p.ldv;
-        });
-        __syncthreads();
-        Acc st[TL::NY], dp[TL::NY];
-        rows_product<T, HDP, TL::PITCH, TL::NY>(q, ks, li, g, st);
-        rows_product<T, HDP, TL::PITCH, TL::NY>(go, vs, li, g, dp);
-#pragma unroll
-        for (int y = 0; y < TL::NY; ++y) {
-            const int64_t j = k0 + 16 * y + li;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const T w = Num<T>::exp_unit(st[y][r] * factor - lse[r]);
-                ws[wave][Num<T>::row(r, g) * TL::WPITCH + 16 * y + li] = j <= last[r] ? w * (dp[y][r] - dot[r]) : (T)0;
-            }
-        }
-        wave_sync();
-        weights_product<T, HDP, TL::COLS, TL::WPITCH, TL::PITCH>(ws[wave], ks, li, g, dq);
-        wave_sync();
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t row = row0 + 16 * wave + Num<T>::row(r, g);
-        if (row >= rows) continue;
-        T* dst = p.dQ + (sp.q0 + row / p.group) * p.lddq + (kv * p.group + row % p.group) * (int64_t)p.head_dim;
-#pragma unroll
-        for (int y = 0; y < HDP / 16; ++y)
-            if (16 * y + li < p.head_dim) dst[16 * y + li] = dq[y][r] * p.scale;
-    }
-}
-
-// ---- the newest tokens of a sequence against its cache --------------------------------------------------------------------
-// Bound by reading the cache once.  Work is cut into units of one sequence: 16 packed rows against one part of its keys, one
-// workgroup each, numbered through all sequences by a scan that every workgroup does for itself (lengths live on the device).
-// A wavefront takes every fourth tile of 16 keys.  Everything is transposed - S^T = K Q^T, O^T = V^T P^T - so that the weights
-// come out of the first product in the lanes where the second wants them, a row's statistics sit in a lane, and K and V go
-// from memory to the registers of the matrix instructions without LDS.  Each operand's registers are filled again for the next
-// tile as soon as its product has read them, so that loads are always in flight.
-template <typename T>
-struct CachedPlan {
-    int most_parts;     // of a sequence
-    T *stat, *data;     // of part i of packed row r: {maximum, sum} and the weighted sum of values, at r * most_parts + i
-    int32_t* part_keys; // how many keys make a part, for the join
+struct Parts {
+    int most;         // of a sequence
+    T *stat, *data;   // of part i of (token, head) number n: {maximum, sum} and the weighted sum of values, at n * most + i
+    int32_t* keys;    // how many keys make a part, for the join
 };
-constexpr int CACHED_WAVES = 4, CACHED_LEAST = 128, CACHED_WHOLE = 512, CACHED_GROUPS = 512;
 
 // Parts of a sequence's keys: of `size` keys, or of more if there would be too many parts, whole tiles.
 __device__ __forceinline__ int64_t part_keys(int64_t keys, int64_t size, int most_parts) {
@@ -559,7 +120,7 @@ __device__ __forceinline__ int64_t part_keys(int64_t keys, int64_t size, int mos
     return ((keys + most_parts - 1) / most_parts + 15) / 16 * 16;
 }
 __device__ __forceinline__ uint32_t part_count(int64_t keys, uint32_t size, int most_parts) {
-    if (keys <= CACHED_WHOLE || keys <= size || most_parts == 1) return 1;
+    if (keys <= WHOLE_KEYS || keys <= size || most_parts == 1) return 1;
     if (keys <= (int64_t)size * most_parts) return ((uint32_t)keys + size - 1) / size;
     const int64_t larger = part_keys(keys, size, most_parts);
     return (uint32_t)((keys + larger - 1) / larger);
@@ -579,7 +140,7 @@ __device__ __forceinline__ uint32_t scan64(uint32_t x) {
 // The sequence of unit `unit` and the unit's number inside it, by a whole wavefront; false: there are not so many.  (Rows fit
 // into 31 bits, so a sequence has less than 2^32 units.  Offsets that overlap may wrap the sum: the caller checks the number.)
 template <typename T>
-__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts, uint32_t size, uint32_t unit, int lane, Span* span, uint32_t* parts, uint32_t* inside) {
+__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int group, int most_parts, uint32_t size, uint32_t unit, int lane, Span* span, uint32_t* parts, uint32_t* inside) {
     uint32_t before = 0;
     for (int s0 = 0; s0 < p.sequences; s0 += 64) {
         Span sp = {0, 0, 0, 0};
@@ -587,7 +148,7 @@ __device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts
         if (s0 + lane < p.sequences) {
             sp = span_of(p, s0 + lane);
             count = part_count(sp.nk, size, most_parts);
-            units = ((uint32_t)sp.nq * (uint32_t)p.group + 15) / 16 * count;
+            units = ((uint32_t)sp.nq * (uint32_t)group + 15) / 16 * count;
         }
         const uint32_t upto = before + scan64(units);
         const uint64_t behind = __ballot(upto > unit);
@@ -624,8 +185,8 @@ __device__ __forceinline__ uint32_t keys_per_part(const CausalArgs<T>& p, int mo
         keys += __shfl_xor(keys, d, 64);
         tiles += __shfl_xor(tiles, d, 64);
     }
-    const float room = fmaxf((float)(CACHED_GROUPS / 2), CACHED_GROUPS - tiles * p.kv_heads), share = keys * p.kv_heads / room;
-    return __builtin_amdgcn_readfirstlane(((uint32_t)fminf(fmaxf(share, (float)CACHED_LEAST), 1e9f) + 63) / 64 * 64);
+    const float room = fmaxf((float)(RUNNING / 2), RUNNING - tiles * p.kv_heads), share = keys * p.kv_heads / room;
+    return __builtin_amdgcn_readfirstlane(((uint32_t)fminf(fmaxf(share, (float)LEAST_KEYS), 1e9f) + 63) / 64 * 64);
 }
 
 // N consecutive elements; columns past the row's end are read at its start, for which nothing uses the result.
@@ -641,22 +202,113 @@ __device__ __forceinline__ Pack<T, N> load_some(const T* __restrict__ row, int d
     return v;
 }
 
+// A row along the reduction of a product over the head dimension: elements CH c + VEC g + t.
 template <typename T, int HDP, bool ALIGNED>
-__global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) cached_attention_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
-    constexpr int VEC = 16 / sizeof(T), CH = 4 * VEC, CHUNKS = HDP / CH, NY = HDP / 16, N = VEC < NY ? VEC : NY, W = CACHED_WAVES, PITCH = HDP + VEC;
+__device__ __forceinline__ void load_along(const T* __restrict__ row, int g, int head_dim, Pack<T, 16 / sizeof(T)> (&to)[HDP * sizeof(T) / 64]) {
+    constexpr int VEC = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < HDP / (4 * VEC); ++c) to[c] = load_some<T, VEC, ALIGNED>(row, 4 * VEC * c + VEC * g, head_dim);
+}
+template <typename T, int HDP>
+__device__ __forceinline__ void zero_past(int g, int head_dim, Pack<T, 16 / sizeof(T)> (&frag)[HDP * sizeof(T) / 64]) {
+    constexpr int VEC = 16 / sizeof(T);
+#pragma unroll
+    for (int c = 0; c < HDP / (4 * VEC); ++c)
+#pragma unroll
+        for (int t = 0; t < VEC; ++t) frag[c].v[t] = 4 * VEC * c + VEC * g + t < head_dim ? frag[c].v[t] : (T)0;
+}
+// A row across, a column per lane: columns 16 N y + N li + t.
+template <typename T, int HDP> constexpr int columns_at_once() { return 16 / (int)sizeof(T) < HDP / 16 ? 16 / (int)sizeof(T) : HDP / 16; }
+template <typename T, int HDP, bool ALIGNED>
+__device__ __forceinline__ void load_across(const T* __restrict__ row, int li, int head_dim, Pack<T, columns_at_once<T, HDP>()> (&to)[HDP / 16 / columns_at_once<T, HDP>()]) {
+    constexpr int N = columns_at_once<T, HDP>();
+#pragma unroll
+    for (int y = 0; y < HDP / 16 / N; ++y) to[y] = load_some<T, N, ALIGNED>(row, 16 * N * y + N * li, head_dim);
+}
+// Zeros for the non-finite values of a tile that is read across; returns a bit for each of its rows that has one.
+template <typename T, int N, int COUNT>
+__device__ __forceinline__ uint32_t zero_bad(Pack<T, N> (&v)[4][COUNT]) {
+    T odd = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < COUNT; ++y)
+#pragma unroll
+            for (int t = 0; t < N; ++t) odd = fma(v[x][y].v[t], (T)0, odd);
+    uint32_t rows = 0;
+    if (__any(!(odd == 0))) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            bool fine = true;
+#pragma unroll
+            for (int y = 0; y < COUNT; ++y)
+#pragma unroll
+                for (int t = 0; t < N; ++t) {
+                    fine = fine && is_finite(v[x][y].v[t]);
+                    v[x][y].v[t] = is_finite(v[x][y].v[t]) ? v[x][y].v[t] : (T)0;
+                }
+            const uint64_t b = __ballot(!fine);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if ((b >> (16 * i)) & 0xFFFFu) rows |= 1u << Num<T>::row(x, i);
+        }
+    }
+    return rows;
+}
+// The product of two tiles over the head dimension: rows of the accumulator are rows of a, columns rows of b.
+template <typename T, int COUNT>
+__device__ __forceinline__ typename Num<T>::Acc product(const Pack<T, 16 / sizeof(T)> (&a)[COUNT], const Pack<T, 16 / sizeof(T)> (&b)[COUNT]) {
+    typename Num<T>::Acc acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c)
+#pragma unroll
+        for (int t = 0; t < 16 / (int)sizeof(T); ++t) acc = Num<T>::mfma(a[c].v[t], b[c].v[t], acc);
+    return acc;
+}
+// out += rows that are read across, transposed, times the weights of those rows.
+template <typename T, int N, int COUNT>
+__device__ __forceinline__ void add_weighted(const Pack<T, N> (&v)[4][COUNT], typename Num<T>::Acc w, typename Num<T>::Acc (&out)[N * COUNT]) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < N * COUNT; ++y) out[y] = Num<T>::mfma(v[x][y / N].v[y % N], w[x], out[y]);
+}
+// A wavefront's sums to LDS: out[N y + t][x] is column 16 N y + N row(x, g) + t of row li.
+template <typename T, int N, int TILES, int PITCH>
+__device__ __forceinline__ void put_sums(const typename Num<T>::Acc (&out)[TILES], int li, int g, T* __restrict__ to) {
+#pragma unroll
+    for (int y = 0; y < TILES / N; ++y)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            Pack<T, N> e;
+#pragma unroll
+            for (int t = 0; t < N; ++t) e.v[t] = out[N * y + t][x];
+            *reinterpret_cast<Pack<T, N>*>(&to[li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]) = e;
+        }
+}
+
+// x / group for x < group + 16
+__device__ __forceinline__ uint32_t heads_over(uint32_t x, uint32_t group, uint32_t inverse) { return group < 16 ? x * inverse >> 16 : x >= group; }
+__device__ __forceinline__ uint32_t inverse_of(uint32_t group) { return (65535 + group) / group; }  // of 2^16, rounded up
+
+// ---- forward, and the newest tokens of a sequence against its cache ---------------------------------------------------------
+template <typename T, int HDP, bool ALIGNED>
+__global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) attention_kernel(const CausalArgs<T> p, const Parts<T> cut) {
+    constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
-    __shared__ __attribute__((aligned(16))) T sums[W][16 * PITCH];
-    __shared__ T stat[W][2][16];
+    __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
+    __shared__ T stat[WAVES][2][16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     // heads of a unit are neighbours, so that workgroups without a unit come last
     const uint32_t stride = gridDim.x / p.kv_heads;
     const int kv = (int)(blockIdx.x % p.kv_heads);
-    const uint32_t keys_each = keys_per_part(p, plan.most_parts, lane);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && plan.most_parts > 1) *plan.part_keys = (int32_t)keys_each;
+    const uint32_t keys_each = keys_per_part(p, cut.most, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && cut.most > 1) *cut.keys = (int32_t)keys_each;
+    const T factor = p.scale * Num<T>::unit();
     for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
         Span sp;
         uint32_t parts, inside;
-        if (!find_unit(p, plan.most_parts, keys_each, unit, lane, &sp, &parts, &inside)) return;
+        if (!find_unit(p, p.group, cut.most, keys_each, unit, lane, &sp, &parts, &inside)) return;
         const uint32_t rows = (uint32_t)sp.nq * (uint32_t)p.group, tile = inside / parts, part = inside % parts, row0 = tile * 16;
         if (tile >= (rows + 15) / 16) return;  // (a wrapped sum)
         const int64_t lead = sp.nk - sp.nq;
@@ -665,38 +317,29 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
         const int64_t token = sp.q0 + first_token + ahead;
         const int head = kv * p.group + (int)(r - (first_token + ahead) * p.group);
         Pack<T, VEC> q[CHUNKS];
-        {
-            const T* __restrict__ row = p.Q + token * p.ldq + head * (int64_t)p.head_dim;
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) q[c] = load_some<T, VEC, ALIGNED>(row, CH * c + VEC * g, p.head_dim);
-        }
+        load_along<T, HDP, ALIGNED>(p.Q + token * p.ldq + head * (int64_t)p.head_dim, g, p.head_dim, q);
         const int64_t first_last = lead + first_token, last = first_last + ahead;  // the last key that the tile's first row sees, that this one does
-        const int64_t size = part_keys(sp.nk, keys_each, plan.most_parts), seen = clamped(first_last + (int)__builtin_amdgcn_readlane(ahead, 15) + 1, sp.nk);
+        const int64_t size = part_keys(sp.nk, keys_each, cut.most), seen = clamped(first_last + (int)__builtin_amdgcn_readlane(ahead, 15) + 1, sp.nk);
         const int64_t from = part * size, to = parts == 1 || seen < from + size ? seen : from + size;
         const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
         const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
-        T m = -(T)INFINITY, l = 0;
-        Acc o[NY];  // element r of o[N y + t]: column 16 N y + N row(r, g) + t of row li
+        T m = -(T)INFINITY, l = 0;  // l: this lane's share
+        Acc o[NY];  // element x of o[N y + t]: column 16 N y + N row(x, g) + t of row li
 #pragma unroll
         for (int y = 0; y < NY; ++y) o[y] = Acc{0, 0, 0, 0};
-        const T factor = p.scale * Num<T>::unit();
-        Pack<T, VEC> k[CHUNKS];   // key li, elements CH c + VEC g + t
-        Pack<T, N> v[4][NY / N];  // keys row(x, g), columns 16 N y + N li + t
+        Pack<T, VEC> k[CHUNKS];   // of key li
+        Pack<T, N> v[4][NY / N];  // of keys row(x, g)
         // keys past the last are the last one again: their scores are masked
         auto load_k = [&](int64_t k0) {
             const int most = (int)(to - 1 - k0 < 15 ? to - 1 - k0 : 15);
-            const T* __restrict__ row = K + k0 * p.ldk + (li < most ? li : most) * p.ldk;
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) k[c] = load_some<T, VEC, ALIGNED>(row, CH * c + VEC * g, p.head_dim);
+            load_along<T, HDP, ALIGNED>(K + k0 * p.ldk + (li < most ? li : most) * p.ldk, g, p.head_dim, k);
         };
         auto load_v = [&](int64_t k0) {
             const int most = (int)(to - 1 - k0 < 15 ? to - 1 - k0 : 15);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int j = Num<T>::row(x, g);
-                const T* __restrict__ row = V + k0 * p.ldv + (j < most ? j : most) * p.ldv;
-#pragma unroll
-                for (int y = 0; y < NY / N; ++y) v[x][y] = load_some<T, N, ALIGNED>(row, 16 * N * y + N * li, p.head_dim);
+                load_across<T, HDP, ALIGNED>(V + k0 * p.ldv + (j < most ? j : most) * p.ldv, li, p.head_dim, v[x]);
             }
         };
         int64_t k0 = from + 16 * wave;
@@ -704,17 +347,10 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
             load_k(k0);
             load_v(k0);
         }
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-            for (int t = 0; t < VEC; ++t) q[c].v[t] = CH * c + VEC * g + t < p.head_dim ? q[c].v[t] : (T)0;
+        zero_past<T, HDP>(g, p.head_dim, q);
         poison_row<T, CHUNKS>(q);
-        for (; k0 < to; k0 += 16 * W) {
-            Acc sc = Acc{0, 0, 0, 0};
-#pragma unroll
-            for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-                for (int t = 0; t < VEC; ++t) sc = Num<T>::mfma(k[c].v[t], q[c].v[t], sc);
+        for (; k0 < to; k0 += 16 * WAVES) {
+            Acc sc = product<T>(k, q);
             // A key with a non-finite value is NaN for the rows that see it and zeros for the others.  In K it makes the scores
             // of its key non-finite whatever the rows hold, so that K is looked at only after such a score.
             uint32_t poisoned = 0;  // bit j: key k0 + j
@@ -730,32 +366,8 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
                 const uint64_t b = __ballot(!fine);
                 poisoned = (uint32_t)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xFFFFu);
             }
-            load_k(k0 + 16 * W);
-            odd = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int y = 0; y < NY / N; ++y)
-#pragma unroll
-                    for (int t = 0; t < N; ++t) odd = fma(v[x][y].v[t], (T)0, odd);
-            if (__any(!(odd == 0))) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    bool fine = true;
-#pragma unroll
-                    for (int y = 0; y < NY / N; ++y)
-#pragma unroll
-                        for (int t = 0; t < N; ++t) {
-                            fine = fine && is_finite(v[x][y].v[t]);
-                            v[x][y].v[t] = is_finite(v[x][y].v[t]) ? v[x][y].v[t] : (T)0;
-                        }
-                    const uint64_t b = __ballot(!fine);
-#pragma unroll
-                    for (int gg = 0; gg < 4; ++gg)
-                        if ((b >> (16 * gg)) & 0xFFFFu) poisoned |= 1u << Num<T>::row(x, gg);
-                }
-            }
-            T top = -(T)INFINITY;
+            load_k(k0 + 16 * WAVES);
+            poisoned |= zero_bad<T>(v);
 #pragma unroll
             for (int x = 0; x < 4; ++x) sc[x] *= factor;
             if (poisoned != 0 || k0 + 15 > first_last) {
@@ -766,6 +378,7 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
                     sc[x] = j >= most ? -(T)INFINITY : (poisoned >> j) & 1 ? nan_of<T>() : sc[x];
                 }
             }
+            T top = -(T)INFINITY;
 #pragma unroll
             for (int x = 0; x < 4; ++x) top = fmax(top, sc[x]);
             // the maximum is raised for a tile only if one of its scores is above it
@@ -787,33 +400,19 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
                 sc[x] = Num<T>::exp_unit(sc[x] - ref);
                 l += sc[x];
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int y = 0; y < NY; ++y) o[y] = Num<T>::mfma(v[x][y / N].v[y % N], sc[x], o[y]);
-            load_v(k0 + 16 * W);
+            add_weighted<T>(v, sc, o);
+            load_v(k0 + 16 * WAVES);
         }
-        // the wavefronts' sums, added in their order
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         if (g == 0) {
             stat[wave][0][li] = m;
             stat[wave][1][li] = l;
         }
-        const int here = (int)(rows - row0 < 16 ? rows - row0 : 16);
-        if (li < here) {
-#pragma unroll
-            for (int y = 0; y < NY / N; ++y)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    Pack<T, N> e;
-#pragma unroll
-                    for (int t = 0; t < N; ++t) e.v[t] = o[N * y + t][x];
-                    *reinterpret_cast<Pack<T, N>*>(&sums[wave][li * PITCH + 16 * N * y + N * Num<T>::row(x, g)]) = e;
-                }
-        }
+        put_sums<T, N, NY, PITCH>(o, li, g, sums[wave]);
         __syncthreads();
-        for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * W) {
+        const int here = (int)(rows - row0 < 16 ? rows - row0 : 16);
+        for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * WAVES) {
             const uint32_t row = at / (HDP / VEC), ahead_of = (row0 % p.group + row) / p.group;
             const int d = at % (HDP / VEC) * VEC;
             if (d >= p.head_dim) continue;
@@ -821,12 +420,12 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
             const int to_head = kv * p.group + (int)(row0 + row - (first_token + ahead_of) * p.group);
             T top = stat[0][0][row], total = 0, sum[VEC];
 #pragma unroll
-            for (int w = 1; w < W; ++w) top = fmax(top, stat[w][0][row]);
+            for (int w = 1; w < WAVES; ++w) top = fmax(top, stat[w][0][row]);
             const T ref = top == -(T)INFINITY ? (T)0 : top;
 #pragma unroll
             for (int t = 0; t < VEC; ++t) sum[t] = 0;
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
+            for (int w = 0; w < WAVES; ++w) {
                 const T f = Num<T>::exp_unit(stat[w][0][row] - ref);
                 total = fma(stat[w][1][row], f, total);
                 const Pack<T, VEC> e = *reinterpret_cast<const Pack<T, VEC>*>(&sums[w][row * PITCH + d]);
@@ -835,16 +434,18 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
             }
             T* __restrict__ dst;
             if (parts == 1) {
-                const T by = first_last + ahead_of >= 0 && sp.nk > 0 ? 1 / total : (T)0;
+                const bool any = first_last + ahead_of >= 0 && sp.nk > 0;
+                const T by = any ? 1 / total : (T)0;
 #pragma unroll
                 for (int t = 0; t < VEC; ++t) sum[t] *= by;
                 dst = p.O + to_token * p.ldo + to_head * (int64_t)p.head_dim;
+                if (d == 0 && p.lse != nullptr) p.lse[to_head * p.q_rows + to_token] = any ? Num<T>::log_sum(top, total) : -(T)INFINITY;
             } else {
-                const int64_t place = (to_token * p.heads + to_head) * plan.most_parts + part;
-                dst = plan.data + place * p.head_dim;
+                const int64_t place = (to_token * p.heads + to_head) * cut.most + part;
+                dst = cut.data + place * p.head_dim;
                 if (d == 0) {
-                    plan.stat[2 * place] = top;
-                    plan.stat[2 * place + 1] = total;
+                    cut.stat[2 * place] = top;
+                    cut.stat[2 * place + 1] = total;
                 }
             }
 #pragma unroll
@@ -858,7 +459,7 @@ __global__ void __launch_bounds__(64 * CACHED_WAVES, sizeof(T) == 4 && ALIGNED ?
 
 // Joins the parts of a row: a wavefront per (token, head).
 template <typename T>
-__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, const CachedPlan<T> plan) {
+__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, const Parts<T> cut) {
     const int lane = threadIdx.x & 63;
     const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (at >= p.q_rows * p.heads) return;
@@ -874,10 +475,10 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p,
     if (begun == 0 || begun > p.sequences) return;
     const Span sp = span_of(p, begun - 1);
     if (token < sp.q0 || token >= sp.q0 + sp.nq) return;
-    const int parts = (int)part_count(sp.nk, (uint32_t)*plan.part_keys, plan.most_parts);
+    const int parts = (int)part_count(sp.nk, (uint32_t)*cut.keys, cut.most);
     if (parts == 1) return;
-    const T m = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane)] : -(T)INFINITY;
-    const T l = lane < parts ? plan.stat[2 * (at * plan.most_parts + lane) + 1] : (T)0;
+    const T m = lane < parts ? cut.stat[2 * (at * cut.most + lane)] : -(T)INFINITY;
+    const T l = lane < parts ? cut.stat[2 * (at * cut.most + lane) + 1] : (T)0;
     T top = m;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d, 64));
@@ -885,7 +486,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p,
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
     f = sp.nk - sp.nq + (token - sp.q0) >= 0 ? f / total : (T)0;
-    const T* __restrict__ mine = plan.data + at * plan.most_parts * (int64_t)p.head_dim;
+    const T* __restrict__ mine = cut.data + at * cut.most * (int64_t)p.head_dim;
     T sum[2] = {0, 0};
     const int d0 = lane < p.head_dim ? lane : 0, d1 = lane + 64 < p.head_dim ? lane + 64 : 0;
 #pragma unroll 8
@@ -899,33 +500,227 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p,
     if (lane + 64 < p.head_dim) dst[lane + 64] = sum[1];
 }
 
-inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
-inline int64_t tile_slots(int64_t rows, int64_t group, int64_t per_tile, int64_t sequences) { return rows * group / per_tile + sequences; }
+// ---- backward -----------------------------------------------------------------------------------------------------------
+// (Queries and keys are the same rows here: token i sees key j iff j <= i.  A row that sees a non-finite value has a NaN in lse,
+// one of dO with a non-finite value a NaN in D: their weights are NaN, and the values themselves are staged as zeros.)
+
+// The sums of the wavefronts of 16 rows, times `by`, to the rows' places.
+template <typename T, int HDP, typename RowOf>
+__device__ __forceinline__ void write_sums(const T (&sums)[WAVES][16 * (HDP + 16 / sizeof(T))], int here, int head_dim, T by, RowOf row_of) {
+    constexpr int VEC = 16 / sizeof(T), PITCH = HDP + VEC;
+    for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * WAVES) {
+        const int row = at / (HDP / VEC), d = at % (HDP / VEC) * VEC;
+        if (d >= head_dim) continue;
+        T sum[VEC];
+#pragma unroll
+        for (int t = 0; t < VEC; ++t) sum[t] = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const Pack<T, VEC> e = *reinterpret_cast<const Pack<T, VEC>*>(&sums[w][row * PITCH + d]);
+#pragma unroll
+            for (int t = 0; t < VEC; ++t) sum[t] += e.v[t];
+        }
+        T* __restrict__ dst = row_of(row);
+#pragma unroll
+        for (int t = 0; t < VEC; ++t)
+            if (d + t < head_dim) dst[d + t] = sum[t] * by;
+    }
+}
+
+// Gradient of Q: 16 packed rows against the keys that they see.  Writes D = rowsum(dO (.) O) for the other kernel.
+template <typename T, int HDP, bool ALIGNED>
+__global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalArgs<T> p) {
+    constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
+    typedef typename Num<T>::Acc Acc;
+    __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const uint32_t stride = gridDim.x / p.kv_heads;
+    const int kv = (int)(blockIdx.x % p.kv_heads);
+    const T factor = p.scale * Num<T>::unit();
+    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+        Span sp;
+        uint32_t parts, inside;
+        if (!find_unit(p, p.group, 1, 0, unit, lane, &sp, &parts, &inside)) return;
+        const uint32_t rows = (uint32_t)sp.nq * (uint32_t)p.group, row0 = inside * 16;
+        if (inside >= (rows + 15) / 16) return;  // (a wrapped sum)
+        const uint32_t r = row0 + li < rows ? row0 + li : rows - 1;
+        const uint32_t first_token = row0 / p.group, ahead = (row0 % p.group + (r - row0)) / p.group, last = first_token + ahead;
+        const int64_t token = sp.q0 + last;
+        const int head = kv * p.group + (int)(r - last * p.group);
+        const int64_t at = head * p.q_rows + token, col = head * (int64_t)p.head_dim;
+        Pack<T, VEC> q[CHUNKS], go[CHUNKS];
+        load_along<T, HDP, ALIGNED>(p.Q + token * p.ldq + col, g, p.head_dim, q);
+        load_along<T, HDP, ALIGNED>(p.dO + token * p.ldo + col, g, p.head_dim, go);
+        T lse = p.lse[at] * Num<T>::unit(), dot = 0;
+        {
+            Pack<T, VEC> o[CHUNKS];
+            load_along<T, HDP, ALIGNED>(p.O + token * p.ldo + col, g, p.head_dim, o);
+            zero_past<T, HDP>(g, p.head_dim, o);
+            zero_past<T, HDP>(g, p.head_dim, go);
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+                for (int t = 0; t < VEC; ++t) dot = fma(go[c].v[t], o[c].v[t], dot);
+            dot += __shfl_xor(dot, 16, 64);
+            dot += __shfl_xor(dot, 32, 64);
+            dot = is_finite(dot) ? dot : nan_of<T>();
+            lse += dot - dot;  // NaN where D is
+        }
+        if (wave == 0 && g == 0 && row0 + li < rows) p.D[at] = dot;
+        zero_past<T, HDP>(g, p.head_dim, q);
+        const uint32_t seen = first_token + (uint32_t)__builtin_amdgcn_readlane(ahead, 15) + 1;  // (of nk = nq keys)
+        const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
+        const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
+        Acc dq[NY];
+#pragma unroll
+        for (int y = 0; y < NY; ++y) dq[y] = Acc{0, 0, 0, 0};
+        for (uint32_t k0 = 16 * wave; k0 < seen; k0 += 16 * WAVES) {
+            const uint32_t most = seen - 1 - k0;
+            const int64_t key = k0 + (li < most ? li : most);
+            Pack<T, VEC> k[CHUNKS], v[CHUNKS];
+            Pack<T, N> across[4][NY / N];
+            load_along<T, HDP, ALIGNED>(K + key * p.ldk, g, p.head_dim, k);
+            load_along<T, HDP, ALIGNED>(V + key * p.ldv, g, p.head_dim, v);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t j = Num<T>::row(x, g);
+                load_across<T, HDP, ALIGNED>(K + (int64_t)(k0 + (j < most ? j : most)) * p.ldk, li, p.head_dim, across[x]);
+            }
+            const Acc s = product<T>(k, q), dp = product<T>(v, go);
+            Acc ds;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const T w = Num<T>::exp_unit(s[x] * factor - lse);
+                ds[x] = k0 + Num<T>::row(x, g) <= last ? w * (dp[x] - dot) : (T)0;
+            }
+            zero_bad<T>(across);
+            add_weighted<T>(across, ds, dq);
+        }
+        put_sums<T, N, NY, PITCH>(dq, li, g, sums[wave]);
+        __syncthreads();
+        write_sums<T, HDP>(sums, (int)(rows - row0 < 16 ? rows - row0 : 16), p.head_dim, p.scale, [&](int row) {
+            const uint32_t to = first_token + (row0 % p.group + row) / p.group;
+            return p.dQ + (sp.q0 + to) * p.lddq + (kv * p.group + (int)(row0 + row - to * p.group)) * (int64_t)p.head_dim;
+        });
+        if (unit > ~0u - stride) return;
+        __syncthreads();
+    }
+}
+
+// Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.
+template <typename T, int HDP, bool ALIGNED>
+__global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalArgs<T> p) {
+    constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
+    typedef typename Num<T>::Acc Acc;
+    __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
+    const uint32_t stride = gridDim.x / p.kv_heads, group = p.group, inverse = inverse_of(group);
+    const int kv = (int)(blockIdx.x % p.kv_heads);
+    const T factor = p.scale * Num<T>::unit();
+    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+        Span sp;
+        uint32_t parts, inside;
+        if (!find_unit(p, 1, 1, 0, unit, lane, &sp, &parts, &inside)) return;
+        const uint32_t keys = (uint32_t)sp.nk, rows = keys * group, key0 = inside * 16;
+        if (inside >= (keys + 15) / 16) return;  // (a wrapped sum)
+        const uint32_t key = key0 + li < keys ? key0 + li : keys - 1;
+        Pack<T, VEC> k[CHUNKS], v[CHUNKS];
+        load_along<T, HDP, ALIGNED>(p.K + (sp.k0 + key) * p.ldk + kv * (int64_t)p.head_dim, g, p.head_dim, k);
+        load_along<T, HDP, ALIGNED>(p.V + (sp.k0 + key) * p.ldv + kv * (int64_t)p.head_dim, g, p.head_dim, v);
+        zero_past<T, HDP>(g, p.head_dim, k);
+        zero_past<T, HDP>(g, p.head_dim, v);
+        Acc dk[NY], dv[NY];
+#pragma unroll
+        for (int y = 0; y < NY; ++y) dk[y] = dv[y] = Acc{0, 0, 0, 0};
+        const T* __restrict__ Q = p.Q + sp.q0 * p.ldq + kv * (int64_t)group * p.head_dim;
+        const T* __restrict__ G = p.dO + sp.q0 * p.ldo + kv * (int64_t)group * p.head_dim;
+        const T* __restrict__ lses = p.lse + kv * (int64_t)group * p.q_rows + sp.q0;
+        const T* __restrict__ dots = p.D + kv * (int64_t)group * p.q_rows + sp.q0;
+        for (uint32_t r0 = key0 * group / 16 * 16 + 16 * wave; r0 < rows; r0 += 16 * WAVES) {
+            const uint32_t most = rows - 1 - r0, token0 = r0 / group, rest0 = r0 - token0 * group;
+            Pack<T, VEC> q[CHUNKS], go[CHUNKS];
+            Pack<T, N> q_across[4][NY / N], g_across[4][NY / N];
+            {
+                const uint32_t i = rest0 + (li < most ? li : most), ahead = heads_over(i, group, inverse);
+                const int64_t token = token0 + ahead, col = (int64_t)(i - ahead * group) * p.head_dim;
+                load_along<T, HDP, ALIGNED>(Q + token * p.ldq + col, g, p.head_dim, q);
+                load_along<T, HDP, ALIGNED>(G + token * p.ldo + col, g, p.head_dim, go);
+            }
+            uint32_t sees[4];
+            T lse[4], dot[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t j = Num<T>::row(x, g), i = rest0 + (j < most ? j : most), ahead = heads_over(i, group, inverse);
+                const int64_t token = token0 + ahead;
+                const uint32_t head = i - ahead * group;
+                load_across<T, HDP, ALIGNED>(Q + token * p.ldq + (int64_t)head * p.head_dim, li, p.head_dim, q_across[x]);
+                load_across<T, HDP, ALIGNED>(G + token * p.ldo + (int64_t)head * p.head_dim, li, p.head_dim, g_across[x]);
+                lse[x] = lses[head * p.q_rows + token];
+                dot[x] = dots[head * p.q_rows + token];
+                sees[x] = j <= most ? token0 + ahead + 1 : 0;  // how many keys the row sees
+            }
+            const Acc s = product<T>(q, k), dp = product<T>(go, v);  // rows are packed rows, columns keys
+            Acc w, ds;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const T e = Num<T>::exp_unit(s[x] * factor - (lse[x] * Num<T>::unit() + (dot[x] - dot[x])));
+                w[x] = key < sees[x] ? e : (T)0;
+                ds[x] = key < sees[x] ? e * (dp[x] - dot[x]) : (T)0;
+            }
+            zero_bad<T>(g_across);
+            add_weighted<T>(g_across, w, dv);
+            zero_bad<T>(q_across);
+            add_weighted<T>(q_across, ds, dk);
+        }
+        const int here = (int)(keys - key0 < 16 ? keys - key0 : 16);
+        put_sums<T, N, NY, PITCH>(dv, li, g, sums[wave]);
+        __syncthreads();
+        write_sums<T, HDP>(sums, here, p.head_dim, (T)1, [&](int row) { return p.dV + (sp.k0 + key0 + row) * p.lddv + kv * (int64_t)p.head_dim; });
+        __syncthreads();
+        put_sums<T, N, NY, PITCH>(dk, li, g, sums[wave]);
+        __syncthreads();
+        write_sums<T, HDP>(sums, here, p.head_dim, p.scale, [&](int row) { return p.dK + (sp.k0 + key0 + row) * p.lddk + kv * (int64_t)p.head_dim; });
+        if (unit > ~0u - stride) return;
+        __syncthreads();
+    }
+}
+
+// Packed rows fit into 31 bits and a launch into its limits.
+template <typename T> inline bool rows_fit(const CausalArgs<T>& a) { return a.q_rows <= INT32_MAX / a.group - 16 && a.k_rows <= INT32_MAX; }
+inline int64_t tile_slots(int64_t rows, int64_t group, int64_t sequences) { return rows * group / 16 + sequences; }
+
+// Parts of a sequence's keys: one where a cache is short, no more than a lane each, and few enough that rows with many
+// units do not need a large workspace.
+template <typename T>
+int most_parts(const CausalArgs<T>& a) {
+    if (a.k_rows <= WHOLE_KEYS) return 1;
+    const int64_t units = tile_slots(a.q_rows, a.group, a.sequences) * a.kv_heads;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({64, (a.k_rows + LEAST_KEYS - 1) / LEAST_KEYS, 8 * RUNNING / units}));
+}
 
 }  // namespace
 
-// A launch of KERNEL<T, HDP> for the smallest padded head dimension that holds head_dim.
-#define BY_HEAD_DIM(KERNEL, GRID, ...)                                                                                  \
-    do {                                                                                                                \
-        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32>), GRID, dim3(256), 0, s, __VA_ARGS__);                  \
-        else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64>), GRID, dim3(256), 0, s, __VA_ARGS__);             \
-        else hipLaunchKernelGGL((KERNEL<T, 128>), GRID, dim3(256), 0, s, __VA_ARGS__);                                  \
-        if (hipError_t e = hipGetLastError()) return e;                                                                 \
+// A launch of KERNEL<T, HDP, ALIGNED> for the smallest padded head dimension that holds head_dim.
+#define BY_HEAD_DIM_OF(KERNEL, ALIGNED, GROUPS, ...)                                                                                              \
+    do {                                                                                                                                          \
+        const dim3 grid((unsigned)(GROUPS)), block(64 * WAVES);                                                                                   \
+        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                       \
+        else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                  \
+        else hipLaunchKernelGGL((KERNEL<T, 128, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                                       \
+        if (hipError_t e = hipGetLastError()) return e;                                                                                           \
     } while (0)
+#define BY_HEAD_DIM(KERNEL, ALIGNED, GROUPS, ...) \
+    do { if (ALIGNED) BY_HEAD_DIM_OF(KERNEL, true, GROUPS, __VA_ARGS__); else BY_HEAD_DIM_OF(KERNEL, false, GROUPS, __VA_ARGS__); } while (0)
 
-#define BY_HEAD_DIM_CACHED(ALIGNED)                                                                                                       \
-    do {                                                                                                                                  \
-        const dim3 block(64 * CACHED_WAVES);                                                                                              \
-        if (a.head_dim <= 32) hipLaunchKernelGGL((cached_attention_kernel<T, 32, ALIGNED>), grid, block, 0, s, a, plan);                  \
-        else if (a.head_dim <= 64) hipLaunchKernelGGL((cached_attention_kernel<T, 64, ALIGNED>), grid, block, 0, s, a, plan);             \
-        else hipLaunchKernelGGL((cached_attention_kernel<T, 128, ALIGNED>), grid, block, 0, s, a, plan);                                  \
-    } while (0)
+// Workgroups for `tiles` units of every key/value head: one each, of very many some take several.
+static int64_t workgroups(int64_t tiles, int64_t most, int64_t kv_heads) { return std::min(tiles, std::max<int64_t>(1, most / kv_heads)) * kv_heads; }
+constexpr int64_t MOST_GROUPS = 1 << 20;
 
 template <typename T>
 hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s) {
-    const int64_t slots = tile_slots(a.q_rows, a.group, 64, a.sequences);
-    if (!grid_fits(slots, 256)) return hipErrorInvalidValue;
-    BY_HEAD_DIM(causal_fwd_kernel, dim3((unsigned)slots, a.kv_heads), a);
+    if (!rows_fit(a)) return hipErrorInvalidValue;
+    const Parts<T> whole = {1, nullptr, nullptr, nullptr};
+    BY_HEAD_DIM(attention_kernel, a.vec_q && a.vec_kv, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a, whole);
     return hipSuccess;
 }
 
@@ -937,46 +732,33 @@ size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a) {
 template <typename T>
 hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     a.D = static_cast<T*>(workspace);
-    const int64_t dots = (a.q_rows * a.heads + 15) / 16, key_slots = tile_slots(a.q_rows, 1, 64, a.sequences), slots = tile_slots(a.q_rows, a.group, 64, a.sequences);
-    if (!grid_fits(dots, 256) || !grid_fits(slots, 256)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(causal_dot_kernel<T>, dim3((unsigned)dots), dim3(256), 0, s, a);
-    if (hipError_t e = hipGetLastError()) return e;
-    BY_HEAD_DIM(causal_bwd_kv_kernel, dim3((unsigned)key_slots, a.kv_heads), a);
-    BY_HEAD_DIM(causal_bwd_q_kernel, dim3((unsigned)slots, a.kv_heads), a);
+    if (!rows_fit(a)) return hipErrorInvalidValue;
+    const bool aligned = a.vec_q && a.vec_kv && a.vec_o;
+    BY_HEAD_DIM(causal_bwd_q_kernel, aligned, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a);
+    BY_HEAD_DIM(causal_bwd_kv_kernel, aligned, workgroups(tile_slots(a.q_rows, 1, a.sequences), MOST_GROUPS, a.kv_heads), a);
     return hipSuccess;
-}
-
-// Parts of a sequence's keys at most: one where a cache is short, no more than a lane each, and few enough that rows with many
-// units do not need a large workspace.
-template <typename T>
-static int most_cached_parts(const CausalArgs<T>& a) {
-    if (a.k_rows <= CACHED_WHOLE) return 1;
-    const int64_t units = tile_slots(a.q_rows, a.group, 16, a.sequences) * a.kv_heads;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({64, (a.k_rows + CACHED_LEAST - 1) / CACHED_LEAST, 8 * CACHED_GROUPS / units}));
 }
 
 template <typename T>
 size_t cached_workspace_bytes(const CausalArgs<T>& a) {
-    const int parts = most_cached_parts(a);
+    const int parts = most_parts(a);
     return parts == 1 ? 0 : 16 + (size_t)a.q_rows * a.heads * parts * (a.head_dim + 2) * sizeof(T);
 }
 
 template <typename T>
 hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s) {
-    CachedPlan<T> plan;
-    plan.most_parts = most_cached_parts(a);
-    plan.part_keys = static_cast<int32_t*>(workspace);
-    plan.data = static_cast<T*>(workspace) + 16 / sizeof(T);
-    plan.stat = plan.data + a.q_rows * a.heads * (int64_t)plan.most_parts * a.head_dim;
-    // a workgroup per unit of a call whose units run at once; of larger calls some take several
-    const int64_t tiles = tile_slots(a.q_rows, a.group, 16, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
-    const int64_t groups = std::min(tiles * plan.most_parts, std::max<int64_t>(1, (tiles * a.kv_heads <= CACHED_GROUPS / 2 ? 1 : 4) * CACHED_GROUPS / a.kv_heads));
-    if (!grid_fits(rows, 256) || a.q_rows > INT32_MAX / a.group - 16 || a.k_rows > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(groups * a.kv_heads));
-    if (a.vec_q && a.vec_kv) BY_HEAD_DIM_CACHED(true); else BY_HEAD_DIM_CACHED(false);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (plan.most_parts > 1) {
-        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, plan);
+    if (!rows_fit(a)) return hipErrorInvalidValue;
+    Parts<T> cut;
+    cut.most = most_parts(a);
+    cut.keys = static_cast<int32_t*>(workspace);
+    cut.data = static_cast<T*>(workspace) + 16 / sizeof(T);
+    cut.stat = cut.data + a.q_rows * a.heads * (int64_t)cut.most * a.head_dim;
+    // where the units run at once there are no more than that of them
+    const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
+    const int64_t most = cut.most == 1 ? MOST_GROUPS : tiles * a.kv_heads <= RUNNING / 2 ? RUNNING : 4 * RUNNING;
+    BY_HEAD_DIM(attention_kernel, a.vec_q && a.vec_kv, workgroups(tiles * cut.most, most, a.kv_heads), a, cut);
+    if (cut.most > 1) {
+        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, cut);
         if (hipError_t e = hipGetLastError()) return e;
     }
     return hipSuccess;
