@@ -1202,8 +1202,20 @@ inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < (
 
 }  // namespace
 
-// (Packed rows of a sequence are counted in 32 bits.)
-bool causal_split_eligible(const CausalArgs<float>& p) { return p.q_rows >= 512 && p.q_rows * p.group < ((int64_t)1 << 31) - 256; }
+// Whether a batch is large enough for these kernels; smaller ones are faster with units of 16 rows.  Three products on halves
+// cost less than one on floats and tiles of 128 rows read less, but their workgroups take more rows each: they want
+// rows * heads >= 2^14 to fill the card, and they have a kernel more to launch and longer prologues, which pay from
+// rows * heads * (mean length) = 2^22 on - in the gradients of shared keys, where there are fewer tiles of keys, from twice
+// that.  Measured, these against the units of 16, head dimension 64, 8 heads on 8 of keys, forward / backward in us:
+//   1024 rows of length 64: 15 / 26 against 9 / 19;  2048 of 64: 18 / 34 against 14 / 31;  2048 of 256: 22 / 46 against 23 / 59;
+//   4096 of 1024: 47 / 108 against 82 / 243;  8 heads on 2 of keys, 2048 of 256: 19 / 86 against 23 / 65, of 1024: 38 / 121
+//   against 47 / 193.  (Packed rows of a sequence are counted in 32 bits.)
+static bool split_pays(const CausalArgs<float>& p, int64_t least) {
+    const int64_t rows = p.q_rows * p.heads;
+    return rows >= ((int64_t)1 << 14) && p.q_rows * p.group < ((int64_t)1 << 31) - 256 && (double)rows * p.q_rows / p.sequences >= (double)least;
+}
+bool causal_split_fwd_pays(const CausalArgs<float>& p) { return split_pays(p, 1 << 22); }
+bool causal_split_bwd_pays(const CausalArgs<float>& p) { return split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23); }
 
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
 

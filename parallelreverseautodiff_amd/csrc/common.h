@@ -467,7 +467,8 @@ template <typename T> hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipSt
 template <typename T> size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a);
 template <typename T> hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s);
 // The same in float on the half-precision matrix instructions (csrc/causal_attention_split.hip), for batches long enough.
-bool causal_split_eligible(const CausalArgs<float>& a);
+bool causal_split_fwd_pays(const CausalArgs<float>& a);
+bool causal_split_bwd_pays(const CausalArgs<float>& a);
 size_t causal_split_bwd_workspace_bytes(const CausalArgs<float>& a);
 hipError_t launch_causal_split_bwd(const CausalArgs<float>& a, void* workspace, hipStream_t s);
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& a);

@@ -2033,7 +2033,7 @@ static int32_t causal_fwd_t(CausalArgs<T> a, prad_buf_t lse, prad_index_t offset
     a.lse = lse != nullptr ? static_cast<T*>(lse->ptr) : nullptr;
     a.q_off = offsets->ptr; a.sequences = (int)(offsets->n - 1);
     if constexpr (sizeof(T) == 4) {
-        if (causal_split_eligible(a)) {
+        if (causal_split_fwd_pays(a)) {
             if (int32_t st = ensure_workspace(causal_split_fwd_workspace_bytes(a))) return st;
             HIP_TRY(launch_causal_split_fwd(a, CUR_WORKSPACE, CUR_STREAM), PRAD_ERR_LAUNCH);
             return PRAD_OK;
@@ -2053,7 +2053,7 @@ static int32_t causal_bwd_t(CausalArgs<T> a, prad_buf_t lse, prad_buf_t dO, cons
     a.dQ = out_column<T>(dQ); a.dK = out_column<T>(dK); a.dV = out_column<T>(dV);
     a.lddq = dQ.buf->cols; a.lddk = dK.buf->cols; a.lddv = dV.buf->cols;
     if constexpr (sizeof(T) == 4) {
-        if (causal_split_eligible(a)) {
+        if (causal_split_bwd_pays(a)) {
             a.vec_dq = packs_of_16<T>({dQ}, a.head_dim);
             a.vec_dkv = packs_of_16<T>({dK, dV}, a.head_dim);
             if (int32_t st = ensure_workspace(causal_split_bwd_workspace_bytes(a))) return st;

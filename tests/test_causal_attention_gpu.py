@@ -166,9 +166,14 @@ CASES = [([1], 1, 1, 1, "fused"), ([5], 2, 1, 3, "apart"), ([0, 0], 2, 2, 8, "fu
          ([16, 15, 17], 4, 2, 33, "apart"), ([64, 63, 65, 1], 2, 1, 40, "fused"), ([31, 32, 33], 6, 2, 64, "fused"), ([130, 2], 5, 1, 64, "apart"),
          ([20, 100], 3, 1, 65, "apart"), ([70, 0, 129], 4, 4, 80, "fused"), ([129], 8, 1, 128, "fused"), ([90, 45], 2, 2, 127, "apart"), ([200], 6, 3, 96, "apart"),
          ([260, 90], 4, 2, 128, "apart"),
-         # long batches
+         # longer ones
          ([300, 0, 129, 64, 1, 77, 40], 4, 2, 64, "fused"), ([520], 3, 1, 40, "apart"), ([63, 65, 130, 255, 100], 2, 2, 32, "fused"), ([257, 256, 31], 4, 1, 128, "fused"),
          ([600, 32], 5, 1, 80, "apart"), ([1] * 530, 2, 1, 64, "fused"), ([1300], 1, 1, 16, "fused"), ([130, 400], 6, 2, 127, "apart")]
+
+
+# Batches whose rows * heads * mean length passes 2^23: those of floats are computed from halves.
+LARGE = [([300, 0, 129, 64, 1, 77, 40], 160, 80, 64, "fused"), ([520], 33, 11, 40, "apart"), ([63, 65, 130, 255, 100], 112, 112, 32, "fused"), ([257, 256, 31], 84, 21, 128, "fused"),
+         ([600, 32], 45, 9, 80, "apart"), ([1] * 20 + [900], 208, 104, 16, "fused"), ([1300], 13, 13, 16, "fused"), ([130, 400], 60, 20, 127, "apart"), ([1, 700, 2], 64, 1, 8, "fused")]
 
 
 @DTYPES
@@ -177,14 +182,26 @@ def test_attention_against_its_definition(gpu, dtype, case):
     compare(Batch(dtype, *case))
 
 
+@pytest.mark.parametrize("case", LARGE, ids=[str((len(c[0]), *c[1:])) for c in LARGE])
+def test_attention_of_large_batches_against_its_definition(gpu, case):
+    batch = Batch(np.float32, *case)
+    assert batch.rows * batch.heads * (batch.rows // len(batch.lengths)) >= 2 ** 23
+    compare(batch)
+
+
+# (long: in the sense of LARGE)
 LONG = pytest.mark.parametrize("long", [False, True], ids=["short", "long"])
+
+
+def times(long, heads, kv_heads, by=32):
+    return (heads * by, kv_heads * by) if long else (heads, kv_heads)
 
 
 @DTYPES
 @LONG
 def test_scores_far_apart_and_far_from_zero(gpu, dtype, long):
     """Scores of several hundreds: the running maximum moves, most weights vanish."""
-    batch = Batch(dtype, [550, 40] if long else [150, 40], 2, 1, 64, "fused")
+    batch = Batch(dtype, [550, 40] if long else [150, 40], *times(long, 2, 1), 64, "fused")
     batch.q *= 12
     batch.k *= 12
     batch.upload()
@@ -195,7 +212,7 @@ def test_scores_far_apart_and_far_from_zero(gpu, dtype, long):
 @LONG
 @pytest.mark.parametrize("scale", [-0.2, 0.0])
 def test_a_scale_that_is_not_positive(gpu, dtype, long, scale):
-    batch = Batch(dtype, [540] if long else [70], 2, 1, 32, "fused")
+    batch = Batch(dtype, [540] if long else [70], *times(long, 2, 1), 32, "fused")
     batch.scale = scale
     batch.tail = batch.tail[:3] + (scale,)
     compare(batch)
@@ -206,7 +223,7 @@ def test_a_scale_that_is_not_positive(gpu, dtype, long, scale):
 def test_rows_of_very_different_size(gpu, dtype, long):
     """Tokens whose values differ by thousands, tiles of zeros among them, everything far below one: every element stays within
     its bound (which grows with the largest values a row mixes)."""
-    batch = Batch(dtype, [560, 30] if long else [190, 30], 2, 1, 64, "fused")
+    batch = Batch(dtype, [560, 30] if long else [190, 30], *times(long, 2, 1), 64, "fused")
     size = 2.0 ** (np.arange(batch.rows) // 37 % 5 * 3.0 - 12)
     for x in (batch.v, batch.g):
         x *= (size * 2.0 ** -20)[:, None].astype(dtype)
@@ -220,7 +237,7 @@ def test_rows_of_very_different_size(gpu, dtype, long):
 @DTYPES
 @LONG
 def test_equal_calls_give_equal_bits(gpu, dtype, long):
-    batch = Batch(dtype, [900, 77, 1, 130] if long else [300, 77, 1, 130], 6, 2, 64, "fused")
+    batch = Batch(dtype, [900, 77, 1, 130] if long else [300, 77, 1, 130], *times(long, 6, 2, 8), 64, "fused")
     first = batch.forward()
     grads = batch.backward(*first)
     for _ in range(2):
@@ -237,7 +254,7 @@ def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, 
     """Token 20 of the second sequence holds one: earlier tokens and other sequences keep every bit of O and of the gradients
     that do not depend on it; whoever sees it gets NaN."""
     lengths = [33, 450, 140] if long else [33, 50, 40]
-    clean, dirty = Batch(dtype, lengths, 2, 1, 40, "fused"), Batch(dtype, lengths, 2, 1, 40, "fused")
+    clean, dirty = (Batch(dtype, lengths, *times(long, 2, 1, 36), 40, "fused") for _ in range(2))
     at = int(clean.starts[1]) + 20
     getattr(dirty, where)[at, 7] = value        # (head 0)
     dirty.upload()
@@ -246,13 +263,13 @@ def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, 
     cg, dg = clean.backward(co, cl), dirty.backward(do, dl)
     a, b = co.download(), do.download()
     first, last, second_end = int(clean.starts[0]), int(clean.starts[-1]), int(clean.starts[2])
-    head0, head1 = slice(0, 40), slice(40, 80)
-    # rows of O that see it: of head 0 the row itself (q), of both heads (k and v are shared) this row and the later ones
+    head0, head1, both = slice(0, 40), slice(40, 80), slice(0, 80)
+    # rows of O that see it: of head 0 the row itself (q), of both heads that share its k and v this row and the later ones
     hit = np.zeros(a.shape, bool)
     if where == "q":
         hit[at, head0] = True
     elif where in "kv":
-        hit[at:second_end] = True
+        hit[at:second_end, both] = True
     inside = np.zeros(a.shape, bool)
     inside[first:last] = True
     assert np.array_equal(a[inside & ~hit], b[inside & ~hit]) and np.isnan(b[hit]).all()
@@ -267,16 +284,19 @@ def test_values_that_are_not_finite_reach_only_who_sees_them(gpu, dtype, where, 
         assert np.array_equal(dq[rest], cg[0][rest])
         later = slice(at + 1, second_end)
         for x, y in ((dk, cg[1]), (dv, cg[2])):
-            assert np.array_equal(x[later], y[later]) and np.isnan(x[int(clean.starts[1]):at + 1]).all()
+            assert np.array_equal(x[later], y[later]) and np.isnan(x[int(clean.starts[1]):at + 1, head0]).all()
     else:                   # a key: the queries from it on
         before = slice(int(clean.starts[1]), at)
-        assert np.array_equal(dq[before], cg[0][before]) and np.isnan(dq[at:second_end]).all()
-        assert np.isnan(dk[int(clean.starts[1]):second_end]).all()
+        assert np.array_equal(dq[before], cg[0][before]) and np.isnan(dq[at:second_end, both]).all()
+        assert np.isnan(dk[int(clean.starts[1]):second_end, head0]).all()
+    for x, y, own in zip(cg, dg, (both, head0, head0)):        # other heads: nothing
+        others = np.delete(np.arange(x.shape[1]), np.r_[own])
+        assert np.array_equal(x[first:last, others], y[first:last, others])
 
 
 @LONG
 def test_rows_of_nobody_are_not_read_for_a_result(gpu, long):
-    clean, dirty = (Batch(np.float32, [470, 20] if long else [70, 20], 4, 2, 64, "fused", front=70, behind=70) for _ in range(2))
+    clean, dirty = (Batch(np.float32, [470, 20] if long else [70, 20], *times(long, 4, 2, 12), 64, "fused", front=70, behind=70) for _ in range(2))
     first, last = int(clean.starts[0]), int(clean.starts[-1])
     for x in (dirty.q, dirty.k, dirty.v, dirty.g):
         x[:first] = np.nan
@@ -290,9 +310,9 @@ def test_rows_of_nobody_are_not_read_for_a_result(gpu, long):
 @DTYPES
 @LONG
 def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype, long):
-    lib, times = _lib.load(), 5 if long else 1
-    batch = Batch(dtype, [60 * times, 60 * times, 30 * times], 4, 2, 64, "fused", front=0, behind=0)
-    o, l = unfilled(dtype, batch.rows, 256), unfilled(dtype, 4, batch.rows)
+    lib, by = _lib.load(), 5 if long else 1
+    batch = Batch(dtype, [60 * by, 60 * by, 30 * by], *times(long, 4, 2, 12), 64, "fused", front=0, behind=0)
+    o, l = unfilled(dtype, batch.rows, batch.heads * 64), unfilled(dtype, batch.heads, batch.rows)
     g, d = dev(batch.g), unfilled(dtype, batch.rows, batch.full[0])
     grads = [x for c in batch.cols for x in (d.handle, c)]
 
@@ -308,7 +328,7 @@ def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype, l
         gr = ctypes.c_void_p()
         check(lib.prad_graph_end(ctypes.byref(gr)))
     for lengths in ([150, 0, 0], [1, 148, 1], [50, 50, 50], [0, 75, 75]):
-        batch.offsets.upload(times * np.concatenate([[0], np.cumsum(lengths)]))
+        batch.offsets.upload(by * np.concatenate([[0], np.cumsum(lengths)]))
         check(lib.prad_graph_launch(gr))
         got = o.download(), l.download(), d.download()
         o.zero(), l.zero(), d.zero()
@@ -321,9 +341,9 @@ def test_a_recorded_training_pass_reads_the_offsets_of_each_launch(gpu, dtype, l
 def test_offsets_that_describe_no_rows_do_no_harm(gpu, long):
     """Offsets past the rows, negative or falling: cut off to rows of the buffers, nothing outside is touched."""
     lib = _lib.load()
-    batch = Batch(np.float32, [40, 540] if long else [40, 40], 2, 1, 32, "fused", front=0, behind=0)
-    room = DeviceBuffer.alloc(np.float32, batch.rows + 64, 64)
-    room.upload(np.full((batch.rows + 64, 64), 7, np.float32))
+    batch = Batch(np.float32, [40, 540] if long else [40, 40], *times(long, 2, 1), 32, "fused", front=0, behind=0)
+    room = DeviceBuffer.alloc(np.float32, batch.rows + 64, batch.heads * 32)
+    room.upload(np.full((room.rows, room.cols), 7, np.float32))
     o = room.view_rows(32, batch.rows)
     for values in ([0, 40, 1000], [-5, 40, 80], [40, 0, 2 ** 31 - 1], [-2 ** 31, 2 ** 31 - 1, -1]):
         batch.offsets.upload(values)
