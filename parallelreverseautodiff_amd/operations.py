@@ -13,6 +13,10 @@ All four matrix-multiply names of the reference - MatrixMultiplyOperation
 (src/RMAD/CudaMatrixMultiplyOperation.cs) and GpuMatrixMultiplyAndSumOperation
 (src/RMAD/GpuMatrixMultiplyAndSumOperation.cs) - resolve to the same device kernels; inputs and
 outputs stay resident on the device between operations.
+
+The operations on token sequences at the end (EmbeddingOperation, DropoutOperation, CausalAttentionOperation,
+CachedAttentionOperation) have no counterpart in the reference and keep the same contract; token ids, sequence offsets and step
+counters are IndexVectors (or plain whole numbers, which become one) and take no gradient.
 """
 import ctypes
 
@@ -21,7 +25,7 @@ import numpy as np
 from . import _lib
 from .cudablas import CudaBlas
 from .exceptions import ArgumentException, CudaNotInitializedException, InvalidOperationException, check
-from .matrix import DeepMatrix, DeviceBuffer, Matrix
+from .matrix import DeepMatrix, DeviceBuffer, IndexVector, Matrix
 
 
 class BackwardResult:
@@ -736,3 +740,160 @@ class CategoricalCrossEntropyLossOperation(Operation):
         dp = DeviceBuffer.alloc_output(output.dtype, output.Rows, output.Cols)
         check(_lib.load().prad_cce_bwd(output.device().handle, self.target.device().handle, dp.handle))
         return BackwardResultBuilder().AddInputGradient(Matrix._from_device(dp)).Build()
+
+
+def _index(values):
+    return values if isinstance(values, IndexVector) else IndexVector.from_values(values)
+
+
+class EmbeddingOperation(Operation):
+    """Rows of a table by token id, times `scale`; an id outside the table (padding) is a row of zeros.  Backward returns the
+    table's gradient: the sum of dOutput's rows over equal ids, in one fixed order."""
+
+    def __init__(self, scale=1.0):
+        super().__init__()
+        self.scale = float(scale)
+        self.table = self.ids = None
+
+    @staticmethod
+    def Instantiate(net):
+        return EmbeddingOperation()
+
+    def _intermediates(self):
+        return [self.table, self.ids]
+
+    def _restore_from(self, items):
+        self.table, self.ids = items
+
+    def Forward(self, table, ids):
+        _ensure_initialized()
+        self.table, self.ids = table, _index(ids)
+        out = DeviceBuffer.alloc_output(table.dtype, self.ids.length, table.Cols)
+        check(_lib.load().prad_embedding_fwd(table.device().handle, self.ids.handle, self.scale, out.handle))
+        self.Output = Matrix._from_device(out)
+        return self.Output
+
+    def Backward(self, dOutput):
+        _ensure_initialized()
+        d = DeviceBuffer.alloc_output(self.table.dtype, self.table.Rows, self.table.Cols)
+        check(_lib.load().prad_embedding_bwd(dOutput.device().handle, self.ids.handle, self.scale, d.handle, 0))
+        return BackwardResultBuilder().AddInputGradient(Matrix._from_device(d)).Build()
+
+
+class DropoutOperation(Operation):
+    """input / (1 - p) where an element is kept and 0 where it is dropped, plus a residual if there is one.  What is kept is a
+    function of (seed, site, step, position) alone and no mask is stored: `site` tells the places of a model apart, `step`
+    (an IndexVector of one element, its value read when the call runs) the iterations.  Backward returns the input's gradient
+    and, if there was a residual, dOutput itself as the residual's; it reads `step` again, so step it afterwards."""
+
+    def __init__(self, p=0.1, seed=0, site=0):
+        super().__init__()
+        self.p, self.seed, self.site = float(p), int(seed), int(site)
+        self.step = None
+        self.has_residual = False
+
+    @staticmethod
+    def Instantiate(net):
+        return DropoutOperation()
+
+    def _intermediates(self):
+        return [self.step, self.has_residual]
+
+    def _restore_from(self, items):
+        self.step, self.has_residual = items
+
+    def _step(self):
+        return self.step.handle if self.step is not None else _null()
+
+    def Forward(self, input, residual=None, step=None):
+        _ensure_initialized()
+        self.step, self.has_residual = None if step is None else _index(step), residual is not None
+        out = DeviceBuffer.alloc_output(input.dtype, input.Rows, input.Cols)
+        check(_lib.load().prad_dropout_fwd(input.device().handle, residual.device().handle if residual is not None else _null(), out.handle,
+                                           self.p, self.seed, self.site, self._step()))
+        self.Output = Matrix._from_device(out)
+        return self.Output
+
+    def Backward(self, dOutput):
+        _ensure_initialized()
+        dx = DeviceBuffer.alloc_output(dOutput.dtype, dOutput.Rows, dOutput.Cols)
+        check(_lib.load().prad_dropout_bwd(dOutput.device().handle, dx.handle, self.p, self.seed, self.site, self._step()))
+        result = BackwardResultBuilder().AddInputGradient(Matrix._from_device(dx))
+        if self.has_residual:
+            result.AddInputGradient(dOutput)
+        return result.Build()
+
+
+class CausalAttentionOperation(Operation):
+    """Causal self-attention over sequences packed one after the other: sequence s is rows [offsets[s], offsets[s+1]) of the
+    inputs.  q has heads * head_dim columns, k and v kv_heads * head_dim; head h works with head h / (heads / kv_heads) of k
+    and v.  Rows of no sequence are zeros in the output and in the gradients.  Backward returns [dq, dk, dv].  The scale is
+    1 / sqrt(head_dim) unless one is given."""
+
+    def __init__(self, heads, kv_heads=None, scale=None):
+        super().__init__()
+        self.heads, self.kv_heads = int(heads), int(heads if kv_heads is None else kv_heads)
+        self.scale = scale
+        self.q = self.k = self.v = self.offsets = self.lse = None
+
+    @staticmethod
+    def Instantiate(net):
+        return CausalAttentionOperation(getattr(getattr(net, "Parameters", None), "NumHeads", 1))
+
+    def _intermediates(self):
+        return [self.q, self.k, self.v, self.offsets, self.lse, self.Output]
+
+    def _restore_from(self, items):
+        self.q, self.k, self.v, self.offsets, self.lse, self.Output = items
+
+    def _shape(self, q, k, v):
+        if self.heads < 1 or q.Cols % self.heads:
+            raise ArgumentException("the columns of q must be a multiple of the number of heads")
+        head_dim = q.Cols // self.heads
+        if k.Cols != self.kv_heads * head_dim or v.Cols != k.Cols:
+            raise ArgumentException("k and v must have head_dim columns for each of their heads")
+        return self.heads, self.kv_heads, head_dim, head_dim ** -0.5 if self.scale is None else float(self.scale)
+
+    def Forward(self, q, k, v, offsets):
+        _ensure_initialized()
+        shape = self._shape(q, k, v)
+        self.q, self.k, self.v, self.offsets = q, k, v, _index(offsets)
+        out = DeviceBuffer.alloc(q.dtype, q.Rows, q.Cols)
+        self.lse = DeviceBuffer.alloc(q.dtype, self.heads, q.Rows)
+        check(_lib.load().prad_causal_attention_fwd(q.device().handle, 0, k.device().handle, 0, v.device().handle, 0, out.handle,
+                                                    self.lse.handle, self.offsets.handle, *shape))
+        self.Output = Matrix._from_device(out)
+        return self.Output
+
+    def Backward(self, dOutput):
+        _ensure_initialized()
+        q, k, v = self.q, self.k, self.v
+        grads = [DeviceBuffer.alloc(x.dtype, x.Rows, x.Cols) for x in (q, k, v)]
+        check(_lib.load().prad_causal_attention_bwd(q.device().handle, 0, k.device().handle, 0, v.device().handle, 0, self.Output.device().handle,
+                                                    self.lse.handle, dOutput.device().handle, grads[0].handle, 0, grads[1].handle, 0,
+                                                    grads[2].handle, 0, self.offsets.handle, *self._shape(q, k, v)))
+        result = BackwardResultBuilder()
+        for g in grads:
+            result.AddInputGradient(Matrix._from_device(g))
+        return result.Build()
+
+
+class CachedAttentionOperation(CausalAttentionOperation):
+    """The newest tokens of each sequence against its cache (generation; no Backward): sequence s has queries
+    [q_offsets[s], q_offsets[s+1]) of q and the rows [k_begin[s], k_end[s]) of the cache k, v, its newest token's included."""
+
+    @staticmethod
+    def Instantiate(net):
+        return CachedAttentionOperation(getattr(getattr(net, "Parameters", None), "NumHeads", 1))
+
+    def Forward(self, q, k, v, q_offsets, k_begin, k_end):
+        _ensure_initialized()
+        out = DeviceBuffer.alloc(q.dtype, q.Rows, q.Cols)
+        offsets, begin, end = _index(q_offsets), _index(k_begin), _index(k_end)
+        check(_lib.load().prad_cached_attention(q.device().handle, 0, k.device().handle, 0, v.device().handle, 0, out.handle, offsets.handle,
+                                                begin.handle, end.handle, *self._shape(q, k, v)))
+        self.Output = Matrix._from_device(out)
+        return self.Output
+
+    def Backward(self, dOutput):
+        raise InvalidOperationException("the attention of the newest tokens against a cache has no gradient")
