@@ -108,7 +108,7 @@ def token_ids(seed, tokens, vocab, kind):
 # chunk of the sums (32), of a wavefront; more rows than one workgroup orders; one token alone; no token at all
 EMBEDDINGS = [(1, 1, 1, "any"), (1, 10, 96, "any"), (49, 1000, 96, "text"), (256, 31, 4, "any"), (257, 31, 4, "any"), (257, 5, 130, "text"), (300, 2000, 7, "any"),
               (1024, 1, 260, "one"), (3000, 50, 33, "one"), (700, 1500, 64, "none"), (5000, 700, 66, "text"), (2049, 520, 256, "any"), (4096, 40000, 8, "text"),
-              (6000, 600000, 4, "any")]
+              (6000, 270000, 4, "any")]
 
 
 @DTYPES
