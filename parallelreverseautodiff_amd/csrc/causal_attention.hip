@@ -685,8 +685,6 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalA
     }
 }
 
-// Packed rows fit into 31 bits and a launch into its limits.
-template <typename T> inline bool rows_fit(const CausalArgs<T>& a) { return a.q_rows <= INT32_MAX / a.group - 16 && a.k_rows <= INT32_MAX; }
 inline int64_t tile_slots(int64_t rows, int64_t group, int64_t sequences) { return rows * group / 16 + sequences; }
 
 // Parts of a sequence's keys: one where a cache is short, no more than a lane each, and few enough that rows with many
@@ -718,7 +716,6 @@ constexpr int64_t MOST_GROUPS = 1 << 20;
 
 template <typename T>
 hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s) {
-    if (!rows_fit(a)) return hipErrorInvalidValue;
     const Parts<T> whole = {1, nullptr, nullptr, nullptr};
     BY_HEAD_DIM(attention_kernel, a.vec_q && a.vec_kv, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a, whole);
     return hipSuccess;
@@ -732,7 +729,6 @@ size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a) {
 template <typename T>
 hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     a.D = static_cast<T*>(workspace);
-    if (!rows_fit(a)) return hipErrorInvalidValue;
     const bool aligned = a.vec_q && a.vec_kv && a.vec_o;
     BY_HEAD_DIM(causal_bwd_q_kernel, aligned, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a);
     BY_HEAD_DIM(causal_bwd_kv_kernel, aligned, workgroups(tile_slots(a.q_rows, 1, a.sequences), MOST_GROUPS, a.kv_heads), a);
@@ -747,7 +743,6 @@ size_t cached_workspace_bytes(const CausalArgs<T>& a) {
 
 template <typename T>
 hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipStream_t s) {
-    if (!rows_fit(a)) return hipErrorInvalidValue;
     Parts<T> cut;
     cut.most = most_parts(a);
     cut.keys = static_cast<int32_t*>(workspace);

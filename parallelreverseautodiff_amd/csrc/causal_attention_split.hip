@@ -1209,10 +1209,10 @@ inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < (
 // that.  Measured, these against the units of 16, head dimension 64, 8 heads on 8 of keys, forward / backward in us:
 //   1024 rows of length 64: 15 / 26 against 9 / 19;  2048 of 64: 18 / 34 against 14 / 31;  2048 of 256: 22 / 46 against 23 / 59;
 //   4096 of 1024: 47 / 108 against 82 / 243;  8 heads on 2 of keys, 2048 of 256: 19 / 86 against 23 / 65, of 1024: 38 / 121
-//   against 47 / 193.  (Packed rows of a sequence are counted in 32 bits.)
+//   against 47 / 193.
 static bool split_pays(const CausalArgs<float>& p, int64_t least) {
     const int64_t rows = p.q_rows * p.heads;
-    return rows >= ((int64_t)1 << 14) && p.q_rows * p.group < ((int64_t)1 << 31) - 256 && (double)rows * p.q_rows / p.sequences >= (double)least;
+    return rows >= ((int64_t)1 << 14) && (double)rows * p.q_rows / p.sequences >= (double)least;
 }
 bool causal_split_fwd_pays(const CausalArgs<float>& p) { return split_pays(p, 1 << 22); }
 bool causal_split_bwd_pays(const CausalArgs<float>& p) { return split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23); }
