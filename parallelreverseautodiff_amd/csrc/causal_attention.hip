@@ -96,8 +96,8 @@ __device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNK
 
 // ---- units of work ----------------------------------------------------------------------------------------------------------
 // A unit is 16 packed rows of one sequence and key/value head against its keys or a part of them, one workgroup each; in the
-// gradients of K and V it is 16 keys against the rows.  Units are numbered through all sequences by a scan that every workgroup
-// does for itself: lengths live on the device.  The wavefronts take every fourth tile of 16 keys (or rows) and add their sums
+// gradients of K and V it is 16 keys against the rows.  Every workgroup finds the sequence of its unit for itself: lengths live
+// on the device.  The wavefronts take every fourth tile of 16 keys (or rows) and add their sums
 // up in LDS at the end, which gives short sequences four times the wavefronts.
 // Everything is transposed - S^T = K Q^T, O^T = V^T P^T - so that the weights come out of the first product in the lanes where
 // the second wants them and a row's statistics sit in a lane; rows go from memory to the registers of the matrix instructions
@@ -109,7 +109,8 @@ constexpr int LEAST_KEYS = 128, WHOLE_KEYS = 512, RUNNING = 512;
 
 template <typename T>
 struct Parts {
-    int most;         // of a sequence
+    uint32_t units;   // at most
+    int most;         // of a sequence; 1: units are tiles
     T *stat, *data;   // of part i of (token, head) number n: {maximum, sum} and the weighted sum of values, at n * most + i
     int32_t* keys;    // how many keys make a part, for the join
 };
@@ -137,31 +138,58 @@ __device__ __forceinline__ uint32_t scan64(uint32_t x) {
     return x;
 }
 
-// The sequence of unit `unit` and the unit's number inside it, by a whole wavefront; false: there are not so many.  (Rows fit
-// into 31 bits, so a sequence has less than 2^32 units.  Offsets that overlap may wrap the sum: the caller checks the number.)
+// The spans of sequences first + lane, and taking one of them from its lane (no value passes 31 bits).
 template <typename T>
-__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int group, int most_parts, uint32_t size, uint32_t unit, int lane, Span* span, uint32_t* parts, uint32_t* inside) {
+__device__ __forceinline__ Span lane_span(const CausalArgs<T>& p, int s) {
+    Span sp = {0, 0, 0, 0};
+    if (s < p.sequences) sp = span_of(p, s);
+    return sp;
+}
+__device__ __forceinline__ Span span_from(const Span& sp, int lane) {
+    return Span{__builtin_amdgcn_readlane((int)sp.q0, lane), __builtin_amdgcn_readlane((int)sp.nq, lane), __builtin_amdgcn_readlane((int)sp.k0, lane),
+                __builtin_amdgcn_readlane((int)sp.nk, lane)};
+}
+
+// Tile `tile` of the packed rows of `group` heads, by a whole wavefront: tiles are numbered through all sequences without a
+// table, sequence s from floor(offset group / 16) + s on, which leaves room for its ceil(n group / 16) tiles.  A search that
+// looks at 64 sequences at a time: one round of loads for up to 63 sequences, two for up to 4095.  false: no such tile.
+template <typename T>
+__device__ __forceinline__ bool find_tile(const CausalArgs<T>& p, uint32_t group, uint32_t tile, int lane, Span* span, uint32_t* inside) {
+    int64_t lo = 0, left = (int64_t)p.sequences + 1;  // the last sequence that begins at or before the tile lies in [lo, lo + left)
+    for (;;) {
+        const int64_t step = (left + 63) / 64, s = lo + lane * step;
+        const bool there = lane * step < left;
+        const uint32_t begin = there ? (uint32_t)clamped(p.q_off[s], p.q_rows) * group / 16 + (uint32_t)s : ~0u;
+        const Span sp = lane_span(p, step == 1 && there ? (int)s : p.sequences);
+        const uint64_t behind = ~__ballot(there && begin <= tile);
+        const int at = behind == 0 ? 63 : __builtin_ctzll(behind) - 1;
+        if (at < 0) return false;
+        if (step == 1) {
+            *span = span_from(sp, at);
+            *inside = tile - (uint32_t)__builtin_amdgcn_readlane((int)begin, at);
+            return *inside < ((uint32_t)span->nq * group + 15) / 16;
+        }
+        lo += at * step;
+        left = left - at * step < step ? left - at * step : step;
+    }
+}
+
+// Unit `unit` where sequences have parts, by a whole wavefront: its sequence, how many parts that has, and the unit's number
+// inside it; false: there are not so many.
+template <typename T>
+__device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int most_parts, uint32_t size, uint32_t unit, int lane, Span* span, uint32_t* parts, uint32_t* inside) {
     uint32_t before = 0;
     for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-        Span sp = {0, 0, 0, 0};
-        uint32_t units = 0, count = 1;
-        if (s0 + lane < p.sequences) {
-            sp = span_of(p, s0 + lane);
-            count = part_count(sp.nk, size, most_parts);
-            units = ((uint32_t)sp.nq * (uint32_t)group + 15) / 16 * count;
-        }
+        const Span sp = lane_span(p, s0 + lane);
+        const uint32_t count = part_count(sp.nk, size, most_parts), units = ((uint32_t)sp.nq * (uint32_t)p.group + 15) / 16 * count;
         const uint32_t upto = before + scan64(units);
         const uint64_t behind = __ballot(upto > unit);
         if (behind != 0) {
             const int at = __builtin_ctzll(behind);
-            // (none of these passes 31 bits)
-            span->q0 = __builtin_amdgcn_readlane((int)sp.q0, at);
-            span->nq = __builtin_amdgcn_readlane((int)sp.nq, at);
-            span->k0 = __builtin_amdgcn_readlane((int)sp.k0, at);
-            span->nk = __builtin_amdgcn_readlane((int)sp.nk, at);
+            *span = span_from(sp, at);
             *parts = __builtin_amdgcn_readlane(count, at);
             *inside = unit - __builtin_amdgcn_readlane(upto - units, at);
-            return true;
+            return *inside < (uint32_t)__builtin_amdgcn_readlane(units, at);  // (offsets that overlap may wrap the sum)
         }
         before = __builtin_amdgcn_readlane(upto, 63);
     }
@@ -170,12 +198,10 @@ __device__ __forceinline__ bool find_unit(const CausalArgs<T>& p, int group, int
 
 // Keys per part that make all units of a call few enough to run at once, each sequence having a part that is not whole.
 template <typename T>
-__device__ __forceinline__ uint32_t keys_per_part(const CausalArgs<T>& p, int most_parts, int lane) {
-    if (most_parts == 1) return 0;
+__device__ __forceinline__ uint32_t keys_per_part(const CausalArgs<T>& p, int lane) {
     float keys = 0, tiles = 0;
     for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-        if (s0 + lane >= p.sequences) break;
-        const Span sp = span_of(p, s0 + lane);
+        const Span sp = lane_span(p, s0 + lane);
         const float here = (float)(((uint32_t)sp.nq * (uint32_t)p.group + 15) / 16);
         tiles += here;
         keys += here * (float)sp.nk;
@@ -292,7 +318,7 @@ __device__ __forceinline__ uint32_t heads_over(uint32_t x, uint32_t group, uint3
 __device__ __forceinline__ uint32_t inverse_of(uint32_t group) { return (65535 + group) / group; }  // of 2^16, rounded up
 
 // ---- forward, and the newest tokens of a sequence against its cache ---------------------------------------------------------
-template <typename T, int HDP, bool ALIGNED>
+template <typename T, int HDP, bool ALIGNED, bool CUT>
 __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) attention_kernel(const CausalArgs<T> p, const Parts<T> cut) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
@@ -302,15 +328,18 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
     // heads of a unit are neighbours, so that workgroups without a unit come last
     const uint32_t stride = gridDim.x / p.kv_heads;
     const int kv = (int)(blockIdx.x % p.kv_heads);
-    const uint32_t keys_each = keys_per_part(p, cut.most, lane);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && cut.most > 1) *cut.keys = (int32_t)keys_each;
+    const uint32_t keys_each = CUT ? keys_per_part(p, lane) : 0;
+    if (CUT && blockIdx.x == 0 && threadIdx.x == 0) *cut.keys = (int32_t)keys_each;
     const T factor = p.scale * Num<T>::unit();
-    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+    for (uint32_t unit = blockIdx.x / p.kv_heads; unit < cut.units; unit += stride) {
         Span sp;
-        uint32_t parts, inside;
-        if (!find_unit(p, p.group, cut.most, keys_each, unit, lane, &sp, &parts, &inside)) return;
+        uint32_t parts = 1, inside;
+        if constexpr (CUT) {
+            if (!find_unit(p, cut.most, keys_each, unit, lane, &sp, &parts, &inside)) return;  // (nor are there any behind it)
+        } else {
+            if (!find_tile(p, p.group, unit, lane, &sp, &inside)) continue;
+        }
         const uint32_t rows = (uint32_t)sp.nq * (uint32_t)p.group, tile = inside / parts, part = inside % parts, row0 = tile * 16;
-        if (tile >= (rows + 15) / 16) return;  // (a wrapped sum)
         const int64_t lead = sp.nk - sp.nq;
         const uint32_t r = row0 + li < rows ? row0 + li : rows - 1;  // the lane's row; past the last it is the last one again
         const uint32_t first_token = row0 / p.group, ahead = (row0 % p.group + (r - row0)) / p.group;  // of the tile; of the row, from there
@@ -319,7 +348,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
         Pack<T, VEC> q[CHUNKS];
         load_along<T, HDP, ALIGNED>(p.Q + token * p.ldq + head * (int64_t)p.head_dim, g, p.head_dim, q);
         const int64_t first_last = lead + first_token, last = first_last + ahead;  // the last key that the tile's first row sees, that this one does
-        const int64_t size = part_keys(sp.nk, keys_each, cut.most), seen = clamped(first_last + (int)__builtin_amdgcn_readlane(ahead, 15) + 1, sp.nk);
+        const int64_t size = CUT ? part_keys(sp.nk, keys_each, cut.most) : 0, seen = clamped(first_last + (int)__builtin_amdgcn_readlane(ahead, 15) + 1, sp.nk);
         const int64_t from = part * size, to = parts == 1 || seen < from + size ? seen : from + size;
         const T* __restrict__ K = p.K + sp.k0 * p.ldk + kv * (int64_t)p.head_dim;
         const T* __restrict__ V = p.V + sp.k0 * p.ldv + kv * (int64_t)p.head_dim;
@@ -433,7 +462,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
                 for (int t = 0; t < VEC; ++t) sum[t] = fma(e.v[t], f, sum[t]);
             }
             T* __restrict__ dst;
-            if (parts == 1) {
+            if (!CUT || parts == 1) {
                 const bool any = first_last + ahead_of >= 0 && sp.nk > 0;
                 const T by = any ? 1 / total : (T)0;
 #pragma unroll
@@ -452,7 +481,6 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
             for (int t = 0; t < VEC; ++t)
                 if (d + t < p.head_dim) dst[d + t] = sum[t];
         }
-        if (unit > ~0u - stride) return;
         __syncthreads();
     }
 }
@@ -529,7 +557,7 @@ __device__ __forceinline__ void write_sums(const T (&sums)[WAVES][16 * (HDP + 16
 
 // Gradient of Q: 16 packed rows against the keys that they see.  Writes D = rowsum(dO (.) O) for the other kernel.
 template <typename T, int HDP, bool ALIGNED>
-__global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalArgs<T> p) {
+__global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalArgs<T> p, uint32_t units) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
     __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
@@ -537,12 +565,11 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalAr
     const uint32_t stride = gridDim.x / p.kv_heads;
     const int kv = (int)(blockIdx.x % p.kv_heads);
     const T factor = p.scale * Num<T>::unit();
-    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+    for (uint32_t unit = blockIdx.x / p.kv_heads; unit < units; unit += stride) {
         Span sp;
-        uint32_t parts, inside;
-        if (!find_unit(p, p.group, 1, 0, unit, lane, &sp, &parts, &inside)) return;
+        uint32_t inside;
+        if (!find_tile(p, p.group, unit, lane, &sp, &inside)) continue;
         const uint32_t rows = (uint32_t)sp.nq * (uint32_t)p.group, row0 = inside * 16;
-        if (inside >= (rows + 15) / 16) return;  // (a wrapped sum)
         const uint32_t r = row0 + li < rows ? row0 + li : rows - 1;
         const uint32_t first_token = row0 / p.group, ahead = (row0 % p.group + (r - row0)) / p.group, last = first_token + ahead;
         const int64_t token = sp.q0 + last;
@@ -602,14 +629,13 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalAr
             const uint32_t to = first_token + (row0 % p.group + row) / p.group;
             return p.dQ + (sp.q0 + to) * p.lddq + (kv * p.group + (int)(row0 + row - to * p.group)) * (int64_t)p.head_dim;
         });
-        if (unit > ~0u - stride) return;
         __syncthreads();
     }
 }
 
 // Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.
 template <typename T, int HDP, bool ALIGNED>
-__global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalArgs<T> p) {
+__global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalArgs<T> p, uint32_t units) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
     __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
@@ -617,12 +643,11 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalA
     const uint32_t stride = gridDim.x / p.kv_heads, group = p.group, inverse = inverse_of(group);
     const int kv = (int)(blockIdx.x % p.kv_heads);
     const T factor = p.scale * Num<T>::unit();
-    for (uint32_t unit = blockIdx.x / p.kv_heads;; unit += stride) {
+    for (uint32_t unit = blockIdx.x / p.kv_heads; unit < units; unit += stride) {
         Span sp;
-        uint32_t parts, inside;
-        if (!find_unit(p, 1, 1, 0, unit, lane, &sp, &parts, &inside)) return;
+        uint32_t inside;
+        if (!find_tile(p, 1, unit, lane, &sp, &inside)) continue;
         const uint32_t keys = (uint32_t)sp.nk, rows = keys * group, key0 = inside * 16;
-        if (inside >= (keys + 15) / 16) return;  // (a wrapped sum)
         const uint32_t key = key0 + li < keys ? key0 + li : keys - 1;
         Pack<T, VEC> k[CHUNKS], v[CHUNKS];
         load_along<T, HDP, ALIGNED>(p.K + (sp.k0 + key) * p.ldk + kv * (int64_t)p.head_dim, g, p.head_dim, k);
@@ -680,7 +705,6 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalA
         put_sums<T, N, NY, PITCH>(dk, li, g, sums[wave]);
         __syncthreads();
         write_sums<T, HDP>(sums, here, p.head_dim, p.scale, [&](int row) { return p.dK + (sp.k0 + key0 + row) * p.lddk + kv * (int64_t)p.head_dim; });
-        if (unit > ~0u - stride) return;
         __syncthreads();
     }
 }
@@ -698,27 +722,32 @@ int most_parts(const CausalArgs<T>& a) {
 
 }  // namespace
 
-// A launch of KERNEL<T, HDP, ALIGNED> for the smallest padded head dimension that holds head_dim.
-#define BY_HEAD_DIM_OF(KERNEL, ALIGNED, GROUPS, ...)                                                                                              \
-    do {                                                                                                                                          \
-        const dim3 grid((unsigned)(GROUPS)), block(64 * WAVES);                                                                                   \
-        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                       \
-        else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                  \
-        else hipLaunchKernelGGL((KERNEL<T, 128, ALIGNED>), grid, block, 0, s, __VA_ARGS__);                                                       \
-        if (hipError_t e = hipGetLastError()) return e;                                                                                           \
+// A launch of KERNEL<T, HDP, ALIGNED, ...> for the smallest padded head dimension that holds head_dim.
+#define BY_HEAD_DIM(KERNEL, GROUPS, ARGS, ...)                                                                       \
+    do {                                                                                                                \
+        const dim3 grid((unsigned)(GROUPS)), block(64 * WAVES);                                                         \
+        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32, __VA_ARGS__>), grid, block, 0, s, UNPACKED ARGS);       \
+        else if (a.head_dim <= 64) hipLaunchKernelGGL((KERNEL<T, 64, __VA_ARGS__>), grid, block, 0, s, UNPACKED ARGS);  \
+        else hipLaunchKernelGGL((KERNEL<T, 128, __VA_ARGS__>), grid, block, 0, s, UNPACKED ARGS);                       \
+        if (hipError_t e = hipGetLastError()) return e;                                                                 \
     } while (0)
-#define BY_HEAD_DIM(KERNEL, ALIGNED, GROUPS, ...) \
-    do { if (ALIGNED) BY_HEAD_DIM_OF(KERNEL, true, GROUPS, __VA_ARGS__); else BY_HEAD_DIM_OF(KERNEL, false, GROUPS, __VA_ARGS__); } while (0)
+#define UNPACKED(...) __VA_ARGS__
 
 // Workgroups for `tiles` units of every key/value head: one each, of very many some take several.
 static int64_t workgroups(int64_t tiles, int64_t most, int64_t kv_heads) { return std::min(tiles, std::max<int64_t>(1, most / kv_heads)) * kv_heads; }
 constexpr int64_t MOST_GROUPS = 1 << 20;
 
+template <typename T, bool CUT>
+static hipError_t launch_attention(const CausalArgs<T>& a, const Parts<T>& cut, int64_t most, hipStream_t s) {
+    const int64_t groups = workgroups(cut.units, most, a.kv_heads);
+    if (a.vec_q && a.vec_kv) BY_HEAD_DIM(attention_kernel, groups, (a, cut), true, CUT);
+    else BY_HEAD_DIM(attention_kernel, groups, (a, cut), false, CUT);
+    return hipSuccess;
+}
+
 template <typename T>
 hipError_t launch_causal_fwd(const CausalArgs<T>& a, hipStream_t s) {
-    const Parts<T> whole = {1, nullptr, nullptr, nullptr};
-    BY_HEAD_DIM(attention_kernel, a.vec_q && a.vec_kv, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a, whole);
-    return hipSuccess;
+    return launch_attention<T, false>(a, {(uint32_t)tile_slots(a.q_rows, a.group, a.sequences), 1, nullptr, nullptr, nullptr}, MOST_GROUPS, s);
 }
 
 template <typename T>
@@ -729,9 +758,15 @@ size_t causal_bwd_workspace_bytes(const CausalArgs<T>& a) {
 template <typename T>
 hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     a.D = static_cast<T*>(workspace);
-    const bool aligned = a.vec_q && a.vec_kv && a.vec_o;
-    BY_HEAD_DIM(causal_bwd_q_kernel, aligned, workgroups(tile_slots(a.q_rows, a.group, a.sequences), MOST_GROUPS, a.kv_heads), a);
-    BY_HEAD_DIM(causal_bwd_kv_kernel, aligned, workgroups(tile_slots(a.q_rows, 1, a.sequences), MOST_GROUPS, a.kv_heads), a);
+    const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences), key_tiles = tile_slots(a.q_rows, 1, a.sequences);
+    const int64_t groups = workgroups(tiles, MOST_GROUPS, a.kv_heads), key_groups = workgroups(key_tiles, MOST_GROUPS, a.kv_heads);
+    if (a.vec_q && a.vec_kv && a.vec_o) {
+        BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), true);
+        BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), true);
+    } else {
+        BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), false);
+        BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), false);
+    }
     return hipSuccess;
 }
 
@@ -748,15 +783,13 @@ hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipS
     cut.keys = static_cast<int32_t*>(workspace);
     cut.data = static_cast<T*>(workspace) + 16 / sizeof(T);
     cut.stat = cut.data + a.q_rows * a.heads * (int64_t)cut.most * a.head_dim;
-    // where the units run at once there are no more than that of them
     const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
-    const int64_t most = cut.most == 1 ? MOST_GROUPS : tiles * a.kv_heads <= RUNNING / 2 ? RUNNING : 4 * RUNNING;
-    BY_HEAD_DIM(attention_kernel, a.vec_q && a.vec_kv, workgroups(tiles * cut.most, most, a.kv_heads), a, cut);
-    if (cut.most > 1) {
-        hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, cut);
-        if (hipError_t e = hipGetLastError()) return e;
-    }
-    return hipSuccess;
+    cut.units = (uint32_t)(tiles * cut.most);
+    if (cut.most == 1) return launch_attention<T, false>(a, cut, MOST_GROUPS, s);
+    // where the units run at once there are no more than that of them
+    if (hipError_t e = launch_attention<T, true>(a, cut, tiles * a.kv_heads <= RUNNING / 2 ? RUNNING : 4 * RUNNING, s)) return e;
+    hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, cut);
+    return hipGetLastError();
 }
 
 #define INSTANTIATE(T)                                                              \
