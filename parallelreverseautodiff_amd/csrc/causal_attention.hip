@@ -150,28 +150,37 @@ __device__ __forceinline__ Span span_from(const Span& sp, int lane) {
                 __builtin_amdgcn_readlane((int)sp.nk, lane)};
 }
 
-// Tile `tile` of the packed rows of `group` heads, by a whole wavefront: tiles are numbered through all sequences without a
-// table, sequence s from floor(offset group / 16) + s on, which leaves room for its ceil(n group / 16) tiles.  A search that
-// looks at 64 sequences at a time: one round of loads for up to 63 sequences, two for up to 4095.  false: no such tile.
-template <typename T>
-__device__ __forceinline__ bool find_tile(const CausalArgs<T>& p, uint32_t group, uint32_t tile, int lane, Span* span, uint32_t* inside) {
-    int64_t lo = 0, left = (int64_t)p.sequences + 1;  // the last sequence that begins at or before the tile lies in [lo, lo + left)
+// The last sequence s whose begin(s, its offset) is not above `value`, by a whole wavefront: its span and begin; false: none.
+// A search that looks at 64 sequences at a time: one round of loads for up to 63 sequences, two for up to 4095.
+template <typename T, typename Begin>
+__device__ __forceinline__ bool find_span(const CausalArgs<T>& p, uint32_t value, int lane, Begin begin, Span* span, uint32_t* begun) {
+    int64_t lo = 0, left = (int64_t)p.sequences + 1;  // it lies in [lo, lo + left); the end counts as a sequence without rows
     for (;;) {
         const int64_t step = (left + 63) / 64, s = lo + lane * step;
         const bool there = lane * step < left;
-        const uint32_t begin = there ? (uint32_t)clamped(p.q_off[s], p.q_rows) * group / 16 + (uint32_t)s : ~0u;
+        const uint32_t mine = there ? begin((uint32_t)s, (uint32_t)clamped(p.q_off[s], p.q_rows)) : ~0u;
         const Span sp = lane_span(p, step == 1 && there ? (int)s : p.sequences);
-        const uint64_t behind = ~__ballot(there && begin <= tile);
-        const int at = behind == 0 ? 63 : __builtin_ctzll(behind) - 1;
+        const uint64_t above = ~__ballot(there && mine <= value);
+        const int at = above == 0 ? 63 : __builtin_ctzll(above) - 1;
         if (at < 0) return false;
         if (step == 1) {
             *span = span_from(sp, at);
-            *inside = tile - (uint32_t)__builtin_amdgcn_readlane((int)begin, at);
-            return *inside < ((uint32_t)span->nq * group + 15) / 16;
+            *begun = __builtin_amdgcn_readlane((int)mine, at);
+            return true;
         }
         lo += at * step;
         left = left - at * step < step ? left - at * step : step;
     }
+}
+
+// Tile `tile` of the packed rows of `group` heads and its number in its sequence.  Tiles are numbered through all sequences
+// without a table, sequence s from floor(offset group / 16) + s on, which leaves room for its ceil(n group / 16) tiles.
+template <typename T>
+__device__ __forceinline__ bool find_tile(const CausalArgs<T>& p, uint32_t group, uint32_t tile, int lane, Span* span, uint32_t* inside) {
+    uint32_t first;
+    if (!find_span(p, tile, lane, [group](uint32_t s, uint32_t offset) { return offset * group / 16 + s; }, span, &first)) return false;
+    *inside = tile - first;
+    return *inside < ((uint32_t)span->nq * group + 15) / 16;
 }
 
 // Unit `unit` where sequences have parts, by a whole wavefront: its sequence, how many parts that has, and the unit's number
@@ -485,28 +494,30 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
     }
 }
 
-// Joins the parts of a row: a wavefront per (token, head).
+// Joins the parts of a row: a workgroup per (token, head), a wavefront every fourth part, whose loads are all in flight at once.
 template <typename T>
-__global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p, const Parts<T> cut) {
-    const int lane = threadIdx.x & 63;
-    const int64_t at = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    if (at >= p.q_rows * p.heads) return;
-    const int64_t token = at / p.heads;
-    // the sequence of the token: rows in front of the first and behind the last are left as they are
-    int begun = 0;  // offsets that are not behind the token
-    for (int s0 = 0; s0 <= p.sequences; s0 += 64) {
-        const int here = __popcll(__ballot(s0 + lane <= p.sequences && clamped(p.q_off[s0 + lane], p.q_rows) <= token));
-        begun += here;
-        if (here < 64) break;
-    }
-    begun = __builtin_amdgcn_readfirstlane(begun);
-    if (begun == 0 || begun > p.sequences) return;
-    const Span sp = span_of(p, begun - 1);
+__global__ void __launch_bounds__(64 * WAVES) cached_join_kernel(const CausalArgs<T> p, const Parts<T> cut) {
+    __shared__ T sums[WAVES][128];
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t at = blockIdx.x, token = at / p.heads;
+    // rows in front of the first sequence and behind the last are left as they are
+    Span sp;
+    uint32_t first;
+    if (!find_span(p, (uint32_t)token, lane, [](uint32_t, uint32_t offset) { return offset; }, &sp, &first)) return;
     if (token < sp.q0 || token >= sp.q0 + sp.nq) return;
     const int parts = (int)part_count(sp.nk, (uint32_t)*cut.keys, cut.most);
     if (parts == 1) return;
     const T m = lane < parts ? cut.stat[2 * (at * cut.most + lane)] : -(T)INFINITY;
     const T l = lane < parts ? cut.stat[2 * (at * cut.most + lane) + 1] : (T)0;
+    constexpr int COUNT = 64 / WAVES;
+    const T* __restrict__ mine = cut.data + at * cut.most * (int64_t)p.head_dim;
+    T v[COUNT][2];
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        const int i = wave + WAVES * j;
+        v[j][0] = i < parts && lane < p.head_dim ? mine[(int64_t)i * p.head_dim + lane] : (T)0;
+        v[j][1] = i < parts && lane + 64 < p.head_dim ? mine[(int64_t)i * p.head_dim + lane + 64] : (T)0;
+    }
     T top = m;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) top = fmax(top, __shfl_xor(top, d, 64));
@@ -514,18 +525,22 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CausalArgs<T> p,
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
     f = sp.nk - sp.nq + (token - sp.q0) >= 0 ? f / total : (T)0;
-    const T* __restrict__ mine = cut.data + at * cut.most * (int64_t)p.head_dim;
     T sum[2] = {0, 0};
-    const int d0 = lane < p.head_dim ? lane : 0, d1 = lane + 64 < p.head_dim ? lane + 64 : 0;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-        const T w = __shfl(f, i, 64);
-        sum[0] += mine[(int64_t)i * p.head_dim + d0] * w;
-        sum[1] += mine[(int64_t)i * p.head_dim + d1] * w;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+        const T w = __shfl(f, wave + WAVES * j, 64);
+        sum[0] = fma(v[j][0], w, sum[0]);
+        sum[1] = fma(v[j][1], w, sum[1]);
     }
-    T* __restrict__ dst = p.O + token * p.ldo + at % p.heads * (int64_t)p.head_dim;
-    if (lane < p.head_dim) dst[lane] = sum[0];
-    if (lane + 64 < p.head_dim) dst[lane + 64] = sum[1];
+    sums[wave][lane] = sum[0];
+    sums[wave][lane + 64] = sum[1];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= p.head_dim) return;
+    T out = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) out += sums[w][d];
+    p.O[token * p.ldo + at % p.heads * (int64_t)p.head_dim + d] = out;
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
@@ -783,12 +798,12 @@ hipError_t launch_cached_attention(const CausalArgs<T>& a, void* workspace, hipS
     cut.keys = static_cast<int32_t*>(workspace);
     cut.data = static_cast<T*>(workspace) + 16 / sizeof(T);
     cut.stat = cut.data + a.q_rows * a.heads * (int64_t)cut.most * a.head_dim;
-    const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences), rows = (a.q_rows * a.heads + 3) / 4;
+    const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences);
     cut.units = (uint32_t)(tiles * cut.most);
     if (cut.most == 1) return launch_attention<T, false>(a, cut, MOST_GROUPS, s);
     // where the units run at once there are no more than that of them
     if (hipError_t e = launch_attention<T, true>(a, cut, tiles * a.kv_heads <= RUNNING / 2 ? RUNNING : 4 * RUNNING, s)) return e;
-    hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, a, cut);
+    hipLaunchKernelGGL(cached_join_kernel<T>, dim3((unsigned)(a.q_rows * a.heads)), dim3(64 * WAVES), 0, s, a, cut);
     return hipGetLastError();
 }
 
