@@ -182,6 +182,11 @@ __device__ __forceinline__ void write_order(const CausalArgs<float>& p, int whic
     }
 }
 
+// Where lane l's 16 bytes lie among the 64 of fragment f.  Two bits of the row are turned over by the lane half and by the
+// fragment's parity: a transposing load asks for 4 rows of 2 fragments and both halves at a time, which lie 1 KB and 512 bytes
+// apart and would be in the same LDS banks.  (Fragments that are read along stay one KB in a row.)
+__device__ __forceinline__ int place_in_fragment(int f, int l) { return l ^ (l >> 5) << 2 ^ (f & 1) << 3; }
+
 template <int HDP>
 __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     constexpr int PITCH = HDP + 4, PER_ROW = HDP / 4, COUNT = 64 * PER_ROW / 256;
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
 #pragma unroll
     for (int u = 0; u < 2 * FRAGS * 64 / 256; ++u) {
         const int at = threadIdx.x + 256 * u, l = at & 63, f = (at >> 6) % FRAGS, block = (at >> 6) / FRAGS;
-        const int64_t hi_at = base + (int64_t)(block * 2 * FRAGS + f) * 512 + l * 8, lo_at = hi_at + FRAGS * 512;
+        const int64_t hi_at = base + (int64_t)(block * 2 * FRAGS + f) * 512 + place_in_fragment(f, l) * 8, lo_at = hi_at + FRAGS * 512;
         float x[8];
         h8 hi[1], lo[1];
         const float* __restrict__ row = tile + (32 * block + (l & 31)) * PITCH + 16 * f + 8 * (l >> 5);
@@ -347,7 +352,7 @@ __device__ __forceinline__ void staged() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
 }
-__device__ __forceinline__ h8 frag(const _Float16* base, int f, int lane) { return *reinterpret_cast<const h8*>(base + f * 512 + lane * 8); }
+__device__ __forceinline__ h8 frag(const _Float16* base, int f, int lane) { return *reinterpret_cast<const h8*>(base + f * 512 + place_in_fragment(f, lane) * 8); }
 
 // Asks the scheduler for this order of instructions in a basic block: `n` LDS reads, `n` matrix instructions.  Without it the
 // fragments are read right before they are used and every step waits for LDS.
@@ -419,15 +424,16 @@ __device__ __forceinline__ void rows_product(const _Float16* block, const h8 (&b
 // gives each 16 lanes 4 rows of 16 columns: its lane i asks for columns 4 (i % 4) .. + 3 of row i / 4 and receives column i.
 typedef short s4 __attribute__((ext_vector_type(4)));
 struct Across {
-    int at;  // of the lane, in halves
+    int at;  // of the lane, in halves; 8 rows on: the other value of that bit
     __device__ __forceinline__ explicit Across(int lane) {
         const int i = lane & 15;
-        at = ((lane >> 4) & 1) * 512 + (4 * (lane >> 5) + (i >> 2) + 32 * ((i >> 1) & 1)) * 8 + (i & 1) * 4;
+        const int f = (lane >> 4) & 1, half = (i >> 1) & 1;
+        at = f * 512 + place_in_fragment(f, 32 * half + 4 * (lane >> 5) + (i >> 2)) * 8 + (i & 1) * 4;
     }
     __device__ __forceinline__ h8 frag(const _Float16* plane, int c, int t) const {
         typedef __attribute__((address_space(3))) s4* lds;
-        const _Float16* first = plane + at + c * 1024 + t * 128;
-        const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)first), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(first + 64));
+        const _Float16* from = plane + c * 1024 + t * 128;
+        const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(from + at)), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(from + (at ^ 64)));
         typedef short s8 __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(h8, s8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
     }
