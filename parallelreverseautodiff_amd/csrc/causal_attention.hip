@@ -6,12 +6,12 @@
 //
 // One pass over the keys with the running maximum and sum of a row: scores never reach memory.  The rows of a tile are
 // (token, head of the group) pairs - token r / group, head r % group - so the query heads that share a key/value head share its
-// tiles, and their gradients of K and V add up in one workgroup's registers in one order.
+// tiles, and their gradients of K and V add up in one workgroup in one order.
 // Statistics and sums are held in the element type (32 or 64 bits); products run on the 16 x 16 x 4 matrix instructions, whose
 // element order along the reduction is free as long as both operands agree: lane group g takes elements CH c + VEC g + t of
 // chunk c, which makes its reads whole 16-byte vectors.
 //
-// Non-finite values.  A key row that holds one (in K or V) is staged as zeros and its scores become NaN where they are seen: a
+// Non-finite values.  A key row that holds one (in K or V) counts as zeros and its scores become NaN where they are seen: a
 // query that sees it has a row of NaN, a query that does not is not touched by it - a product with a masked weight of zero
 // would carry 0 * NaN into every row of the tile.
 #include "common.h"
@@ -97,14 +97,17 @@ __device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNK
 // ---- units of work ----------------------------------------------------------------------------------------------------------
 // A unit is 16 packed rows of one sequence and key/value head against its keys or a part of them, one workgroup each; in the
 // gradients of K and V it is 16 keys against the rows.  Every workgroup finds the sequence of its unit for itself: lengths live
-// on the device.  The wavefronts take every fourth tile of 16 keys (or rows) and add their sums
-// up in LDS at the end, which gives short sequences four times the wavefronts.
+// on the device.  The wavefronts take every fourth tile of 16 keys (or rows) and add their sums up in LDS at the end, which gives
+// short sequences four times the wavefronts.  (Against 64 rows a workgroup and tiles in LDS: 86 us for 301, the batch of doubles
+// below; 401 for 743, two sequences of 1024, 8 heads of 64 doubles.  Eight wavefronts: 80 and 467.)
 // Everything is transposed - S^T = K Q^T, O^T = V^T P^T - so that the weights come out of the first product in the lanes where
 // the second wants them and a row's statistics sit in a lane; rows go from memory to the registers of the matrix instructions
 // without LDS, along for a product over the head dimension and across for one over the rows.  The registers of an operand are
 // filled again for the next tile as soon as its product has read them, so that loads are always in flight.
 constexpr int WAVES = 4;
-// parts of the keys: the least keys in one, sequences that are not cut, units that run at once (two workgroups per compute unit)
+// Parts of the keys: the least keys in one, sequences that are not cut (300 keys in parts of 64 and joined: 15.2 us, whole: 13.2),
+// units that run at once, two workgroups per compute unit.  Parts are as large as lets all units of a call run at once: the cache
+// of 24 sequences below in 71 us, in parts of 256 keys in 86.
 constexpr int LEAST_KEYS = 128, WHOLE_KEYS = 512, RUNNING = 512;
 
 template <typename T>
@@ -327,6 +330,10 @@ __device__ __forceinline__ uint32_t heads_over(uint32_t x, uint32_t group, uint3
 __device__ __forceinline__ uint32_t inverse_of(uint32_t group) { return (65535 + group) / group; }  // of 2^16, rounded up
 
 // ---- forward, and the newest tokens of a sequence against its cache ---------------------------------------------------------
+// A cache is read once and bounds the call from some MB on: 24 sequences of 0 to 8192 keys, 16 heads on 4 of 128 floats, in
+// 64 us, and 5 for joining the parts (332 MB, 4.5 TB/s of the 5.0 that a copy reaches).  Small calls are bound by their latency,
+// about 1 us to find the sequence, 1.5 for the first rows, 1 per tile and 0.6 for the sums: 300 keys, 8 heads on 2 of 64
+// floats, in 9.4 us.  Doubles, forward over sequences of 512, 256, 200 and 37, 6 heads on 3 of 32: 20 us.
 template <typename T, int HDP, bool ALIGNED, bool CUT>
 __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) attention_kernel(const CausalArgs<T> p, const Parts<T> cut) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(64 * WAVES) cached_join_kernel(const CausalArg
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 // (Queries and keys are the same rows here: token i sees key j iff j <= i.  A row that sees a non-finite value has a NaN in lse,
-// one of dO with a non-finite value a NaN in D: their weights are NaN, and the values themselves are staged as zeros.)
+// one of dO with a non-finite value a NaN in D: their weights are NaN, and the values themselves count as zeros.)
 
 // The sums of the wavefronts of 16 rows, times `by`, to the rows' places.
 template <typename T, int HDP, typename RowOf>
@@ -570,7 +577,8 @@ __device__ __forceinline__ void write_sums(const T (&sums)[WAVES][16 * (HDP + 16
     }
 }
 
-// Gradient of Q: 16 packed rows against the keys that they see.  Writes D = rowsum(dO (.) O) for the other kernel.
+// Gradient of Q: 16 packed rows against the keys that they see.  Writes D = rowsum(dO (.) O) for the other kernel.  Bound by the
+// latency of a tile (the batch of doubles above: 22 us, 2.3 us a tile).
 template <typename T, int HDP, bool ALIGNED>
 __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalArgs<T> p, uint32_t units) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
@@ -648,7 +656,9 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalAr
     }
 }
 
-// Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.
+// Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.  As above: 44 us, 16
+// tiles of rows to a wavefront at most.  Reading a tile ahead in these two was measured: up to 16 % faster on sequences from
+// 512 on, as much slower on many short ones, whose registers then let fewer wavefronts run; it was left out.
 template <typename T, int HDP, bool ALIGNED>
 __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalArgs<T> p, uint32_t units) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
