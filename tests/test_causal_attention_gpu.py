@@ -434,7 +434,13 @@ def against_definition(dtype, new, ranges, rows, heads, kv_heads, d, odd=False):
 CACHED = [([1], [(0, 1)], 1, 1, 1, 4), ([1], [(3, 3)], 9, 2, 1, 32), ([1, 1, 1], [(0, 16), (20, 35), (40, 57)], 64, 4, 2, 64), ([1], [(7, 2007)], 2048, 8, 2, 128),
           ([1, 1], [(0, 300), (0, 300)], 512, 3, 1, 33), ([5, 1, 0, 9], [(0, 40), (30, 80), (80, 90), (95, 104)], 120, 4, 1, 80), ([4], [(10, 12)], 30, 2, 2, 16),
           ([1], [(0, 70)], 70, 20, 1, 64), ([33], [(0, 100)], 128, 6, 2, 40), ([1] * 40, [(10 * i, 10 * i + i) for i in range(40)], 400, 2, 1, 64),
-          ([1], [(100, 4100)], 4200, 16, 1, 128), ([200], [(0, 350)], 400, 2, 1, 64)]
+          ([1], [(100, 4100)], 4200, 16, 1, 128), ([200], [(0, 350)], 400, 2, 1, 64),
+          # caches of more than 512 rows, whose keys are cut into parts: some sequences with parts and some without, an empty one,
+          # several tiles of rows, fewer keys than queries, more than 64 sequences, none or few keys in the last part, as many
+          # parts as there may be
+          ([1, 1, 1], [(0, 700), (700, 700), (650, 2000)], 2048, 2, 1, 33), ([9, 40], [(5, 900), (300, 1700)], 1800, 6, 2, 40), ([700], [(0, 600)], 640, 2, 2, 16),
+          ([1] * 70, [(20 * i, 20 * i + i * 37 % 900) for i in range(70)], 2400, 2, 1, 64), ([2, 0, 3], [(0, 5000), (10, 5000), (4990, 5000)], 5000, 20, 1, 128),
+          ([1], [(0, 513)], 513, 1, 1, 1), ([1, 1], [(0, 9000), (0, 640)], 9001, 4, 4, 8)]
 
 
 @DTYPES
@@ -442,6 +448,60 @@ CACHED = [([1], [(0, 1)], 1, 1, 1, 4), ([1], [(3, 3)], 9, 2, 1, 32), ([1, 1, 1],
 @pytest.mark.parametrize("odd", [False, True], ids=["even", "odd"])
 def test_cached_attention_against_its_definition(gpu, dtype, case, odd):
     against_definition(dtype, *case, odd=odd)
+
+
+def test_thousands_of_sequences(gpu):
+    """Sequences are found by a search of three rounds; short and empty ones in between, packed and against a cache."""
+    compare(Batch(np.float64, [1, 0, 2] * 1400, 2, 1, 4, "fused"))
+    against_definition(np.float32, [1, 0, 2] * 1400, [(i % 500, i % 500 + i % 13) for i in range(4200)], 512, 2, 1, 4)
+
+
+def test_calls_of_several_threads_at_once(gpu):
+    """Each with operands of its own, sharing the library's one workspace: what each gets is what it gets alone."""
+    import threading
+    large, short = (lambda i: Batch(np.float32, [500, 200 + i], 64, 32, 16, "fused", seed=i)), (lambda i: Batch(np.float64, [40 + i, 90], 2, 1, 32, "fused", seed=i))
+    batches = [make(i) for i in range(4) for make in (large, short)]
+    alone = [(b.forward(), None) for b in batches]
+    alone = [(o.download(), b.backward(o, l)) for b, ((o, l), _) in zip(batches, alone)]
+    wrong = []
+
+    def run(b, want):
+        for _ in range(3):
+            o, l = b.forward()
+            got = o.download(), b.backward(o, l)
+            if not (np.array_equal(got[0], want[0], equal_nan=True) and all(np.array_equal(x, y, equal_nan=True) for x, y in zip(got[1], want[1]))):
+                wrong.append(b.lengths)
+
+    threads = [threading.Thread(target=run, args=(b, w)) for b, w in zip(batches, alone)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert wrong == []
+
+
+def test_a_workspace_that_grows_behind_a_recording(gpu):
+    """A recorded call keeps the workspace of its recording when a larger eager call takes another."""
+    lib, gr = _lib.load(), ctypes.c_void_p()
+    small, large = (Batch(np.float32, lengths, 64, 32, d, "fused", front=0, behind=0) for lengths, d in (([300, 200], 16), ([1500, 900], 64)))
+    o, l = small.forward()
+    g, d = dev(small.g), unfilled(np.float32, small.rows, small.full[0])
+    grads = [x for c in small.cols for x in (d.handle, c)]
+    step = lambda: check(lib.prad_causal_attention_bwd(*small.operands(), o.handle, l.handle, g.handle, *grads, small.offsets.handle, *small.tail))
+    step()
+    want = d.download()
+    check(lib.prad_graph_begin())
+    try:
+        step()
+    finally:
+        check(lib.prad_graph_end(ctypes.byref(gr)))
+    first = large.backward(*large.forward())
+    for _ in range(3):
+        d.zero()
+        check(lib.prad_graph_launch(gr))
+        assert np.array_equal(d.download(), want)
+        assert all(np.array_equal(x, y) for x, y in zip(large.backward(*large.forward()), first))
+    check(lib.prad_graph_destroy(gr))
 
 
 @DTYPES
