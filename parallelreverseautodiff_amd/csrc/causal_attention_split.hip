@@ -56,8 +56,9 @@ __device__ __forceinline__ float pow2(int e) { return __builtin_ldexpf(1.0f, e <
 
 // Tiles of 64 packed rows (token, head of the group) are numbered as in causal_attention.hip: sequence s begins at
 // floor(offset G / R) + s.
-__device__ __forceinline__ int64_t first_tile(const CausalArgs<float>& p, int s, int group, int R) { return clamped(p.q_off[s], p.q_rows) * group / R + s; }
-__device__ __forceinline__ bool find_tile(const CausalArgs<float>& p, int group, int R, int64_t tile, int* sequence, int64_t* inside) {
+// (Packed rows, with some tiles behind the last, are counted in 31 bits; tiles and sequences together in 32.)
+__device__ __forceinline__ uint32_t first_tile(const CausalArgs<float>& p, int s, uint32_t group, uint32_t R) { return (uint32_t)clamped(p.q_off[s], p.q_rows) * group / R + s; }
+__device__ __forceinline__ bool find_tile(const CausalArgs<float>& p, uint32_t group, uint32_t R, uint32_t tile, int* sequence, uint32_t* inside) {
     int lo = 0, hi = p.sequences;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -69,9 +70,9 @@ __device__ __forceinline__ bool find_tile(const CausalArgs<float>& p, int group,
     *inside = tile - first_tile(p, lo - 1, group, R);
     return true;
 }
-__device__ __forceinline__ void sequence_rows(const CausalArgs<float>& p, int s, int64_t* q0, int64_t* n) {
-    *q0 = clamped(p.q_off[s], p.q_rows);
-    const int64_t q1 = clamped(p.q_off[s + 1], p.q_rows);
+__device__ __forceinline__ void sequence_rows(const CausalArgs<float>& p, int s, uint32_t* q0, uint32_t* n) {
+    *q0 = (uint32_t)clamped(p.q_off[s], p.q_rows);
+    const uint32_t q1 = (uint32_t)clamped(p.q_off[s + 1], p.q_rows);
     *n = q1 > *q0 ? q1 - *q0 : 0;
 }
 
@@ -142,18 +143,19 @@ constexpr int ORDER_BINS = 1024;
 __device__ __forceinline__ void write_order(const CausalArgs<float>& p, int which, int slots, int shift, int4* __restrict__ order, int* bins) {
     __shared__ int wave_total[4];
     const int lane = threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
-    const int group = which == 0 ? p.group : 1;
+    const uint32_t group = which == 0 ? p.group : 1;
     for (int i = threadIdx.x; i < ORDER_BINS; i += 256) bins[i] = 0;
     __syncthreads();
     for (int pass = 0; pass < 2; ++pass) {
         for (int slot = threadIdx.x; slot < slots; slot += 256) {
             int s = -1;
-            int64_t inside = 0, q0 = 0, n = 0, work = -1;  // in tiles of 64 keys or tokens
+            uint32_t inside = 0, q0 = 0, n = 0;
+            int work = -1;  // in tiles of 64 keys or tokens
             if (find_tile(p, group, 128, slot, &s, &inside)) {
                 sequence_rows(p, s, &q0, &n);
-                if (inside * 128 < n * group) work = which == 0 ? (inside * 128 + 127) / group / 64 : (n - 1 - inside * 128) / 64;
+                if (inside < (n * group + 127) / 128) work = which == 0 ? (inside * 128 + 127) / group / 64 : (n - 1 - inside * 128) / 64;
             }
-            const int64_t bin = work < 0 ? ORDER_BINS - 1 : (work >> shift) > ORDER_BINS - 2 ? 0 : ORDER_BINS - 2 - (work >> shift);
+            const int bin = work < 0 ? ORDER_BINS - 1 : (work >> shift) > ORDER_BINS - 2 ? 0 : ORDER_BINS - 2 - (work >> shift);
             const int at = atomicAdd(&bins[bin], 1);
             if (pass == 1) order[at] = int4{work < 0 ? -1 : s, (int)inside, (int)q0, (int)n};
         }
@@ -203,11 +205,13 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     const SplitSource t = a.t[blockIdx.z];
     const int kv = blockIdx.y;
     int s;
-    int64_t inside, q0, n;
-    if (!find_tile(p, t.group, 64, blockIdx.x, &s, &inside)) return;
-    sequence_rows(p, s, &q0, &n);
-    const int64_t rows = n * t.group, row0 = inside * 64;
-    if (row0 >= rows) return;
+    uint32_t inside, first, n;
+    const uint32_t group = t.group;
+    if (!find_tile(p, group, 64, blockIdx.x, &s, &inside)) return;
+    sequence_rows(p, s, &first, &n);
+    const uint32_t rows = n * group, row0 = inside * 64;
+    if (inside >= (rows + 63) / 64) return;
+    const int64_t q0 = first;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     __syncthreads();
@@ -216,10 +220,10 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) {
         const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
-        const int64_t r = row0 + j;
+        const uint32_t r = row0 + j, token = r / group;
         v[u] = f4{0.f, 0.f, 0.f, 0.f};
         if (r < rows && d < p.head_dim) {
-            const float* __restrict__ src = t.src + (q0 + r / t.group) * t.ld + (kv * t.group + r % t.group) * (int64_t)p.head_dim + d;
+            const float* __restrict__ src = t.src + (q0 + token) * t.ld + (kv * group + (r - token * group)) * (int64_t)p.head_dim + d;
             if (t.vec) {
                 v[u] = *reinterpret_cast<const f4*>(src);
             } else {
@@ -249,7 +253,8 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
 #pragma unroll
         for (int u = 0; u < COUNT; ++u) {
             const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
-            const int64_t r = row0 + j, token = q0 + r / t.group, head = kv * t.group + r % t.group;
+            const uint32_t r = row0 + j, down = r / group;
+            const int64_t token = q0 + down, head = kv * group + (r - down * group);
             float dot = 0.f;
             if (r < rows && d < p.head_dim) {
                 const float* __restrict__ o = p.O + token * p.ldo + head * p.head_dim + d;
@@ -270,7 +275,8 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
         }
         __syncthreads();
         if (threadIdx.x < 64) {
-            const int64_t r = row0 + threadIdx.x, token = q0 + r / t.group, head = kv * t.group + r % t.group;
+            const uint32_t r = row0 + threadIdx.x, down = r / group;
+            const int64_t token = q0 + down, head = kv * group + (r - down * group);
             float dot = row_dots[threadIdx.x], lse = -INFINITY;
             if (r < rows) {
                 if (!is_finite(dot) || bad[threadIdx.x] != 0) dot = NAN;
