@@ -1810,7 +1810,7 @@ int32_t prad_index_alloc(int64_t n, prad_index_t* out) {
     REQUIRE_INIT();
     if (out == nullptr) return fail(PRAD_ERR_ARG, "out is NULL");
     *out = nullptr;
-    if (n <= 0) return fail(PRAD_ERR_ARG, "an index vector needs at least one element");
+    if (n <= 0 || n > INT64_MAX / 4) return fail(PRAD_ERR_ARG, "an index vector needs at least one element and no more than there are addresses");
     prad_index* v = new (std::nothrow) prad_index{INDEX_MAGIC, n, nullptr, true, 0};
     if (v == nullptr) return fail(PRAD_ERR_ALLOC, "out of host memory");
     std::lock_guard<std::mutex> lock(g_ctx.mu);
@@ -1838,7 +1838,7 @@ int32_t prad_index_wrap(int64_t n, void* device_ptr, prad_index_t* out) {
     REQUIRE_INIT();
     if (out == nullptr || device_ptr == nullptr) return fail(PRAD_ERR_ARG, "NULL argument");
     *out = nullptr;
-    if (n <= 0) return fail(PRAD_ERR_ARG, "an index vector needs at least one element");
+    if (n <= 0 || n > INT64_MAX / 4) return fail(PRAD_ERR_ARG, "an index vector needs at least one element and no more than there are addresses");
     if (reinterpret_cast<uintptr_t>(device_ptr) % 4 != 0) return fail(PRAD_ERR_ARG, "an index vector starts on a multiple of 4 bytes");
     prad_index* v = new (std::nothrow) prad_index{INDEX_MAGIC, n, static_cast<int32_t*>(device_ptr), false, 0};
     if (v == nullptr) return fail(PRAD_ERR_ALLOC, "out of host memory");

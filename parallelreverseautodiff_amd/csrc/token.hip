@@ -136,12 +136,10 @@ __global__ void __launch_bounds__(SORT_THREADS) embedding_sort_kernel(const int3
     for (int e = threadIdx.x; e < SORT_WAVES * span; e += SORT_THREADS) cursor[e] = 0;
     __syncthreads();
     // parts of whole wavefronts of positions
-    const int part = ((tokens + SORT_WAVES - 1) / SORT_WAVES + 63) & ~63;
-    const int64_t from = (int64_t)wave * part, to = from + part < tokens ? from + part : tokens;
+    const int64_t part = (((int64_t)tokens + SORT_WAVES - 1) / SORT_WAVES + 63) & ~(int64_t)63;
+    const int64_t from = wave * part, to = from + part < tokens ? from + part : tokens;
     int32_t* __restrict__ mine = cursor + wave * span;
-    // (ids have 31 bits: rows from 2^31 on have none; a negative id is none of them)
-    const uint32_t first32 = (uint32_t)(first < ((int64_t)1 << 31) ? first : (int64_t)1 << 31);
-    const uint32_t reach = first32 + (uint32_t)rows <= 0x80000000u ? (uint32_t)rows : 0x80000000u - first32;
+    const uint32_t first32 = (uint32_t)first, reach = (uint32_t)rows;  // (rows end below 2^31, where negative ids begin)
     int below = 0;
     for (int64_t i0 = from; i0 < to; i0 += 256) {
         int32_t id[4];
@@ -391,11 +389,12 @@ hipError_t embedding_bwd_n(const T* dout, const int32_t* ids, T* dtable, int64_t
     const int64_t chunks = sum_chunks(tokens);
     double* head = reinterpret_cast<double*>(at);
     double* tail = head + chunks * width;
+    const unsigned slices = (unsigned)((packs + 63) / 64);
+    if (slices > 65535 || !grid_fits(chunks, 256)) return hipErrorInvalidValue;
     const int span = (int)std::min<int64_t>(SORT_MOST_SPAN, (vocab + 255) / 256);
     hipLaunchKernelGGL((embedding_sort_kernel<T, N>), dim3((unsigned)((vocab + span - 1) / span)), dim3(SORT_THREADS), (size_t)SORT_WAVES * span * 4, s, ids,
                        (int)tokens, vocab, span, order, order_ids, valid, dtable, packs, accumulate);
     if (hipError_t e = hipGetLastError()) return e;
-    const unsigned slices = (unsigned)((packs + 63) / 64);
     hipLaunchKernelGGL((embedding_sum_kernel<T, N>), dim3((unsigned)((chunks + 3) / 4), slices), dim3(256), 0, s, dout, order, order_ids, valid, head, tail,
                        dtable, packs, scale, accumulate);
     if (hipError_t e = hipGetLastError()) return e;

@@ -63,7 +63,8 @@ def test_index_vector_round_trip_and_addition(gpu):
 def test_index_vector_refusals(gpu):
     lib = _lib.load()
     h = ctypes.c_void_p()
-    assert lib.prad_index_alloc(0, ctypes.byref(h)) == _lib.PRAD_ERR_ARG and not h.value
+    for n in (0, -1, 2 ** 62):
+        assert lib.prad_index_alloc(n, ctypes.byref(h)) == _lib.PRAD_ERR_ARG and not h.value
     assert lib.prad_index_wrap(1, None, ctypes.byref(h)) == _lib.PRAD_ERR_ARG
     v = IndexVector.alloc(4)
     assert lib.prad_index_wrap(1, ctypes.c_void_p(lib.prad_index_device_ptr(v.handle) + 2), ctypes.byref(h)) == _lib.PRAD_ERR_ARG
