@@ -104,7 +104,7 @@ __device__ __forceinline__ void poison_row(Pack<T, 16 / sizeof(T)> (&frag)[CHUNK
 // the second wants them and a row's statistics sit in a lane; rows go from memory to the registers of the matrix instructions
 // without LDS, along for a product over the head dimension and across for one over the rows.  The registers of an operand are
 // filled again for the next tile as soon as its product has read them, so that loads are always in flight.
-constexpr int WAVES = 4;
+constexpr int WAVES = 4, MANY_WAVES = 8;
 // Parts of the keys: the least keys in one, sequences that are not cut (300 keys in parts of 64 and joined: 15.2 us, whole: 13.2),
 // units that run at once, two workgroups per compute unit.  Parts are as large as lets all units of a call run at once: the cache
 // of 24 sequences below in 71 us, in parts of 256 keys in 86.
@@ -333,13 +333,13 @@ __device__ __forceinline__ uint32_t inverse_of(uint32_t group) { return (65535 +
 // A cache is read once and bounds the call from some MB on: 24 sequences of 0 to 8192 keys, 16 heads on 4 of 128 floats, in
 // 64 us, and 5 for joining the parts (332 MB, 4.5 TB/s of the 5.0 that a copy reaches).  Small calls are bound by their latency,
 // about 1 us to find the sequence, 1.5 for the first rows, 1 per tile and 0.6 for the sums: 300 keys, 8 heads on 2 of 64
-// floats, in 9.4 us.  Doubles, forward over sequences of 512, 256, 200 and 37, 6 heads on 3 of 32: 20 us.
-template <typename T, int HDP, bool ALIGNED, bool CUT>
-__global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1) attention_kernel(const CausalArgs<T> p, const Parts<T> cut) {
+// floats, in 8.9 us.  Doubles, forward over sequences of 512, 256, 200 and 37, 6 heads on 3 of 32: 20 us.
+template <typename T, int HDP, bool ALIGNED, bool CUT, int W>
+__global__ void __launch_bounds__(64 * W, W == 4 && sizeof(T) == 4 && ALIGNED ? 2 : 1) attention_kernel(const CausalArgs<T> p, const Parts<T> cut) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
-    __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
-    __shared__ T stat[WAVES][2][16];
+    __shared__ __attribute__((aligned(16))) T sums[W][16 * PITCH];
+    __shared__ T stat[W][2][16];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     // heads of a unit are neighbours, so that workgroups without a unit come last
     const uint32_t stride = gridDim.x / p.kv_heads;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
         }
         zero_past<T, HDP>(g, p.head_dim, q);
         poison_row<T, CHUNKS>(q);
-        for (; k0 < to; k0 += 16 * WAVES) {
+        for (; k0 < to; k0 += 16 * W) {
             Acc sc = product<T>(k, q);
             // A key with a non-finite value is NaN for the rows that see it and zeros for the others.  In K it makes the scores
             // of its key non-finite whatever the rows hold, so that K is looked at only after such a score.
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
                 const uint64_t b = __ballot(!fine);
                 poisoned = (uint32_t)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xFFFFu);
             }
-            load_k(k0 + 16 * WAVES);
+            load_k(k0 + 16 * W);
             poisoned |= zero_bad<T>(v);
 #pragma unroll
             for (int x = 0; x < 4; ++x) sc[x] *= factor;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
                 l += sc[x];
             }
             add_weighted<T>(v, sc, o);
-            load_v(k0 + 16 * WAVES);
+            load_v(k0 + 16 * W);
         }
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
         put_sums<T, N, NY, PITCH>(o, li, g, sums[wave]);
         __syncthreads();
         const int here = (int)(rows - row0 < 16 ? rows - row0 : 16);
-        for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * WAVES) {
+        for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * W) {
             const uint32_t row = at / (HDP / VEC), ahead_of = (row0 % p.group + row) / p.group;
             const int d = at % (HDP / VEC) * VEC;
             if (d >= p.head_dim) continue;
@@ -465,12 +465,12 @@ __global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && ALIGNED ? 2 : 1)
             const int to_head = kv * p.group + (int)(row0 + row - (first_token + ahead_of) * p.group);
             T top = stat[0][0][row], total = 0, sum[VEC];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) top = fmax(top, stat[w][0][row]);
+            for (int w = 1; w < W; ++w) top = fmax(top, stat[w][0][row]);
             const T ref = top == -(T)INFINITY ? (T)0 : top;
 #pragma unroll
             for (int t = 0; t < VEC; ++t) sum[t] = 0;
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
+            for (int w = 0; w < W; ++w) {
                 const T f = Num<T>::exp_unit(stat[w][0][row] - ref);
                 total = fma(stat[w][1][row], f, total);
                 const Pack<T, VEC> e = *reinterpret_cast<const Pack<T, VEC>*>(&sums[w][row * PITCH + d]);
@@ -765,8 +765,19 @@ constexpr int64_t MOST_GROUPS = 1 << 20;
 template <typename T, bool CUT>
 static hipError_t launch_attention(const CausalArgs<T>& a, const Parts<T>& cut, int64_t most, hipStream_t s) {
     const int64_t groups = workgroups(cut.units, most, a.kv_heads);
-    if (a.vec_q && a.vec_kv) BY_HEAD_DIM(attention_kernel, groups, (a, cut), true, CUT);
-    else BY_HEAD_DIM(attention_kernel, groups, (a, cut), false, CUT);
+    // No more units than compute units, of many keys: eight wavefronts each.  One token against 300 keys, 8 heads on 2 of 64, 9.7 us
+    // for 10.2; 1024 tokens, 2 heads of 64, 19.1 for 21.3; level for heads of 128 and up to 256 keys.  In double the registers
+    // of two wavefronts per SIMD do not hold a tile.
+    if constexpr (!CUT && sizeof(T) == 4) {
+        if (a.vec_q && a.vec_kv && groups <= RUNNING / 2 && a.k_rows > (int64_t)256 * a.sequences && a.head_dim <= 64) {
+            const dim3 grid((unsigned)groups), block(64 * MANY_WAVES);
+            if (a.head_dim <= 32) hipLaunchKernelGGL((attention_kernel<T, 32, true, CUT, MANY_WAVES>), grid, block, 0, s, a, cut);
+            else hipLaunchKernelGGL((attention_kernel<T, 64, true, CUT, MANY_WAVES>), grid, block, 0, s, a, cut);
+            return hipGetLastError();
+        }
+    }
+    if (a.vec_q && a.vec_kv) BY_HEAD_DIM(attention_kernel, groups, (a, cut), true, CUT, WAVES);
+    else BY_HEAD_DIM(attention_kernel, groups, (a, cut), false, CUT, WAVES);
     return hipSuccess;
 }
 
