@@ -456,6 +456,29 @@ def test_thousands_of_sequences(gpu):
     against_definition(np.float32, [1, 0, 2] * 1400, [(i % 500, i % 500 + i % 13) for i in range(4200)], 512, 2, 1, 4)
 
 
+def test_more_units_than_a_launch_has_workgroups(gpu):
+    """With 40000 heads of one column a launch has 26 workgroups to a head and the sequences 30 tiles: some take two.  All heads
+    hold the same, so all results do."""
+    lib, heads, lengths = _lib.load(), 40000, [433, 16]
+    rows, starts = sum(lengths), [0, 433, 449]
+    x = [seeded.normal(77, i, (rows, 1), 1.0, np.float64) for i in range(4)]
+    q, k, v, g = (dev(np.repeat(y, heads, axis=1)) for y in x)
+    o, l, dq, dk, dv = (unfilled(np.float64, *s) for s in ((rows, heads), (heads, rows), (rows, heads), (rows, heads), (rows, heads)))
+    off = IndexVector.from_values(starts)
+    check(lib.prad_causal_attention_fwd(q.handle, 0, k.handle, 0, v.handle, 0, o.handle, l.handle, off.handle, heads, heads, 1, 1.0))
+    check(lib.prad_causal_attention_bwd(q.handle, 0, k.handle, 0, v.handle, 0, o.handle, l.handle, g.handle, dq.handle, 0, dk.handle, 0, dv.handle, 0,
+                                        off.handle, heads, heads, 1, 1.0))
+    got = [b.download() for b in (o, dq, dk, dv)]
+    assert all((y == y[:, :1]).all() for y in got)
+    u = float(np.finfo(np.float64).eps) / 2
+    for first, last in zip(starts[:-1], starts[1:]):
+        args = [y[first:last] for y in x[:3]]
+        ro, _, *rg = attention(*args, 1.0, x[3][first:last])
+        eo, _, *eg = attention_bounds(*args, 1.0, 2 * u, x[3][first:last])
+        for y, r, e in zip(got, [ro] + rg, [eo] + eg):
+            close(y[first:last, :1], r, e, "a head")
+
+
 def test_calls_of_several_threads_at_once(gpu):
     """Each with operands of its own, sharing the library's one workspace: what each gets is what it gets alone."""
     import threading
@@ -478,6 +501,26 @@ def test_calls_of_several_threads_at_once(gpu):
     for x in threads:
         x.join()
     assert wrong == []
+
+
+def test_rows_behind_two_to_the_31_elements(gpu):
+    """A cache of 8.6 GB, keys and values in its last rows; its rows as a table."""
+    lib, cols, rows, n = _lib.load(), 1024, 2 ** 21 + 700, 650
+    whole = DeviceBuffer.alloc(np.float32, rows, cols)
+    end = seeded.normal(78, 1, (n, cols), 1.0, np.float32)
+    whole.view_rows(rows - n, n).upload(end)
+    x = seeded.normal(78, 2, (2, 128), 1.0, np.float32)
+    q, o, off = dev(x), unfilled(np.float32, 2, 128), IndexVector.from_values([0, 1, 2])
+    begin, last = IndexVector.from_values([rows - n, rows - 40]), IndexVector.from_values([rows - 3, rows])
+    check(lib.prad_cached_attention(q.handle, 0, whole.handle, 64, whole.handle, 640, o.handle, off.handle, begin.handle, last.handle, 2, 1, 64, 0.125))
+    got, u = o.download(), float(np.finfo(np.float32).eps) / 2
+    for i, keys in enumerate((slice(0, n - 3), slice(n - 40, n))):
+        for h in (slice(0, 64), slice(64, 128)):
+            args = x[i:i + 1, h], end[keys, 64:128], end[keys, 640:704], 0.125
+            close(got[i:i + 1, h], attention(*args)[0], attention_bounds(*args, 2 * u, np.zeros((1, 64)))[0], "o")
+    ids, out = IndexVector.from_values([rows - 1, rows - n, rows]), unfilled(np.float32, 3, cols)
+    check(lib.prad_embedding_fwd(whole.handle, ids.handle, 1.0, out.handle))
+    assert np.array_equal(out.download(), np.stack([end[-1], end[0], np.zeros(cols, np.float32)]))
 
 
 def test_a_workspace_that_grows_behind_a_recording(gpu):
