@@ -555,17 +555,17 @@ __global__ void __launch_bounds__(64 * WAVES) cached_join_kernel(const CausalArg
 // one of dO with a non-finite value a NaN in D: their weights are NaN, and the values themselves count as zeros.)
 
 // The sums of the wavefronts of 16 rows, times `by`, to the rows' places.
-template <typename T, int HDP, typename RowOf>
-__device__ __forceinline__ void write_sums(const T (&sums)[WAVES][16 * (HDP + 16 / sizeof(T))], int here, int head_dim, T by, RowOf row_of) {
+template <typename T, int HDP, int W, typename RowOf>
+__device__ __forceinline__ void write_sums(const T (&sums)[W][16 * (HDP + 16 / sizeof(T))], int here, int head_dim, T by, RowOf row_of) {
     constexpr int VEC = 16 / sizeof(T), PITCH = HDP + VEC;
-    for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * WAVES) {
+    for (int at = threadIdx.x; at < here * (HDP / VEC); at += 64 * W) {
         const int row = at / (HDP / VEC), d = at % (HDP / VEC) * VEC;
         if (d >= head_dim) continue;
         T sum[VEC];
 #pragma unroll
         for (int t = 0; t < VEC; ++t) sum[t] = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
+        for (int w = 0; w < W; ++w) {
             const Pack<T, VEC> e = *reinterpret_cast<const Pack<T, VEC>*>(&sums[w][row * PITCH + d]);
 #pragma unroll
             for (int t = 0; t < VEC; ++t) sum[t] += e.v[t];
@@ -648,7 +648,7 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalAr
         }
         put_sums<T, N, NY, PITCH>(dq, li, g, sums[wave]);
         __syncthreads();
-        write_sums<T, HDP>(sums, (int)(rows - row0 < 16 ? rows - row0 : 16), p.head_dim, p.scale, [&](int row) {
+        write_sums<T, HDP, WAVES>(sums, (int)(rows - row0 < 16 ? rows - row0 : 16), p.head_dim, p.scale, [&](int row) {
             const uint32_t to = first_token + (row0 % p.group + row) / p.group;
             return p.dQ + (sp.q0 + to) * p.lddq + (kv * p.group + (int)(row0 + row - to * p.group)) * (int64_t)p.head_dim;
         });
@@ -656,14 +656,14 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_q_kernel(const CausalAr
     }
 }
 
-// Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.  As above: 44 us, 16
+// Gradients of K and V: 16 keys against the packed rows that see them, all heads of the group among them.  As above: 35 us, 8
 // tiles of rows to a wavefront at most.  Reading a tile ahead in these two was measured: up to 16 % faster on sequences from
 // 512 on, as much slower on many short ones, whose registers then let fewer wavefronts run; it was left out.
-template <typename T, int HDP, bool ALIGNED>
-__global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalArgs<T> p, uint32_t units) {
+template <typename T, int HDP, bool ALIGNED, int W>
+__global__ void __launch_bounds__(64 * W) causal_bwd_kv_kernel(const CausalArgs<T> p, uint32_t units) {
     constexpr int VEC = 16 / sizeof(T), CHUNKS = HDP / (4 * VEC), NY = HDP / 16, N = columns_at_once<T, HDP>(), PITCH = HDP + VEC;
     typedef typename Num<T>::Acc Acc;
-    __shared__ __attribute__((aligned(16))) T sums[WAVES][16 * PITCH];
+    __shared__ __attribute__((aligned(16))) T sums[W][16 * PITCH];
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, li = lane & 15, g = lane >> 4;
     const uint32_t stride = gridDim.x / p.kv_heads, group = p.group, inverse = inverse_of(group);
     const int kv = (int)(blockIdx.x % p.kv_heads);
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalA
         const T* __restrict__ G = p.dO + sp.q0 * p.ldo + kv * (int64_t)group * p.head_dim;
         const T* __restrict__ lses = p.lse + kv * (int64_t)group * p.q_rows + sp.q0;
         const T* __restrict__ dots = p.D + kv * (int64_t)group * p.q_rows + sp.q0;
-        for (uint32_t r0 = key0 * group / 16 * 16 + 16 * wave; r0 < rows; r0 += 16 * WAVES) {
+        for (uint32_t r0 = key0 * group / 16 * 16 + 16 * wave; r0 < rows; r0 += 16 * W) {
             const uint32_t most = rows - 1 - r0, token0 = r0 / group, rest0 = r0 - token0 * group;
             Pack<T, VEC> q[CHUNKS], go[CHUNKS];
             Pack<T, N> q_across[4][NY / N], g_across[4][NY / N];
@@ -725,11 +725,11 @@ __global__ void __launch_bounds__(64 * WAVES) causal_bwd_kv_kernel(const CausalA
         const int here = (int)(keys - key0 < 16 ? keys - key0 : 16);
         put_sums<T, N, NY, PITCH>(dv, li, g, sums[wave]);
         __syncthreads();
-        write_sums<T, HDP>(sums, here, p.head_dim, (T)1, [&](int row) { return p.dV + (sp.k0 + key0 + row) * p.lddv + kv * (int64_t)p.head_dim; });
+        write_sums<T, HDP, W>(sums, here, p.head_dim, (T)1, [&](int row) { return p.dV + (sp.k0 + key0 + row) * p.lddv + kv * (int64_t)p.head_dim; });
         __syncthreads();
         put_sums<T, N, NY, PITCH>(dk, li, g, sums[wave]);
         __syncthreads();
-        write_sums<T, HDP>(sums, here, p.head_dim, p.scale, [&](int row) { return p.dK + (sp.k0 + key0 + row) * p.lddk + kv * (int64_t)p.head_dim; });
+        write_sums<T, HDP, W>(sums, here, p.head_dim, p.scale, [&](int row) { return p.dK + (sp.k0 + key0 + row) * p.lddk + kv * (int64_t)p.head_dim; });
         __syncthreads();
     }
 }
@@ -756,6 +756,14 @@ int most_parts(const CausalArgs<T>& a) {
         else hipLaunchKernelGGL((KERNEL<T, 128, __VA_ARGS__>), grid, block, 0, s, UNPACKED ARGS);                       \
         if (hipError_t e = hipGetLastError()) return e;                                                                 \
     } while (0)
+// With MANY_WAVES, for head dimensions of up to 256 bytes: more would not leave each wavefront the registers of a tile.
+#define BY_HEAD_DIM_MANY(KERNEL, GROUPS, ARGS, ...)                                                                              \
+    do {                                                                                                                         \
+        const dim3 grid((unsigned)(GROUPS)), block(64 * MANY_WAVES);                                                             \
+        if (a.head_dim <= 32) hipLaunchKernelGGL((KERNEL<T, 32, __VA_ARGS__, MANY_WAVES>), grid, block, 0, s, UNPACKED ARGS);    \
+        else hipLaunchKernelGGL((KERNEL<T, 256 / sizeof(T), __VA_ARGS__, MANY_WAVES>), grid, block, 0, s, UNPACKED ARGS);        \
+        if (hipError_t e = hipGetLastError()) return e;                                                                          \
+    } while (0)
 #define UNPACKED(...) __VA_ARGS__
 
 // Workgroups for `tiles` units of every key/value head: one each, of very many some take several.
@@ -766,14 +774,12 @@ template <typename T, bool CUT>
 static hipError_t launch_attention(const CausalArgs<T>& a, const Parts<T>& cut, int64_t most, hipStream_t s) {
     const int64_t groups = workgroups(cut.units, most, a.kv_heads);
     // No more units than compute units, of many keys: eight wavefronts each.  One token against 300 keys, 8 heads on 2 of 64, 9.7 us
-    // for 10.2; 1024 tokens, 2 heads of 64, 19.1 for 21.3; level for heads of 128 and up to 256 keys.  In double the registers
-    // of two wavefronts per SIMD do not hold a tile.
+    // for 10.2; 1024 tokens, 2 heads of 64, 19.1 for 21.3; level up to 256 keys, and for heads of 128; slower in double (four
+    // sequences of doubles, forward, 23 for 21).
     if constexpr (!CUT && sizeof(T) == 4) {
-        if (a.vec_q && a.vec_kv && groups <= RUNNING / 2 && a.k_rows > (int64_t)256 * a.sequences && a.head_dim <= 64) {
-            const dim3 grid((unsigned)groups), block(64 * MANY_WAVES);
-            if (a.head_dim <= 32) hipLaunchKernelGGL((attention_kernel<T, 32, true, CUT, MANY_WAVES>), grid, block, 0, s, a, cut);
-            else hipLaunchKernelGGL((attention_kernel<T, 64, true, CUT, MANY_WAVES>), grid, block, 0, s, a, cut);
-            return hipGetLastError();
+        if (a.vec_q && a.vec_kv && a.head_dim <= 64 && groups <= RUNNING / 2 && a.k_rows > (int64_t)256 * a.sequences) {
+            BY_HEAD_DIM_MANY(attention_kernel, groups, (a, cut), true, CUT);
+            return hipSuccess;
         }
     }
     if (a.vec_q && a.vec_kv) BY_HEAD_DIM(attention_kernel, groups, (a, cut), true, CUT, WAVES);
@@ -796,13 +802,17 @@ hipError_t launch_causal_bwd(CausalArgs<T> a, void* workspace, hipStream_t s) {
     a.D = static_cast<T*>(workspace);
     const int64_t tiles = tile_slots(a.q_rows, a.group, a.sequences), key_tiles = tile_slots(a.q_rows, 1, a.sequences);
     const int64_t groups = workgroups(tiles, MOST_GROUPS, a.kv_heads), key_groups = workgroups(key_tiles, MOST_GROUPS, a.kv_heads);
-    if (a.vec_q && a.vec_kv && a.vec_o) {
-        BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), true);
-        BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), true);
-    } else {
-        BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), false);
-        BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), false);
-    }
+    const bool aligned = a.vec_q && a.vec_kv && a.vec_o;
+    if (aligned) BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), true);
+    else BY_HEAD_DIM(causal_bwd_q_kernel, groups, (a, (uint32_t)tiles), false);
+    // Few units of long walks: eight wavefronts each.  With the kernel above, the four sequences of doubles 56 us for 65; 1024
+    // doubles, 8 heads of 32, 80 for 88; 700 floats, 8 heads on 2 of 32, 64 for 77; 800, 4 heads of 64, 50 for 53.  Beyond these
+    // bounds: two sequences of 1024 doubles 150 for 137, ten of 100 39 for 28, eight of 64, 16 heads on 4 of 64 floats, 25 for
+    // 23.  (The kernel above has nothing from it.)
+    if (aligned && a.head_dim * sizeof(T) <= 256 && a.q_rows * a.kv_heads <= 16 * RUNNING && a.q_rows * a.group > (int64_t)256 * a.sequences)
+        BY_HEAD_DIM_MANY(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), true);
+    else if (aligned) BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), true, WAVES);
+    else BY_HEAD_DIM(causal_bwd_kv_kernel, key_groups, (a, (uint32_t)key_tiles), false, WAVES);
     return hipSuccess;
 }
 
