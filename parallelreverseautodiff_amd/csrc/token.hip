@@ -68,8 +68,10 @@ __global__ void __launch_bounds__(256) embedding_fwd_kernel(const T* __restrict_
 // Sums are held in double.
 
 // Few tokens: one launch.  A wavefront owns a table row, finds its positions among the ids by ballots and adds them up.  Bound
-// by its latency: 49 tokens, 1000 rows of 96 doubles in 2.9 us.
-constexpr int EMB_DIRECT_TOKENS = 256;
+// by its latency: 49 tokens, 1000 rows of 96 doubles in 2.9 us.  Against the three launches below, 512 tokens: 3.7 us for 17.2
+// (1000 rows of 96 floats), 16 for 25 (32768 of 512); where all tokens are one, which a single wavefront then adds up, 35 for 14
+// and 83 for 22.  With 1024 tokens that would be 71 and 161.
+constexpr int EMB_DIRECT_TOKENS = 512;
 
 template <typename T, int N>
 __global__ void __launch_bounds__(256) embedding_bwd_direct_kernel(const T* __restrict__ dout, const int32_t* __restrict__ ids, T* __restrict__ dtable,
@@ -93,11 +95,22 @@ __global__ void __launch_bounds__(256) embedding_bwd_direct_kernel(const T* __re
         for (int e = 0; e < N; ++e) sum[e] = 0.0;
 #pragma unroll
         for (int b = 0; b < EMB_DIRECT_TOKENS / 64; ++b) {
-            for (uint64_t left = found[b]; left != 0; left &= left - 1) {
-                const int64_t i = 64 * b + __builtin_ctzll(left);
-                const P v = reinterpret_cast<const P*>(dout)[i * packs + c];
+            uint64_t left = found[b];
+            while (left != 0) {  // eight at a time, their loads in flight together
+                const int n = __builtin_popcountll(left);
+                P v[8];
 #pragma unroll
-                for (int e = 0; e < N; ++e) sum[e] += (double)v.v[e];
+                for (int u = 0; u < 8; ++u) {
+                    if (u >= n) break;
+                    v[u] = reinterpret_cast<const P*>(dout)[(int64_t)(64 * b + __builtin_ctzll(left)) * packs + c];
+                    left &= left - 1;
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    if (u >= n) break;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) sum[e] += (double)v[u].v[e];
+                }
             }
         }
         P* dst = reinterpret_cast<P*>(dtable) + row * packs + c;

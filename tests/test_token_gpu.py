@@ -105,11 +105,11 @@ def token_ids(seed, tokens, vocab, kind):
     return ids.astype(np.int32)
 
 
-# (tokens, vocabulary, width, ids): one token, one row; odd widths; counts on both sides of the one-launch form (256), of a
+# (tokens, vocabulary, width, ids): one token, one row; odd widths; counts on both sides of the one-launch form (512), of a
 # chunk of the sums (32), of a wavefront; more rows than one workgroup orders; one token alone; no token at all
 EMBEDDINGS = [(1, 1, 1, "any"), (1, 10, 96, "any"), (49, 1000, 96, "text"), (256, 31, 4, "any"), (257, 31, 4, "any"), (257, 5, 130, "text"), (300, 2000, 7, "any"),
               (1024, 1, 260, "one"), (3000, 50, 33, "one"), (700, 1500, 64, "none"), (5000, 700, 66, "text"), (2049, 520, 256, "any"), (4096, 40000, 8, "text"),
-              (6000, 270000, 4, "any")]
+              (6000, 270000, 4, "any"), (512, 70, 33, "text"), (512, 900, 64, "one"), (513, 70, 33, "text"), (400, 40, 8, "any")]
 
 
 @DTYPES
