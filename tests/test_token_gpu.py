@@ -175,8 +175,9 @@ def test_embedding_refusals(gpu):
     assert call(handle_of(DeviceBuffer.alloc(np.float32, 10, 8, depth=2)), ids.handle, 1.0, out.handle) == (_lib.PRAD_ERR_SHAPE,) * 2
 
 
-def test_a_recorded_embedding_reads_the_ids_of_each_launch(gpu):
-    lib, dtype, vocab, width, tokens = _lib.load(), np.float32, 50, 16, 400
+@pytest.mark.parametrize("tokens", [400, 900])
+def test_a_recorded_embedding_reads_the_ids_of_each_launch(gpu, tokens):
+    lib, dtype, vocab, width = _lib.load(), np.float32, 50, 16
     table, dout = seeded.normal(13, 1, (vocab, width), 1.0, dtype), seeded.normal(13, 2, (tokens, width), 1.0, dtype)
     bt, bd, ids = dev(table), dev(dout), IndexVector.alloc(tokens)
     out, d_table = unfilled(dtype, tokens, width), unfilled(dtype, vocab, width)
