@@ -424,8 +424,8 @@ int32_t prad_dropout_bwd(prad_buf_t dy, prad_buf_t dx, double p, int64_t seed, i
  *              buffers; results are then undefined, memory is not harmed.)
  *   O:         tokens x heads*head_dim.
  *   lse:       heads x tokens, receives log sum exp of every row's visible scores, which backward needs; NULL: not kept.
- * heads is a multiple of kv_heads, head_dim 1 .. 128, rows * heads / kv_heads at most 2^31 - 513; float and double.  Sums are
- * held in the element type.  Large batches of floats are computed on the half-precision matrix instructions from two halves of
+ * heads is a multiple of kv_heads, head_dim 1 .. 128, (rows + 128) * heads / kv_heads at most 2^31 - 513; float and double.
+ * Sums are held in the element type.  Large batches of floats are computed on the half-precision matrix instructions from two halves of
  * each value (22 bits); the results keep the error of single precision.
  * A query that sees a value that is not finite, in Q, K or V, gets rows of NaN; one that does not see it is not affected. */
 int32_t prad_causal_attention_fwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,

@@ -2086,9 +2086,9 @@ static int32_t causal_check(const HeadColumns& Q, const HeadColumns& K, const He
     if (int32_t st = columns_check(V, K.buf->rows)) return st;
     if (O->depth != 1 || O->rows != Q.buf->rows || O->cols != heads * head_dim)
         return fail(PRAD_ERR_SHAPE, "O must be %lld x %lld", (long long)Q.buf->rows, (long long)(heads * head_dim));
-    // the kernels count the rows of all heads that share a key head in 32 bits, some tiles past the last one
-    if (Q.buf->rows > (INT32_MAX - 512) / (Q.width / K.width) || K.buf->rows > INT32_MAX)
-        return fail(PRAD_ERR_ARG, "at most 2^31 - 513 rows times heads per key/value head, 2^31 - 1 rows of keys");
+    // the kernels count the rows of all heads that share a key head in 32 bits, a tile of tokens and some of rows past the last one
+    if (Q.buf->rows > (INT32_MAX - 512) / (Q.width / K.width) - 128 || K.buf->rows > INT32_MAX)
+        return fail(PRAD_ERR_ARG, "(rows + 128) times heads per key/value head is at most 2^31 - 513, rows of keys 2^31 - 1");
     if (offsets->n < 2 || offsets->n > INT32_MAX) return fail(PRAD_ERR_SHAPE, "the offsets of n sequences are n + 1 elements");
     return PRAD_OK;
 }

@@ -368,7 +368,7 @@ def test_attention_refusals(gpu):
         assert fwd(**change) == status, change
     # more rows than the kernels count (borrowed views of the same few rows: refused before anything is read)
     tall = lambda b, rows: DeviceBuffer.wrap(np.float32, rows, b.cols, b.ptr, parent=b)
-    n = 2 ** 30 - 256
+    n = 2 ** 30 - 384
     assert fwd(q=tall(x, n), k=tall(x, n), v=tall(x, n), o=tall(o, n), lse=None) == _lib.PRAD_ERR_ARG
     wide = f(20, 32)
     assert fwd(q=wide.view_rows(0, 10), o=wide.view_rows(5, 10), k=x, v=x) == _lib.PRAD_ERR_ARG     # an output over an input
@@ -618,7 +618,7 @@ def test_cached_attention_refusals(gpu):
         q.handle, 0, k.handle, 0, v.handle, 0, o.handle, off.handle, b.handle, e.handle, 2, 1, d, 0.25)
     assert call() == _lib.PRAD_OK
     tall = lambda b, rows: DeviceBuffer.wrap(np.float32, rows, b.cols, b.ptr, parent=b)     # (refused before anything is read)
-    assert call(q=tall(q, 2 ** 30 - 256), o=tall(o, 2 ** 30 - 256)) == _lib.PRAD_ERR_ARG
+    assert call(q=tall(q, 2 ** 30 - 384), o=tall(o, 2 ** 30 - 384)) == _lib.PRAD_ERR_ARG
     assert call(k=tall(k, 2 ** 31), v=tall(v, 2 ** 31)) == _lib.PRAD_ERR_ARG
     for change, status in (({"v": f(21, 16)}, _lib.PRAD_ERR_SHAPE), ({"b": IndexVector.alloc(3)}, _lib.PRAD_ERR_SHAPE), ({"e": IndexVector.alloc(1)}, _lib.PRAD_ERR_SHAPE),
                            ({"e": q}, _lib.PRAD_ERR_BAD_HANDLE), ({"o": f(3, 16)}, _lib.PRAD_ERR_SHAPE), ({"o": q}, _lib.PRAD_ERR_ARG), ({"k": f(20, 8)}, _lib.PRAD_ERR_SHAPE),
