@@ -1276,7 +1276,8 @@ hipError_t launch_causal_split_bwd(const CausalArgs<float>& p, void* workspace, 
                   row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
     if (!grid_fits(row_tiles, 256) || !grid_fits(row_groups * p.kv_heads, 256) || !grid_fits(key_groups * p.kv_heads * b.main.chunks, 256))
         return hipErrorInvalidValue;
-    const dim3 split((unsigned)row_tiles, p.kv_heads, 5), row_grid((unsigned)(row_groups * p.kv_heads));
+    // (at least two wide: the workgroups 0 and 1 of the last plane make the schedules, however few tiles there are)
+    const dim3 split((unsigned)std::max<int64_t>(row_tiles, 2), p.kv_heads, 5), row_grid((unsigned)(row_groups * p.kv_heads));
     switch (padded(p.head_dim)) {
         case 32: enqueue_backward<32>(b, split, (unsigned)(key_groups * p.kv_heads), row_grid, s); break;
         case 64: enqueue_backward<64>(b, split, (unsigned)(key_groups * p.kv_heads), row_grid, s); break;

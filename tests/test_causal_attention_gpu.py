@@ -638,3 +638,23 @@ def test_key_ranges_that_describe_no_rows_do_no_harm(gpu):
         assert np.isfinite(got).all()
         if begin >= end:
             assert np.all(got == 0)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,d", [(63, 1100, 1100, 2), (50, 1700, 1700, 4), (40, 6000, 6000, 1)])
+def test_one_sequence_within_a_tile_of_very_many_heads(gpu, rows, heads, kv_heads, d):
+    """Fewer than 64 rows of one sequence, but so many heads that the batch is computed from halves: a single tile of rows, and
+    the gradients of K and V have their schedule all the same.  Heads hold one of eight values."""
+    lib, few = _lib.load(), 8
+    small = Batch(np.float32, [rows], few, few, d, "fused", seed=83, front=0, behind=0)
+    spread = lambda x: np.tile(x, (1, -(-heads // few)))[:, :heads * d]
+    q, k, v, g = (dev(spread(x)) for x in (small.q, small.k, small.v, small.g))
+    o, l, dq, dk, dv = (unfilled(np.float32, *s) for s in ((rows, heads * d), (heads, rows)) + ((rows, heads * d),) * 3)
+    tail = (small.offsets.handle, heads, kv_heads, d, small.scale)
+    check(lib.prad_causal_attention_fwd(q.handle, 0, k.handle, 0, v.handle, 0, o.handle, l.handle, *tail))
+    check(lib.prad_causal_attention_bwd(q.handle, 0, k.handle, 0, v.handle, 0, o.handle, l.handle, g.handle, dq.handle, 0, dk.handle, 0, dv.handle, 0, *tail))
+    (ro, rl, *rg), (eo, el, *eg) = small.reference()
+    for b, r, e, name in zip((o, dq, dk, dv), (ro, *rg), (eo, *eg), ("o", "dq", "dk", "dv")):
+        got = b.download()
+        assert np.array_equal(got, spread(got[:, :few * d])), name
+        close(got[:, :few * d], r, e, name)
+    close(l.download()[:few], rl, el, "lse")
