@@ -844,13 +844,14 @@ __device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, cons
     rows_products<HDP>(t.q[block], st.k_hi, st.k_lo, s, t.g[block], st.v_hi, st.v_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
     const int e_ratio = notes.e_q - st.top_q;
-    const float x_v = (float)st.x_v;
+    // (not as part of the exponent: an argument of a hundred has 17 bits behind its point)
+    const float scale_v = pow2(st.x_v);
     float w[16], ds[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const f4 lse = *reinterpret_cast<const f4*>(t.lse + 32 * block + 8 * q + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e]) + x_v);
+        for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e])) * scale_v;
     }
     if (row0 < wave_last) {  // some key is not seen by some row
 #pragma unroll

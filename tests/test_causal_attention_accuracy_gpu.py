@@ -1,0 +1,121 @@
+"""How exact causal attention is: errors in norm, and batches in whose sequences rows differ widely in size - what a row does not
+see, and what it sees with a weight of next to nothing, leaves its results alone.  The short batches run on units of 16 rows, the
+long ones of floats are computed from halves; both are held to the same bounds."""
+import numpy as np
+import pytest
+
+from parallelreverseautodiff_amd import _lib
+from parallelreverseautodiff_amd.exceptions import check
+from test_causal_attention_gpu import Batch, close, dev, unfilled
+from token_reference import attention
+
+pytestmark = pytest.mark.gpu
+
+
+def bounds(q, k, v, scale, u, g):
+    """As token_reference.attention_bounds, with the error of each score taken for itself: err_ij of the score of query i and key
+    j moves the weight p_ij by p_ij (err_ij + sum_l p_il err_il) to first order - the second term is the sum of the weights - and
+    lse_i by sum_l p_il err_il, so that a score of great size whose weight is nothing loosens no bound."""
+    q, k, v, g = (np.asarray(x, np.float64) for x in (q, k, v, g))
+    n, m, d = len(q), len(k), q.shape[1]
+    seen = np.arange(m)[None, :] <= np.arange(n)[:, None] + (m - n)
+    with np.errstate(over="ignore", invalid="ignore"):     # (products with what is not seen)
+        s, size = np.where(seen, q @ k.T * scale, -np.inf), np.where(seen, np.abs(q) @ np.abs(k).T, 0)
+    top = s.max(axis=1)
+    e = np.exp(s - top[:, None])
+    p = e / e.sum(axis=1)[:, None]
+    lse = top + np.log(e.sum(axis=1))
+    err = (d + 4) * u * size * abs(scale)
+    err += u * (np.abs(s, where=seen, out=np.zeros_like(s)) + np.abs(top)[:, None])
+    mean = (p * err).sum(axis=1)[:, None]
+    e_o = (p * (err + mean + (m + 8) * u)) @ np.abs(v) + (m + 4) * u * (p @ np.abs(v))
+    e_lse = mean[:, 0] + (m + 8) * u + 4 * u * np.abs(lse)
+    o = p @ v
+    again = err + e_lse[:, None] + (4 * np.abs(lse)[:, None] + 8) * u
+    with np.errstate(over="ignore", invalid="ignore"):
+        dp, dp_size = np.where(seen, g @ v.T, 0), np.where(seen, np.abs(g) @ np.abs(v).T, 0)
+    dot = (g * o).sum(axis=1)[:, None]
+    e_dot = ((d + 2) * u * (np.abs(g) * np.abs(o)).sum(axis=1) + (np.abs(g) * e_o).sum(axis=1))[:, None]
+    e_ds = p * (np.abs(dp - dot) * (again + 4 * u) + (d + 2) * u * dp_size + e_dot + 2 * u * (np.abs(dp) + np.abs(dot)))
+    ds = p * np.abs(dp - dot)
+    return (e_o, e_lse, abs(scale) * ((e_ds + (m + 4) * u * ds) @ np.abs(k)), abs(scale) * ((e_ds + (n + 4) * u * ds).T @ np.abs(q)),
+            (p * (again + (n + 4) * u)).T @ np.abs(g))
+
+
+class Spread(Batch):
+    """A batch whose few heads are repeated `by` times on the device: large enough for the halves, quick to define."""
+
+    def repeat(self, by):
+        self.few = self.heads, self.kv_heads, self.q, self.k, self.v, self.g
+        self.by = by
+        self.heads, self.kv_heads = by * self.heads, by * self.kv_heads
+        self.q, self.k, self.v, self.g = (np.tile(x, (1, by)) for x in (self.q, self.k, self.v, self.g))
+        self.cols = (0, self.q.shape[1], self.q.shape[1] + self.k.shape[1])
+        self.full = [self.q.shape[1] + 2 * self.k.shape[1]] * 3
+        self.tail = (self.heads, self.kv_heads) + self.tail[2:]
+        self.upload()
+        return self
+
+    def run(self):
+        """(o, lse, dq, dk, dv) of the few heads, after a look at whether all copies of them are the same."""
+        o, l = self.forward()
+        out = [o.download(), l.download(), *self.backward(o, l)]
+        self.heads, self.kv_heads, self.q, self.k, self.v, self.g = self.few
+        for i, x in enumerate(out):
+            few = x[:x.shape[0] // self.by] if i == 1 else x[:, :x.shape[1] // self.by]
+            assert np.array_equal(x, np.tile(few, (self.by, 1) if i == 1 else (1, self.by)), equal_nan=True)
+            out[i] = few
+        return out
+
+    def definition(self):
+        o, lse = np.zeros(self.q.shape), np.zeros((self.heads, self.rows))
+        dq, dk, dv = np.zeros(self.q.shape), np.zeros(self.k.shape), np.zeros(self.v.shape)
+        errors = [np.zeros_like(x) for x in (o, lse, dq, dk, dv)]
+        u = float(np.finfo(self.dtype).eps) / 2
+        for rows, h, qc, kc in self.each():
+            args = self.q[rows, qc], self.k[rows, kc], self.v[rows, kc], self.scale
+            o[rows, qc], lse[h, rows], dq[rows, qc], a, b = attention(*args, self.g[rows, qc])
+            dk[rows, kc] += a
+            dv[rows, kc] += b
+            # a shared head's gradient is a sum over its group: one more rounding per head, in the bound's own terms
+            e = bounds(*args, u * (1 + self.heads // self.kv_heads / (rows.stop - rows.start + 8)), self.g[rows, qc])
+            errors[0][rows, qc], errors[1][h, rows], errors[2][rows, qc] = e[0], e[1], e[2]
+            errors[3][rows, kc] += e[3]
+            errors[4][rows, kc] += e[4]
+        return (o, lse, dq, dk, dv), errors
+
+
+NAMES = "o", "lse", "dq", "dk", "dv"
+
+
+def compare(batch, names=NAMES, without=()):
+    """The named results within their bounds in all rows of the sequences but `without`."""
+    got = batch.run()
+    want, error = batch.definition()
+    rows = np.setdiff1d(np.arange(batch.starts[0], batch.starts[-1]), np.asarray(without, int))
+    for name, x, r, e in zip(NAMES, got, want, error):
+        if name in names:
+            at = np.s_[:, rows] if name == "lse" else rows
+            close(x[at], r[at], e[at], name)
+
+
+KINDS = pytest.mark.parametrize("dtype,by", [(np.float64, 1), (np.float32, 1), (np.float32, 160)], ids=["f64", "f32", "f32-halves"])
+SHAPES = pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (4, 2, 40), (3, 1, 128)], ids=str)
+LENGTHS = [190, 64, 100]
+
+
+@KINDS
+@pytest.mark.parametrize("lengths", [LENGTHS, [64] * 8, [400]], ids=str)
+def test_errors_in_norm(gpu, dtype, by, lengths):
+    """Normal data, the norm of a result's error over the result's: 16 unit roundoffs u.  A score is a chain of 64 products whose
+    partial sums grow to 1.1: additions off by u / sqrt(3) of them in the mean, 1.1 * 0.7 * sqrt(64 / 3) = 4 u together; lse, of
+    size 5, is rounded, taken in other units and rounded again, 2 * 5 / sqrt(3) = 6 u; their difference moves a weight by
+    sqrt(4 ** 2 + 6 ** 2) = 7 u, a difference dP - D is off by as much, and a gradient by both, 10 u, before its sum over the
+    rows evens out a part of that."""
+    batch = Spread(dtype, lengths, 2, 2, 64, "fused").repeat(by)
+    got, (want, _) = batch.run(), batch.definition()
+    inside = slice(int(batch.starts[0]), int(batch.starts[-1]))
+    for name, x, r in zip(NAMES, got, want):
+        at = np.s_[:, inside] if name == "lse" else inside
+        off = np.linalg.norm(x[at] - r[at]) / np.linalg.norm(r[at])
+        assert off <= 8 * float(np.finfo(dtype).eps), (name, off)
