@@ -844,22 +844,19 @@ __device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, cons
     rows_products<HDP>(t.q[block], st.k_hi, st.k_lo, s, t.g[block], st.v_hi, st.v_lo, dp, lane);
     const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
     const int e_ratio = notes.e_q - st.top_q;
-    // (not as part of the exponent: an argument of a hundred has 17 bits behind its point)
-    const float scale_v = pow2(st.x_v);
     float w[16], ds[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const f4 lse = *reinterpret_cast<const f4*>(t.lse + 32 * block + 8 * q + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e])) * scale_v;
+        for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e]));
     }
     if (row0 < wave_last) {  // some key is not seen by some row
 #pragma unroll
         for (int r = 0; r < 16; ++r) w[r] = row0 + acc_row(r, h) >= st.first_row ? w[r] : 0.f;
     }
-    fit(w, st.x_v, st.dv);
-    // |P (dP - D)| 2^(1 - top_t) is at most 1; the ratio of Q's powers goes in, the weights' own power comes out
-    const int e_one = 1 - st.top_t + e_ratio + st.x_k - st.x_v;
+    // |P (dP - D)| 2^(1 - top_t) is at most 1; the ratio of Q's powers goes in
+    const int e_one = 1 - st.top_t + e_ratio + st.x_k;
     const float a1 = __builtin_ldexpf(1.f, notes.e_g + st.e_v + e_one);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -871,11 +868,12 @@ __device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, cons
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = row0 + acc_row(r, h) >= st.first_row ? ds[r] : 0.f;
     }
-    if (notes.e_g != st.top_g) {
-        const float f = pow2(notes.e_g - st.top_g);
+    // The weights of dV, with the ratio of dO's powers: what is made to fit into halves is what really enters the sum.  (The power
+    // multiplies the exponential: as a part of its argument, a hundred or so, it would leave that 17 bits behind the point.)
+    const float f = pow2(st.x_v + notes.e_g - st.top_g);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] *= f;
-    }
+    for (int r = 0; r < 16; ++r) w[r] *= f;
+    fit(w, st.x_v, st.dv);
     h8 hi[2], lo[2];
     split_regs<16>(w, minus_one, hi, lo);
     columns_product<HDP>(t.g[block], hi, lo, across, st.dv);
@@ -919,7 +917,8 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
         st.e_k = a.hk[key_tile].e;
         st.e_v = a.hv[key_tile].e;
         int tq = NO_EXPONENT, tg = NO_EXPONENT, td = NO_EXPONENT;
-        for (int tile = first + lane; tile < tiles; tile += 64) {
+        // (rows in front of the wavefront's keys see none of them)
+        for (int tile = max(first, key0 * p.group / 64) + lane; tile < tiles; tile += 64) {
             tq = max(tq, a.hq[tile_at(tile)].e);
             tg = max(tg, a.hg[tile_at(tile)].e);
             td = max(td, a.hg[tile_at(tile)].e_dot);

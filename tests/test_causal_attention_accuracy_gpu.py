@@ -119,3 +119,34 @@ def test_errors_in_norm(gpu, dtype, by, lengths):
         at = np.s_[:, inside] if name == "lse" else inside
         off = np.linalg.norm(x[at] - r[at]) / np.linalg.norm(r[at])
         assert off <= 8 * float(np.finfo(dtype).eps), (name, off)
+
+
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("down", [16, 24, 60])
+def test_large_gradients_that_have_no_weight(gpu, dtype, by, heads, kv_heads, d, down):
+    """The gradients of a sequence's tokens from 64 to 127 are 2^down times the others; to keys in front of them these tokens give
+    weights of less than e^-90.  (The gradient of K is held as well: what those tokens add to it vanishes with their weight.)"""
+    batch = Spread(dtype, [190, 64, 130], heads, kv_heads, d, "fused")
+    large, front = np.zeros(batch.rows, bool), np.zeros(batch.rows, bool)
+    for s in (batch.starts[0], batch.starts[2]):
+        front[s:s + 64] = True
+        large[s + 64:s + 128] = True
+    large &= np.arange(batch.rows) < batch.starts[-1]
+    batch.g[large] *= dtype(2.0 ** down)
+    for i in range(kv_heads):
+        batch.k[front, i * d] = -40
+    for i in range(heads):
+        batch.q[large, i * d] = 120 / (40 * batch.scale)
+    compare(batch.repeat(by), ("dv", "dk"))
+
+
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("down", [16, 24, 100])
+def test_large_gradients_that_do_not_reach_a_key(gpu, dtype, by, heads, kv_heads, d, down):
+    """The gradients of a sequence's first 64 tokens are 2^down times the others: keys behind them are not seen by them."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    for s in batch.starts[:-1]:
+        batch.g[s:s + 64] *= dtype(2.0 ** down)
+    compare(batch.repeat(by), ("dq", "dk", "dv"))
