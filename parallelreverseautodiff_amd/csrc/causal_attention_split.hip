@@ -9,10 +9,11 @@
 //
 // Scaling.  Halves reach from 2^-24 to 2^16, so the rows of a tile (64 rows of one head) are scaled by one power of two that
 // takes the largest magnitude in it to [2^11, 2^12).  An element 2^-26 times that still has its 11 + 11 bits, one further down
-// an absolute error of 2^-37 of the largest.  Where tiles are summed in one accumulator, the ratio of a tile's power to the
-// largest one of all tiles that go into the sum is folded into the weights.  The weights of a column (a query forward, a key or a
-// query backward) are scaled by a power of two that belongs to the column and falls when a weight no longer fits, the
-// accumulators of the column with it: forward that is the running maximum of the softmax, backward `fit`.
+// an absolute error of 2^-37 of the largest.  Where tiles are summed in one accumulator, the ratio of their powers is folded into
+// the weights, in float.  The weights of a column (a query forward, a key or a query backward), with that ratio, are scaled by a
+// power of two that belongs to the column and falls when one no longer fits into a half, the accumulators of the column with it:
+// forward that is a running maximum beside the softmax's own, backward `fit`.  So it follows what really enters the sum: a tile of
+// large values that a column does not see, or gives next to no weight, costs it no bits.
 //
 // Layout.  A first launch splits the operands and writes them in the order in which the 32 x 32 x 16 matrix instruction takes
 // its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the head dimension; a fragment is
@@ -515,8 +516,9 @@ template <int HDP>
 struct ForwardState {
     h8 q_hi[HDP / 16], q_lo[HDP / 16];
     f16v o[HDP / 32];
-    float m, l;        // the maximum the weights refer to (in units of log2 e) and their sum, this lane half's share
-    int e_row, e_v;    // exponent of the row of Q; exponent that o is kept at
+    float m, l;        // the maximum the sum refers to (in units of log2 e, whole): sum of 2^(score - m + 8), this lane half's share
+    float x;           // the same for o: sum of 2^(score + e - x + 8) V 2^-e, e the power of V's tile
+    int e_row;         // exponent of the row of Q
     int last;          // the last key that the lane's row sees
 };
 
@@ -532,20 +534,29 @@ __device__ __forceinline__ void forward_mask(f16v& s, uint32_t marks, int k0, in
         }
     }
 }
-// Scores to weights, split.  The reference of the weights follows the maximum only when it has risen by more than 2^6: weights reach
-// 2^6 2^8, and the accumulators are rarely rescaled (by the factor returned).  No key seen yet: m = -inf, and a top of -inf
-// keeps the weights at 0.
+// Scores to weights, split.  A weight meets V scaled by 2^-e_tile: what enters the accumulators is 2^(score + e_tile), and the
+// reference x of the weights follows the largest of those, so that a tile of large values whose weight is next to nothing takes no
+// bits from the others.  The sum of the weights follows the largest score, m: it takes the weights of a block with the ratio of the
+// two references, which are whole numbers.  Both are raised only when the largest has risen by more than 2^6 (weights reach
+// 2^6 2^8), so that the accumulators are rarely rescaled (by the factor returned).  No key seen yet: -inf, and a top of -inf keeps
+// the weights at 0.
+constexpr float FAR = 60.f;
 template <int HDP>
-__device__ __forceinline__ float forward_weights(f16v& s, float c, float minus_one, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2]) {
+__device__ __forceinline__ float forward_weights(f16v& s, float c, float e_tile, float minus_one, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2], bool* far) {
     float top = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
     top = max_halves(top) * c;
-    const bool raise = top > st.m + 6.f;
-    const float m = raise ? top : st.m;
-    const float f = __builtin_amdgcn_exp2f(raise ? st.m - m : 0.f);  // (m = -inf before: 0)
+    const bool raise = top > st.m + 6.f, raise_o = top + e_tile > st.x + 6.f;
+    const float whole = ceilf(top), m = raise ? whole : st.m, x = raise_o ? whole + e_tile : st.x;
+    const float f = __builtin_amdgcn_exp2f(raise ? st.m - m : 0.f), fo = __builtin_amdgcn_exp2f(raise_o ? st.x - x : 0.f);  // (-inf before: 0)
     st.m = m;
-    const float ref = m == -INFINITY ? 0.f : m - 8.f;
+    st.x = x;
+    // A tile so small that all of it is below 2^-40 of what the accumulators hold (or zeros): its weights are formed for the sum
+    // alone, where the reference of the accumulators would take them below the smallest float.
+    const bool none = m == -INFINITY;
+    *far = x - e_tile > m + FAR;
+    const float up = *far ? FAR : x - e_tile - m, ref = none ? 0.f : m + up - 8.f;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     float w[16];
 #pragma unroll
@@ -553,30 +564,26 @@ __device__ __forceinline__ float forward_weights(f16v& s, float c, float minus_o
         w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
         sum[r & 3] += w[r];
     }
-    st.l = __builtin_fmaf(st.l, f, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+    st.l = __builtin_fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), none ? 1.f : __builtin_amdgcn_exp2f(up), st.l * f);
     split_regs<16>(w, minus_one, hi, lo);
     keep_here(hi, lo);
-    return f;
+    return fo;
 }
-// Before the weights of a block meet V: the accumulators follow the weights' reference, and the larger of their exponent and the
-// tile's; a tile of smaller values has the ratio in its weights (a power of two: exact, down to where halves end).
+// Before the weights of a block meet V: the accumulators follow the weights' reference.
 template <int HDP>
-__device__ __forceinline__ void forward_rescale(float f, int e_tile, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2]) {
-    const int e_v = max(e_tile, st.e_v);
-    if (__ballot(f != 1.f) != 0 || e_v != st.e_v) {
-        const float fo = __builtin_ldexpf(f, max(st.e_v - e_v, -200));
+__device__ __forceinline__ void forward_rescale(float f, bool far, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2]) {
+    if (__ballot(f != 1.f) != 0) {
 #pragma unroll
         for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st.o[d][r] *= fo;
-        st.e_v = e_v;
+            for (int r = 0; r < 16; ++r) st.o[d][r] *= f;
     }
-    if (e_tile != st.e_v) {
-        const _Float16 ratio = (_Float16)pow2(max(e_tile - st.e_v, -40));
+    if (__ballot(far) != 0) {
+        const _Float16 keep = far ? 0.f : 1.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            hi[i] *= ratio;
-            lo[i] *= ratio;
+            hi[i] *= keep;
+            lo[i] *= keep;
         }
     }
 }
@@ -588,20 +595,21 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
                                              int lane, ForwardState<HDP>& st) {
     const int h = lane >> 5, first_mark = k0 / 32 % 2;
     const Across across(lane);
-    const float c = pow2(st.e_row + notes.k.e);
+    const float c = pow2(st.e_row + notes.k.e), e_v = (float)notes.v.e;
     f16v s[KEYS / 32];
     h8 hi[2], lo[2];
+    bool far;
     rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
     forward_mask<HDP>(s[0], notes.k.bad[KEYS == 64 ? 0 : first_mark], k0, wave_first, h, st);
     if constexpr (KEYS == 64) rows_product<HDP, true>(&t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
-    float f = forward_weights<HDP>(s[0], c, minus_one, st, hi, lo);
-    forward_rescale<HDP>(f, notes.v.e, st, hi, lo);
+    float f = forward_weights<HDP>(s[0], c, e_v, minus_one, st, hi, lo, &far);
+    forward_rescale<HDP>(f, far, st, hi, lo);
     if constexpr (KEYS == 64) {
         forward_mask<HDP>(s[1], notes.k.bad[1], k0 + 32, wave_first, h, st);
         columns_product<HDP, true>(&t.v[0][0], hi, lo, across, st.o);
         h8 hi2[2], lo2[2];
-        f = forward_weights<HDP>(s[1], c, minus_one, st, hi2, lo2);
-        forward_rescale<HDP>(f, notes.v.e, st, hi2, lo2);
+        f = forward_weights<HDP>(s[1], c, e_v, minus_one, st, hi2, lo2, &far);
+        forward_rescale<HDP>(f, far, st, hi2, lo2);
         columns_product<HDP>(&t.v[1][0], hi2, lo2, across, st.o);
     } else {
         columns_product<HDP>(&t.v[0][0], hi, lo, across, st.o);
@@ -682,7 +690,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     st.last = row < rows ? seen_by_row : job.w - 1;
     st.m = -INFINITY;
     st.l = 0.f;
-    st.e_v = NO_EXPONENT;
+    st.x = -INFINITY;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
@@ -701,6 +709,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     if (row >= rows) return;
     const float l = sum_halves(st.l);
     const float inv = row_bad ? NAN : 1.f / l;
+    const int e_o = st.x == -INFINITY ? 0 : (int)(st.x - st.m);
     float* __restrict__ dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
@@ -709,7 +718,7 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
             const int at = 32 * d + 8 * q + 4 * h;
             f4 y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(st.o[d][4 * q + e] * inv, st.e_v);
+            for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(st.o[d][4 * q + e] * inv, e_o);
             if (at >= p.head_dim) continue;
             if (p.vec_o) {
                 *reinterpret_cast<f4*>(dst + at) = y;

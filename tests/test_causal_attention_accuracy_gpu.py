@@ -150,3 +150,22 @@ def test_large_gradients_that_do_not_reach_a_key(gpu, dtype, by, heads, kv_heads
     for s in batch.starts[:-1]:
         batch.g[s:s + 64] *= dtype(2.0 ** down)
     compare(batch.repeat(by), ("dq", "dk", "dv"))
+
+
+# ---- tiles of different size, of which the large one has next to no weight -----------------------------------------------
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("down", [16, 24, 60])
+def test_large_values_that_have_no_weight(gpu, dtype, by, heads, kv_heads, d, down):
+    """The values of a sequence's first 64 tokens are 2^down times the others, and later queries give them weights of less than
+    e^-90: 2^-130 of the sum, which is less than a rounding of what the others give."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    first = np.zeros(batch.rows, bool)
+    for s in batch.starts[:-1]:
+        first[s:s + 64] = True
+    batch.v[first] *= dtype(2.0 ** down)
+    for i in range(kv_heads):
+        batch.k[first, i * d] = -40
+    for i in range(heads):
+        batch.q[~first, i * d] = 120 / (40 * batch.scale)
+    compare(batch.repeat(by), ("o", "lse"))
