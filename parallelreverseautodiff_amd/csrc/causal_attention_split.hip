@@ -7,13 +7,15 @@
 // (library products on this card: 1060 TFLOP/s in half, 153 in float) - and they overlap with vector instructions, which the
 // float ones do not.
 //
-// Scaling.  Halves reach from 2^-24 to 2^16, so the rows of a tile (64 rows of one head) are scaled by one power of two that
-// takes the largest magnitude in it to [2^11, 2^12).  An element 2^-26 times that still has its 11 + 11 bits, one further down
-// an absolute error of 2^-37 of the largest.  Where tiles are summed in one accumulator, the ratio of their powers is folded into
-// the weights, in float.  The weights of a column (a query forward, a key or a query backward), with that ratio, are scaled by a
-// power of two that belongs to the column and falls when one no longer fits into a half, the accumulators of the column with it:
-// forward that is a running maximum beside the softmax's own, backward `fit`.  So it follows what really enters the sum: a tile of
-// large values that a column does not see, or gives next to no weight, costs it no bits.
+// Scaling.  A half has 11 bits from 2^-14 on and ends at 2^-24, so an element keeps its 11 + 11 bits down to 2^-2 or so; what is
+// below that is off by 2^-25.  The rows of a tile (64 rows of one head) are scaled by one power of two that takes the largest
+// magnitude in it to [2^11, 2^15), as long as no row's largest is more than 2^10 below that: every row is then right to 2^-24 of
+// its own largest.  In an uneven tile each row has a power of its own; those go onto the scores, onto dP and onto the weights, row
+// by row.  Where tiles are summed in one accumulator, the ratio of their powers is folded into the weights, in float.  The weights
+// of a column (a query forward, a key or a query backward), with that ratio, are scaled by a power of two that belongs to the
+// column and falls when one no longer fits into a half, the accumulators of the column with it: forward that is a running maximum
+// beside the softmax's own, backward `fit`.  So it follows what really enters the sum: large values that a column does not see,
+// or gives next to no weight, cost it no bits.
 //
 // Layout.  A first launch splits the operands and writes them in the order in which the 32 x 32 x 16 matrix instruction takes
 // its fragments: lane l of a fragment holds 8 halves, row l % 32, elements 8 (l / 32) + e along the head dimension; a fragment is
@@ -41,17 +43,29 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr int NO_EXPONENT = -1000;   // of a tile that holds nothing but zeros
+constexpr int NO_EXPONENT = -1000;   // of zeros
+// How far (powers of two) the largest values of two rows of a tile lie apart before rows get powers of their own.
+constexpr int MOST_SPREAD = 10;
 
 // What the first launch notes about a tile of 64 rows.
 struct Header {
-    int e;                  // values were scaled by 2^-e
+    int e;                  // the power of its largest value: an even tile was scaled by 2^-e
+    int uneven;             // rows were scaled by powers of their own
     uint32_t bad[2];        // rows that hold a non-finite value
-    int e_dot;              // of dO: |D| < 2^e_dot
 };
 
 __device__ __forceinline__ int64_t clamped(int64_t v, int64_t most) { return v < 0 ? 0 : v > most ? most : v; }
 __device__ __forceinline__ bool is_finite(float x) { return fabsf(x) < INFINITY; }
+// x < 2^power_of(x)
+__device__ __forceinline__ int power_of(float x) {
+    if (!(x > 0.f)) return NO_EXPONENT;
+    int e;
+    (void)frexpf(x, &e);
+    return e;
+}
+// The power that takes the largest magnitude of some values to [2^11, 2^15).  A multiple of 4, so that tiles of about the same size
+// have the same.
+__device__ __forceinline__ int power_for(float top) { return top > 0.f ? (power_of(top) - 12) & ~3 : NO_EXPONENT; }
 // 2^e, within the normal numbers
 __device__ __forceinline__ float pow2(int e) { return __builtin_ldexpf(1.0f, e < -126 ? -126 : e > 127 ? 127 : e); }
 
@@ -124,6 +138,7 @@ struct SplitSource {
     int vec;
     _Float16* split;
     Header* header;
+    int* powers;       // of the 64 rows of a tile: scaled by 2^-power
     int dots;          // dO: D and lse of the rows as well
 };
 struct SplitArgs {
@@ -134,6 +149,7 @@ struct SplitArgs {
     int order_slots[2];
     int shift;
     float* row_notes;  // [slot][kv][2][64]: -lse log2 e (-inf for a row that is not there), then D
+    int* e_dot;        // [slot][kv]: |D| < 2^e_dot
 };
 
 // The groups of 128 packed rows (which = 0) or 128 keys (1) of all sequences as (sequence, number inside it, first row of the
@@ -195,7 +211,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     constexpr int PITCH = HDP + 4, PER_ROW = HDP / 4, COUNT = 64 * PER_ROW / 256;
     static_assert(64 * PITCH >= ORDER_BINS, "the tile's room also holds the bins of a schedule");
     __shared__ __attribute__((aligned(16))) float tile[64 * PITCH];
-    __shared__ float wave_max[4], row_dots[64], largest_dot;
+    __shared__ float row_top[64], row_dots[64];
     __shared__ int bad[64];
     const CausalArgs<float>& p = a.p;
     if ((int)blockIdx.z == a.tensors) {
@@ -217,7 +233,6 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     if (threadIdx.x < 64) bad[threadIdx.x] = 0;
     __syncthreads();
     f4 v[COUNT];
-    float top = 0.f;
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) {
         const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
@@ -237,6 +252,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) {
         const int j = (threadIdx.x + 256 * u) / PER_ROW;
+        float top = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (!is_finite(v[u][e])) {
@@ -245,12 +261,12 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
             }
             top = fmaxf(top, fabsf(v[u][e]));
         }
+#pragma unroll
+        for (int m = 1; m < PER_ROW; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+        row_top[j] = top;  // (every lane of the row the same)
     }
-    top = wave_max_t(top);
-    if (lane == 0) wave_max[wave] = top;
     // D = rowsum(dO (.) O): the PER_ROW lanes that hold a row of dO
     if (t.dots) {
-        float size = 0.f;
 #pragma unroll
         for (int u = 0; u < COUNT; ++u) {
             const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
@@ -274,55 +290,44 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
             for (int m = 1; m < PER_ROW; m <<= 1) dot += __shfl_xor(dot, m, 64);
             row_dots[j] = dot;  // (every lane of the row the same)
         }
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            const uint32_t r = row0 + threadIdx.x, down = r / group;
+    }
+    __syncthreads();
+    // One power for the tile, or one for each row where some are far below the largest: each wavefront for itself, a row per lane.
+    const float top_here = row_top[lane], top = wave_max_t(top_here);
+    const int e = power_for(top);
+    const bool uneven = __ballot(row0 + lane < rows && top > 0.f && power_of(top) - power_of(top_here) > MOST_SPREAD) != 0;
+    const int64_t tile_at = (int64_t)blockIdx.x * p.kv_heads + kv;
+    if (wave == 0) {
+        const uint64_t marks = __ballot(bad[lane] != 0);
+        if (lane == 0) t.header[tile_at] = Header{e, uneven, {(uint32_t)marks, (uint32_t)(marks >> 32)}};
+        t.powers[tile_at * 64 + lane] = uneven ? power_for(top_here) : e;
+        if (t.dots) {
+            const uint32_t r = row0 + lane, down = r / group;
             const int64_t token = q0 + down, head = kv * group + (r - down * group);
-            float dot = row_dots[threadIdx.x], lse = -INFINITY;
+            float dot = row_dots[lane], lse = -INFINITY, size = 0.f;
             if (r < rows) {
-                if (!is_finite(dot) || bad[threadIdx.x] != 0) dot = NAN;
+                if (!is_finite(dot) || bad[lane] != 0) dot = NAN;
                 else size = fabsf(dot);
                 lse = (dot - dot) - p.lse[head * p.q_rows + token] * LOG2E;  // NaN where D is
             }
-            const int64_t at = ((int64_t)blockIdx.x * p.kv_heads + kv) * 128 + threadIdx.x;
-            a.row_notes[at] = lse;
-            a.row_notes[at + 64] = dot;
-            size = wave_max_t(size);
-            if (lane == 0) largest_dot = size;
-        }
-    }
-    __syncthreads();
-    top = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
-    int e = NO_EXPONENT;
-    if (top > 0.f) {
-        (void)frexpf(top, &e);  // top = m 2^e, m in [1/2, 1)
-        e -= 12;
-    }
-    if (threadIdx.x < 64) {
-        const uint64_t marks = __ballot(bad[threadIdx.x] != 0);
-        if (threadIdx.x == 0) {
-            Header h;
-            h.e = e;
-            h.bad[0] = (uint32_t)marks;
-            h.bad[1] = (uint32_t)(marks >> 32);
-            h.e_dot = NO_EXPONENT;
-            if (t.dots) {
-                if (largest_dot > 0.f) (void)frexpf(largest_dot, &h.e_dot);
-            }
-            t.header[(int64_t)blockIdx.x * p.kv_heads + kv] = h;
+            a.row_notes[tile_at * 128 + lane] = lse;
+            a.row_notes[tile_at * 128 + 64 + lane] = dot;
+            const int e_dot = power_of(wave_max_t(size));
+            if (lane == 0) a.e_dot[tile_at] = e_dot;
         }
     }
 #pragma unroll
     for (int u = 0; u < COUNT; ++u) {
         const int at = threadIdx.x + 256 * u, j = at / PER_ROW, d = (at % PER_ROW) * 4;
+        const int by = uneven ? power_for(row_top[j]) : e;
         f4 w;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) w[c] = top > 0.f ? __builtin_ldexpf(v[u][c], -e) : 0.f;
+        for (int c = 0; c < 4; ++c) w[c] = top > 0.f ? __builtin_ldexpf(v[u][c], -by) : 0.f;
         *reinterpret_cast<f4*>(tile + j * PITCH + d) = w;
     }
     __syncthreads();
     const float minus_one = opaque_minus_one();
-    const int64_t base = ((int64_t)blockIdx.x * p.kv_heads + kv) * (128 * HDP);  // halves
+    const int64_t base = tile_at * (128 * HDP);  // halves
     constexpr int FRAGS = HDP / 16;  // per block and plane
 #pragma unroll
     for (int u = 0; u < 2 * FRAGS * 64 / 256; ++u) {
@@ -473,6 +478,8 @@ struct ForwardArgs {
     const _Float16* v;
     const Header* hk;
     const Header* hv;
+    const int* powers_k;
+    const int* powers_v;
     const int4* order;
 };
 
@@ -486,6 +493,30 @@ struct ForwardTile {
     _Float16 v[BLOCKS][64 * HDP];
 };
 
+// x[r] times 2^(power of its row + by): rows of a block of an uneven tile.
+template <typename X>
+__device__ __forceinline__ void take_powers(X& x, const int* __restrict__ powers, int by, int h) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int4 e = *reinterpret_cast<const int4*>(powers + 8 * q + 4 * h);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[4 * q + c] = __builtin_ldexpf(x[4 * q + c], (&e.x)[c] + by);
+    }
+}
+// The same for dP, with D and another power p2 of the row: (dP 2^(power + by) - D) 2^(p2 + by2).  D of the row, or of the lane.
+__device__ __forceinline__ void take_powers(f16v& dp, const int* __restrict__ powers, int by, int h, const int* __restrict__ powers2, int by2, const float* dot,
+                                            int dot_step = 1) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int4 e = *reinterpret_cast<const int4*>(powers + 8 * q + 4 * h), e2 = *reinterpret_cast<const int4*>(powers2 + 8 * q + 4 * h);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int out = (&e2.x)[c] + by2;
+            dp[4 * q + c] = __builtin_ldexpf(dp[4 * q + c], (&e.x)[c] + by + out) - __builtin_ldexpf(dot[dot_step * (8 * q + 4 * h + c)], out);
+        }
+    }
+}
+
 // What the headers of a tile of keys say.  They are asked for with the copies of the tile and looked at (`uniform`) once those have
 // arrived: touching them earlier would wait for the copies.
 struct KeyNotes {
@@ -495,6 +526,7 @@ struct KeyNotes {
         KeyNotes n;
         n.k.e = __builtin_amdgcn_readfirstlane(k.e);
         n.v.e = __builtin_amdgcn_readfirstlane(v.e);
+        n.k.uneven = __builtin_amdgcn_readfirstlane(k.uneven | v.uneven);
         n.k.bad[0] = __builtin_amdgcn_readfirstlane(k.bad[0] | v.bad[0]);
         n.k.bad[1] = __builtin_amdgcn_readfirstlane(k.bad[1] | v.bad[1]);
         return n;
@@ -554,9 +586,8 @@ __device__ __forceinline__ float forward_weights(f16v& s, float c, float e_tile,
     st.x = x;
     // A tile so small that all of it is below 2^-40 of what the accumulators hold (or zeros): its weights are formed for the sum
     // alone, where the reference of the accumulators would take them below the smallest float.
-    const bool none = m == -INFINITY;
-    *far = x - e_tile > m + FAR;
-    const float up = *far ? FAR : x - e_tile - m, ref = none ? 0.f : m + up - 8.f;
+    const float ref = fmaxf(fminf(x - (e_tile + 8.f), m + (FAR - 8.f)), -1e30f);  // (finite where both are not)
+    *far = x - (e_tile + 8.f) > m + (FAR - 8.f);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     float w[16];
 #pragma unroll
@@ -564,7 +595,7 @@ __device__ __forceinline__ float forward_weights(f16v& s, float c, float e_tile,
         w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
         sum[r & 3] += w[r];
     }
-    st.l = __builtin_fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), none ? 1.f : __builtin_amdgcn_exp2f(up), st.l * f);
+    st.l = __builtin_fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref + 8.f - m), st.l * f);
     split_regs<16>(w, minus_one, hi, lo);
     keep_here(hi, lo);
     return fo;
@@ -588,28 +619,57 @@ __device__ __forceinline__ void forward_rescale(float f, bool far, ForwardState<
     }
 }
 
+// In an uneven tile the weights that meet V take its values' powers (`powers`: of the 32 keys of the block); those that
+// `forward_weights` made are for the sum.
+template <int HDP>
+__device__ __forceinline__ void forward_uneven_weights(const f16v& s, const int* __restrict__ powers, float minus_one, int h, ForwardState<HDP>& st,
+                                                       h8 (&hi)[2], h8 (&lo)[2]) {
+    float top = -INFINITY, w[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int4 e = *reinterpret_cast<const int4*>(powers + 8 * q + 4 * h);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            w[4 * q + c] = s[4 * q + c] + (float)(&e.x)[c];
+            top = fmaxf(top, w[4 * q + c]);
+        }
+    }
+    top = max_halves(top);
+    const bool raise = top > st.x + 6.f;
+    const float x = raise ? ceilf(top) : st.x, f = __builtin_amdgcn_exp2f(raise ? st.x - x : 0.f), ref = x == -INFINITY ? 0.f : x - 8.f;
+    st.x = x;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(w[r] - ref);
+    split_regs<16>(w, minus_one, hi, lo);
+    forward_rescale<HDP>(f, false, st, hi, lo);
+}
+
 // A tile of KEYS keys against the wavefront's rows, block by block: the second block's scores are formed beside the first one's
-// softmax, the first one's product with V beside the second one's softmax.
-template <int HDP, int KEYS>
-__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int k0, int wave_first, float minus_one,
-                                             int lane, ForwardState<HDP>& st) {
+// softmax, the first one's product with V beside the second one's softmax.  powers_k, powers_v: of the tile's keys.
+template <int HDP, int KEYS, bool UNEVEN>
+__device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, const int* __restrict__ powers_k,
+                                             const int* __restrict__ powers_v, int k0, int wave_first, float minus_one, int lane, ForwardState<HDP>& st) {
     const int h = lane >> 5, first_mark = k0 / 32 % 2;
     const Across across(lane);
-    const float c = pow2(st.e_row + notes.k.e), e_v = (float)notes.v.e;
+    const float c = UNEVEN ? 1.f : pow2(st.e_row + notes.k.e), e_v = (float)(UNEVEN ? NO_EXPONENT : notes.v.e);
     f16v s[KEYS / 32];
     h8 hi[2], lo[2];
     bool far;
     rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
+    if constexpr (UNEVEN) take_powers(s[0], powers_k, st.e_row, h);  // (to units of log2 e)
     forward_mask<HDP>(s[0], notes.k.bad[KEYS == 64 ? 0 : first_mark], k0, wave_first, h, st);
     if constexpr (KEYS == 64) rows_product<HDP, true>(&t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
     float f = forward_weights<HDP>(s[0], c, e_v, minus_one, st, hi, lo, &far);
     forward_rescale<HDP>(f, far, st, hi, lo);
+    if constexpr (UNEVEN) forward_uneven_weights<HDP>(s[0], powers_v, minus_one, h, st, hi, lo);
     if constexpr (KEYS == 64) {
+        if constexpr (UNEVEN) take_powers(s[1], powers_k + 32, st.e_row, h);
         forward_mask<HDP>(s[1], notes.k.bad[1], k0 + 32, wave_first, h, st);
         columns_product<HDP, true>(&t.v[0][0], hi, lo, across, st.o);
         h8 hi2[2], lo2[2];
         f = forward_weights<HDP>(s[1], c, e_v, minus_one, st, hi2, lo2, &far);
         forward_rescale<HDP>(f, far, st, hi2, lo2);
+        if constexpr (UNEVEN) forward_uneven_weights<HDP>(s[1], powers_v + 32, minus_one, h, st, hi2, lo2);
         columns_product<HDP>(&t.v[1][0], hi2, lo2, across, st.o);
     } else {
         columns_product<HDP>(&t.v[0][0], hi, lo, across, st.o);
@@ -620,7 +680,7 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
 // keys, head dimension 64, 8192 tokens in 420 us, 330 TFLOP/s of the visible pairs, 990 with the three products each - 93 %
 // of a large library product of halves.  Twelve sequences of up to 2048 in 75 us.
 template <int HDP, int KEYS>
-__global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardArgs a) {
+__global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel(const ForwardArgs a) {
     __shared__ __attribute__((aligned(16))) ForwardTile<HDP, KEYS> even, odd;
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
@@ -695,16 +755,33 @@ __global__ void __launch_bounds__(256, 2) causal_split_fwd_kernel(const ForwardA
     for (int d = 0; d < HDP / 32; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.o[d][r] = 0.f;
-    for (int k0 = 0; k0 < seen; k0 += 2 * KEYS) {
-        staged();
-        KeyNotes notes = notes_even.uniform();
-        if (k0 + KEYS < seen) forward_stage<HDP, KEYS>(a, odd, notes_odd, tile0, kv, k0 + KEYS, wave, lane);
-        if (k0 < wave_seen) forward_tile<HDP, KEYS>(even, notes, k0, wave_first, minus_one, lane, st);
-        if (k0 + KEYS >= seen) break;
-        staged();
-        notes = notes_odd.uniform();
-        if (k0 + 2 * KEYS < seen) forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, k0 + 2 * KEYS, wave, lane);
-        if (k0 + KEYS < wave_seen) forward_tile<HDP, KEYS>(odd, notes, k0 + KEYS, wave_first, minus_one, lane, st);
+    auto use = [&](auto uneven, const ForwardTile<HDP, KEYS>& t, const KeyNotes& notes, int k0) __attribute__((always_inline)) {
+        const int64_t at = ((tile0 + k0 / 64) * p.kv_heads + kv) * 64 + k0 % 64;
+        if (k0 < wave_seen) forward_tile<HDP, KEYS, uneven()>(t, notes, a.powers_k + at, a.powers_v + at, k0, wave_first, minus_one, lane, st);
+    };
+    // From key k0 on, whose tile is being copied; returns where an uneven tile is met by the form that takes none.  (The code for those
+    // is apart, and used from there on: inside the common one its registers cost that up to 20 %.)
+    auto walk = [&](auto uneven, int k0) __attribute__((always_inline)) {
+        for (; k0 < seen; k0 += 2 * KEYS) {
+            staged();
+            KeyNotes notes = notes_even.uniform();
+            if (!uneven() && notes.k.uneven != 0) break;
+            if (k0 + KEYS < seen) forward_stage<HDP, KEYS>(a, odd, notes_odd, tile0, kv, k0 + KEYS, wave, lane);
+            use(uneven, even, notes, k0);
+            if (k0 + KEYS >= seen) return seen;
+            staged();
+            notes = notes_odd.uniform();
+            if (!uneven() && notes.k.uneven != 0) return k0 + KEYS;
+            if (k0 + 2 * KEYS < seen) forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, k0 + 2 * KEYS, wave, lane);
+            use(uneven, odd, notes, k0 + KEYS);
+        }
+        return k0;
+    };
+    const int at = walk(std::false_type(), 0);
+    if (__builtin_expect(at < seen, 0)) {
+        // (all wavefronts are past what either buffer held before that tile)
+        forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, at, wave, lane);
+        walk(std::true_type(), at);
     }
     if (row >= rows) return;
     const float l = sum_halves(st.l);
@@ -740,7 +817,9 @@ struct BackwardArgs {
     const _Float16* q; const _Float16* g;   // g: dO
     const _Float16* k; const _Float16* v;
     const Header* hq; const Header* hg; const Header* hk; const Header* hv;
+    const int* powers_q; const int* powers_g; const int* powers_k; const int* powers_v;
     const float* row_notes;
+    const int* e_dot;
     const int4* row_order; const int4* key_order;
     int chunk_tiles, chunks;    // tiles of rows that a workgroup of the key kernel takes at most, and parts that makes of the longest
     float* part;                // [chunk][token][kv][dK | dV][hd4] where a group of keys has more than one part
@@ -752,8 +831,22 @@ __device__ __forceinline__ int wave_max_int(int v) {
     for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
     return __builtin_amdgcn_readfirstlane(v);
 }
-// dP - D is below 2^(e - 1) in magnitude, e from the exponents of dO, V and D: a sum of up to 2^7 products of values below 2^12
-__device__ __forceinline__ int e_difference(int e_g, int e_v, int e_dot) { return max(31 + e_g + e_v, e_dot + 1) + 1; }
+// dP - D is below 2^(e - 1) in magnitude, e from the exponents of dO, V and D: a sum of up to 2^7 products of values below 2^15
+__device__ __forceinline__ int e_difference(int e_g, int e_v, int e_dot) { return max(37 + e_g + e_v, e_dot + 1) + 1; }
+// The largest of the values of the lanes up to lane n, or from lane n on; a lane asks with an n of its own (outside 0 .. 63: none of
+// them, or all).
+__device__ __forceinline__ int max_upto(int v, int n) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = max(v, __shfl_up(v, off, 64));
+    const int got = __shfl(v, n > 63 ? 63 : n < 0 ? 0 : n, 64);
+    return n < 0 ? NO_EXPONENT : got;
+}
+__device__ __forceinline__ int max_from(int v, int n) {
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) v = max(v, __shfl_down(v, off, 64));
+    const int got = __shfl(v, n < 0 ? 0 : n > 63 ? 63 : n, 64);
+    return n > 63 ? NO_EXPONENT : got;
+}
 
 // Makes weights fit into halves: where a column's largest has passed 2^15, the column and its accumulators come down to 2^11, so
 // that it takes another factor of 16 before the next time.  x: the power of two that the column is scaled by.
@@ -819,13 +912,13 @@ struct RowTile {
     float lse[64], dot[64];
 };
 struct RowNotes {
-    int e_q, e_g;
+    int e_q, e_g, uneven;
 };
 
 template <int HDP>
 __device__ __forceinline__ void row_stage(const BackwardArgs& a, RowTile<HDP>& t, RowNotes& notes, int64_t tile_at, int wave, int lane) {
-    notes.e_q = a.hq[tile_at].e;
-    notes.e_g = a.hg[tile_at].e;
+    const Header hq = a.hq[tile_at], hg = a.hg[tile_at];
+    notes = RowNotes{hq.e, hg.e, hq.uneven | hg.uneven};
     stage<256 * HDP, 4>(a.q + tile_at * (128 * HDP), &t.q[0][0], wave, lane);
     stage<256 * HDP, 4>(a.g + tile_at * (128 * HDP), &t.g[0][0], wave, lane);
     if (wave < 2) {
@@ -838,21 +931,29 @@ template <int HDP>
 struct KeyState {
     h8 k_hi[HDP / 16], k_lo[HDP / 16], v_hi[HDP / 16], v_lo[HDP / 16];
     f16v dk[HDP / 32], dv[HDP / 32];
-    int e_k, e_v;            // of the lane's keys
-    int top_q, top_g, top_t; // the largest exponents of Q, dO and dP - D over all rows that go into the sums
+    int e_k, e_v;            // of the lane's key
     int x_v, x_k;            // the powers of two that the lane's key is scaled by in the weights of dV and dK
     int first_row;           // the first packed row that sees the lane's key
 };
 
-template <int HDP>
-__device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, const RowNotes& notes, int row0, int wave_last, float factor, float minus_one, int lane,
-                                          KeyState<HDP>& st) {
+// powers_q, powers_g: of the block's rows.
+template <int HDP, bool UNEVEN>
+__device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, const RowNotes& notes, const int* __restrict__ powers_q,
+                                          const int* __restrict__ powers_g, int row0, int wave_last, float factor, float minus_one, int lane, KeyState<HDP>& st) {
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
     rows_products<HDP>(t.q[block], st.k_hi, st.k_lo, s, t.g[block], st.v_hi, st.v_lo, dp, lane);
-    const float c = __builtin_ldexpf(factor, notes.e_q + st.e_k);
-    const int e_ratio = notes.e_q - st.top_q;
+    // The weights of dV are 2^x_v P with dO's power, those of dK 2^x_k P (dP - D) with Q's: what is made to fit into halves is what
+    // really enters the sums.  (The power multiplies the exponential: as a part of its argument, a hundred or so, it would leave
+    // that 17 bits behind the point.)  In an uneven tile the powers are those of the rows.
+    if constexpr (UNEVEN) {
+        take_powers(s, powers_q, st.e_k, h);
+        take_powers(dp, powers_g, st.e_v, h, powers_q, st.x_k, t.dot + 32 * block);
+    }
+    const float c = __builtin_ldexpf(factor, UNEVEN ? 0 : notes.e_q + st.e_k);
+    const int e_one = UNEVEN ? 2 * NO_EXPONENT : notes.e_q + st.x_k;  // (D is in dP already: what is left of it is 0, or NaN)
+    const float a1 = __builtin_ldexpf(1.f, UNEVEN ? 0 : notes.e_g + st.e_v + e_one), f = pow2(UNEVEN ? 0 : notes.e_g + st.x_v);
     float w[16], ds[16];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -860,28 +961,23 @@ __device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, cons
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], c, lse[e]));
     }
-    if (row0 < wave_last) {  // some key is not seen by some row
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] = row0 + acc_row(r, h) >= st.first_row ? w[r] : 0.f;
-    }
-    // |P (dP - D)| 2^(1 - top_t) is at most 1; the ratio of Q's powers goes in
-    const int e_one = 1 - st.top_t + e_ratio + st.x_k;
-    const float a1 = __builtin_ldexpf(1.f, notes.e_g + st.e_v + e_one);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const f4 dot = *reinterpret_cast<const f4*>(t.dot + 32 * block + 8 * q + 4 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) ds[4 * q + e] = w[4 * q + e] * __builtin_fmaf(dp[4 * q + e], a1, -__builtin_ldexpf(dot[e], e_one));
     }
-    if (row0 < wave_last) {  // (a weight of zero times a D that is not finite)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] = row0 + acc_row(r, h) >= st.first_row ? ds[r] : 0.f;
-    }
-    // The weights of dV, with the ratio of dO's powers: what is made to fit into halves is what really enters the sum.  (The power
-    // multiplies the exponential: as a part of its argument, a hundred or so, it would leave that 17 bits behind the point.)
-    const float f = pow2(st.x_v + notes.e_g - st.top_g);
 #pragma unroll
     for (int r = 0; r < 16; ++r) w[r] *= f;
+    if constexpr (UNEVEN) take_powers(w, powers_g, st.x_v, h);
+    if (row0 < wave_last) {  // some key is not seen by some row (whose weight, D or dP may be anything)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const bool seen = row0 + acc_row(r, h) >= st.first_row;
+            w[r] = seen ? w[r] : 0.f;
+            ds[r] = seen ? ds[r] : 0.f;
+        }
+    }
     fit(w, st.x_v, st.dv);
     h8 hi[2], lo[2];
     split_regs<16>(w, minus_one, hi, lo);
@@ -923,22 +1019,30 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
         const int64_t at = key_tile * (128 * HDP) + from / 32 % 2 * (64 * HDP);
         load_fragments<HDP>(a.k + at, lane, st.k_hi, st.k_lo);
         load_fragments<HDP>(a.v + at, lane, st.v_hi, st.v_lo);
-        st.e_k = a.hk[key_tile].e;
-        st.e_v = a.hv[key_tile].e;
+        st.e_k = a.powers_k[key_tile * 64 + from % 64 + (lane & 31)];
+        st.e_v = a.powers_v[key_tile * 64 + from % 64 + (lane & 31)];
+        // tiles of rows that see all of the wavefront's keys, then those of which some rows do not see some key
+        const int first_row = (key0 + (lane & 31)) * p.group, whole = max(first, ((key0 + 31) * p.group + 63) / 64);
         int tq = NO_EXPONENT, tg = NO_EXPONENT, td = NO_EXPONENT;
-        // (rows in front of the wavefront's keys see none of them)
-        for (int tile = max(first, key0 * p.group / 64) + lane; tile < tiles; tile += 64) {
+        for (int tile = whole + lane; tile < tiles; tile += 64) {
             tq = max(tq, a.hq[tile_at(tile)].e);
             tg = max(tg, a.hg[tile_at(tile)].e);
-            td = max(td, a.hg[tile_at(tile)].e_dot);
+            td = max(td, a.e_dot[tile_at(tile)]);
         }
-        st.top_q = wave_max_int(tq);
-        st.top_g = wave_max_int(tg);
-        st.e_k = __builtin_amdgcn_readfirstlane(st.e_k);
-        st.e_v = __builtin_amdgcn_readfirstlane(st.e_v);
-        st.top_t = e_difference(st.top_g, st.e_v, wave_max_int(td));
+        tq = wave_max_int(tq);
+        tg = wave_max_int(tg);
+        td = wave_max_int(td);
+        for (int tile = max(first, key0 * p.group / 64); tile < min(whole, tiles); ++tile) {
+            const int64_t at = tile_at(tile);
+            const int from_row = first_row - 64 * tile;
+            tq = max(tq, max_from(a.powers_q[at * 64 + lane], from_row));
+            tg = max(tg, max_from(a.powers_g[at * 64 + lane], from_row));
+            td = max(td, max_from(power_of(fabsf(a.row_notes[at * 128 + 64 + lane])), from_row));
+        }
+        // P is at most 1, |P (dP - D)| 2^(1 - e_difference) too
+        st.x_v = FIT_FROM - tg;
+        st.x_k = FIT_FROM + 1 - e_difference(tg, st.e_v, td) - tq;
     }
-    st.x_v = st.x_k = FIT_FROM;
     st.first_row = (key0 + (lane & 31)) * p.group;
     const int wave_first = key0 * p.group, wave_last = (key0 + 31) * p.group;
 #pragma unroll
@@ -946,22 +1050,36 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.dk[d][r] = st.dv[d][r] = 0.f;
     const float factor = p.scale * LOG2E;
-    auto uniform = [](const RowNotes& x) { return RowNotes{__builtin_amdgcn_readfirstlane(x.e_q), __builtin_amdgcn_readfirstlane(x.e_g)}; };
-    auto use = [&](const RowTile<HDP>& t, const RowNotes& notes, int i) {
+    auto uniform = [](const RowNotes& x) {
+        return RowNotes{__builtin_amdgcn_readfirstlane(x.e_q), __builtin_amdgcn_readfirstlane(x.e_g), __builtin_amdgcn_readfirstlane(x.uneven)};
+    };
+    auto use = [&](auto uneven, const RowTile<HDP>& t, const RowNotes& notes, int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int block = 0; block < 2; ++block)
-            if (active && 64 * i + 32 * block + 31 >= wave_first) row_block<HDP>(t, block, notes, 64 * i + 32 * block, wave_last, factor, minus_one, lane, st);
+            if (active && 64 * i + 32 * block + 31 >= wave_first)
+                row_block<HDP, uneven()>(t, block, notes, a.powers_q + tile_at(i) * 64 + 32 * block, a.powers_g + tile_at(i) * 64 + 32 * block,
+                                         64 * i + 32 * block, wave_last, factor, minus_one, lane, st);
     };
-    for (int i = first; i < tiles; i += 2) {
-        staged();
-        RowNotes notes = uniform(notes_even);
-        if (i + 1 < tiles) row_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
-        use(even, notes, i);
-        if (i + 1 >= tiles) break;
-        staged();
-        notes = uniform(notes_odd);
-        if (i + 2 < tiles) row_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
-        use(odd, notes, i + 1);
+    auto walk = [&](auto uneven, int i) __attribute__((always_inline)) {  // (as in the forward kernel)
+        for (; i < tiles; i += 2) {
+            staged();
+            RowNotes notes = uniform(notes_even);
+            if (!uneven() && notes.uneven != 0) break;
+            if (i + 1 < tiles) row_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
+            use(uneven, even, notes, i);
+            if (i + 1 >= tiles) return tiles;
+            staged();
+            notes = uniform(notes_odd);
+            if (!uneven() && notes.uneven != 0) return i + 1;
+            if (i + 2 < tiles) row_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
+            use(uneven, odd, notes, i + 1);
+        }
+        return i;
+    };
+    const int at = walk(std::false_type(), first);
+    if (__builtin_expect(at < tiles, 0)) {
+        row_stage<HDP>(a, even, notes_even, tile_at(at), wave, lane);
+        walk(std::true_type(), at);
     }
     const int64_t key = key0 + (lane & 31);
     if (key >= n) return;
@@ -975,8 +1093,8 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
         width = a.hd4;  // (columns past the head dimension are zeros)
         vec = true;
     }
-    store_column<HDP>(dst_k, st.dk, p.scale, st.top_t - 1 + st.top_q - st.x_k, h, width, vec);
-    store_column<HDP>(dst_v, st.dv, 1.f, st.top_g - st.x_v, h, width, vec);
+    store_column<HDP>(dst_k, st.dk, p.scale, -st.x_k, h, width, vec);
+    store_column<HDP>(dst_v, st.dv, 1.f, -st.x_v, h, width, vec);
 }
 
 // Adds the parts of the groups of keys that have several, in their order (16 us behind the 187 above, by memory).
@@ -1016,13 +1134,13 @@ struct KeyTile {
     _Float16 k[2][64 * HDP], v[2][64 * HDP];   // two blocks of 32 keys
 };
 struct BlockNotes {
-    int e_k, e_v;
+    int e_k, e_v, uneven;
 };
 
 template <int HDP>
 __device__ __forceinline__ void key_stage(const BackwardArgs& a, KeyTile<HDP>& t, BlockNotes& notes, int64_t tile_at, int wave, int lane) {
-    notes.e_k = a.hk[tile_at].e;
-    notes.e_v = a.hv[tile_at].e;
+    const Header hk = a.hk[tile_at], hv = a.hv[tile_at];
+    notes = BlockNotes{hk.e, hv.e, hk.uneven | hv.uneven};
     stage<256 * HDP, 4>(a.k + tile_at * (128 * HDP), &t.k[0][0], wave, lane);
     stage<256 * HDP, 4>(a.v + tile_at * (128 * HDP), &t.v[0][0], wave, lane);
 }
@@ -1032,26 +1150,30 @@ struct RowState {
     h8 q_hi[HDP / 16], q_lo[HDP / 16], g_hi[HDP / 16], g_lo[HDP / 16];
     f16v dq[HDP / 32];
     float lse, dot;
-    int e_q, e_g, top_k, top_t;
+    int e_q, e_g;   // of the lane's row
     int x_q;        // the power of two that the lane's row is scaled by in the weights
     int last;       // the last key that the lane's row sees
 };
 
-template <int HDP>
-__device__ __forceinline__ void key_block(const KeyTile<HDP>& t, int block, const BlockNotes& notes, int k0, int wave_first, float factor, float minus_one, int lane,
-                                          RowState<HDP>& st) {
+// powers_k, powers_v: of the block's keys.
+template <int HDP, bool UNEVEN>
+__device__ __forceinline__ void key_block(const KeyTile<HDP>& t, int block, const BlockNotes& notes, const int* __restrict__ powers_k,
+                                          const int* __restrict__ powers_v, int k0, int wave_first, float factor, float minus_one, int lane, RowState<HDP>& st) {
     const int h = lane >> 5;
     const Across across(lane);
     f16v s, dp;
     rows_products<HDP>(t.k[block], st.q_hi, st.q_lo, s, t.v[block], st.g_hi, st.g_lo, dp, lane);
-    const float c = __builtin_ldexpf(factor, st.e_q + notes.e_k);
-    const int e_ratio = notes.e_k - st.top_k;
-    const int e_one = 1 - st.top_t + e_ratio + st.x_q;
-    const float a1 = __builtin_ldexpf(1.f, st.e_g + notes.e_v + e_one), b = -__builtin_ldexpf(st.dot, e_one);
+    if constexpr (UNEVEN) {  // (as above)
+        take_powers(s, powers_k, st.e_q, h);
+        take_powers(dp, powers_v, st.e_g, h, powers_k, st.x_q, &st.dot, 0);
+    }
+    const float c = __builtin_ldexpf(factor, UNEVEN ? 0 : st.e_q + notes.e_k);
+    const int e_one = UNEVEN ? 2 * NO_EXPONENT : notes.e_k + st.x_q;
+    const float a1 = __builtin_ldexpf(1.f, UNEVEN ? 0 : st.e_g + notes.e_v + e_one), b = -__builtin_ldexpf(st.dot, e_one);
     float ds[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, st.lse)) * __builtin_fmaf(dp[r], a1, b);
-    if (k0 + 31 > wave_first) {
+    if (k0 + 31 > wave_first) {  // some key is not seen by some row (whose weight or dP may be anything)
 #pragma unroll
         for (int r = 0; r < 16; ++r) ds[r] = k0 + acc_row(r, h) <= st.last ? ds[r] : 0.f;
     }
@@ -1087,18 +1209,23 @@ __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const Backwa
         load_fragments<HDP>(a.g + at, lane, st.g_hi, st.g_lo);
         st.lse = a.row_notes[row_tile * 128 + from % 64 + (lane & 31)];
         st.dot = a.row_notes[row_tile * 128 + 64 + from % 64 + (lane & 31)];
-        const Header hq = a.hq[row_tile], hg = a.hg[row_tile];
+        st.e_q = a.powers_q[row_tile * 64 + from % 64 + (lane & 31)];
+        st.e_g = a.powers_g[row_tile * 64 + from % 64 + (lane & 31)];
+        // tiles of keys that all of the wavefront's rows see, then those of which some rows do not see some key
+        const int last = row < rows ? row / p.group : job.w - 1, whole = min((wave_first + 1) / 64, tiles);
         int tk = NO_EXPONENT, tv = NO_EXPONENT;
-        for (int tile = lane; tile < tiles; tile += 64) {
+        for (int tile = lane; tile < whole; tile += 64) {
             tk = max(tk, a.hk[tile_at(tile)].e);
             tv = max(tv, a.hv[tile_at(tile)].e);
         }
-        st.e_q = __builtin_amdgcn_readfirstlane(hq.e);
-        st.e_g = __builtin_amdgcn_readfirstlane(hg.e);
-        st.top_k = wave_max_int(tk);
-        st.top_t = e_difference(st.e_g, wave_max_int(tv), __builtin_amdgcn_readfirstlane(hg.e_dot));
+        tk = wave_max_int(tk);
+        tv = wave_max_int(tv);
+        for (int tile = whole; 64 * tile < wave_seen; ++tile) {
+            tk = max(tk, max_upto(a.powers_k[tile_at(tile) * 64 + lane], last - 64 * tile));
+            tv = max(tv, max_upto(a.powers_v[tile_at(tile) * 64 + lane], last - 64 * tile));
+        }
+        st.x_q = FIT_FROM + 1 - e_difference(st.e_g, tv, power_of(fabsf(st.dot))) - tk;
     }
-    st.x_q = FIT_FROM;
     const int seen_by_row = row / p.group;
     st.last = row < rows ? seen_by_row : job.w - 1;
 #pragma unroll
@@ -1106,26 +1233,40 @@ __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const Backwa
 #pragma unroll
         for (int r = 0; r < 16; ++r) st.dq[d][r] = 0.f;
     const float factor = p.scale * LOG2E;
-    auto uniform = [](const BlockNotes& x) { return BlockNotes{__builtin_amdgcn_readfirstlane(x.e_k), __builtin_amdgcn_readfirstlane(x.e_v)}; };
-    auto use = [&](const KeyTile<HDP>& t, const BlockNotes& notes, int i) {
+    auto uniform = [](const BlockNotes& x) {
+        return BlockNotes{__builtin_amdgcn_readfirstlane(x.e_k), __builtin_amdgcn_readfirstlane(x.e_v), __builtin_amdgcn_readfirstlane(x.uneven)};
+    };
+    auto use = [&](auto uneven, const KeyTile<HDP>& t, const BlockNotes& notes, int i) __attribute__((always_inline)) {
 #pragma unroll
         for (int block = 0; block < 2; ++block)
-            if (64 * i + 32 * block < wave_seen) key_block<HDP>(t, block, notes, 64 * i + 32 * block, wave_first, factor, minus_one, lane, st);
+            if (64 * i + 32 * block < wave_seen)
+                key_block<HDP, uneven()>(t, block, notes, a.powers_k + tile_at(i) * 64 + 32 * block, a.powers_v + tile_at(i) * 64 + 32 * block,
+                                         64 * i + 32 * block, wave_first, factor, minus_one, lane, st);
     };
-    for (int i = 0; i < tiles; i += 2) {
-        staged();
-        BlockNotes notes = uniform(notes_even);
-        if (i + 1 < tiles) key_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
-        use(even, notes, i);
-        if (i + 1 >= tiles) break;
-        staged();
-        notes = uniform(notes_odd);
-        if (i + 2 < tiles) key_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
-        use(odd, notes, i + 1);
+    auto walk = [&](auto uneven, int i) __attribute__((always_inline)) {  // (as in the forward kernel)
+        for (; i < tiles; i += 2) {
+            staged();
+            BlockNotes notes = uniform(notes_even);
+            if (!uneven() && notes.uneven != 0) break;
+            if (i + 1 < tiles) key_stage<HDP>(a, odd, notes_odd, tile_at(i + 1), wave, lane);
+            use(uneven, even, notes, i);
+            if (i + 1 >= tiles) return tiles;
+            staged();
+            notes = uniform(notes_odd);
+            if (!uneven() && notes.uneven != 0) return i + 1;
+            if (i + 2 < tiles) key_stage<HDP>(a, even, notes_even, tile_at(i + 2), wave, lane);
+            use(uneven, odd, notes, i + 1);
+        }
+        return i;
+    };
+    const int at = walk(std::false_type(), 0);
+    if (__builtin_expect(at < tiles, 0)) {
+        key_stage<HDP>(a, even, notes_even, tile_at(at), wave, lane);
+        walk(std::true_type(), at);
     }
     if (row >= rows) return;
     store_column<HDP>(p.dQ + ((int64_t)q0 + seen_by_row) * p.lddq + (kv * p.group + row - seen_by_row * p.group) * (int64_t)p.head_dim, st.dq, p.scale,
-                      st.top_t - 1 + st.top_k - st.x_q, h, p.head_dim, p.vec_dq);
+                      -st.x_q, h, p.head_dim, p.vec_dq);
 }
 
 // ---- workspace --------------------------------------------------------------------------------------------------------------
@@ -1166,15 +1307,17 @@ ForwardPlan forward_plan(const CausalArgs<float>& p, void* workspace) {
     _Float16* v = c.take<_Float16>((size_t)key_tiles * 256 * hdp);
     Header* hk = c.take<Header>((size_t)key_tiles * sizeof(Header));
     Header* hv = c.take<Header>((size_t)key_tiles * sizeof(Header));
+    int* powers_k = c.take<int>((size_t)key_tiles * 64 * sizeof(int));
+    int* powers_v = c.take<int>((size_t)key_tiles * 64 * sizeof(int));
     const int64_t row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
     f.split.order = c.take<int4>((size_t)row_groups * sizeof(int4));
     f.split.order_slots[0] = (int)row_groups;
     f.split.tensors = 2;
     f.split.shift = order_shift(p.q_rows);
     f.split.p = p;
-    f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, hk, 0};
-    f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, v, hv, 0};
-    f.main = {p, k, v, hk, hv, f.split.order};
+    f.split.t[0] = {p.K, p.ldk, 1, p.vec_kv, k, hk, powers_k, 0};
+    f.split.t[1] = {p.V, p.ldv, 1, p.vec_kv, v, hv, powers_v, 0};
+    f.main = {p, k, v, hk, hv, powers_k, powers_v, f.split.order};
     f.bytes = c.used;
     return f;
 }
@@ -1192,17 +1335,20 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     BackwardPlan b{};
     _Float16* split[4];
     Header* headers[4];
+    int* powers[4];
     for (int i = 0; i < 4; ++i) {  // Q, dO, K, V
         const int64_t tiles = i < 2 ? row_tiles : key_tiles;
         split[i] = c.take<_Float16>((size_t)tiles * 256 * hdp);
         headers[i] = c.take<Header>((size_t)tiles * sizeof(Header));
+        powers[i] = c.take<int>((size_t)tiles * 64 * sizeof(int));
     }
     float* notes = c.take<float>((size_t)row_tiles * 128 * 4);
+    int* e_dot = c.take<int>((size_t)row_tiles * sizeof(int));
     b.split.p = p;
-    b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, split[0], headers[0], 0};
-    b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, split[1], headers[1], 1};
-    b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, split[2], headers[2], 0};
-    b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, split[3], headers[3], 0};
+    b.split.t[0] = {p.Q, p.ldq, p.group, p.vec_q, split[0], headers[0], powers[0], 0};
+    b.split.t[1] = {p.dO, p.ldo, p.group, p.vec_o, split[1], headers[1], powers[1], 1};
+    b.split.t[2] = {p.K, p.ldk, 1, p.vec_kv, split[2], headers[2], powers[2], 0};
+    b.split.t[3] = {p.V, p.ldv, 1, p.vec_kv, split[3], headers[3], powers[3], 0};
     const int64_t row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences);
     b.split.order = c.take<int4>((size_t)(row_groups + key_groups) * sizeof(int4));
     b.split.order_slots[0] = (int)row_groups;
@@ -1220,7 +1366,8 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     const int chunks = (int)((most_tiles + chunk - 1) / chunk);
     float* part = chunks > 1 ? c.take<float>((size_t)(part_bytes * chunks)) : nullptr;
     b.split.row_notes = notes;
-    b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], notes,
+    b.split.e_dot = e_dot;
+    b.main = {p, split[0], split[1], split[2], split[3], headers[0], headers[1], headers[2], headers[3], powers[0], powers[1], powers[2], powers[3], notes, e_dot,
               b.split.order, b.split.order + row_groups, (int)chunk, chunks, part, hd4};
     b.bytes = c.used;
     return b;

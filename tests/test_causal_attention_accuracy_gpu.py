@@ -91,7 +91,8 @@ NAMES = "o", "lse", "dq", "dk", "dv"
 def compare(batch, names=NAMES, without=()):
     """The named results within their bounds in all rows of the sequences but `without`."""
     got = batch.run()
-    want, error = batch.definition()
+    with np.errstate(over="ignore", invalid="ignore"):      # (the rows that see a large value)
+        want, error = batch.definition()
     rows = np.setdiff1d(np.arange(batch.starts[0], batch.starts[-1]), np.asarray(without, int))
     for name, x, r, e in zip(NAMES, got, want, error):
         if name in names:
@@ -169,3 +170,78 @@ def test_large_values_that_have_no_weight(gpu, dtype, by, heads, kv_heads, d, do
     for i in range(heads):
         batch.q[~first, i * d] = 120 / (40 * batch.scale)
     compare(batch.repeat(by), ("o", "lse"))
+
+
+# ---- one row of a tile much larger than the others ------------------------------------------------------------------------
+LARGER = pytest.mark.parametrize("up", [14, 20, 40, 100, "lowest"])
+
+
+def value_of(up, dtype):
+    return np.finfo(dtype).min if up == "lowest" else dtype(2.0 ** up)
+
+
+@KINDS
+@SHAPES
+@LARGER
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_a_large_row_that_is_not_seen(gpu, dtype, by, heads, kv_heads, d, where, up):
+    """The last token of each sequence, which no other sees, has a K or V that is 2^up times the others or the type's lowest value
+    throughout."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    last = batch.starts[1:] - 1
+    x = getattr(batch, where)
+    if up == "lowest":
+        x[last] = np.finfo(dtype).min
+    else:
+        x[last] *= value_of(up, dtype)
+    compare(batch.repeat(by), ("o", "lse"), without=last)
+
+
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("up", [20, 40, 80])
+def test_large_values_within_a_tile_that_have_no_weight(gpu, dtype, by, heads, kv_heads, d, up):
+    """Every fifth token has values 2^up times the others, and all queries give those weights of less than e^-90 (2^-130)."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    large = np.arange(batch.rows) % 5 == 3
+    for s in batch.starts[:-1]:
+        large[s:s + 4] = False
+    batch.v[large] *= dtype(2.0 ** min(up, 30))
+    for i in range(kv_heads):
+        batch.k[large, i * d] = -40
+    for i in range(heads):
+        batch.q[:, i * d] = 120 / (40 * batch.scale)
+    batch.v[~large] *= dtype(2.0 ** (min(up, 30) - up))
+    compare(batch.repeat(by), ("o", "lse"))
+
+
+@KINDS
+@SHAPES
+@LARGER
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_gradients_beside_a_large_row_that_is_not_seen(gpu, dtype, by, heads, kv_heads, d, where, up):
+    """The same; the last token's own gradient is zero, so that it adds nothing to those of the keys that it sees."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    last = batch.starts[1:] - 1
+    x = getattr(batch, where)
+    if up == "lowest":
+        x[last] = np.finfo(dtype).min
+    else:
+        x[last] *= value_of(up, dtype)
+    batch.g[last] = 0
+    batch.q[last] = 0       # (a score of 2^up, whose lse has an error of 2^up / 2^24, would give a weight of any size)
+    compare(batch.repeat(by), ("dq", "dk", "dv"), without=last)
+
+
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("up", [14, 20, 40, 100])
+@pytest.mark.parametrize("where", ["q", "g"])
+def test_a_large_query_in_front(gpu, dtype, by, heads, kv_heads, d, where, up):
+    """The second token of each sequence has a Q (of small keys) or a gradient 2^up times the others: keys behind it get nothing
+    from it, the others' gradients of Q nothing either."""
+    batch = Spread(dtype, LENGTHS, heads, kv_heads, d, "fused")
+    getattr(batch, where)[batch.starts[:-1] + 1] *= dtype(2.0 ** up)
+    if where == "q":
+        batch.k *= dtype(2.0 ** -up)
+    compare(batch.repeat(by), ("dq", "dk", "dv"))
