@@ -206,6 +206,18 @@ __device__ __forceinline__ void write_order(const CausalArgs<float>& p, int whic
 // apart and would be in the same LDS banks.  (Fragments that are read along stay one KB in a row.)
 __device__ __forceinline__ int place_in_fragment(int f, int l) { return l ^ (l >> 5) << 2 ^ (f & 1) << 3; }
 
+// Over each LANES lanes, in all of them.
+template <int LANES>
+__device__ __forceinline__ float max_of(float x) {
+    auto with = [&](int other) { x = fmaxf(x, __int_as_float(other)); };
+    with(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, true));
+    with(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, true));
+    with(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, true));
+    if (LANES > 8) with(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, true));
+    if (LANES > 16) x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return x;
+}
+
 template <int HDP>
 __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     constexpr int PITCH = HDP + 4, PER_ROW = HDP / 4, COUNT = 64 * PER_ROW / 256;
@@ -261,9 +273,7 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
             }
             top = fmaxf(top, fabsf(v[u][e]));
         }
-#pragma unroll
-        for (int m = 1; m < PER_ROW; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-        row_top[j] = top;  // (every lane of the row the same)
+        row_top[j] = max_of<PER_ROW>(top);  // (every lane of the row the same)
     }
     // D = rowsum(dO (.) O): the PER_ROW lanes that hold a row of dO
     if (t.dots) {
@@ -461,6 +471,15 @@ __device__ __forceinline__ void columns_product(const _Float16* block, const h8 
         [&](int i, h8 hi, h8 lo) { mfma3(hi, lo, w_hi[i % 2], w_lo[i % 2], out[i / 2]); });
 }
 
+__device__ __forceinline__ int wave_max_int(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xf, 0xf, false));   // inside each 2 lanes, 4, 8, 16
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));  // with the 16 before, with the 32 before
+    v = max(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
 // Over the two lanes that share a column (lane halves).
 __device__ __forceinline__ float max_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -521,12 +540,13 @@ __device__ __forceinline__ void take_powers(f16v& dp, const int* __restrict__ po
 // arrived: touching them earlier would wait for the copies.
 struct KeyNotes {
     Header k, v;
+    int power;  // (of uniform()) K's, or one above all if the tile is uneven
     // the same value in every lane: to scalar registers
     __device__ __forceinline__ KeyNotes uniform() const {
         KeyNotes n;
         n.k.e = __builtin_amdgcn_readfirstlane(k.e);
         n.v.e = __builtin_amdgcn_readfirstlane(v.e);
-        n.k.uneven = __builtin_amdgcn_readfirstlane(k.uneven | v.uneven);
+        n.power = __builtin_amdgcn_readfirstlane((k.uneven | v.uneven) != 0 ? -NO_EXPONENT : k.e);
         n.k.bad[0] = __builtin_amdgcn_readfirstlane(k.bad[0] | v.bad[0]);
         n.k.bad[1] = __builtin_amdgcn_readfirstlane(k.bad[1] | v.bad[1]);
         return n;
@@ -549,7 +569,7 @@ struct ForwardState {
     h8 q_hi[HDP / 16], q_lo[HDP / 16];
     f16v o[HDP / 32];
     float m, l;        // the maximum the sum refers to (in units of log2 e, whole): sum of 2^(score - m + 8), this lane half's share
-    float x;           // the same for o: sum of 2^(score + e - x + 8) V 2^-e, e the power of V's tile
+    float x;           // the same for o: sum of 2^(score + e - x + 8) V 2^-e, e the power of V; behind the last tile x - m
     int e_row;         // exponent of the row of Q
     int last;          // the last key that the lane's row sees
 };
@@ -571,8 +591,9 @@ __device__ __forceinline__ void forward_mask(f16v& s, uint32_t marks, int k0, in
 // bits from the others.  The sum of the weights follows the largest score, m: it takes the weights of a block with the ratio of the
 // two references, which are whole numbers.  Both are raised only when the largest has risen by more than 2^6 (weights reach
 // 2^6 2^8), so that the accumulators are rarely rescaled (by the factor returned).  No key seen yet: -inf, and a top of -inf keeps
-// the weights at 0.
+// the weights at 0.  (Scores of up to 2^MOST_SCORE: the references, and powers beside them, are whole numbers of 24 bits.)
 constexpr float FAR = 60.f;
+constexpr int MOST_SCORE = 23;
 template <int HDP>
 __device__ __forceinline__ float forward_weights(f16v& s, float c, float e_tile, float minus_one, ForwardState<HDP>& st, h8 (&hi)[2], h8 (&lo)[2], bool* far) {
     float top = s[0];
@@ -619,29 +640,41 @@ __device__ __forceinline__ void forward_rescale(float f, bool far, ForwardState<
     }
 }
 
-// In an uneven tile the weights that meet V take its values' powers (`powers`: of the 32 keys of the block); those that
-// `forward_weights` made are for the sum.
+// The same in uneven tiles (scores are in units of log2 e, `powers` those of the 32 values of the block) and for scores of any size:
+// all that enters an exponential is a difference from m, and x is kept as one.
 template <int HDP>
-__device__ __forceinline__ void forward_uneven_weights(const f16v& s, const int* __restrict__ powers, float minus_one, int h, ForwardState<HDP>& st,
-                                                       h8 (&hi)[2], h8 (&lo)[2]) {
-    float top = -INFINITY, w[16];
+__device__ __forceinline__ float forward_uneven_weights(f16v& s, const int* __restrict__ powers, float minus_one, int h, ForwardState<HDP>& st, h8 (&hi)[2],
+                                                        h8 (&lo)[2]) {
+    float top = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = max_halves(top);
+    const bool raise = top - st.m > 6.f;
+    const float m = raise ? ceilf(top) : st.m, down = raise ? st.m - m : 0.f, zero = m == -INFINITY ? 0.f : m;  // (m = -inf before: -inf)
+    st.m = m;
+    st.x += down;
+    float sum = 0.f, top_o = -INFINITY;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         const int4 e = *reinterpret_cast<const int4*>(powers + 8 * q + 4 * h);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            w[4 * q + c] = s[4 * q + c] + (float)(&e.x)[c];
-            top = fmaxf(top, w[4 * q + c]);
+            const float z = s[4 * q + c] - zero;
+            sum += __builtin_amdgcn_exp2f(z + 8.f);
+            s[4 * q + c] = z + (float)(&e.x)[c];
+            top_o = fmaxf(top_o, s[4 * q + c]);
         }
     }
-    top = max_halves(top);
-    const bool raise = top > st.x + 6.f;
-    const float x = raise ? ceilf(top) : st.x, f = __builtin_amdgcn_exp2f(raise ? st.x - x : 0.f), ref = x == -INFINITY ? 0.f : x - 8.f;
+    st.l = __builtin_fmaf(st.l, __builtin_amdgcn_exp2f(down), sum);
+    top_o = max_halves(top_o);
+    const bool raise_o = top_o - st.x > 6.f;
+    const float x = raise_o ? ceilf(top_o) : st.x, f = __builtin_amdgcn_exp2f(raise_o ? st.x - x : 0.f);
     st.x = x;
+    float w[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(w[r] - ref);
+    for (int r = 0; r < 16; ++r) w[r] = __builtin_amdgcn_exp2f(s[r] - (x - 8.f));
     split_regs<16>(w, minus_one, hi, lo);
-    forward_rescale<HDP>(f, false, st, hi, lo);
+    return f;
 }
 
 // A tile of KEYS keys against the wavefront's rows, block by block: the second block's scores are formed beside the first one's
@@ -651,25 +684,27 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
                                              const int* __restrict__ powers_v, int k0, int wave_first, float minus_one, int lane, ForwardState<HDP>& st) {
     const int h = lane >> 5, first_mark = k0 / 32 % 2;
     const Across across(lane);
-    const float c = UNEVEN ? 1.f : pow2(st.e_row + notes.k.e), e_v = (float)(UNEVEN ? NO_EXPONENT : notes.v.e);
+    const float c = pow2(st.e_row + notes.k.e), e_v = (float)notes.v.e;
     f16v s[KEYS / 32];
     h8 hi[2], lo[2];
-    bool far;
+    bool far = false;
+    auto weights = [&](f16v& s, int block, h8(&hi)[2], h8(&lo)[2]) __attribute__((always_inline)) {
+        if constexpr (UNEVEN) return forward_uneven_weights<HDP>(s, powers_v + 32 * block, minus_one, h, st, hi, lo);
+        else return forward_weights<HDP>(s, c, e_v, minus_one, st, hi, lo, &far);
+    };
     rows_product<HDP>(&t.k[0][0], st.q_hi, st.q_lo, s[0], lane);
-    if constexpr (UNEVEN) take_powers(s[0], powers_k, st.e_row, h);  // (to units of log2 e)
+    if constexpr (UNEVEN) take_powers(s[0], powers_k, st.e_row, h);
     forward_mask<HDP>(s[0], notes.k.bad[KEYS == 64 ? 0 : first_mark], k0, wave_first, h, st);
     if constexpr (KEYS == 64) rows_product<HDP, true>(&t.k[1][0], st.q_hi, st.q_lo, s[1], lane);
-    float f = forward_weights<HDP>(s[0], c, e_v, minus_one, st, hi, lo, &far);
+    float f = weights(s[0], 0, hi, lo);
     forward_rescale<HDP>(f, far, st, hi, lo);
-    if constexpr (UNEVEN) forward_uneven_weights<HDP>(s[0], powers_v, minus_one, h, st, hi, lo);
     if constexpr (KEYS == 64) {
         if constexpr (UNEVEN) take_powers(s[1], powers_k + 32, st.e_row, h);
         forward_mask<HDP>(s[1], notes.k.bad[1], k0 + 32, wave_first, h, st);
         columns_product<HDP, true>(&t.v[0][0], hi, lo, across, st.o);
         h8 hi2[2], lo2[2];
-        f = forward_weights<HDP>(s[1], c, e_v, minus_one, st, hi2, lo2, &far);
+        f = weights(s[1], 1, hi2, lo2);
         forward_rescale<HDP>(f, far, st, hi2, lo2);
-        if constexpr (UNEVEN) forward_uneven_weights<HDP>(s[1], powers_v + 32, minus_one, h, st, hi2, lo2);
         columns_product<HDP>(&t.v[1][0], hi2, lo2, across, st.o);
     } else {
         columns_product<HDP>(&t.v[0][0], hi, lo, across, st.o);
@@ -682,6 +717,7 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
 template <int HDP, int KEYS>
 __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel(const ForwardArgs a) {
     __shared__ __attribute__((aligned(16))) ForwardTile<HDP, KEYS> even, odd;
+    __shared__ int wave_power[4];
     const CausalArgs<float>& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     // all heads of a group of rows next to each other: consecutive workgroups go to different chiplets, so a chiplet's cache
@@ -737,6 +773,8 @@ __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel
             e -= 12;
         }
         st.e_row = e + e_factor;
+        const int power = wave_max_int(top > 0.f ? st.e_row : NO_EXPONENT);
+        if (lane == 0) wave_power[wave] = power;
 #pragma unroll
         for (int k = 0; k < HDP / 16; ++k) {
             h8 hi[1], lo[1];
@@ -759,25 +797,29 @@ __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel
         const int64_t at = ((tile0 + k0 / 64) * p.kv_heads + kv) * 64 + k0 % 64;
         if (k0 < wave_seen) forward_tile<HDP, KEYS, uneven()>(t, notes, a.powers_k + at, a.powers_v + at, k0, wave_first, minus_one, lane, st);
     };
-    // From key k0 on, whose tile is being copied; returns where an uneven tile is met by the form that takes none.  (The code for those
-    // is apart, and used from there on: inside the common one its registers cost that up to 20 %.)
+    // Scores are sums of up to 2^7 products of a row's values, below 2^12 times its power, and a key's, below 2^15.
+    __syncthreads();
+    const int most_power = MOST_SCORE - 34 - __builtin_amdgcn_readfirstlane(max(max(wave_power[0], wave_power[1]), max(wave_power[2], wave_power[3])));
+    // From key k0 on, whose tile is being copied; returns where a tile is met that needs the uneven form, by the other one.  (The code
+    // for those is apart, and used from there on: inside the common one its registers cost that up to 20 %.)
     auto walk = [&](auto uneven, int k0) __attribute__((always_inline)) {
         for (; k0 < seen; k0 += 2 * KEYS) {
             staged();
             KeyNotes notes = notes_even.uniform();
-            if (!uneven() && notes.k.uneven != 0) break;
+            if (!uneven() && notes.power > most_power) break;
             if (k0 + KEYS < seen) forward_stage<HDP, KEYS>(a, odd, notes_odd, tile0, kv, k0 + KEYS, wave, lane);
             use(uneven, even, notes, k0);
             if (k0 + KEYS >= seen) return seen;
             staged();
             notes = notes_odd.uniform();
-            if (!uneven() && notes.k.uneven != 0) return k0 + KEYS;
+            if (!uneven() && notes.power > most_power) return k0 + KEYS;
             if (k0 + 2 * KEYS < seen) forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, k0 + 2 * KEYS, wave, lane);
             use(uneven, odd, notes, k0 + KEYS);
         }
         return k0;
     };
     const int at = walk(std::false_type(), 0);
+    st.x = st.m == -INFINITY ? 0.f : st.x - st.m;
     if (__builtin_expect(at < seen, 0)) {
         // (all wavefronts are past what either buffer held before that tile)
         forward_stage<HDP, KEYS>(a, even, notes_even, tile0, kv, at, wave, lane);
@@ -786,7 +828,6 @@ __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel
     if (row >= rows) return;
     const float l = sum_halves(st.l);
     const float inv = row_bad ? NAN : 1.f / l;
-    const int e_o = st.x == -INFINITY ? 0 : (int)(st.x - st.m);
     float* __restrict__ dst = p.O + token * p.ldo + head * (int64_t)p.head_dim;
 #pragma unroll
     for (int d = 0; d < HDP / 32; ++d)
@@ -795,7 +836,7 @@ __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel
             const int at = 32 * d + 8 * q + 4 * h;
             f4 y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(st.o[d][4 * q + e] * inv, e_o);
+            for (int e = 0; e < 4; ++e) y[e] = __builtin_ldexpf(st.o[d][4 * q + e] * inv, (int)st.x);
             if (at >= p.head_dim) continue;
             if (p.vec_o) {
                 *reinterpret_cast<f4*>(dst + at) = y;
@@ -826,11 +867,6 @@ struct BackwardArgs {
     int hd4;                    // head_dim rounded up to whole vectors
 };
 
-__device__ __forceinline__ int wave_max_int(int v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, 64));
-    return __builtin_amdgcn_readfirstlane(v);
-}
 // dP - D is below 2^(e - 1) in magnitude, e from the exponents of dO, V and D: a sum of up to 2^7 products of values below 2^15
 __device__ __forceinline__ int e_difference(int e_g, int e_v, int e_dot) { return max(37 + e_g + e_v, e_dot + 1) + 1; }
 // The largest of the values of the lanes up to lane n, or from lane n on; a lane asks with an n of its own (outside 0 .. 63: none of

@@ -245,3 +245,41 @@ def test_a_large_query_in_front(gpu, dtype, by, heads, kv_heads, d, where, up):
     if where == "q":
         batch.k *= dtype(2.0 ** -up)
     compare(batch.repeat(by), ("dq", "dk", "dv"))
+
+
+# ---- scores far beyond what a weight resolves ------------------------------------------------------------------------------
+@KINDS
+@SHAPES
+@pytest.mark.parametrize("size", [10, 22, 26, 31, 40, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(gpu, dtype, by, heads, kv_heads, d, size, sign):
+    """One column of Q and K makes all scores, each a multiple of 2^size and without any rounding; the values grow and shrink by
+    2^20 from one tile of 64 tokens to the next.  A query's largest score is 2^size above the others, at its own token or at the
+    first: its weight is one and all others are nothing, so O is that token's value and lse that score.
+    How far they may be off, in unit roundoffs u = 2^-24 of single precision.  In two halves x = hi + lo + r: hi has 11 bits, so
+    |lo| <= 2^-11 |x|, and lo 11 more, |r| <= 2^-23 |x| = 2 u |x|.  O is a weight times a value without the product of the two lo, at
+    most 2^-22 = 4 u, each off by 2 u, a sum of three products (1 u) over the sum of the weights (1 u): 10 u of the row's largest.
+    The score is scale log2 e (2 u) times Q (1 u), split (2 u), times K (a half: exact), summed (1 u), times ln 2 (2 u): 8 u.  The
+    other kernels have fewer roundings."""
+    batch = Spread(dtype, [300, 64, 100], heads, kv_heads, d, "fused")
+    batch.scale = 0.5
+    batch.tail = batch.tail[:3] + (0.5,)
+    batch.q[:], batch.k[:] = 0, 0
+    want_at = np.arange(batch.rows)
+    for a, b in zip(batch.starts[:-1], batch.starts[1:]):
+        place = np.arange(b - a)
+        batch.k[a:b, ::d] = sign * dtype(2.0) * (place[:, None] + 1)
+        batch.v[a:b] *= (2.0 ** (20 * (place // 64 % 2)))[:, None].astype(dtype)
+        if sign < 0:
+            want_at[a:b] = a
+    batch.q[:, ::d] = dtype(2.0 ** size)
+    got = batch.repeat(by).run()
+    inside = np.arange(batch.starts[0], batch.starts[-1])
+    u, group = float(np.finfo(dtype).eps) / 2, heads // kv_heads
+    for h in range(heads):
+        kv = h // group
+        v = batch.v[want_at[inside], kv * d:kv * d + d].astype(np.float64)
+        o = got[0][inside, h * d:h * d + d].astype(np.float64)
+        assert (np.abs(o - v) <= 10 * u * np.abs(v).max(axis=1, keepdims=True)).all(), (h, np.abs(o - v).max())
+        score = batch.k[want_at[inside], kv * d].astype(np.float64) * 2.0 ** size * 0.5
+        assert (np.abs(got[1][h, inside] - score) <= 8 * u * np.abs(score)).all(), h
