@@ -1421,12 +1421,18 @@ inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < (
 //   1024 rows of length 64: 15 / 26 against 9 / 19;  2048 of 64: 18 / 34 against 14 / 31;  2048 of 256: 22 / 46 against 23 / 59;
 //   4096 of 1024: 47 / 108 against 82 / 243;  8 heads on 2 of keys, 2048 of 256: 19 / 86 against 23 / 65, of 1024: 38 / 121
 //   against 47 / 193.
-static bool split_pays(const CausalArgs<float>& p, int64_t least) {
+// And sequences have to fill the tiles of 128 packed rows and 64 keys, of which each takes whole ones: from 40 packed rows a sequence
+// on, in the gradients from 32 keys too.  As above, by mean length, 32768 rows, forward / backward in us:
+//   8 heads on 8: 16: 383 / 791 against 233 / 673;  32: 208 / 444 against 159 / 429;  48: 155 / 357 against 188 / 554;
+//   16 heads on 4: 8: 454 / 942 against 331 / 625;  16: 243 / 618 against 282 / 604;  24: 190 / 539 against 280 / 522;
+//   32: 156 / 457 against 279 / 507.
+static bool split_pays(const CausalArgs<float>& p, int64_t least, int64_t least_keys) {
     const int64_t rows = p.q_rows * p.heads;
-    return rows >= ((int64_t)1 << 14) && (double)rows * p.q_rows / p.sequences >= (double)least;
+    return rows >= ((int64_t)1 << 14) && (double)rows * p.q_rows / p.sequences >= (double)least && p.q_rows >= least_keys * p.sequences &&
+           p.q_rows * p.group >= (int64_t)40 * p.sequences;
 }
-bool causal_split_fwd_pays(const CausalArgs<float>& p) { return split_pays(p, 1 << 22); }
-bool causal_split_bwd_pays(const CausalArgs<float>& p) { return split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23); }
+bool causal_split_fwd_pays(const CausalArgs<float>& p) { return split_pays(p, 1 << 22, 0); }
+bool causal_split_bwd_pays(const CausalArgs<float>& p) { return split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23, 32); }
 
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
 

@@ -1,6 +1,8 @@
 """How exact causal attention is: errors in norm, and batches in whose sequences rows differ widely in size - what a row does not
 see, and what it sees with a weight of next to nothing, leaves its results alone.  The short batches run on units of 16 rows, the
 long ones of floats are computed from halves; both are held to the same bounds."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -283,3 +285,19 @@ def test_scores_of_any_size(gpu, dtype, by, heads, kv_heads, d, size, sign):
         assert (np.abs(o - v) <= 10 * u * np.abs(v).max(axis=1, keepdims=True)).all(), (h, np.abs(o - v).max())
         score = batch.k[want_at[inside], kv * d].astype(np.float64) * 2.0 ** size * 0.5
         assert (np.abs(got[1][h, inside] - score) <= 8 * u * np.abs(score)).all(), h
+
+
+# ---- which kernels a batch takes --------------------------------------------------------------------------------------------
+def device_memory_left():
+    free, total = ctypes.c_size_t(), ctypes.c_size_t()
+    assert ctypes.CDLL("libamdhip64.so").hipMemGetInfo(ctypes.byref(free), ctypes.byref(total)) == 0
+    return free.value
+
+
+def test_thousands_of_short_sequences_of_many_heads(gpu):
+    """Sequences of one to three tokens: kernels that give each a tile of 64 rows a head would work on 30 times the rows, in a
+    workspace of 18 GB forward and 36 backward for operands of 74 MB."""
+    batch = Spread(np.float32, [1, 2, 3] * 2000, 1, 1, 8, "fused")
+    before = device_memory_left()
+    compare(batch.repeat(192))
+    assert before - device_memory_left() < 2 ** 31
