@@ -30,6 +30,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace prad {
@@ -1409,8 +1410,6 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
     return b;
 }
 
-inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
-
 }  // namespace
 
 // Whether a batch is large enough for these kernels; smaller ones are faster with units of 16 rows.  Three products on halves
@@ -1431,15 +1430,28 @@ static bool split_pays(const CausalArgs<float>& p, int64_t least, int64_t least_
     return rows >= ((int64_t)1 << 14) && (double)rows * p.q_rows / p.sequences >= (double)least && p.q_rows >= least_keys * p.sequences &&
            p.q_rows * p.group >= (int64_t)40 * p.sequences;
 }
-bool causal_split_fwd_pays(const CausalArgs<float>& p) { return split_pays(p, 1 << 22, 0); }
-bool causal_split_bwd_pays(const CausalArgs<float>& p) { return split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23, 32); }
+// The other kernels take what these cannot: launches of 2^32 lanes, and a workspace that is out of proportion - head dimensions are
+// padded to 32, so that it can be many times the operands - where it is large.
+static bool split_fits(const CausalArgs<float>& p, std::initializer_list<int64_t> groups, size_t bytes) {
+    for (int64_t g : groups)
+        if (g * 256 >= ((int64_t)1 << 32)) return false;
+    return bytes <= std::max((size_t)1 << 32, (size_t)(8 * sizeof(float) * 2) * p.q_rows * (p.heads + p.kv_heads) * p.head_dim);
+}
+bool causal_split_fwd_pays(const CausalArgs<float>& p) {
+    return split_pays(p, 1 << 22, 0) && split_fits(p, {tile_slots(p.q_rows, 1, 64, p.sequences), tile_slots(p.q_rows, p.group, 128, p.sequences) * p.kv_heads}, causal_split_fwd_workspace_bytes(p));
+}
+bool causal_split_bwd_pays(const CausalArgs<float>& p) {
+    if (!split_pays(p, p.group == 1 ? 1 << 22 : 1 << 23, 32)) return false;
+    const BackwardPlan b = backward_plan(p, nullptr);
+    return split_fits(p, {tile_slots(p.q_rows, p.group, 64, p.sequences), tile_slots(p.q_rows, p.group, 128, p.sequences) * p.kv_heads,
+                          tile_slots(p.q_rows, 1, 128, p.sequences) * p.kv_heads * b.main.chunks}, b.bytes);
+}
 
 size_t causal_split_fwd_workspace_bytes(const CausalArgs<float>& p) { return forward_plan(p, nullptr).bytes; }
 
 hipError_t launch_causal_split_fwd(const CausalArgs<float>& p, void* workspace, hipStream_t s) {
     const ForwardPlan f = forward_plan(p, workspace);
     const int64_t key_slots = tile_slots(p.q_rows, 1, 64, p.sequences), slots = tile_slots(p.q_rows, p.group, 128, p.sequences);
-    if (!grid_fits(key_slots, 256) || !grid_fits(slots * p.kv_heads, 256)) return hipErrorInvalidValue;
     const dim3 split((unsigned)key_slots, p.kv_heads, 3), grid((unsigned)(slots * p.kv_heads)), block(256);
     switch (padded(p.head_dim)) {
         case 32:
@@ -1472,8 +1484,6 @@ hipError_t launch_causal_split_bwd(const CausalArgs<float>& p, void* workspace, 
     const BackwardPlan b = backward_plan(p, workspace);
     const int64_t row_tiles = tile_slots(p.q_rows, p.group, 64, p.sequences), key_groups = tile_slots(p.q_rows, 1, 128, p.sequences),
                   row_groups = tile_slots(p.q_rows, p.group, 128, p.sequences);
-    if (!grid_fits(row_tiles, 256) || !grid_fits(row_groups * p.kv_heads, 256) || !grid_fits(key_groups * p.kv_heads * b.main.chunks, 256))
-        return hipErrorInvalidValue;
     // (at least two wide: the workgroups 0 and 1 of the last plane make the schedules, however few tiles there are)
     const dim3 split((unsigned)std::max<int64_t>(row_tiles, 2), p.kv_heads, 5), row_grid((unsigned)(row_groups * p.kv_heads));
     switch (padded(p.head_dim)) {

@@ -301,3 +301,12 @@ def test_thousands_of_short_sequences_of_many_heads(gpu):
     before = device_memory_left()
     compare(batch.repeat(192))
     assert before - device_memory_left() < 2 ** 31
+
+
+def test_very_many_heads_of_one_column(gpu):
+    """Head dimensions are padded to 32 where a batch is computed from halves: 8192 heads of one column would take 10 GB of
+    workspace for operands of 67 MB."""
+    batch = Spread(np.float32, [1500, 548], 2, 2, 1, "fused")
+    before = device_memory_left()
+    compare(batch.repeat(4096))
+    assert before - device_memory_left() < 2 ** 31
