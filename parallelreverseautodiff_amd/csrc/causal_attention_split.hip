@@ -304,9 +304,10 @@ __global__ void __launch_bounds__(256) causal_split_kernel(const SplitArgs a) {
     }
     __syncthreads();
     // One power for the tile, or one for each row where some are far below the largest: each wavefront for itself, a row per lane.
+    // (A row with a non-finite value does not count: whoever sees it gets NaN, and the others keep their bits.)
     const float top_here = row_top[lane], top = wave_max_t(top_here);
     const int e = power_for(top);
-    const bool uneven = __ballot(row0 + lane < rows && top > 0.f && power_of(top) - power_of(top_here) > MOST_SPREAD) != 0;
+    const bool uneven = __ballot(row0 + lane < rows && bad[lane] == 0 && top > 0.f && power_of(top) - power_of(top_here) > MOST_SPREAD) != 0;
     const int64_t tile_at = (int64_t)blockIdx.x * p.kv_heads + kv;
     if (wave == 0) {
         const uint64_t marks = __ballot(bad[lane] != 0);

@@ -310,3 +310,25 @@ def test_very_many_heads_of_one_column(gpu):
     before = device_memory_left()
     compare(batch.repeat(4096))
     assert before - device_memory_left() < 2 ** 31
+
+
+@KINDS
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("where", ["q", "k", "v", "g"])
+def test_rows_without_a_finite_value(gpu, dtype, by, where, value):
+    """Token 20 of the first sequence holds nothing finite: who does not see it keeps every bit."""
+    clean, dirty = (Spread(dtype, LENGTHS, 2, 1, 64, "fused") for _ in range(2))
+    at, end, last = int(clean.starts[0]) + 20, int(clean.starts[1]), int(clean.starts[-1])
+    getattr(dirty, where)[at] = value
+    a, b = clean.repeat(by).run(), dirty.repeat(by).run()
+    before, others, behind = np.arange(clean.starts[0], at), np.arange(end, last), np.arange(at + 1, end)
+    keep = {"o": np.r_[before, others], "lse": np.r_[before, others], "dq": np.r_[before, others], "dk": others, "dv": others}
+    if where in "qg":       # one row that is not to be had, and the keys that it sees
+        keep.update(o=np.r_[before, behind, others], lse=np.r_[before, behind, others], dq=np.r_[before, behind, others],
+                    dk=np.r_[behind, others], dv=np.r_[behind, others])
+    if where == "g":
+        keep.update(o=np.r_[before, at, behind, others], lse=np.r_[before, at, behind, others])
+    for name, x, y in zip(NAMES, a, b):
+        rows = np.s_[:, keep[name]] if name == "lse" else keep[name]
+        assert np.array_equal(x[rows], y[rows]), name
+    assert where == "g" or np.isnan(b[0][at]).all()
