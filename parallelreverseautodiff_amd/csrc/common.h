@@ -435,7 +435,7 @@ hipError_t launch_window_attention_bwd(const float* QKV, const float* P, const f
 // Embedding lookup and gradient, dropout, index vectors (csrc/token.hip).
 template <typename T> hipError_t launch_embedding_fwd(const T* table, const int32_t* ids, T* out, int64_t tokens, int64_t vocab, int64_t width, T scale,
                                                       hipStream_t s);
-size_t embedding_bwd_workspace_bytes(int64_t tokens, int64_t width);
+size_t embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t width);
 template <typename T> hipError_t launch_embedding_bwd(const T* dout, const int32_t* ids, T* dtable, int64_t tokens, int64_t vocab, int64_t width,
                                                       double scale, int accumulate, void* workspace, hipStream_t s);
 // residual may be nullptr; step nullptr: step 0

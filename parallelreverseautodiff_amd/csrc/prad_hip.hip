@@ -1927,7 +1927,7 @@ int32_t prad_embedding_bwd(prad_buf_t dout, prad_index_t ids, double scale, prad
     if (int32_t st = embedding_check(dtable, dout, ids, scale)) return st;
     if (overlap(dtable, dout) || overlap(dtable, ids)) return fail(PRAD_ERR_ARG, "dtable must not overlap an input");
     ENQUEUE_LOCK();
-    if (int32_t st = ensure_workspace(embedding_bwd_workspace_bytes(dout->rows, dout->cols))) return st;
+    if (int32_t st = ensure_workspace(embedding_bwd_workspace_bytes(dout->rows, dtable->rows, dout->cols))) return st;
     const int acc = accumulate != 0 ? 1 : 0;
     if (dtable->dtype == PRAD_F64)
         HIP_TRY(launch_embedding_bwd<double>(static_cast<const double*>(dout->ptr), ids->ptr, static_cast<double*>(dtable->ptr), dout->rows, dtable->rows,

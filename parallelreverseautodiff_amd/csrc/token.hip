@@ -380,14 +380,15 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const int32_t* __re
 inline bool grid_fits(int64_t groups, int64_t lanes) { return groups * lanes < ((int64_t)1 << 32); }
 
 inline size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
+// (a table of more rows than a launch has wavefronts takes the other launches, which have a workgroup for 960 rows)
+inline bool one_launch(int64_t tokens, int64_t vocab) { return tokens <= EMB_DIRECT_TOKENS && grid_fits((vocab + 3) / 4, 256); }
 inline int64_t sum_chunks(int64_t tokens) { return (tokens + SUM_CHUNK - 1) / SUM_CHUNK; }
 
 template <typename T, int N>
 hipError_t embedding_bwd_n(const T* dout, const int32_t* ids, T* dtable, int64_t tokens, int64_t vocab, int64_t width, double scale, int accumulate,
                            void* workspace, hipStream_t s) {
     const int64_t packs = width / N;
-    if (tokens <= EMB_DIRECT_TOKENS) {
-        if (!grid_fits((vocab + 3) / 4, 256)) return hipErrorInvalidValue;
+    if (one_launch(tokens, vocab)) {
         hipLaunchKernelGGL((embedding_bwd_direct_kernel<T, N>), dim3((unsigned)((vocab + 3) / 4)), dim3(256), 0, s, dout, ids, dtable, (int)tokens, vocab,
                            packs, scale, accumulate);
         return hipGetLastError();
@@ -521,8 +522,8 @@ hipError_t launch_embedding_fwd(const T* table, const int32_t* ids, T* out, int6
     return hipGetLastError();
 }
 
-size_t embedding_bwd_workspace_bytes(int64_t tokens, int64_t width) {
-    if (tokens <= EMB_DIRECT_TOKENS) return 0;
+size_t embedding_bwd_workspace_bytes(int64_t tokens, int64_t vocab, int64_t width) {
+    if (one_launch(tokens, vocab)) return 0;
     return 256 + 2 * round256((size_t)tokens * 4) + 2 * (size_t)sum_chunks(tokens) * width * sizeof(double);
 }
 

@@ -312,3 +312,21 @@ def test_another_thread_is_refused_while_one_records(gpu):
     check(lib.prad_graph_destroy(gr))
     with pytest.raises(InvalidOperationException):
         check(_lib.PRAD_ERR_RECORDING)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 512, 600])
+def test_gradient_of_a_table_of_very_many_rows(gpu, tokens):
+    """More than 2^26 rows, whatever the number of tokens."""
+    lib, vocab = _lib.load(), 2 ** 26 + 1000
+    ids = np.array([vocab - 1, 0, vocab - 1, -1, 2 ** 26 - 1] * (tokens // 5 + 1), np.int64)[:tokens]
+    dout = seeded.normal(19, 1, (tokens, 1), 1.0, np.float32)
+    bd, bi, d_table = dev(dout), IndexVector.from_values(ids), DeviceBuffer.alloc_output(np.float32, vocab, 1)
+    check(lib.prad_embedding_bwd(bd.handle, bi.handle, 0.5, d_table.handle, 0))
+    flat = DeviceBuffer.wrap(np.float32, 1, vocab, d_table.ptr, parent=d_table)      # (one row: a download goes row by row)
+    got = flat.download()[0]
+    want = np.zeros(vocab, np.float32)
+    for r in set(ids[ids >= 0].tolist()):       # (sums in double, rounded once)
+        want[r] = np.float32(dout[ids == r, 0].astype(np.float64).sum() * 0.5)
+    assert np.allclose(got, want, rtol=2.0 ** -23, atol=0)
+    check(lib.prad_embedding_bwd(bd.handle, bi.handle, 0.5, d_table.handle, 1))
+    assert np.allclose(flat.download()[0], 2 * want, rtol=2.0 ** -22, atol=0)
