@@ -1897,6 +1897,9 @@ int32_t prad_index_add(prad_index_t v, int32_t delta) {
     return PRAD_OK;
 }
 
+// Finite in the element type, and times log2 e as well.
+static bool scale_fits(double scale, int32_t dtype) { return std::isfinite(scale) && (dtype == PRAD_F64 || std::fabs(scale) < 0x1p127); }
+
 // rows x width against a table of the same width, `rows` ids
 static int32_t embedding_check(prad_buf_t table, prad_buf_t rows, prad_index_t ids, double scale) {
     REQUIRE_BUF(table); REQUIRE_BUF(rows); REQUIRE_INDEX(ids);
@@ -1905,7 +1908,7 @@ static int32_t embedding_check(prad_buf_t table, prad_buf_t rows, prad_index_t i
     if (table->cols != rows->cols) return fail(PRAD_ERR_SHAPE, "the table has %lld columns, the rows %lld", (long long)table->cols, (long long)rows->cols);
     if (ids->n != rows->rows) return fail(PRAD_ERR_SHAPE, "%lld ids for %lld rows", (long long)ids->n, (long long)rows->rows);
     if (table->rows > INT32_MAX || rows->rows > INT32_MAX || table->cols > INT32_MAX) return fail(PRAD_ERR_ARG, "an embedding holds at most 2^31 - 1 rows and columns");
-    if (!std::isfinite(scale)) return fail(PRAD_ERR_ARG, "scale must be finite");
+    if (!scale_fits(scale, table->dtype)) return fail(PRAD_ERR_ARG, "scale must be finite in the element type");
     return PRAD_OK;
 }
 
@@ -1993,11 +1996,10 @@ static int32_t columns_check(const HeadColumns& c, int64_t rows) {
         return fail(PRAD_ERR_SHAPE, "%s: columns [%lld, %lld) lie outside its %lld", c.name, (long long)c.col, (long long)(c.col + c.width), (long long)c.buf->cols);
     return PRAD_OK;
 }
-static int32_t heads_check(int64_t heads, int64_t kv_heads, int64_t head_dim, double scale) {
+static int32_t heads_check(int64_t heads, int64_t kv_heads, int64_t head_dim) {
     if (heads < 1 || kv_heads < 1 || heads > 65535 || kv_heads > heads || heads % kv_heads != 0)
         return fail(PRAD_ERR_ARG, "the heads must be a multiple of the key/value heads, 1 to 65535 of them");
     if (head_dim < 1 || head_dim > 128) return fail(PRAD_ERR_ARG, "the head dimension must be 1 to 128");
-    if (!std::isfinite(scale)) return fail(PRAD_ERR_ARG, "scale must be finite");
     return PRAD_OK;
 }
 extern "C++" {
@@ -2078,9 +2080,10 @@ static int32_t cached_t(CausalArgs<T> a, prad_index_t q_offsets, prad_index_t k_
 
 // Operands common to the three calls; rows of K and V may differ from Q's with a cache.
 static int32_t causal_check(const HeadColumns& Q, const HeadColumns& K, const HeadColumns& V, prad_buf_t O, prad_index_t offsets, int64_t heads,
-                            int64_t head_dim, bool cache) {
+                            int64_t head_dim, double scale, bool cache) {
     REQUIRE_BUF(Q.buf); REQUIRE_BUF(K.buf); REQUIRE_BUF(V.buf); REQUIRE_BUF(O); REQUIRE_INDEX(offsets);
     if (int32_t st = same_dtype({Q.buf, K.buf, V.buf, O})) return st;
+    if (!scale_fits(scale, O->dtype)) return fail(PRAD_ERR_ARG, "scale must be finite in the element type");
     if (int32_t st = columns_check(Q, Q.buf->rows)) return st;
     if (int32_t st = columns_check(K, cache ? K.buf->rows : Q.buf->rows)) return st;
     if (int32_t st = columns_check(V, K.buf->rows)) return st;
@@ -2096,9 +2099,9 @@ static int32_t causal_check(const HeadColumns& Q, const HeadColumns& K, const He
 int32_t prad_causal_attention_fwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t k_col, prad_buf_t V, int64_t v_col, prad_buf_t O,
                                   prad_buf_t lse, prad_index_t offsets, int64_t heads, int64_t kv_heads, int64_t head_dim, double scale) {
     REQUIRE_INIT();
-    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    if (int32_t st = heads_check(heads, kv_heads, head_dim)) return st;
     const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
-    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, false)) return st;
+    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, scale, false)) return st;
     if (lse != nullptr) {
         REQUIRE_BUF(lse);
         if (int32_t st = same_dtype({Q, lse})) return st;
@@ -2119,9 +2122,9 @@ int32_t prad_causal_attention_bwd(prad_buf_t Q, int64_t q_col, prad_buf_t K, int
                                   prad_buf_t dV, int64_t dv_col, prad_index_t offsets, int64_t heads, int64_t kv_heads,
                                   int64_t head_dim, double scale) {
     REQUIRE_INIT();
-    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    if (int32_t st = heads_check(heads, kv_heads, head_dim)) return st;
     const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
-    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, false)) return st;
+    if (int32_t st = causal_check(q, k, v, O, offsets, heads, head_dim, scale, false)) return st;
     REQUIRE_BUF(lse); REQUIRE_BUF(dO); REQUIRE_BUF(dQ); REQUIRE_BUF(dK); REQUIRE_BUF(dV);
     if (int32_t st = same_dtype({Q, lse, dO, dQ, dK, dV})) return st;
     if (int32_t st = expect_rows(lse, heads, Q->rows, "lse")) return st;
@@ -2145,9 +2148,9 @@ int32_t prad_cached_attention(prad_buf_t Q, int64_t q_col, prad_buf_t K, int64_t
                               prad_index_t q_offsets, prad_index_t k_begin, prad_index_t k_end, int64_t heads, int64_t kv_heads,
                               int64_t head_dim, double scale) {
     REQUIRE_INIT();
-    if (int32_t st = heads_check(heads, kv_heads, head_dim, scale)) return st;
+    if (int32_t st = heads_check(heads, kv_heads, head_dim)) return st;
     const HeadColumns q{Q, q_col, heads * head_dim, "Q"}, k{K, k_col, kv_heads * head_dim, "K"}, v{V, v_col, kv_heads * head_dim, "V"};
-    if (int32_t st = causal_check(q, k, v, O, q_offsets, heads, head_dim, true)) return st;
+    if (int32_t st = causal_check(q, k, v, O, q_offsets, heads, head_dim, scale, true)) return st;
     REQUIRE_INDEX(k_begin); REQUIRE_INDEX(k_end);
     if (k_begin->n != q_offsets->n - 1 || k_end->n != q_offsets->n - 1)
         return fail(PRAD_ERR_SHAPE, "%lld sequences need as many key ranges", (long long)(q_offsets->n - 1));

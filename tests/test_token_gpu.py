@@ -330,3 +330,19 @@ def test_gradient_of_a_table_of_very_many_rows(gpu, tokens):
     assert np.allclose(got, want, rtol=2.0 ** -23, atol=0)
     check(lib.prad_embedding_bwd(bd.handle, bi.handle, 0.5, d_table.handle, 1))
     assert np.allclose(flat.download()[0], 2 * want, rtol=2.0 ** -22, atol=0)
+
+
+@DTYPES
+def test_a_scale_that_the_element_type_does_not_hold(gpu, dtype):
+    """1e39 is a number in double and infinite in float."""
+    lib, wanted = _lib.load(), _lib.PRAD_OK if dtype == np.float64 else _lib.PRAD_ERR_ARG
+    table, out, ids = DeviceBuffer.alloc(dtype, 10, 8), DeviceBuffer.alloc(dtype, 5, 8), IndexVector.alloc(5)
+    assert lib.prad_embedding_fwd(table.handle, ids.handle, 1e39, out.handle) == wanted
+    assert lib.prad_embedding_bwd(out.handle, ids.handle, 1e39, table.handle, 0) == wanted
+    x, o, lse, dx = (DeviceBuffer.alloc(dtype, r, c) for r, c in ((5, 24), (5, 8), (2, 5), (5, 24)))
+    off, begin, end = IndexVector.from_values([0, 5]), IndexVector.alloc(1), IndexVector.from_values([5])
+    qkv = x.handle, 0, x.handle, 8, x.handle, 16
+    for scale, status in ((1e39, wanted), (-1e39, wanted), (1e300, wanted), (1e38, _lib.PRAD_OK), (float("inf"), _lib.PRAD_ERR_ARG)):
+        assert lib.prad_causal_attention_fwd(*qkv, o.handle, lse.handle, off.handle, 2, 2, 4, scale) == status
+        assert lib.prad_causal_attention_bwd(*qkv, o.handle, lse.handle, o.handle, dx.handle, 0, dx.handle, 8, dx.handle, 16, off.handle, 2, 2, 4, scale) == status
+        assert lib.prad_cached_attention(*qkv, o.handle, off.handle, begin.handle, end.handle, 2, 2, 4, scale) == status
