@@ -714,8 +714,11 @@ __device__ __forceinline__ void forward_tile(const ForwardTile<HDP, KEYS>& t, co
 }
 
 // Bound by the matrix instructions (busy 60 % of the time) and by what of the softmax does not hide behind them: 16 heads on 4 of
-// keys, head dimension 64, 8192 tokens in 420 us, 330 TFLOP/s of the visible pairs, 990 with the three products each - 93 %
-// of a large library product of halves.  Twelve sequences of up to 2048 in 75 us.
+// keys, head dimension 64, 8192 tokens in 432 us, 318 TFLOP/s of the visible pairs, 954 with the three products each - 90 %
+// of a large library product of halves.  Twelve sequences of up to 2048 in 75 us (busy 47 %: their lengths leave compute units idle at
+// the end).  8 heads of 128, 4096 tokens, in 187 us: a workgroup to a compute unit, so that its latencies show (busy 45 %).  Where an
+// uneven tile is met, the rest of a workgroup's walk takes its code: the 8192 tokens then 575 us for 444, with 4096 tokens and 8 heads
+// of 128 300 us for 207, of 32 161 for 88 (calls with both launches).
 template <int HDP, int KEYS>
 __global__ void __launch_bounds__(256, HDP > 32 ? 2 : 3) causal_split_fwd_kernel(const ForwardArgs a) {
     __shared__ __attribute__((aligned(16))) ForwardTile<HDP, KEYS> even, odd;
@@ -888,7 +891,9 @@ __device__ __forceinline__ int max_from(int v, int n) {
 
 // Makes weights fit into halves: where a column's largest has passed 2^15, the column and its accumulators come down to 2^11, so
 // that it takes another factor of 16 before the next time.  x: the power of two that the column is scaled by.
-constexpr int FIT_FROM = 110;  // (the smallest normal weight, 2^-126, still shows)
+// Weights start at 2^FIT_FROM times what is at most 1: a sum all of whose terms are below 2^-100 of the largest |dO||V| that it might have
+// held - a weight of 2^-60 beside values 2^40 times the others' - loses bits, one with larger terms does not.
+constexpr int FIT_FROM = 110;
 template <int N>
 __device__ __forceinline__ void fit(float (&w)[16], int& x, f16v (&acc)[N]) {
     float top = fabsf(w[0]);
@@ -1027,7 +1032,8 @@ __device__ __forceinline__ void row_block(const RowTile<HDP>& t, int block, cons
 
 // Bound by vector instructions beside the products (two exponent-sized passes, two splits and two looks for the largest weight per
 // score) and, one third, by the last workgroups: 16 heads on 4 of keys, head dimension 64, sequences of 2048, 1901, 1536, 1000,
-// 800, 511, 300 and 64 tokens in 187 us, 4 of the 7 products of a training step.
+// 800, 511, 300 and 64 tokens in 177 us, 4 of the 7 products of a training step (matrix instructions busy 56 % of the time).  With
+// uneven tiles all through 5 to 40 % slower.
 template <int HDP>
 __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_kernel(const BackwardArgs a) {
     __shared__ __attribute__((aligned(16))) RowTile<HDP> even, odd;
@@ -1135,7 +1141,7 @@ __global__ void __launch_bounds__(256, HDP > 64 ? 1 : 2) causal_split_bwd_kv_ker
     store_column<HDP>(dst_v, st.dv, 1.f, -st.x_v, h, width, vec);
 }
 
-// Adds the parts of the groups of keys that have several, in their order (16 us behind the 187 above, by memory).
+// Adds the parts of the groups of keys that have several, in their order (16 us behind the 177 above, by memory).
 __global__ void __launch_bounds__(256) causal_split_join_kernel(const BackwardArgs a) {
     const CausalArgs<float>& p = a.p;
     const int kv = blockIdx.x % (unsigned)p.kv_heads;
@@ -1221,7 +1227,7 @@ __device__ __forceinline__ void key_block(const KeyTile<HDP>& t, int block, cons
     columns_product<HDP>(t.k[block], hi, lo, across, st.dq);
 }
 
-// Bound as the forward kernel: the batch above in 114 us, 3 products of the 7.
+// Bound as the forward kernel: the batch above in 115 us, 3 products of the 7.
 template <int HDP>
 __global__ void __launch_bounds__(256, 2) causal_split_bwd_q_kernel(const BackwardArgs a) {
     __shared__ __attribute__((aligned(16))) KeyTile<HDP> even, odd;
