@@ -44,10 +44,16 @@ def bounds(q, k, v, scale, u, g):
             (p * (again + (n + 4) * u)).T @ np.abs(g))
 
 
+HALVES = 0
+
+
 class Spread(Batch):
-    """A batch whose few heads are repeated `by` times on the device: large enough for the halves, quick to define."""
+    """A batch whose few heads are repeated `by` times on the device, or (HALVES) as often as makes it large enough for the
+    halves: rows * heads * mean length of 2^23."""
 
     def repeat(self, by):
+        if by == HALVES:
+            by = -(-2 ** 23 * len(self.lengths) // (self.rows ** 2 * self.heads))
         self.few = self.heads, self.kv_heads, self.q, self.k, self.v, self.g
         self.by = by
         self.heads, self.kv_heads = by * self.heads, by * self.kv_heads
@@ -102,7 +108,7 @@ def compare(batch, names=NAMES, without=()):
             close(x[at], r[at], e[at], name)
 
 
-KINDS = pytest.mark.parametrize("dtype,by", [(np.float64, 1), (np.float32, 1), (np.float32, 160)], ids=["f64", "f32", "f32-halves"])
+KINDS = pytest.mark.parametrize("dtype,by", [(np.float64, 1), (np.float32, 1), (np.float32, HALVES)], ids=["f64", "f32", "f32-halves"])
 SHAPES = pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (4, 2, 40), (3, 1, 128)], ids=str)
 LENGTHS = [190, 64, 100]
 
