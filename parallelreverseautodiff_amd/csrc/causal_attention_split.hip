@@ -7,9 +7,9 @@
 // (library products on this card: 1060 TFLOP/s in half, 153 in float) - and they overlap with vector instructions, which the
 // float ones do not.
 //
-// Scaling.  A half has 11 bits from 2^-14 on and ends at 2^-24, so an element keeps its 11 + 11 bits down to 2^-2 or so; what is
-// below that is off by 2^-25.  The rows of a tile (64 rows of one head) are scaled by one power of two that takes the largest
-// magnitude in it to [2^11, 2^15), as long as no row's largest is more than 2^10 below that: every row is then right to 2^-24 of
+// Scaling.  A half has 11 bits from 2^-14 on and ends at 2^-24, so an element keeps its 11 + 11 bits, off by 2^-23 of itself at most,
+// down to 2^-2 or so; what is below that is off by 2^-25.  The rows of a tile (64 rows of one head) are scaled by one power of two that takes the largest
+// magnitude in it to [2^11, 2^15), as long as no row's largest is more than 2^10 below that: every row is then right to 2^-23 of
 // its own largest.  In an uneven tile each row has a power of its own; those go onto the scores, onto dP and onto the weights, row
 // by row.  Where tiles are summed in one accumulator, the ratio of their powers is folded into the weights, in float.  The weights
 // of a column (a query forward, a key or a query backward), with that ratio, are scaled by a power of two that belongs to the
@@ -642,8 +642,8 @@ __device__ __forceinline__ void forward_rescale(float f, bool far, ForwardState<
     }
 }
 
-// The same in uneven tiles (scores are in units of log2 e, `powers` those of the 32 values of the block) and for scores of any size:
-// all that enters an exponential is a difference from m, and x is kept as one.
+// `forward_weights` in uneven tiles (scores are in units of log2 e, `powers` those of the 32 values of the block) and for scores of
+// any size: all that enters an exponential is a difference from m, and x is kept as one.
 template <int HDP>
 __device__ __forceinline__ float forward_uneven_weights(f16v& s, const int* __restrict__ powers, float minus_one, int h, ForwardState<HDP>& st, h8 (&hi)[2],
                                                         h8 (&lo)[2]) {
@@ -1428,7 +1428,8 @@ BackwardPlan backward_plan(const CausalArgs<float>& p, void* workspace) {
 //   4096 of 1024: 47 / 108 against 82 / 243;  8 heads on 2 of keys, 2048 of 256: 19 / 86 against 23 / 65, of 1024: 38 / 121
 //   against 47 / 193.
 // And sequences have to fill the tiles of 128 packed rows and 64 keys, of which each takes whole ones: from 40 packed rows a sequence
-// on, in the gradients from 32 keys too.  As above, by mean length, 32768 rows, forward / backward in us:
+// on, in the gradients from 32 keys too.  (The mean stands for the lengths, which the host does not know.)  As above, by mean length,
+// 32768 rows, forward / backward in us:
 //   8 heads on 8: 16: 383 / 791 against 233 / 673;  32: 208 / 444 against 159 / 429;  48: 155 / 357 against 188 / 554;
 //   16 heads on 4: 8: 454 / 942 against 331 / 625;  16: 243 / 618 against 282 / 604;  24: 190 / 539 against 280 / 522;
 //   32: 156 / 457 against 279 / 507.
